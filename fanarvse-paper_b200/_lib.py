@@ -65,7 +65,25 @@ SIGNATURES = {
     "fvs_rows_scatter": (I32, [P, P, I32, I32, P, I32, P, P, P]),
     "fvs_exact_scores": (I32, [P, P, I32, P, I32, I32, P, I32, P]),
     "fvs_merge_topk": (I32, [P, P, P, I32, I32, I32, I32, P, P]),
+    "fvs_kv_append": (I32, [P, P, I32, P, I64, I64, P, I64, I64, P, I64, I64, I32, P, P, I32, I32, I64, P, P, P, I32,
+                             P, P, I32, I32, I32]),
+    "fvs_kv_read": (I32, [P, P, I32, P, P, P, I32, I32, I64, P, P, I32]),
+    "fvs_kv_attend_work": (I32, [I32, I32, I32]),
+    "fvs_kv_attend": (I32, [P, P, I32, P, I64, I64, I32, P, I32, I32, I64, P, F32, P, P, P]),
 }
+
+
+class KvCache(C.Structure):
+    """fvs_kv_cache of include/fanar_b200.h"""
+    _fields_ = [("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("fill", P), ("status", P),
+                ("page_stride", I64), ("head_stride", I64), ("slot_stride", I64),
+                ("scale_page_stride", I64), ("scale_head_stride", I64), ("scale_slot_stride", I64),
+                ("pages", C.c_int32), ("heads", C.c_int32), ("page", C.c_int32), ("dim", C.c_int32),
+                ("type", C.c_int32)]
+
+
+F16, BF16, I8, F32T = 0, 1, 2, 3        # element type codes
+PAIRS = {"halves": 0, "neighbours": 1}  # which elements of a head the rotation pairs
 
 ERRORS = {-1: "FVS_EINVAL (bad argument)", -2: "FVS_ERANGE (size above the kernel's limit)"}
 

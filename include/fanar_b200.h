@@ -439,6 +439,81 @@ int fvs_rows_scatter(fvs_stream_t stream, const int32_t* rows, int FB, int B, ui
 int fvs_merge_topk(fvs_stream_t stream, const int64_t* ids_g, const float* score_g, int G, int B, int kin, int k,
                    int64_t* I, float* S);
 
+/*
+ * Paged key-value cache (new: what follows a search when a model answers from the found passages).  The reference has
+ * no counterpart.
+ *
+ * Keys and values of one layer lie in pages of `page` token slots: k and v are [pages, heads, page, dim] with the given
+ * strides in ELEMENTS (the same for both; a head's dim elements are contiguous).  type FVS_F16 / FVS_BF16: the values;
+ * FVS_I8: codes, with one fp32 scale per (page, head, slot) in k_scale / v_scale (strides in elements): value = code *
+ * scale.  dim is 64, 96, 128, 192 or 256; k, v and every stride are multiples of 16 bytes.
+ * fill (nullable) [pages]: only the first fill[p] slots of page p hold a token (a passage whose last page is partly
+ * filled); without it every slot does.
+ * status: one device word, set to FVS_KV_BAD_INDEX when a call meets an index outside its table (a page number >=
+ * pages, a sequence outside the page table, a token past its row, a position past the rotation table); that access is
+ * skipped.  The caller clears it.
+ *
+ * A page table is int32 [seqs, wide] (rows table_stride elements apart): logical token t of sequence b lies in page
+ * table[b, t / page], slot t % page; a negative entry is a hole (a search result -1, an unused place).
+ */
+#define FVS_F16 0
+#define FVS_BF16 1
+#define FVS_I8 2
+#define FVS_F32 3
+#define FVS_KV_BAD_INDEX 1
+typedef struct fvs_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    const int32_t* fill;
+    int32_t* status;
+    int64_t page_stride, head_stride, slot_stride;
+    int64_t scale_page_stride, scale_head_stride, scale_slot_stride;
+    int32_t pages, heads, page, dim, type;
+} fvs_kv_cache;
+
+/*
+ * Appends the keys k and values v [tokens, heads, dim] (type: FVS_F16 or FVS_BF16, the cache's own unless that is
+ * FVS_I8; token and head strides in elements) of new tokens: token n goes to logical place idx[n] of sequence seq[n]
+ * (seq NULL: sequence n).  idx[n] < 0 or a hole: nothing is stored.  Two tokens at one place: either one is kept.
+ * Before that the first `rot` elements of each key head (rot a multiple of 16, <= dim; 0: none) and of each head of q
+ * [tokens, hq, dim] (hq 0: none) are rotated by cos / sin [positions, rot / 2] at position pos[n] (pos NULL: idx[n]),
+ * pairs (i, i + rot / 2) or (2i, 2i + 1): (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once.  q_out is
+ * contiguous [tokens, hq, dim] and may be q; zeros for a token without a place.
+ * Codes of an FVS_I8 cache: scale = amax * (1 / 127), code = rint(x * ((1 / amax) * 127)) in fp32, codes and scale 0
+ * for a row of zeros; a row with an infinity or a not-a-number reads back as not-a-numbers.
+ */
+#define FVS_PAIRS_HALVES 0
+#define FVS_PAIRS_NEIGHBOURS 1
+int fvs_kv_append(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* k, int64_t k_token,
+                  int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* q, int64_t q_token,
+                  int64_t q_head, int hq, void* q_out, const int32_t* table, int seqs, int wide, int64_t table_stride,
+                  const int32_t* seq, const int32_t* idx, const int32_t* pos, int tokens, const float* cos,
+                  const float* sin, int positions, int rot, int pairs);
+
+/*
+ * Reads the rows of tokens idx[n] of sequences seq[n] (NULL: sequence n) back: k and v contiguous [tokens, heads, dim]
+ * of `type` FVS_F16, FVS_BF16 or FVS_F32, codes times their scale in fp32, rounded once.  Zeros where there is no place.
+ * fill is not looked at.
+ */
+int fvs_kv_read(fvs_stream_t stream, const fvs_kv_cache* cache, int type, void* k, void* v, const int32_t* table,
+                int seqs, int wide, int64_t table_stride, const int32_t* seq, const int32_t* idx, int tokens);
+
+/*
+ * Attention of one new token per sequence over its visible keys: q [seqs, hq, dim] (type FVS_F16 or FVS_BF16, the
+ * cache's own unless that is FVS_I8; strides in elements), hq a multiple of the cache's heads, query head h reads key
+ * head h / (hq / heads).  Token t of sequence b is visible if t < lens[b], its table entry is a page and its slot <
+ * fill.  out[b, h] = sum_t p_t v_t with p the softmax of scale * <q, k_t> over the visible tokens, contiguous
+ * [seqs, hq, dim] of `type`; lse[b, h] (nullable, fp32) = ln sum_t exp(scale * <q, k_t>).  No visible token: out 0,
+ * lse -infinity.  Slots that are not visible are never multiplied, whatever they hold.
+ * A length above the table's row (or below 0) is cut to it, with FVS_KV_BAD_INDEX for the former.
+ * work: fvs_kv_attend_work(...) bytes of device memory, 16-byte aligned, whose first seqs * hq words are zero at the
+ * first call (each call leaves them zero); calls that may run at the same time need one each.
+ */
+int fvs_kv_attend_work(int seqs, int hq, int dim);
+int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,
+                  int64_t q_head, int hq, const int32_t* table, int seqs, int wide, int64_t table_stride,
+                  const int32_t* lens, float scale, void* out, float* lse, void* work);
+
 #ifdef __cplusplus
 }
 #endif
