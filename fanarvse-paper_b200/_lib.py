@@ -68,8 +68,8 @@ SIGNATURES = {
     "fvs_kv_append": (I32, [P, P, I32, P, I64, I64, P, I64, I64, P, I64, I64, I32, P, P, I32, I32, I64, P, P, P, I32,
                              P, P, I32, I32, I32]),
     "fvs_kv_read": (I32, [P, P, I32, P, P, P, I32, I32, I64, P, P, I32]),
-    "fvs_kv_attend_work": (I32, [I32, I32, I32]),
-    "fvs_kv_attend": (I32, [P, P, I32, P, I64, I64, I32, P, I32, I32, I64, P, F32, P, P, P]),
+    "fvs_kv_attend_work": (I32, [I32]),
+    "fvs_kv_attend": (I32, [P, P, I32, P, I64, I64, I32, P, I32, I32, I64, P, F32, P, P, P, P]),
 }
 
 

@@ -173,8 +173,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     extern __shared__ __align__(16) uint8_t ring_all[];
     __shared__ int64_t s_sum[WARPS];
     __shared__ int s_some[WARPS];
-    __shared__ int s_start[WARPS][4];    // b, hh, u, - of a team's first unit
-    __shared__ int64_t s_base[WARPS];    // units before sequence b
+    __shared__ int s_start[WARPS + 1][3];  // b, hh, u of a team's first unit
+    __shared__ int64_t s_base[WARPS + 1];  // units before sequence b
+    __shared__ int64_t s_at[WARPS + 1];    // where ranges begin
     __shared__ float s_ml[WARPS][Sh::ROWS][2];
     __shared__ int s_last[WARPS];
 
@@ -184,16 +185,16 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     const int per_seq = a.c.heads * split;
     const int B = a.tb.seqs;
 
-    // ---- units of all sequences, and where this team's range begins
+    // ---- units of all sequences (each thread a run of them)
     const int chunk = (B + THREADS - 1) / THREADS;
     const int b_lo = min(B, tid * chunk), b_hi = min(B, b_lo + chunk);
     int64_t mine = 0;
     int some = 0;
+#pragma unroll 8
     for (int b = b_lo; b < b_hi; b++) {
         const int n = units_of(seq_len(a, b));
         mine += n;
         some += n > 0;
-        if (blockIdx.x == 0 && __ldg(a.lens + b) > (int64_t)a.tb.wide * a.c.page) atomicOr(a.c.status, BAD_INDEX);
     }
     int64_t incl = mine;
 #pragma unroll
@@ -214,38 +215,51 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         some += s_some[w];
     }
     total *= per_seq;
-    // sequences without a token
-    for (int b = blockIdx.x; b < B; b += gridDim.x) {
-        if (__ldg(a.lens + b) > 0) continue;
-        uint4* o = (uint4*)((uint16_t*)a.out + (int64_t)b * a.hq * D);
-        for (int i = tid; i < a.hq * D / 8; i += THREADS) o[i] = make_uint4(0, 0, 0, 0);
-        if (a.lse)
-            for (int i = tid; i < a.hq; i += THREADS) a.lse[(int64_t)b * a.hq + i] = -INFINITY;
+    if (blockIdx.x == 0)
+        for (int b = tid; b < B; b += THREADS)
+            if (__ldg(a.lens + b) > (int64_t)a.tb.wide * a.c.page) atomicOr(a.c.status, BAD_INDEX);
+    if (some < B) {  // sequences without a token: this CTA's share of all
+        for (int b0 = 0; b0 < B; b0 += gridDim.x * 32) {
+            const int b = b0 + lane * gridDim.x + blockIdx.x;
+            for (uint32_t none = __ballot_sync(0xffffffffu, b < B && __ldg(a.lens + (b < B ? b : 0)) <= 0); none; none &= none - 1) {
+                const int64_t z = b0 + (int64_t)(__ffs(none) - 1) * gridDim.x + blockIdx.x;
+                uint4* o = (uint4*)((uint16_t*)a.out + z * a.hq * D);
+                for (int i = tid; i < a.hq * D / 8; i += THREADS) o[i] = make_uint4(0, 0, 0, 0);
+                if (a.lse)
+                    for (int i = tid; i < a.hq; i += THREADS) a.lse[z * a.hq + i] = -INFINITY;
+            }
+        }
+        if (total == 0) return;
     }
-    if (total == 0) return;
-    // a warp works alone where that still leaves each warp two items and more
-    const bool solo = (int64_t)some * per_seq >= 2ll * WARPS * gridDim.x;
+    // ---- this team's range of the units: `per` for each team, moved up to the end of an item of at most `keep` units
+    // that it would cut (such an item costs less than joining its parts)
+    const bool solo = (int64_t)some * per_seq >= 2ll * WARPS * gridDim.x;  // two items and more for every warp
     const int64_t most = solo ? (int64_t)gridDim.x * WARPS : gridDim.x;
-    const int64_t least = solo ? 1 : 2 * WARPS;  // units of a range
-    int64_t teams64 = (total + least - 1) / least;
-    if (teams64 > most) teams64 = most;
-    const int teams = (int)teams64;
+    int64_t per = (total + most - 1) / most;
+    if (!solo && per < WARPS) per = WARPS;
+    const int64_t keep = per > 64 ? per / 8 : 8;
     const int team = solo ? blockIdx.x * WARPS + warp : blockIdx.x;
-    if (blockIdx.x * (solo ? WARPS : 1) >= teams) return;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-        const int tm = solo ? blockIdx.x * WARPS + w : blockIdx.x;
-        if (tm >= teams || (!solo && w)) break;
-        const int64_t g0 = total * tm / teams;
-        if (g0 < before * per_seq || g0 >= (before + mine) * per_seq) continue;
+    const int team0 = solo ? blockIdx.x * WARPS : blockIdx.x;
+    if (team0 * per >= total) return;
+#pragma unroll 1
+    for (int w = 0; w <= (solo ? WARPS : 1); w++) {
+        const int64_t g = (int64_t)(team0 + w) * per;
+        if (g >= total) {
+            if (tid == 0) s_at[w] = total;
+            continue;
+        }
+        if (g < before * per_seq || g >= (before + mine) * per_seq) continue;
         int64_t base = before;
         for (int b = b_lo; b < b_hi; b++) {
             const int n = units_of(seq_len(a, b));
-            if (g0 < (base + n) * per_seq) {
-                const int64_t at = g0 - base * per_seq;
+            const int64_t in = g - base * per_seq;
+            if (in < (int64_t)n * per_seq) {
+                const int hh = (int)(in / n), u = (int)(in - (int64_t)hh * n);
+                const bool up = u && n <= keep;
+                s_at[w] = up ? g + n - u : g;
                 s_start[w][0] = b;
-                s_start[w][1] = (int)(at / n);
-                s_start[w][2] = (int)(at % n);
+                s_start[w][1] = hh + up;  // per_seq: the next sequence's first item
+                s_start[w][2] = up ? 0 : u;
                 s_base[w] = base;
                 break;
             }
@@ -253,10 +267,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         }
     }
     __syncthreads();
-    if (team >= teams) return;  // solo: a whole warp; no block barrier follows in that mode
     const int w0 = solo ? warp : 0;
-    const int64_t g_begin = total * team / teams;
-    const int count = (int)(total * (team + 1) / teams - g_begin);
+    const int64_t g_begin = s_at[w0];
+    const int count = (int)(s_at[w0 + 1] - g_begin);
+    if (count <= 0) return;  // solo: a whole warp, and no block barrier follows in that mode
     const int step = solo ? 1 : WARPS, first = solo ? 0 : warp;
     auto team_sync = [&]() {
         if (solo)
@@ -272,8 +286,17 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     ahead.len = seq_len(a, ahead.b);
     ahead.n = units_of(ahead.len);
     ahead.left = count;
-    int cb = ahead.b, chh = ahead.hh, cu = ahead.u, cn = ahead.n;  // the segment under computation
     int64_t c_base = s_base[w0];
+    if (ahead.hh == per_seq) {
+        ahead.hh = 0;
+        do {
+            c_base += ahead.n;
+            ahead.b++;
+            ahead.len = seq_len(a, ahead.b);
+            ahead.n = units_of(ahead.len);
+        } while (ahead.n == 0);
+    }
+    int cb = ahead.b, chh = ahead.hh, cu = ahead.u, cn = ahead.n;  // the segment under computation
     if (first) advance(a, ahead, first, per_seq);
 
     uint8_t* ring = ring_all + warp * Sh::RING;
@@ -571,7 +594,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         const bool whole = seg_end - seg_begin == cn;
         const int tt = solo ? lane : tid, nthr = solo ? 32 : THREADS;
         const int w_lo = solo ? warp : 0, w_hi = solo ? warp + 1 : WARPS;
-        float* part = a.parts + (int64_t)(2 * team + (g_begin < i_begin ? 1 : 0)) * Sh::PART;
+        float* part = a.parts + (int64_t)(2 * team + (team * per < i_begin ? 1 : 0)) * Sh::PART;
         constexpr int Q4 = D / 4;
         for (int i = tt; i < rows * Q4; i += nthr) {
             const int row = i / Q4, d = (i - row * Q4) * 4;
@@ -603,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         if (!whole) {
             __threadfence();
             team_sync();
-            const int t_lo = (int)(((i_begin + 1) * teams - 1) / total), t_hi = (int)((i_end * teams - 1) / total);
+            const int t_lo = (int)(i_begin / per), t_hi = (int)((i_end - 1) / per);
             int last = 0;
             if (tt == 0) {
                 last = atomicAdd(a.arrived + item, 1) == t_hi - t_lo;
@@ -622,7 +645,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     const int row = i / Q4, d = (i - row * Q4) * 4;
                     const float* from = a.parts + (int64_t)2 * t_lo * Sh::PART;
                     // the first part is its team's second one unless the item begins with the team's range
-                    const int lead = total * t_lo / teams < i_begin ? 1 : 0;
+                    const int lead = t_lo * per < i_begin ? 1 : 0;
                     float mx = -INFINITY;
                     for (int t = 0; t <= t_hi - t_lo; t++)
                         mx = fmaxf(mx, __ldcg(from + (int64_t)(2 * t + (t ? 0 : lead)) * Sh::PART + Sh::ROWS * D + 2 * row));
@@ -704,18 +727,17 @@ static int launch_types(fvs_stream_t stream, const AttendArgs& a, int type) {
 
 using namespace fvs::kv;
 
-// arrival counters, then two partial results for each of up to 3 CTAs' warps on every SM
-static int64_t counters_bytes(int seqs, int hq) { return ((int64_t)seqs * hq * 4 + 15) / 16 * 16; }
-
-extern "C" int fvs_kv_attend_work(int seqs, int hq, int dim) {
-    if (seqs < 1 || hq < 1 || dim < 1) return FVS_EINVAL;
-    if ((int64_t)seqs * hq > (1 << 28) || dim > 256) return FVS_ERANGE;
-    return (int)(counters_bytes(seqs, hq) + (int64_t)2 * 3 * WARPS * fvs_sm_count() * 16 * (dim + 2) * 4);
+// two partial results for each of up to 3 CTAs' warps on every SM
+extern "C" int fvs_kv_attend_work(int dim) {
+    if (dim < 1) return FVS_EINVAL;
+    if (dim > 256) return FVS_ERANGE;
+    return 2 * 3 * WARPS * fvs_sm_count() * 16 * (dim + 2) * 4;
 }
 
 extern "C" int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,
                              int64_t q_head, int hq, const int32_t* table, int seqs, int wide, int64_t table_stride,
-                             const int32_t* lens, float scale, void* out, float* lse, void* work) {
+                             const int32_t* lens, float scale, void* out, float* lse, void* work,
+                             int32_t* arrived) {
     if (int rc = check_cache(cache)) return rc;
     FVS_CHECK_ARG(type == FVS_F16 || type == FVS_BF16);
     FVS_CHECK_ARG(cache->type == FVS_I8 || cache->type == type);
@@ -723,11 +745,11 @@ extern "C" int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int
     if (seqs == 0) return FVS_OK;
     if (int rc = check_table(table, seqs, wide, table_stride)) return rc;
     FVS_CHECK_ARG(q && ((uintptr_t)q & 15) == 0 && q_seq % 8 == 0 && q_head % 8 == 0 && q_seq >= 0 && q_head >= 0);
-    FVS_CHECK_ARG(lens && out && ((uintptr_t)out & 15) == 0 && work && ((uintptr_t)work & 15) == 0);
+    FVS_CHECK_ARG(lens && out && ((uintptr_t)out & 15) == 0 && work && ((uintptr_t)work & 15) == 0 &&
+                  arrived);
     if ((int64_t)seqs * hq > (1 << 28)) return FVS_ERANGE;
-    AttendArgs a{*cache, {table, table_stride, seqs, wide}, q, q_seq, q_head, lens, out, lse, (int32_t*)work,
-                 (float*)((uint8_t*)work + counters_bytes(seqs, hq)), hq, hq / cache->heads,
-                 scale * 1.4426950408889634f};
+    AttendArgs a{*cache, {table, table_stride, seqs, wide}, q, q_seq, q_head, lens, out, lse, arrived,
+                 (float*)work, hq, hq / cache->heads, scale * 1.4426950408889634f};
     switch (cache->dim) {
         case 64: return launch_types<64>(stream, a, type);
         case 96: return launch_types<96>(stream, a, type);

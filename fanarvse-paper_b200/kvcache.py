@@ -70,7 +70,7 @@ class PagedKV:
         self._c = _lib.KvCache(p(k), p(v), p(k_scale), p(v_scale), p(fill), p(self.status), *k.stride()[:3], *ss,
                                self.pages, self.heads, self.page, self.dim, _CODE[k.dtype])
         self._ref = C.byref(self._c)
-        self._work = {}      # stream -> workspace of attend
+        self._work = {}      # stream -> workspace of attend: addresses, counters held, tensors
         self._captured = []  # workspaces of captured calls
         self.L = _lib.lib()
         self.launches = 0
@@ -187,28 +187,31 @@ class PagedKV:
         if n == 0:
             return out, lse
         stream = _lib.stream_handle()
-        work = self._workspace(stream.value, n, hq)
+        work, arrived = self._workspace(stream.value, n * hq)
         check(self.L.fvs_kv_attend(stream, self._ref, ty, *qa, hq, *self._table(table), self._ints(lens, n, "lens"),
                                    1.0 / math.sqrt(self.dim) if scale is None else scale, out.data_ptr(),
-                                   lse.data_ptr(), work), "kv_attend")
+                                   lse.data_ptr(), work, arrived), "kv_attend")
         self.launches += 1
         return out, lse
 
-    def _workspace(self, stream, n, hq):
-        """Zeroed once and left zeroed by every call, one for each stream; a captured call gets its own, which its graph
-        zeroes, because the graph may be replayed beside calls on any stream."""
-        held = self._work.get(stream)
+    def _workspace(self, stream, n):
+        """Addresses of the partial results and of n arrival counters (zeroed once, left zeroed by every call), one pair for
+        each stream; a captured call gets its own, whose counters its graph zeroes, because the graph may be replayed
+        beside calls on any stream."""
         capturing = torch.cuda.is_current_stream_capturing()
-        if held is None or held[1] < n * hq or capturing:
-            need = self.L.fvs_kv_attend_work(n, hq, self.dim)
+        held = None if capturing else self._work.get(stream)
+        if held is None or held[2] < n:
+            need = self.L.fvs_kv_attend_work(self.dim)
             if need < 0:
                 check(need, "kv_attend_work")
-            t = torch.zeros((need + 3) // 4, dtype=torch.int32, device=self.device)
+            work = torch.empty(need, dtype=torch.uint8, device=self.device)
+            arrived = torch.zeros(n, dtype=torch.int32, device=self.device)
+            held = (work.data_ptr(), arrived.data_ptr(), n, work, arrived)
             if capturing:
-                self._captured.append(t)
-                return t.data_ptr()
-            held = self._work[stream] = (t, n * hq, t.data_ptr())
-        return held[2]
+                self._captured.append(held)
+            else:
+                self._work[stream] = held
+        return held[:2]
 
     def check_status(self):
         """Raises if a call since the last check met an index outside its table (synchronises)."""

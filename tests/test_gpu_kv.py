@@ -180,6 +180,35 @@ def test_attend_splits_over_the_length(kv, B, heads, group, dim, longest, store)
     check_attend(cache, q[perm].contiguous(), table[perm].contiguous(), lens[perm].contiguous())
 
 
+def test_attend_batches_of_changing_size(kv):
+    """Calls of different batch and head counts share a stream's workspace; every one is split over its length."""
+    g = torch.Generator().manual_seed(77)
+    lens = torch.tensor([3000, 2500, 2700, 100, 2900], dtype=torch.int32)
+    table, pages = full_table(lens.tolist(), 32, g)
+    cache = make_cache(kv, pages, 2, 32, 64, BF16, g)
+    table, lens = table.to(DEV), lens.to(DEV)
+    for n, hq in ((2, 4), (5, 16), (1, 2), (5, 16), (3, 40), (2, 4), (5, 16), (3, 40)):
+        q = torch.randn(n, hq, 64, generator=g).to(DEV, BF16)
+        check_attend(cache, q, table[:n], lens[:n])
+
+
+@pytest.mark.parametrize("store", [F16, I8])
+@pytest.mark.parametrize("B,lens", [(300, (1, 300)), (900, (1, 40)), (3000, (0, 3)), (2500, (100, 130)), (129, (0, 2000))])
+def test_attend_many_short_and_a_few_long(kv, store, B, lens):
+    """Ranges of work that begin and end inside items, at their ends and over sequences without tokens."""
+    g = torch.Generator().manual_seed(B)
+    n = torch.randint(lens[0], lens[1] + 1, (B,), generator=g)
+    n[torch.rand(B, generator=g) < 0.2] = 0
+    n[B // 3] = 1500
+    n[B // 3 + 1:B // 3 + 40] = 0
+    n[0] = n[-1] = 0
+    table, pages = full_table(n.tolist(), 16, g)
+    cache = make_cache(kv, pages, 1, 16, 64, store, g)
+    q = torch.randn(B, 2, 64, generator=g).to(DEV, F16)
+    check_attend(cache, q, table.to(DEV), n.to(DEV, torch.int32))
+    cache.check_status()
+
+
 @pytest.mark.parametrize("store", [BF16, I8])
 def test_attend_scores_far_apart(kv, store):
     """A running maximum that keeps rising, one that falls, one key that takes all the weight."""
