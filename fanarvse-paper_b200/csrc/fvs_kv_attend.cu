@@ -4,12 +4,12 @@
 // m' = max(m, max s), l' = l 2^(m - m') + sum 2^(s - m'), and the accumulated output by o' = o 2^(m - m') + sum
 // 2^(s - m') v.  Scores are in units of log2 (scale * log2 e); m, l, o and all sums are fp32.
 //
-// Work.  A unit is 16 keys of one (sequence, key head, group of up to 8 NT query heads) item.  The units of all items in
-// order are cut into equal ranges, one for each team -- a CTA of four warps whose warps take the range's units in turn,
-// or, where there are many items, a single warp -- so that any mix of lengths keeps every SM busy and a long sequence is
-// split without the host knowing any length.  A range that holds a whole item writes its output; parts of an item go to
-// the workspace, and the team that finishes an item's last part (counted by an atomic, joined in range order, so that
-// results do not depend on the order of arrival) joins them.
+// Work.  A unit is 16 keys of one (sequence, key head, group of up to 8 NT query heads) item.  The items in order, each
+// of ITEM_COST + its units, are cut into ranges of equal cost, one for each CTA of four warps, so that any mix of
+// lengths keeps every SM busy and a long sequence is split without the host knowing any length.  The warps of a CTA take
+// an item's units in turn and add up their results in shared memory; an item of few units is one warp's.  A range that
+// holds a whole item writes its output; parts of an item go to the workspace, and the CTA that finishes an item's last
+// part (counted by an atomic, joined in range order, so that results do not depend on the order of arrival) joins them.
 //
 // A warp copies its units' key and value rows with cp.async into a ring of its own (no block barrier between units; page
 // numbers are looked up two units ahead of the copy) and multiplies with mma.sync m16n8k16.  Both products run
@@ -47,6 +47,7 @@ struct AttendArgs {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int UNIT = 16;       // keys
+constexpr int ITEM_COST = 3;   // of an item beside its units (loading q, adding up and writing), in units
 constexpr float SLACK = 8.f;   // how far (log2) a score may pass the running maximum before it moves
 
 template <int D, int STORE, int NT_>
@@ -130,11 +131,6 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t sel) {
     return *reinterpret_cast<const uint32_t*>(&y);
 }
 
-// Where a warp stands in its team's range: unit u of n of sequence b (len keys), item hh of the sequence's items.
-struct Cursor {
-    int b, hh, u, n, len, left;
-};
-
 __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
     const int len = __ldg(a.lens + b);
     const int64_t room = (int64_t)a.tb.wide * a.c.page;
@@ -142,26 +138,37 @@ __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
 }
 __device__ __forceinline__ int units_of(int len) { return (int)(((unsigned)len + UNIT - 1) / UNIT); }
 
-__device__ __forceinline__ void advance(const AttendArgs& a, Cursor& c, int by, int per_seq) {
-    c.left -= by;
-    c.u += by;
-    if (c.left <= 0) return;
-    while (c.u >= c.n) {
-        c.u -= c.n;
-        if (++c.hh == per_seq) {
-            c.hh = 0;
-            do {
-                c.b++;
-                c.len = seq_len(a, c.b);
-                c.n = units_of(c.len);
-            } while (c.n == 0);
-        }
+// A place in the order of all items: unit u of item hh (of per_seq) of sequence b.
+struct Place {
+    int b, hh, u;
+};
+
+// An item, with the units [u, end) of it that lie in a CTA's range.
+struct Item {
+    int b, hh, len, n, u, end;
+};
+__device__ __forceinline__ void clip(Item& it, const Place& stop) {
+    it.end = it.b == stop.b && it.hh == stop.hh ? stop.u : it.n;
+}
+// the next item of the range; false at its end
+__device__ __forceinline__ bool next_item(const AttendArgs& a, Item& it, const Place& stop, int per_seq) {
+    if (++it.hh == per_seq) {
+        it.hh = 0;
+        do {
+            if (++it.b > stop.b || it.b >= a.tb.seqs) return false;
+            it.len = seq_len(a, it.b);
+            it.n = units_of(it.len);
+        } while (it.n == 0);
     }
+    it.u = 0;
+    clip(it, stop);
+    return it.b < stop.b || (it.b == stop.b && it.hh <= stop.hh && it.end > 0);
 }
 
 // One key of a unit on its way from the page table to the copy.
 struct Lookup {
     int entry, slot, head, fill;
+    bool live;  // there is such a unit
 };
 
 template <int D, int TYPE, int STORE, int NT>
@@ -172,12 +179,12 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     constexpr int S = Sh::S;
     extern __shared__ __align__(16) uint8_t ring_all[];
     __shared__ int64_t s_sum[WARPS];
-    __shared__ int s_some[WARPS];
-    __shared__ int s_start[WARPS + 1][3];  // b, hh, u of a team's first unit
-    __shared__ int64_t s_base[WARPS + 1];  // units before sequence b
-    __shared__ int64_t s_at[WARPS + 1];    // where ranges begin
+    __shared__ int s_none[WARPS];
+    __shared__ int64_t s_before[THREADS];  // cost (for one item of each sequence) before each thread's sequences
+    __shared__ Place s_place[2];           // where this CTA's range begins and ends
+    __shared__ int64_t s_base;             // cost before the first sequence of the range
     __shared__ float s_ml[WARPS][Sh::ROWS][2];
-    __shared__ int s_last[WARPS];
+    __shared__ int s_tile[WARPS], s_last;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = lane >> 2, c4 = lane & 3;
@@ -185,16 +192,22 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     const int per_seq = a.c.heads * split;
     const int B = a.tb.seqs;
 
-    // ---- units of all sequences (each thread a run of them)
+    // ---- cost of all sequences (each thread a run of them)
     const int chunk = (B + THREADS - 1) / THREADS;
-    const int b_lo = min(B, tid * chunk), b_hi = min(B, b_lo + chunk);
+    const int b_hi = min(B, (tid + 1) * chunk);
     int64_t mine = 0;
-    int some = 0;
-#pragma unroll 8
-    for (int b = b_lo; b < b_hi; b++) {
-        const int n = units_of(seq_len(a, b));
-        mine += n;
-        some += n > 0;
+    int none = 0;
+    for (int b0 = tid * chunk; b0 < b_hi; b0 += 8) {
+        unsigned sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (b0 + j < b_hi) {
+                const int n = units_of(seq_len(a, b0 + j));
+                sum += n ? n + ITEM_COST : 0;
+                none += n == 0;
+            }
+        }
+        mine += sum;
     }
     int64_t incl = mine;
 #pragma unroll
@@ -202,102 +215,108 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += x;
     }
-    some = __reduce_add_sync(0xffffffffu, some);
+    none = __reduce_add_sync(0xffffffffu, none);
     if (lane == 31) s_sum[warp] = incl;
-    if (lane == 0) s_some[warp] = some;
+    if (lane == 0) s_none[warp] = none;
     __syncthreads();
     int64_t before = incl - mine, total = 0;
-    some = 0;
+    none = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; w++) {
         if (w < warp) before += s_sum[w];
         total += s_sum[w];
-        some += s_some[w];
+        none += s_none[w];
     }
+    s_before[tid] = before;
     total *= per_seq;
     if (blockIdx.x == 0)
         for (int b = tid; b < B; b += THREADS)
             if (__ldg(a.lens + b) > (int64_t)a.tb.wide * a.c.page) atomicOr(a.c.status, BAD_INDEX);
-    if (some < B) {  // sequences without a token: this CTA's share of all
+    if (none) {  // sequences without a token: this CTA's share of all
         for (int b0 = 0; b0 < B; b0 += gridDim.x * 32) {
             const int b = b0 + lane * gridDim.x + blockIdx.x;
-            for (uint32_t none = __ballot_sync(0xffffffffu, b < B && __ldg(a.lens + (b < B ? b : 0)) <= 0); none; none &= none - 1) {
-                const int64_t z = b0 + (int64_t)(__ffs(none) - 1) * gridDim.x + blockIdx.x;
-                uint4* o = (uint4*)((uint16_t*)a.out + z * a.hq * D);
+            for (uint32_t z = __ballot_sync(0xffffffffu, b < B && __ldg(a.lens + (b < B ? b : 0)) <= 0); z; z &= z - 1) {
+                const int64_t bz = b0 + (int64_t)(__ffs(z) - 1) * gridDim.x + blockIdx.x;
+                uint4* o = (uint4*)((uint16_t*)a.out + bz * a.hq * D);
                 for (int i = tid; i < a.hq * D / 8; i += THREADS) o[i] = make_uint4(0, 0, 0, 0);
                 if (a.lse)
-                    for (int i = tid; i < a.hq; i += THREADS) a.lse[z * a.hq + i] = -INFINITY;
+                    for (int i = tid; i < a.hq; i += THREADS) a.lse[bz * a.hq + i] = -INFINITY;
             }
         }
-        if (total == 0) return;
     }
-    // ---- this team's range of the units: `per` for each team, moved up to the end of an item of at most `keep` units
-    // that it would cut (such an item costs less than joining its parts)
-    const bool solo = (int64_t)some * per_seq >= 2ll * WARPS * gridDim.x;  // two items and more for every warp
-    const int64_t most = solo ? (int64_t)gridDim.x * WARPS : gridDim.x;
-    int64_t per = (total + most - 1) / most;
-    if (!solo && per < WARPS) per = WARPS;
-    const int64_t keep = per > 64 ? per / 8 : 8;
-    const int team = solo ? blockIdx.x * WARPS + warp : blockIdx.x;
-    const int team0 = solo ? blockIdx.x * WARPS : blockIdx.x;
-    if (team0 * per >= total) return;
-#pragma unroll 1
-    for (int w = 0; w <= (solo ? WARPS : 1); w++) {
-        const int64_t g = (int64_t)(team0 + w) * per;
+    // ---- this CTA's range of the cost.  Unit u of an item that begins at cost x lies at x + ITEM_COST + u.  A cut nearer
+    // than `near` units to an item's begin or end moves there: joining two parts costs more than that
+    int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    if (per < 16) per = 16;
+    if (blockIdx.x * per >= total) return;
+    const int near = per > 64 ? (int)(per / 8) : 8;
+    const int alone = per > 128 ? 16 : (int)(per / 8);  // items of up to so many units are one warp's
+    __syncthreads();
+    if (warp < 2) {
+        const int64_t g = (blockIdx.x + warp) * per;
         if (g >= total) {
-            if (tid == 0) s_at[w] = total;
-            continue;
-        }
-        if (g < before * per_seq || g >= (before + mine) * per_seq) continue;
-        int64_t base = before;
-        for (int b = b_lo; b < b_hi; b++) {
-            const int n = units_of(seq_len(a, b));
-            const int64_t in = g - base * per_seq;
-            if (in < (int64_t)n * per_seq) {
-                const int hh = (int)(in / n), u = (int)(in - (int64_t)hh * n);
-                const bool up = u && n <= keep;
-                s_at[w] = up ? g + n - u : g;
-                s_start[w][0] = b;
-                s_start[w][1] = hh + up;  // per_seq: the next sequence's first item
-                s_start[w][2] = up ? 0 : u;
-                s_base[w] = base;
-                break;
+            if (lane == 0) s_place[warp] = Place{B, 0, 0};
+        } else {
+            int at = 0;  // the last run of sequences that begins at or before g
+#pragma unroll
+            for (int j = 0; j < THREADS / 32; j++) at += s_before[j * 32 + lane] * per_seq <= g;
+            at = (int)__reduce_add_sync(0xffffffffu, (unsigned)at) - 1;
+            int64_t base = s_before[at];
+            for (int b0 = at * chunk; b0 < B; b0 += 32) {
+                const int n = b0 + lane < B ? units_of(seq_len(a, b0 + lane)) : 0;
+                const int64_t cost = n ? n + ITEM_COST : 0;
+                int64_t upto = cost;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                const uint32_t past = __ballot_sync(0xffffffffu, (base + upto) * per_seq > g);
+                if (past) {
+                    if (lane == __ffs(past) - 1) {
+                        const int64_t in = g - (base + upto - cost) * per_seq;
+                        const int hh = (int)(in / cost), u = (int)(in - hh * cost) - ITEM_COST;
+                        s_place[warp] = u < near ? Place{b0 + lane, hh, 0} : n - u < near ? Place{b0 + lane, hh + 1, 0} : Place{b0 + lane, hh, u};
+                        if (warp == 0) s_base = base + upto - cost;
+                    }
+                    break;
+                }
+                base += __shfl_sync(0xffffffffu, upto, 31);
             }
-            base += n;
         }
     }
     __syncthreads();
-    const int w0 = solo ? warp : 0;
-    const int64_t g_begin = s_at[w0];
-    const int count = (int)(s_at[w0 + 1] - g_begin);
-    if (count <= 0) return;  // solo: a whole warp, and no block barrier follows in that mode
-    const int step = solo ? 1 : WARPS, first = solo ? 0 : warp;
-    auto team_sync = [&]() {
-        if (solo)
-            __syncwarp();
-        else
-            __syncthreads();
-    };
-
-    Cursor ahead;
-    ahead.b = s_start[w0][0];
-    ahead.hh = s_start[w0][1];
-    ahead.u = s_start[w0][2];
-    ahead.len = seq_len(a, ahead.b);
-    ahead.n = units_of(ahead.len);
-    ahead.left = count;
-    int64_t c_base = s_base[w0];
-    if (ahead.hh == per_seq) {
-        ahead.hh = 0;
-        do {
-            c_base += ahead.n;
-            ahead.b++;
-            ahead.len = seq_len(a, ahead.b);
-            ahead.n = units_of(ahead.len);
-        } while (ahead.n == 0);
+    const Place stop = s_place[1];
+    Item now;  // the item under computation
+    now.b = s_place[0].b;
+    now.hh = s_place[0].hh;
+    now.len = seq_len(a, now.b);
+    now.n = units_of(now.len);
+    now.u = s_place[0].u;
+    clip(now, stop);
+    int64_t base = s_base;
+    bool more = true;
+    if (now.hh == per_seq) {  // moved past the sequence's last item
+        const int b = now.b;
+        now.hh--;
+        more = next_item(a, now, stop, per_seq);
+        if (now.b != b) base += units_of(seq_len(a, b)) + ITEM_COST;
+    } else {
+        more = now.b < stop.b || (now.b == stop.b && (now.hh < stop.hh || (now.hh == stop.hh && now.u < stop.u)));
     }
-    int cb = ahead.b, chh = ahead.hh, cu = ahead.u, cn = ahead.n;  // the segment under computation
-    if (first) advance(a, ahead, first, per_seq);
+    if (!more) return;
+    // the units that this warp copies: every fourth of an item, all of one that it has alone
+    Item ahead = now;
+    bool any = true;
+    auto owner = [&](const Item& it) { return (it.b * per_seq + it.hh) % WARPS; };
+    auto settle = [&]() {
+        while (any && ahead.u >= ahead.end) {
+            any = next_item(a, ahead, stop, per_seq);
+            if (any) ahead.u = ahead.n > alone ? warp : owner(ahead) == warp ? 0 : ahead.end;
+        }
+    };
+    ahead.u = ahead.n > alone ? ahead.u + warp : owner(ahead) == warp ? 0 : ahead.end;
+    settle();
 
     uint8_t* ring = ring_all + warp * Sh::RING;
     const uint32_t ring_at = smem_addr(ring);
@@ -308,7 +327,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         k.entry = -1;
         k.slot = 0;
         k.head = 0;
-        if (ahead.left > 0) {
+        k.live = any;
+        if (any) {
             const int t = ahead.u * UNIT + (lane & 15);
             if (t < ahead.len) {
                 const int p = (int)((unsigned)t / (unsigned)a.c.page);
@@ -316,7 +336,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 k.entry = __ldg(a.tb.at + (int64_t)ahead.b * a.tb.stride + p);
             }
             k.head = ahead.hh / split;
-            advance(a, ahead, step, per_seq);
+            ahead.u += ahead.n > alone ? WARPS : 1;
+            settle();
         }
         return k;
     };
@@ -356,12 +377,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     look_fill(la);
     Lookup lb = look();
     int ready = 0;                                         // next slot to fill
-    int to_issue = count > first ? (count - first + step - 1) / step : 0;  // this warp's units not yet issued
     auto feed = [&]() {
-        if (to_issue > 0) {
-            issue(la, ready);
-            to_issue--;
-        }
+        if (la.live) issue(la, ready);
         copies_commit();
         ready = ready + 1 == S ? 0 : ready + 1;
         la = lb;
@@ -371,13 +388,24 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
 #pragma unroll 1
     for (int i = 0; i < S - 1; i++) feed();
 
-    // ---- segments of the range: an item's units that lie in it
-    int offset = first, seg_begin = 0, slot = 0;
+    // ---- the range's items
+    int slot = 0;
 #pragma unroll 1
-    while (seg_begin < count) {
-        const int seg_end = min(count, seg_begin + cn - cu);
-        const int kvh = chh / split, h0 = kvh * a.group + (chh % split) * Sh::ROWS;
-        const int rows = min(Sh::ROWS, a.group - (chh % split) * Sh::ROWS);
+    for (; more;) {
+        const bool solo = now.n <= alone;
+        const int kvh = now.hh / split, h0 = kvh * a.group + (now.hh % split) * Sh::ROWS;
+        const int rows = min(Sh::ROWS, a.group - (now.hh % split) * Sh::ROWS);
+        const Item it = now;
+        const int64_t it_begin = base * per_seq + (int64_t)now.hh * (now.n + ITEM_COST);
+        more = next_item(a, now, stop, per_seq);
+        if (now.b != it.b) base += it.n + ITEM_COST;
+        if (solo && owner(it) != warp) continue;
+        auto team_sync = [&]() {
+            if (solo)
+                __syncwarp();
+            else
+                __syncthreads();
+        };
 
         // q as the B operand: head r of each 8, elements of the order in which the keys' rows come
         uint32_t qf[NT][D / 16][2];
@@ -385,7 +413,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int h = t * 8 + r;
-            const uint16_t* qp = (const uint16_t*)a.q + cb * a.q_seq + (int64_t)(h0 + h) * a.q_head;
+            const uint16_t* qp = (const uint16_t*)a.q + it.b * a.q_seq + (int64_t)(h0 + h) * a.q_head;
             if (I8) {
                 uint2 raw[D / 16];
                 float top = 0.f;
@@ -429,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 for (int x = 0; x < 4; x++) o[i][t][x] = 0.f;
 
 #pragma unroll 1
-        for (; offset < seg_end; offset += step) {
+        for (int u = solo ? it.u : it.u + warp; u < it.end; u += solo ? 1 : WARPS) {
             copies_wait<S - 2>();
             __syncwarp();
             feed();
@@ -564,7 +592,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             }
         }
 
-        // ---- the segment's result: the warps' tiles through shared memory (a warp's ring slot that the next copy fills)
+        // ---- the item's result: the warps' tiles through shared memory (each warp's ring slot that its next copy fills)
         __syncwarp();
         float* tile = Sh::O_IN_RING ? (float*)(ring + ready * Sh::STAGE)
                                     : (float*)(ring_all + WARPS * Sh::RING + warp * Sh::OBYTES);
@@ -586,16 +614,22 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 }
             }
         }
-        // where the tile of a warp lies: the warps of a team may stand at different slots
-        if (!solo && lane == 0) s_last[warp] = (int)((uint8_t*)tile - ring_all);
+        if (lane == 0) s_tile[warp] = (int)((uint8_t*)tile - ring_all);
         team_sync();
-        const int64_t item = (int64_t)cb * per_seq + chh;
-        const int64_t i_begin = c_base * per_seq + (int64_t)chh * cn, i_end = i_begin + cn;
-        const bool whole = seg_end - seg_begin == cn;
+        const bool whole = it.u == 0 && it.end == it.n;
         const int tt = solo ? lane : tid, nthr = solo ? 32 : THREADS;
         const int w_lo = solo ? warp : 0, w_hi = solo ? warp + 1 : WARPS;
-        float* part = a.parts + (int64_t)(2 * team + (team * per < i_begin ? 1 : 0)) * Sh::PART;
+        // an item's first part is its CTA's second one: that CTA may hold the last part of another
+        float* part = a.parts + (int64_t)(2 * blockIdx.x + (it.u == 0)) * Sh::PART;
         constexpr int Q4 = D / 4;
+        auto finish = [&](int row, int d, float mx, float sum, const float4& acc) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t h = (int64_t)it.b * a.hq + h0 + row;
+            *(uint2*)((uint16_t*)a.out + h * D + d) =
+                sum == 0.f ? make_uint2(0, 0)
+                           : make_uint2(Elem<TYPE>::down(acc.x * inv, acc.y * inv), Elem<TYPE>::down(acc.z * inv, acc.w * inv));
+            if (d == 0 && a.lse) a.lse[h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+        };
         for (int i = tt; i < rows * Q4; i += nthr) {
             const int row = i / Q4, d = (i - row * Q4) * 4;
             float mx = -INFINITY;
@@ -604,55 +638,43 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int w = w_lo; w < w_hi; w++) {
                 const float f = weight(make_float2(s_ml[w][row][0], s_ml[w][row][1]), mx);
-                const float* src = (const float*)(solo ? (const uint8_t*)tile : ring_all + s_last[w]) + row * Sh::OS + d;
-                const float4 x = *(const float4*)src;
+                const float4 x = *(const float4*)((const float*)(ring_all + s_tile[w]) + row * Sh::OS + d);
                 if (f != 0.f) {
                     sum += s_ml[w][row][1] * f;
                     acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
                 }
             }
             if (whole) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const int64_t h = (int64_t)cb * a.hq + h0 + row;
-                *(uint2*)((uint16_t*)a.out + h * D + d) =
-                    sum == 0.f ? make_uint2(0, 0)
-                               : make_uint2(Elem<TYPE>::down(acc.x * inv, acc.y * inv), Elem<TYPE>::down(acc.z * inv, acc.w * inv));
-                if (d == 0 && a.lse) a.lse[h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+                finish(row, d, mx, sum, acc);
             } else {
                 *(float4*)(part + row * D + d) = acc;
                 if (d == 0) *(float2*)(part + Sh::ROWS * D + 2 * row) = make_float2(mx, sum);
             }
         }
-        if (!whole) {
+        if (!whole) {  // never alone: an item of so few units is not cut
             __threadfence();
-            team_sync();
-            const int t_lo = (int)(i_begin / per), t_hi = (int)((i_end - 1) / per);
-            int last = 0;
-            if (tt == 0) {
-                last = atomicAdd(a.arrived + item, 1) == t_hi - t_lo;
-                if (last) a.arrived[item] = 0;
-                if (!solo) s_last[0] = last;
+            __syncthreads();
+            // the cuts inside the item lie at multiples of per; parts - 1 of them, the first at t_lo * per
+            const int t_lo = (int)((it_begin + ITEM_COST + near + per - 1) / per);
+            const int parts = (int)((it_begin + ITEM_COST + it.n - near) / per) - t_lo + 2;
+            if (tid == 0) {
+                const int64_t item = (int64_t)it.b * per_seq + it.hh;
+                s_last = atomicAdd(a.arrived + item, 1) == parts - 1;
+                if (s_last) a.arrived[item] = 0;
             }
-            if (solo)
-                last = __shfl_sync(0xffffffffu, last, 0);
-            else {
-                __syncthreads();
-                last = s_last[0];
-            }
-            if (last) {
+            __syncthreads();
+            if (s_last) {
                 __threadfence();
-                for (int i = tt; i < rows * Q4; i += nthr) {
+                for (int i = tid; i < rows * Q4; i += THREADS) {
                     const int row = i / Q4, d = (i - row * Q4) * 4;
-                    const float* from = a.parts + (int64_t)2 * t_lo * Sh::PART;
-                    // the first part is its team's second one unless the item begins with the team's range
-                    const int lead = t_lo * per < i_begin ? 1 : 0;
+                    const float* from = a.parts + (int64_t)2 * (t_lo - 1) * Sh::PART;
                     float mx = -INFINITY;
-                    for (int t = 0; t <= t_hi - t_lo; t++)
-                        mx = fmaxf(mx, __ldcg(from + (int64_t)(2 * t + (t ? 0 : lead)) * Sh::PART + Sh::ROWS * D + 2 * row));
+                    for (int t = 0; t < parts; t++)
+                        mx = fmaxf(mx, __ldcg(from + (int64_t)(2 * t + (t == 0)) * Sh::PART + Sh::ROWS * D + 2 * row));
                     float sum = 0.f;
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int t = 0; t <= t_hi - t_lo; t++) {
-                        const float* p = from + (int64_t)(2 * t + (t ? 0 : lead)) * Sh::PART;
+                    for (int t = 0; t < parts; t++) {
+                        const float* p = from + (int64_t)(2 * t + (t == 0)) * Sh::PART;
                         const float2 ml = __ldcg((const float2*)(p + Sh::ROWS * D + 2 * row));
                         const float4 x = __ldcg((const float4*)(p + row * D + d));
                         const float f = weight(ml, mx);
@@ -661,29 +683,11 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                             acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
                         }
                     }
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                    const int64_t h = (int64_t)cb * a.hq + h0 + row;
-                    *(uint2*)((uint16_t*)a.out + h * D + d) =
-                        sum == 0.f ? make_uint2(0, 0)
-                                   : make_uint2(Elem<TYPE>::down(acc.x * inv, acc.y * inv), Elem<TYPE>::down(acc.z * inv, acc.w * inv));
-                    if (d == 0 && a.lse) a.lse[h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+                    finish(row, d, mx, sum, acc);
                 }
             }
         }
         team_sync();  // the tiles' slots may be filled again
-
-        // ---- next item
-        seg_begin = seg_end;
-        if (seg_begin >= count) break;
-        cu = 0;
-        if (++chh == per_seq) {
-            chh = 0;
-            do {
-                c_base += cn;
-                cb++;
-                cn = units_of(seq_len(a, cb));
-            } while (cn == 0);
-        }
     }
     copies_wait<0>();
 }
@@ -727,11 +731,11 @@ static int launch_types(fvs_stream_t stream, const AttendArgs& a, int type) {
 
 using namespace fvs::kv;
 
-// two partial results for each of up to 3 CTAs' warps on every SM
+// two partial results for each of up to 3 CTAs on every SM
 extern "C" int fvs_kv_attend_work(int dim) {
     if (dim < 1) return FVS_EINVAL;
     if (dim > 256) return FVS_ERANGE;
-    return 2 * 3 * WARPS * fvs_sm_count() * 16 * (dim + 2) * 4;
+    return 2 * 3 * fvs_sm_count() * 16 * (dim + 2) * 4;
 }
 
 extern "C" int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,
