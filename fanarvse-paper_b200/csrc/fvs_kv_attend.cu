@@ -26,6 +26,8 @@
 // itself; l sums them in fp32 before that.  int8 codes are exact in fp16; their key scale multiplies the fp32 score, their
 // value scale the probability, divided by the largest power of two met so far so that it stays in fp16's range; queries
 // over int8 codes are brought to fp16 by a power of two for each head.
+#include <limits.h>
+
 #include "fvs_kv.cuh"
 
 namespace fvs {
@@ -39,14 +41,15 @@ struct AttendArgs {
     const int32_t* lens;
     void* out;
     float* lse;
-    int32_t* arrived;  // [items], zero between calls
+    int32_t* arrived;  // [items], then the next piece of work and the CTAs that are done; zero between calls
     float* parts;
     int hq, group;     // query heads, query heads of a key head
+    int split;         // items of a key head
     float scale2;      // scale * log2 e
+    uint32_t page_mul, page_shift;  // t / page = t * page_mul >> page_shift for t < 2^31
 };
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int UNIT = 16;       // keys
 constexpr int ITEM_COST = 3;   // of an item beside its units (loading q, adding up and writing), in units
 constexpr float SLACK = 8.f;   // how far (log2) a score may pass the running maximum before it moves
 
@@ -56,24 +59,34 @@ struct Shape {
     static constexpr int NT = NT_;
     static constexpr int ROWS = 8 * NT;              // query heads of an item
     static constexpr int RB = D * (I8 ? 1 : 2);      // bytes of a row
-    // row strides in shared memory that keep every access below free of bank conflicts: 16-bit rows are read by ldmatrix
-    // (an odd number of 16-byte chunks); int8 keys 8 bytes a lane from 4 rows at a time (stride
-    // = 32 or 96 mod 128), int8 values 4 bytes a lane from every second row (twice the stride = 32 or 96 mod 128)
-    static constexpr int KS = I8 ? (D == 96 ? 160 : D + 32) : RB + 16;
-    static constexpr int VS = RB + 16;
-    static constexpr int SCALES = UNIT * (KS + VS);  // byte offset of the scales [2][16]
-    static constexpr int MASK = SCALES + (I8 ? 128 : 0);
+    static constexpr int TILES = RB <= 128 ? 2 : 1;  // of 16 keys in a unit
+    static constexpr int UNIT = 16 * TILES;
+    // Rows in shared memory, so that no access below has bank conflicts.  Rows of 128 bytes: their 16-byte chunks permuted
+    // by the row; others: padded, 16-bit rows (read by ldmatrix) to an odd number of chunks, int8 keys (8 bytes a lane from
+    // 4 rows at a time) to 32 or 96 mod 128 bytes, int8 values (4 bytes a lane from every second row) to half of that.
+    static constexpr bool SWZ = RB == 128;
+    static constexpr int KS = SWZ ? RB : I8 ? (D == 96 ? 160 : D + 32) : RB + 16;
+    static constexpr int VS = SWZ ? RB : RB + 16;
+    static __device__ __forceinline__ int k_chunk(int row, int ch) { return !SWZ ? ch : I8 ? ch ^ (2 * (row & 3)) : ch ^ (row & 7); }
+    static __device__ __forceinline__ int v_chunk(int row, int ch) { return !SWZ ? ch : I8 ? ch ^ (row & 6) : ch ^ (row & 7); }
+    static constexpr int VALUES = UNIT * KS;                  // byte offset of the value rows
+    static constexpr int SCALES = VALUES + UNIT * VS;         // of the scales [2][UNIT]
+    static constexpr int MASK = SCALES + (I8 ? 8 * UNIT : 0);  // of the word of visible keys
     static constexpr int STAGE = MASK + 16;
     static constexpr int OS = D + 4;                 // row stride (floats) of a staged output tile
     static constexpr int OBYTES = ROWS * OS * 4;
     static constexpr bool O_IN_RING = OBYTES <= STAGE;
-    static constexpr int CTAS = RB <= 128 && NT == 1 ? 3 : RB <= 256 ? 2 : 1;  // per SM
-    static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 1024 - (O_IN_RING ? 0 : WARPS * OBYTES);
+    static constexpr bool Q_SMEM = D > 128 && NT > 1;         // q's fragments would not fit the registers
+    static constexpr int QBYTES = Q_SMEM ? ROWS * D * 2 : 0;
+    static constexpr int FIXED = (O_IN_RING ? 0 : WARPS * OBYTES) + QBYTES;
+    // CTAs per SM: three (12 warps hide each other's latencies; 168 registers a thread) where two stages fit
+    static constexpr int CTAS = NT == 1 && D <= 128 ? 3 : RB <= 256 && !Q_SMEM ? 2 : 1;
+    static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 2560 - FIXED;
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
-    static constexpr int S = FIT > 6 ? 6 : FIT;      // ring stages
+    static constexpr int S = FIT > 4 ? 4 : FIT;      // ring stages
     static_assert(S >= 2, "ring");
     static constexpr int RING = S * STAGE;           // bytes per warp
-    static constexpr int SMEM = WARPS * (RING + (O_IN_RING ? 0 : OBYTES));
+    static constexpr int SMEM = WARPS * RING + FIXED;
     static constexpr int PART = ROWS * (D + 2);      // floats of a partial result
 };
 
@@ -124,51 +137,80 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ float weight(float2 ml, float mx) {
     return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - mx);
 }
-// two codes (bytes chosen by `sel` from w ^ 0x80808080) as fp16: 0x6400 | u is 1024 + u, less 1152 is the signed code
-__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t sel) {
-    const uint32_t x = __byte_perm(w, 0x64646464u, sel);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&y);
-}
+// Codes as fp16 without arithmetic: the byte u = code + 128 with a zero byte above it is the subnormal u 2^-24.  The 128 is
+// taken out by the matrix instructions too (see below), so the codes' values stay exact.
+__device__ __forceinline__ uint32_t codes2(uint32_t u, uint32_t sel) { return __byte_perm(u, 0u, sel); }
+constexpr uint32_t LOW = 0x4140, HIGH = 0x4342;  // the lower and the upper two codes of a word
+constexpr uint32_t MINUS_128 = 0x80808080u;      // two fp16: -128 2^-24
 
 __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
     const int len = __ldg(a.lens + b);
     const int64_t room = (int64_t)a.tb.wide * a.c.page;
     return len > room ? (int)room : max(len, 0);
 }
-__device__ __forceinline__ int units_of(int len) { return (int)(((unsigned)len + UNIT - 1) / UNIT); }
-
-// A place in the order of all items: unit u of item hh (of per_seq) of sequence b.
-struct Place {
-    int b, hh, u;
-};
-
-// An item, with the units [u, end) of it that lie in a CTA's range.
-struct Item {
-    int b, hh, len, n, u, end;
-};
-__device__ __forceinline__ void clip(Item& it, const Place& stop) {
-    it.end = it.b == stop.b && it.hh == stop.hh ? stop.u : it.n;
+template <int UNIT>
+__device__ __forceinline__ int units_of(int len) {
+    return (int)(((unsigned)len + UNIT - 1) / UNIT);
 }
-// the next item of the range; false at its end
-__device__ __forceinline__ bool next_item(const AttendArgs& a, Item& it, const Place& stop, int per_seq) {
-    if (++it.hh == per_seq) {
-        it.hh = 0;
-        do {
-            if (++it.b > stop.b || it.b >= a.tb.seqs) return false;
-            it.len = seq_len(a, it.b);
-            it.n = units_of(it.len);
-        } while (it.n == 0);
+
+// A place in the order of all items: unit u of part `sub` (of `split`) of the query heads of key head `head` of sequence b.
+struct Place {
+    int b, head, sub, u;
+    __device__ __forceinline__ bool same_item(int ob, int oh, int os) const { return b == ob && head == oh && sub == os; }
+};
+
+// An item, with the units [u, end) of it that lie in a piece.
+struct Item {
+    int b, head, sub, len, n, u, end;
+};
+// the next item of the piece that ends at `stop`; false if there is none
+template <int UNIT>
+__device__ __forceinline__ bool next_item(const AttendArgs& a, Item& it, const Place& stop) {
+    if (it.end < it.n || stop.same_item(it.b, it.head, it.sub)) return false;  // the piece ends in this one
+    if (++it.sub == a.split) {
+        it.sub = 0;
+        if (++it.head == a.c.heads) {
+            it.head = 0;
+            do {
+                if (++it.b > stop.b || it.b >= a.tb.seqs) return false;
+                it.len = seq_len(a, it.b);
+                it.n = units_of<UNIT>(it.len);
+            } while (it.n == 0);
+        }
     }
     it.u = 0;
-    clip(it, stop);
-    return it.b < stop.b || (it.b == stop.b && it.hh <= stop.hh && it.end > 0);
+    it.end = stop.same_item(it.b, it.head, it.sub) ? stop.u : it.n;
+    return it.end > 0;
 }
 
 // One key of a unit on its way from the page table to the copy.
 struct Lookup {
-    int entry, slot, head, fill;
-    bool live;  // there is such a unit
+    int entry;  // page, < 0: none, NO_UNIT: the range has no such unit
+    int slot, head, fill;
+};
+constexpr int NO_UNIT = INT_MIN;
+
+// Cuts of the cost of all items: equal shares, one for each CTA, each share cut into `runs` pieces, the first of them
+// long.  A CTA begins with its share's long piece; the short ones are taken as CTAs finish.  (SMs differ in how fast memory
+// serves them: with equal pieces alone the slowest of 296 CTAs ran 110 us where half were done after 80 us.)
+struct Cuts {
+    int64_t share, lead;  // of the cost: a share, its first piece
+    int runs, small;      // pieces of a share, the cost of each but the first (the last one may be shorter)
+    // pieces are numbered in the order of the cost
+    __device__ __forceinline__ int64_t at(int64_t piece) const {
+        const int64_t s = piece / runs;
+        const int k = (int)(piece - s * runs);
+        return s * share + (k ? min(share, lead + (int64_t)(k - 1) * small) : 0);
+    }
+    // number of the last cut at or before g
+    __device__ __forceinline__ int upto(int64_t g) const {
+        const int64_t s = g / share, in = g - s * share;
+        return (int)(s * runs + (in < lead ? 0 : min((int64_t)runs - 1, 1 + (in - lead) / small)));
+    }
+    // number of the first cut at or after g
+    __device__ __forceinline__ int from(int64_t g) const { return upto(g - 1) + 1; }
+    // the n-th of the pieces that are taken as CTAs finish
+    __device__ __forceinline__ int64_t taken(int n) const { return (int64_t)(n / (runs - 1)) * runs + 1 + n % (runs - 1); }
 };
 
 template <int D, int TYPE, int STORE, int NT>
@@ -176,19 +218,20 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     using Sh = Shape<D, STORE, NT>;
     constexpr bool I8 = Sh::I8;
     constexpr int MT = I8 ? FVS_F16 : TYPE;  // type of the matrix instructions' operands
-    constexpr int S = Sh::S;
-    extern __shared__ __align__(16) uint8_t ring_all[];
+    constexpr int S = Sh::S, UNIT = Sh::UNIT, TILES = Sh::TILES;
+    extern __shared__ __align__(128) uint8_t ring_all[];
     __shared__ int64_t s_sum[WARPS];
     __shared__ int s_none[WARPS];
     __shared__ int64_t s_before[THREADS];  // cost (for one item of each sequence) before each thread's sequences
-    __shared__ Place s_place[2];           // where this CTA's range begins and ends
-    __shared__ int64_t s_base;             // cost before the first sequence of the range
+    __shared__ Place s_place[2];           // where a piece begins and ends
+    __shared__ int64_t s_base;             // cost before the first sequence of the piece
     __shared__ float s_ml[WARPS][Sh::ROWS][2];
-    __shared__ int s_tile[WARPS], s_last;
+    __shared__ int s_tile[WARPS], s_last, s_next;
+    __shared__ Cuts s_cuts;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = lane >> 2, c4 = lane & 3;
-    const int split = (a.group + Sh::ROWS - 1) / Sh::ROWS;  // items of a key head
+    const int split = a.split;
     const int per_seq = a.c.heads * split;
     const int B = a.tb.seqs;
 
@@ -197,12 +240,12 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     const int b_hi = min(B, (tid + 1) * chunk);
     int64_t mine = 0;
     int none = 0;
-    for (int b0 = tid * chunk; b0 < b_hi; b0 += 8) {
+    for (int b0 = tid * chunk; b0 < b_hi; b0 += 16) {
         unsigned sum = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < 16; j++) {
             if (b0 + j < b_hi) {
-                const int n = units_of(seq_len(a, b0 + j));
+                const int n = units_of<UNIT>(seq_len(a, b0 + j));
                 sum += n ? n + ITEM_COST : 0;
                 none += n == 0;
             }
@@ -244,18 +287,39 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             }
         }
     }
-    // ---- this CTA's range of the cost.  Unit u of an item that begins at cost x lies at x + ITEM_COST + u.  A cut nearer
-    // than `near` units to an item's begin or end moves there: joining two parts costs more than that
-    int64_t per = (total + gridDim.x - 1) / gridDim.x;
-    if (per < 16) per = 16;
-    if (blockIdx.x * per >= total) return;
-    const int near = per > 64 ? (int)(per / 8) : 8;
-    const int alone = per > 128 ? 16 : (int)(per / 8);  // items of up to so many units are one warp's
+    // ---- the pieces.  Unit u of an item that begins at cost x lies at x + ITEM_COST + u.  A cut nearer than `near` units
+    // to an item's begin or end moves there: joining two parts costs more than that
+    Cuts cuts;
+    cuts.share = max((int64_t)16, (total + gridDim.x - 1) / gridDim.x);
+    const bool shared = cuts.share >= 192;  // with less, setting up another piece costs more than it evens out
+    if (shared) {
+        cuts.small = (int)((cuts.share + 7) / 8);
+        cuts.lead = cuts.share - 2 * cuts.small;
+        cuts.runs = 3;
+    } else {
+        cuts.small = (int)cuts.share;
+        cuts.lead = cuts.share;
+        cuts.runs = 1;
+    }
+    if (tid == 0) s_cuts = cuts;
+    const int near = max(8, cuts.small / 8);
+    // items of up to so many units are one warp's; fewer than 2 near, so that none of them is cut
+    const int alone = Sh::Q_SMEM ? 0 : (int)min((int64_t)15, cuts.share / 8);
+    uint8_t* ring = ring_all + warp * Sh::RING;
+    const uint32_t ring_at = smem_addr(ring);
+    const bool aligned = a.c.page % 16 == 0;  // a tile's keys lie in one page
+    auto page_of = [&](int t) { return (int)(((uint64_t)(unsigned)t * a.page_mul) >> a.page_shift); };
+
+    int64_t piece = (int64_t)blockIdx.x * cuts.runs;
+#pragma unroll 1
+    for (;; piece = s_cuts.taken(s_next)) {
     __syncthreads();
+    if (s_cuts.at(piece) >= total) break;
+    if (tid == THREADS - 1 && shared) s_next = atomicAdd(a.arrived + (int64_t)B * per_seq, 1);
     if (warp < 2) {
-        const int64_t g = (blockIdx.x + warp) * per;
+        const int64_t g = s_cuts.at(piece + warp);
         if (g >= total) {
-            if (lane == 0) s_place[warp] = Place{B, 0, 0};
+            if (lane == 0) s_place[warp] = Place{B, 0, 0, 0};
         } else {
             int at = 0;  // the last run of sequences that begins at or before g
 #pragma unroll
@@ -263,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             at = (int)__reduce_add_sync(0xffffffffu, (unsigned)at) - 1;
             int64_t base = s_before[at];
             for (int b0 = at * chunk; b0 < B; b0 += 32) {
-                const int n = b0 + lane < B ? units_of(seq_len(a, b0 + lane)) : 0;
+                const int n = b0 + lane < B ? units_of<UNIT>(seq_len(a, b0 + lane)) : 0;
                 const int64_t cost = n ? n + ITEM_COST : 0;
                 int64_t upto = cost;
 #pragma unroll
@@ -275,8 +339,12 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 if (past) {
                     if (lane == __ffs(past) - 1) {
                         const int64_t in = g - (base + upto - cost) * per_seq;
-                        const int hh = (int)(in / cost), u = (int)(in - hh * cost) - ITEM_COST;
-                        s_place[warp] = u < near ? Place{b0 + lane, hh, 0} : n - u < near ? Place{b0 + lane, hh + 1, 0} : Place{b0 + lane, hh, u};
+                        int hh = (int)(in / cost), u = (int)(in - hh * cost) - ITEM_COST;
+                        if (u < near)
+                            u = 0;
+                        else if (n - u < near)
+                            hh++, u = 0;  // heads: past the sequence's last item
+                        s_place[warp] = Place{b0 + lane, hh / split, hh % split, u};
                         if (warp == 0) s_base = base + upto - cost;
                     }
                     break;
@@ -289,53 +357,53 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     const Place stop = s_place[1];
     Item now;  // the item under computation
     now.b = s_place[0].b;
-    now.hh = s_place[0].hh;
-    now.len = seq_len(a, now.b);
-    now.n = units_of(now.len);
+    now.head = s_place[0].head;
+    now.sub = s_place[0].sub;
     now.u = s_place[0].u;
-    clip(now, stop);
+    now.len = seq_len(a, now.b);
+    now.n = units_of<UNIT>(now.len);
     int64_t base = s_base;
-    bool more = true;
-    if (now.hh == per_seq) {  // moved past the sequence's last item
-        const int b = now.b;
-        now.hh--;
-        more = next_item(a, now, stop, per_seq);
-        if (now.b != b) base += units_of(seq_len(a, b)) + ITEM_COST;
+    bool more;
+    if (now.head == a.c.heads) {  // moved past the sequence's last item
+        const int cost = now.n + ITEM_COST;
+        now.head--;
+        now.sub = split - 1;
+        now.end = now.n;
+        more = next_item<UNIT>(a, now, stop);
+        base += cost;
     } else {
-        more = now.b < stop.b || (now.b == stop.b && (now.hh < stop.hh || (now.hh == stop.hh && now.u < stop.u)));
+        now.end = stop.same_item(now.b, now.head, now.sub) ? stop.u : now.n;
+        more = now.u < now.end;
     }
-    if (!more) return;
     // the units that this warp copies: every fourth of an item, all of one that it has alone
     Item ahead = now;
-    bool any = true;
-    auto owner = [&](const Item& it) { return (it.b * per_seq + it.hh) % WARPS; };
+    bool any = more;
+    auto owner = [&](const Item& it) { return ((it.b * a.c.heads + it.head) * split + it.sub) % WARPS; };
     auto settle = [&]() {
         while (any && ahead.u >= ahead.end) {
-            any = next_item(a, ahead, stop, per_seq);
+            any = next_item<UNIT>(a, ahead, stop);
             if (any) ahead.u = ahead.n > alone ? warp : owner(ahead) == warp ? 0 : ahead.end;
         }
     };
-    ahead.u = ahead.n > alone ? ahead.u + warp : owner(ahead) == warp ? 0 : ahead.end;
+    if (any) ahead.u = ahead.n > alone ? ahead.u + warp : owner(ahead) == warp ? 0 : ahead.end;
     settle();
-
-    uint8_t* ring = ring_all + warp * Sh::RING;
-    const uint32_t ring_at = smem_addr(ring);
 
     // ---- copies, two lookups ahead
     auto look = [&]() {
         Lookup k;
-        k.entry = -1;
-        k.slot = 0;
-        k.head = 0;
-        k.live = any;
+        k.entry = NO_UNIT;
+        k.slot = k.head = 0;
         if (any) {
-            const int t = ahead.u * UNIT + (lane & 15);
-            if (t < ahead.len) {
-                const int p = (int)((unsigned)t / (unsigned)a.c.page);
-                k.slot = t - p * a.c.page;
-                k.entry = __ldg(a.tb.at + (int64_t)ahead.b * a.tb.stride + p);
+            const int t = ahead.u * UNIT + (lane & (UNIT - 1));
+            const int from = aligned ? t & ~15 : t;
+            k.entry = -1;
+            k.slot = INT_MAX;  // not one of the sequence's keys
+            if (from < ahead.len) {
+                const int p = page_of(from);
+                if (t < ahead.len) k.slot = t - p * a.c.page;
+                k.entry = max(-1, __ldg(a.tb.at + (int64_t)ahead.b * a.tb.stride + p));
             }
-            k.head = ahead.hh / split;
+            k.head = ahead.head;
             ahead.u += ahead.n > alone ? WARPS : 1;
             settle();
         }
@@ -346,70 +414,114 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             atomicOr(a.c.status, BAD_INDEX);
             k.entry = -1;
         }
-        k.fill = a.c.fill && k.entry >= 0 ? __ldg(a.c.fill + k.entry) : 0x7fffffff;
+        k.fill = a.c.fill && k.entry >= 0 ? __ldg(a.c.fill + k.entry) : INT_MAX;
     };
     auto issue = [&](const Lookup& k, int slot) {
         const bool live = k.entry >= 0 && k.slot < k.fill;
-        const uint32_t mask = __ballot_sync(0xffffffffu, live);
-        const int64_t row = live ? (int64_t)k.entry * a.c.page_stride + (int64_t)k.head * a.c.head_stride +
-                                       (int64_t)k.slot * a.c.slot_stride
-                                 : 0;
+        const uint32_t mask = __ballot_sync(0xffffffffu, live) & (UNIT == 32 ? 0xffffffffu : 0xffffu);
         const uint32_t st = ring_at + slot * Sh::STAGE;
         constexpr int PER = Sh::RB / 16;  // chunks of a row
         constexpr int ESZ = I8 ? 1 : 2;
+        if (aligned) {
+            // a tile's rows are one slot apart: each lane copies its chunk of every RPI-th row
+            constexpr int RPI = PER > 16 ? 1 : PER > 8 ? 2 : PER > 4 ? 4 : 8;
+            const int row = lane / PER, ch = lane % PER;
 #pragma unroll
-        for (int i = 0; i < UNIT * PER / 32; i++) {
-            const int at = i * 32 + lane, key = at / PER, ch = at % PER;
-            const int64_t off = __shfl_sync(0xffffffffu, row, key) * ESZ + ch * 16;
-            const bool on = (mask >> key) & 1;
-            copy16(st + key * Sh::KS + ch * 16, (const uint8_t*)a.c.k + off, on);
-            copy16(st + UNIT * Sh::KS + key * Sh::VS + ch * 16, (const uint8_t*)a.c.v + off, on);
+            for (int j = 0; j < TILES; j++) {
+                const uint32_t m = (mask >> (16 * j)) & 0xffffu;
+                const int slot0 = __shfl_sync(0xffffffffu, k.slot, 16 * j), entry = __shfl_sync(0xffffffffu, k.entry, 16 * j);
+                if (m && row < RPI) {
+                    const int64_t off = ((int64_t)entry * a.c.page_stride + (int64_t)k.head * a.c.head_stride +
+                                         (int64_t)(slot0 + row) * a.c.slot_stride) * ESZ + ch * 16;
+                    const uint8_t *pk = (const uint8_t*)a.c.k + off, *pv = (const uint8_t*)a.c.v + off;
+                    const int64_t step = a.c.slot_stride * (RPI * ESZ);
+                    const bool dense = a.c.slot_stride == D && m == 0xffffu;  // fixed distances: no address arithmetic
+#pragma unroll
+                    for (int i = 0; i < 16 / RPI; i++) {
+                        const int key = 16 * j + i * RPI + row;
+                        const uint32_t dk = st + key * Sh::KS + Sh::k_chunk(key, ch) * 16;
+                        const uint32_t dv = st + Sh::VALUES + key * Sh::VS + Sh::v_chunk(key, ch) * 16;
+                        if (dense) {
+                            copy16(dk, pk + i * RPI * Sh::RB, true);
+                            copy16(dv, pv + i * RPI * Sh::RB, true);
+                        } else {
+                            const bool on = (m >> (i * RPI + row)) & 1;
+                            copy16(dk, on ? pk + i * step : (const uint8_t*)a.c.k, on);
+                            copy16(dv, on ? pv + i * step : (const uint8_t*)a.c.v, on);
+                        }
+                    }
+                }
+            }
+        } else {
+            const int64_t at0 = live ? (int64_t)k.entry * a.c.page_stride + (int64_t)k.head * a.c.head_stride +
+                                           (int64_t)k.slot * a.c.slot_stride
+                                     : 0;
+#pragma unroll
+            for (int i = 0; i < UNIT * PER / 32; i++) {
+                const int at = i * 32 + lane, key = at / PER, ch = at % PER;
+                const int64_t off = __shfl_sync(0xffffffffu, at0, key) * ESZ + ch * 16;
+                const bool on = (mask >> key) & 1;
+                copy16(st + key * Sh::KS + Sh::k_chunk(key, ch) * 16, (const uint8_t*)a.c.k + off, on);
+                copy16(st + Sh::VALUES + key * Sh::VS + Sh::v_chunk(key, ch) * 16, (const uint8_t*)a.c.v + off, on);
+            }
         }
         if (I8) {
             const int64_t at = live ? (int64_t)k.entry * a.c.scale_page_stride + (int64_t)k.head * a.c.scale_head_stride +
                                           (int64_t)k.slot * a.c.scale_slot_stride
                                     : 0;
-            copy4(st + Sh::SCALES + lane * 4, (lane < 16 ? a.c.k_scale : a.c.v_scale) + at, live);
+            if (UNIT == 32) {
+                copy4(st + Sh::SCALES + lane * 4, a.c.k_scale + at, live);
+                copy4(st + Sh::SCALES + 128 + lane * 4, a.c.v_scale + at, live);
+            } else {
+                copy4(st + Sh::SCALES + lane * 4, (lane < 16 ? a.c.k_scale : a.c.v_scale) + at, live);
+            }
         }
-        if (lane == 0) *(uint32_t*)(ring + slot * Sh::STAGE + Sh::MASK) = mask & 0xffffu;
+        if (lane == 0) *(uint32_t*)(ring + slot * Sh::STAGE + Sh::MASK) = mask;
     };
-    Lookup la = look();
-    look_fill(la);
-    Lookup lb = look();
-    int ready = 0;                                         // next slot to fill
+    Lookup la, lb;
+    int ready = S - 1;  // the slot to be filled next
+    {
+        // the first lookups side by side, so that their latencies overlap
+        Lookup l0[S + 1];
+#pragma unroll
+        for (int i = 0; i <= S; i++) l0[i] = look();
+#pragma unroll
+        for (int i = 0; i < S; i++) look_fill(l0[i]);
+#pragma unroll
+        for (int i = 0; i < S - 1; i++) {
+            if (l0[i].entry != NO_UNIT) issue(l0[i], i);
+            copies_commit();
+        }
+        la = l0[S - 1];
+        lb = l0[S];
+    }
     auto feed = [&]() {
-        if (la.live) issue(la, ready);
+        if (la.entry != NO_UNIT) issue(la, ready);
         copies_commit();
         ready = ready + 1 == S ? 0 : ready + 1;
         la = lb;
         look_fill(la);
         lb = look();
     };
-#pragma unroll 1
-    for (int i = 0; i < S - 1; i++) feed();
 
-    // ---- the range's items
+    // ---- the piece's items
     int slot = 0;
 #pragma unroll 1
     for (; more;) {
         const bool solo = now.n <= alone;
-        const int kvh = now.hh / split, h0 = kvh * a.group + (now.hh % split) * Sh::ROWS;
-        const int rows = min(Sh::ROWS, a.group - (now.hh % split) * Sh::ROWS);
+        const int h0 = now.head * a.group + now.sub * Sh::ROWS;
+        const int rows = min(Sh::ROWS, a.group - now.sub * Sh::ROWS);
         const Item it = now;
-        const int64_t it_begin = base * per_seq + (int64_t)now.hh * (now.n + ITEM_COST);
-        more = next_item(a, now, stop, per_seq);
+        const int64_t it_begin = base * per_seq + (int64_t)(now.head * split + now.sub) * (now.n + ITEM_COST);
+        more = next_item<UNIT>(a, now, stop);
         if (now.b != it.b) base += it.n + ITEM_COST;
         if (solo && owner(it) != warp) continue;
-        auto team_sync = [&]() {
-            if (solo)
-                __syncwarp();
-            else
-                __syncthreads();
-        };
 
         // q as the B operand: head r of each 8, elements of the order in which the keys' rows come
-        uint32_t qf[NT][D / 16][2];
-        float mul[NT][2];  // what a raw product is multiplied with, for heads 2 c4 and 2 c4 + 1
+        uint32_t qf[Sh::Q_SMEM ? 1 : NT][Sh::Q_SMEM ? 1 : D / 16][2];
+        uint2* q_all = (uint2*)(ring_all + Sh::SMEM - Sh::QBYTES);
+        float mul[NT][2];   // what a raw product is multiplied with, for heads 2 c4 and 2 c4 + 1
+        float bias[NT][2];  // int8: what the codes' 128 adds to it
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int h = t * 8 + r;
@@ -425,26 +537,53 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = max(1, min(252, (int)(__float_as_uint(top) >> 23)));  // 2^(e - 127) <= top
+                const int e = max(1, min(230, (int)(__float_as_uint(top) >> 23)));  // 2^(e - 127) <= top
                 const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                float sum = 0.f;  // of the rounded values
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const float2 x = Elem<TYPE>::up(raw[k].x), y = Elem<TYPE>::up(raw[k].y);
-                    qf[t][k][0] = Elem<FVS_F16>::down(x.x * down, x.y * down);
-                    qf[t][k][1] = Elem<FVS_F16>::down(y.x * down, y.y * down);
+                    const uint32_t f0 = Elem<FVS_F16>::down(x.x * down, x.y * down), f1 = Elem<FVS_F16>::down(y.x * down, y.y * down);
+                    const float2 u = Elem<FVS_F16>::up(f0), v = Elem<FVS_F16>::up(f1);
+                    sum += (u.x + u.y) + (v.x + v.y);
+                    if (Sh::Q_SMEM) {
+                        if (k % WARPS == warp) q_all[(t * (D / 16) + k) * 32 + lane] = make_uint2(f0, f1);
+                    } else {
+                        qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][0] = f0;
+                        qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][1] = f1;
+                    }
                 }
-                const float up = a.scale2 * __uint_as_float((uint32_t)e << 23);
-                mul[t][0] = __shfl_sync(0xffffffffu, up, c4 * 8);
-                mul[t][1] = __shfl_sync(0xffffffffu, up, c4 * 8 + 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                const float up = a.scale2 * __uint_as_float((uint32_t)(e + 24) << 23);
+                sum *= -0x1p-17f;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    mul[t][x] = __shfl_sync(0xffffffffu, up, c4 * 8 + 4 * x);
+                    bias[t][x] = __shfl_sync(0xffffffffu, sum, c4 * 8 + 4 * x);
+                }
             } else {
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
-                    qf[t][k][0] = h < rows ? __ldg((const uint32_t*)(qp + k * 16 + c4 * 2)) : 0u;
-                    qf[t][k][1] = h < rows ? __ldg((const uint32_t*)(qp + k * 16 + c4 * 2 + 8)) : 0u;
+                    if (Sh::Q_SMEM && k % WARPS != warp) continue;
+                    const uint32_t f0 = h < rows ? __ldg((const uint32_t*)(qp + k * 16 + c4 * 2)) : 0u;
+                    const uint32_t f1 = h < rows ? __ldg((const uint32_t*)(qp + k * 16 + c4 * 2 + 8)) : 0u;
+                    if (Sh::Q_SMEM) {
+                        q_all[(t * (D / 16) + k) * 32 + lane] = make_uint2(f0, f1);
+                    } else {
+                        qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][0] = f0;
+                        qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][1] = f1;
+                    }
                 }
                 mul[t][0] = mul[t][1] = a.scale2;
+                bias[t][0] = bias[t][1] = 0.f;
             }
         }
+        if (Sh::Q_SMEM) __syncthreads();
+        auto q_frag = [&](int t, int k) {
+            if (Sh::Q_SMEM) return q_all[(t * (D / 16) + k) * 32 + lane];
+            return make_uint2(qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][0], qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][1]);
+        };
         float m[NT][2], l[NT][2], o[D / 16][NT][4];
         int vexp = 1;  // int8: value scales are divided by 2^(vexp - 126)
 #pragma unroll
@@ -466,66 +605,81 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             slot = slot + 1 == S ? 0 : slot + 1;
             const uint32_t mask = *(const uint32_t*)(stp + Sh::MASK);
             if (mask == 0) continue;
-            // S^T = K Q^T, in two chains
-            float s[NT][4], s2[NT][4];
+            // S^T = K Q^T, each tile in two chains
+            float s[TILES][NT][4];
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int j = 0; j < TILES; j++) {
+                float s2[NT][4];
 #pragma unroll
-                for (int x = 0; x < 4; x++) s[t][x] = s2[t][x] = 0.f;
-            if (I8) {
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int k = 0; k < D / 32; k++) {
-                    uint2 lo = *(const uint2*)(stp + r * Sh::KS + k * 32 + c4 * 8);
-                    uint2 hi = *(const uint2*)(stp + (r + 8) * Sh::KS + k * 32 + c4 * 8);
-                    lo.x ^= 0x80808080u, lo.y ^= 0x80808080u, hi.x ^= 0x80808080u, hi.y ^= 0x80808080u;
-                    const uint32_t f0[4] = {codes2(lo.x, 0x4140), codes2(hi.x, 0x4140), codes2(lo.x, 0x4342), codes2(hi.x, 0x4342)};
-                    const uint32_t f1[4] = {codes2(lo.y, 0x4140), codes2(hi.y, 0x4140), codes2(lo.y, 0x4342), codes2(hi.y, 0x4342)};
+                    for (int x = 0; x < 4; x++) s[j][t][x] = I8 ? bias[t][x & 1] : 0.f, s2[t][x] = 0.f;
+                if (I8) {
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        mma<MT>(s[t], f0, qf[t][2 * k][0], qf[t][2 * k][1]);
-                        mma<MT>(s2[t], f1, qf[t][2 * k + 1][0], qf[t][2 * k + 1][1]);
+                    for (int k = 0; k < D / 32; k++) {
+                        const int at = (16 * j + r) * Sh::KS + Sh::k_chunk(r, 2 * k) * 16 + c4 * 8;
+                        uint2 lo = *(const uint2*)(stp + at), hi = *(const uint2*)(stp + at + 8 * Sh::KS);
+                        lo.x ^= 0x80808080u, lo.y ^= 0x80808080u, hi.x ^= 0x80808080u, hi.y ^= 0x80808080u;
+                        const uint32_t f0[4] = {codes2(lo.x, LOW), codes2(hi.x, LOW), codes2(lo.x, HIGH), codes2(hi.x, HIGH)};
+                        const uint32_t f1[4] = {codes2(lo.y, LOW), codes2(hi.y, LOW), codes2(lo.y, HIGH), codes2(hi.y, HIGH)};
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            const uint2 q0 = q_frag(t, 2 * k), q1 = q_frag(t, 2 * k + 1);
+                            mma<MT>(s[j][t], f0, q0.x, q0.y);
+                            mma<MT>(s2[t], f1, q1.x, q1.y);
+                        }
+                    }
+                } else {
+                    const uint32_t at = st + (16 * j + (lane & 15)) * Sh::KS;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k += 2) {
+                        uint32_t f0[4], f1[4];
+                        ldm4(f0, at + Sh::k_chunk(lane, 2 * k + (lane >> 4)) * 16);
+                        ldm4(f1, at + Sh::k_chunk(lane, 2 * k + 2 + (lane >> 4)) * 16);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            const uint2 q0 = q_frag(t, k), q1 = q_frag(t, k + 1);
+                            mma<MT>(s[j][t], f0, q0.x, q0.y);
+                            mma<MT>(s2[t], f1, q1.x, q1.y);
+                        }
                     }
                 }
-            } else {
-                const uint32_t at = st + (lane & 15) * Sh::KS + (lane >> 4) * 16;
 #pragma unroll
-                for (int k = 0; k < D / 16; k += 2) {
-                    uint32_t f0[4], f1[4];
-                    ldm4(f0, at + k * 32);
-                    ldm4(f1, at + k * 32 + 32);
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        mma<MT>(s[t], f0, qf[t][k][0], qf[t][k][1]);
-                        mma<MT>(s2[t], f1, qf[t][k + 1][0], qf[t][k + 1][1]);
-                    }
-                }
+                    for (int x = 0; x < 4; x++) s[j][t][x] = (s[j][t][x] + s2[t][x]) * mul[t][x & 1];
             }
-            const bool on0 = (mask >> r) & 1, on1 = (mask >> (r + 8)) & 1;
-            float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f;
-            if (I8) {
-                const float* sc = (const float*)(stp + Sh::SCALES);
-                ks0 = sc[r], ks1 = sc[r + 8], vs0 = sc[16 + r], vs1 = sc[24 + r];
-            }
+            float vs[TILES][2];
             bool moved = false;
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
+            for (int j = 0; j < TILES; j++) {
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const float raw = s[t][x] + s2[t][x];
-                    const float y = I8 ? raw * (x < 2 ? ks0 : ks1) * mul[t][x & 1] : raw * mul[t][x & 1];
-                    s[t][x] = (x < 2 ? on0 : on1) ? y : -INFINITY;
+                for (int x = 0; x < 2; x++) {
+                    const int key = 16 * j + 8 * x + r;
+                    const float* sc = (const float*)(stp + Sh::SCALES);
+                    const float ks = I8 ? sc[key] : 1.f;
+                    vs[j][x] = I8 ? sc[UNIT + key] : 1.f;
+                    const bool on = (mask >> key) & 1;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            float& y = s[j][t][2 * x + h];
+                            y = on ? (I8 ? y * ks : y) : -INFINITY;
+                            moved |= y > m[t][h] + SLACK;
+                        }
                 }
-                moved |= fmaxf(s[t][0], s[t][2]) > m[t][0] + SLACK || fmaxf(s[t][1], s[t][3]) > m[t][1] + SLACK;
             }
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        float y = fmaxf(s[t][x], s[t][x + 2]);
+                        float y = m[t][x];
+#pragma unroll
+                        for (int j = 0; j < TILES; j++) y = fmaxf(y, fmaxf(s[j][t][x], s[j][t][x + 2]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
-                        y = fmaxf(y, m[t][x]);
                         const float f = y == -INFINITY ? 1.f : exp2_fast(m[t][x] - y);
                         m[t][x] = y;
                         l[t][x] *= f;
@@ -535,7 +689,11 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 }
             }
             if (I8) {
-                const uint32_t big = max(__float_as_uint(vs0) & 0x7fffffffu, __float_as_uint(vs1) & 0x7fffffffu);
+                uint32_t big = 0;
+#pragma unroll
+                for (int j = 0; j < TILES; j++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) big = max(big, __float_as_uint(vs[j][x]) & 0x7fffffffu);
                 const int e = min(252, (int)(__reduce_max_sync(0xffffffffu, big) >> 23));
                 if (e > vexp) {
                     const float f = e - vexp >= 126 ? 0.f : __uint_as_float((uint32_t)(127 - (e - vexp)) << 23);
@@ -548,166 +706,229 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                             for (int x = 0; x < 4; x++) o[i][t][x] *= f;
                 }
                 const float down = __uint_as_float((uint32_t)(253 - vexp) << 23);
-                vs0 *= down, vs1 *= down;
+#pragma unroll
+                for (int j = 0; j < TILES; j++) vs[j][0] *= down, vs[j][1] *= down;
             }
-            // p, and p as the B operand of the second product
-            uint32_t pf[NT][2];
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const float z0 = m[t][0] == -INFINITY ? 0.f : m[t][0], z1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
-                float p0 = exp2_fast(s[t][0] - z0), p1 = exp2_fast(s[t][1] - z1);
-                float p2 = exp2_fast(s[t][2] - z0), p3 = exp2_fast(s[t][3] - z1);
-                l[t][0] += p0 + p2;
-                l[t][1] += p1 + p3;
-                if (I8) p0 *= vs0, p1 *= vs0, p2 *= vs1, p3 *= vs1;
-                pf[t][0] = transpose8x8(Elem<MT>::down(p0, p1));
-                pf[t][1] = transpose8x8(Elem<MT>::down(p2, p3));
-            }
-            // O^T += V^T P^T
-            if (I8) {
-                const uint8_t* v = stp + UNIT * Sh::KS + r * 4;
+            for (int j = 0; j < TILES; j++) {
+                if (TILES > 1 && ((mask >> (16 * j)) & 0xffffu) == 0) continue;  // its rows were not copied
+                // p, and p as the B operand of the second product
+                uint32_t pf[NT][2];
 #pragma unroll
-                for (int j = 0; j < D / 32; j++) {
-                    const uint32_t v0 = *(const uint32_t*)(v + (2 * c4) * Sh::VS + j * 32) ^ 0x80808080u;
-                    const uint32_t v1 = *(const uint32_t*)(v + (2 * c4 + 1) * Sh::VS + j * 32) ^ 0x80808080u;
-                    const uint32_t v2 = *(const uint32_t*)(v + (2 * c4 + 8) * Sh::VS + j * 32) ^ 0x80808080u;
-                    const uint32_t v3 = *(const uint32_t*)(v + (2 * c4 + 9) * Sh::VS + j * 32) ^ 0x80808080u;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t x = __byte_perm(v0, v1, h ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, h ? 0x7362 : 0x5140);
-                        const uint32_t f[4] = {codes2(x, 0x4140), codes2(x, 0x4342), codes2(y, 0x4140), codes2(y, 0x4342)};
-#pragma unroll
-                        for (int t = 0; t < NT; t++) mma<MT>(o[2 * j + h][t], f, pf[t][0], pf[t][1]);
-                    }
+                for (int t = 0; t < NT; t++) {
+                    const float z0 = m[t][0] == -INFINITY ? 0.f : m[t][0], z1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
+                    float p0 = exp2_fast(s[j][t][0] - z0), p1 = exp2_fast(s[j][t][1] - z1);
+                    float p2 = exp2_fast(s[j][t][2] - z0), p3 = exp2_fast(s[j][t][3] - z1);
+                    l[t][0] += p0 + p2;
+                    l[t][1] += p1 + p3;
+                    if (I8) p0 *= vs[j][0], p1 *= vs[j][0], p2 *= vs[j][1], p3 *= vs[j][1];
+                    pf[t][0] = transpose8x8(Elem<MT>::down(p0, p1));
+                    pf[t][1] = transpose8x8(Elem<MT>::down(p2, p3));
                 }
-            } else {
-                const uint32_t at = st + UNIT * Sh::KS + ((lane >> 4) * 8 + (lane & 7)) * Sh::VS + ((lane >> 3) & 1) * 16;
+                // O^T += V^T P^T
+                if (I8) {
+                    const uint32_t minus[4] = {MINUS_128, MINUS_128, MINUS_128, MINUS_128};
 #pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    uint32_t f[4];
-                    ldm4t(f, at + i * 32);
+                    for (int k = 0; k < D / 32; k++) {
+                        // rows 2 c4, 2 c4 + 1 and 8 further: their chunks are permuted alike
+                        const uint8_t* v = stp + Sh::VALUES + (16 * j + 2 * c4) * Sh::VS + Sh::v_chunk(2 * c4, 2 * k) * 16 + r * 4;
+                        const uint32_t v0 = *(const uint32_t*)v ^ 0x80808080u, v1 = *(const uint32_t*)(v + Sh::VS) ^ 0x80808080u;
+                        const uint32_t v2 = *(const uint32_t*)(v + 8 * Sh::VS) ^ 0x80808080u, v3 = *(const uint32_t*)(v + 9 * Sh::VS) ^ 0x80808080u;
 #pragma unroll
-                    for (int t = 0; t < NT; t++) mma<MT>(o[i][t], f, pf[t][0], pf[t][1]);
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t x = __byte_perm(v0, v1, h ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, h ? 0x7362 : 0x5140);
+                            const uint32_t f[4] = {codes2(x, LOW), codes2(x, HIGH), codes2(y, LOW), codes2(y, HIGH)};
+#pragma unroll
+                            for (int t = 0; t < NT; t++) {
+                                mma<MT>(o[2 * k + h][t], f, pf[t][0], pf[t][1]);
+                                mma<MT>(o[2 * k + h][t], minus, pf[t][0], pf[t][1]);
+                            }
+                        }
+                    }
+                } else {
+                    const int row = (lane >> 4) * 8 + (lane & 7);
+                    const uint32_t at = st + Sh::VALUES + (16 * j + row) * Sh::VS;
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++) {
+                        uint32_t f[4];
+                        ldm4t(f, at + Sh::v_chunk(lane, 2 * i + ((lane >> 3) & 1)) * 16);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) mma<MT>(o[i][t], f, pf[t][0], pf[t][1]);
+                    }
                 }
             }
         }
 
-        // ---- the item's result: the warps' tiles through shared memory (each warp's ring slot that its next copy fills)
+        // ---- the item's result.  Each lane brings its heads' outputs to the maximum over the warps, and to their end where
+        // the item is whole; the warps' tiles are then added up in shared memory (in each warp's ring slot that its next
+        // copy fills)
+        const bool whole = it.u == 0 && it.end == it.n;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[t][x] += __shfl_xor_sync(0xffffffffu, l[t][x], d);
+                if (r == 0) *(float2*)s_ml[warp][t * 8 + 2 * c4 + x] = make_float2(m[t][x], l[t][x]);
+            }
         __syncwarp();
         float* tile = Sh::O_IN_RING ? (float*)(ring + ready * Sh::STAGE)
                                     : (float*)(ring_all + WARPS * Sh::RING + warp * Sh::OBYTES);
-        const float vup = I8 ? __uint_as_float((uint32_t)(vexp + 1) << 23) : 1.f;
+        if (lane == 0) s_tile[warp] = (int)((uint8_t*)tile - ring_all);
+        if (!solo) __syncthreads();
+        const float vup = I8 ? __uint_as_float((uint32_t)(vexp + 1) << 23) * 0x1p24f : 1.f;
+        auto log_sum = [](float mx, float sum) { return sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f; };
 #pragma unroll
         for (int t = 0; t < NT; t++) {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                float y = l[t][x];
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) y += __shfl_xor_sync(0xffffffffu, y, d);
                 const int row = t * 8 + 2 * c4 + x;
-                if (r == 0) s_ml[warp][row][0] = m[t][x], s_ml[warp][row][1] = y;
+                float mx = m[t][x], sum = l[t][x], f = 1.f;
+                if (!solo) {
+                    const float2 own = make_float2(mx, sum);
+#pragma unroll
+                    for (int w = 0; w < WARPS; w++) mx = fmaxf(mx, s_ml[w][row][0]);
+                    sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WARPS; w++) {
+                        const float2 ml = *(const float2*)s_ml[w][row];
+                        sum += ml.y * weight(ml, mx);
+                    }
+                    f = weight(own, mx);
+                }
+                if (whole) {
+                    f = sum == 0.f ? 0.f : f / sum;
+                    if (a.lse && r == 0 && (solo || warp == 0) && row < rows)
+                        a.lse[(int64_t)it.b * a.hq + h0 + row] = log_sum(mx, sum);
+                } else if (r == 0 && warp == 0) {
+                    *(float2*)(a.parts + (2 * piece + (it.u == 0)) * Sh::PART + Sh::ROWS * D + 2 * row) = make_float2(mx, sum);
+                }
+                const bool none = f == 0.f;
+                f *= vup;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
                     float* p = tile + row * Sh::OS + (I8 ? (i / 2) * 32 + 4 * r + 2 * (i & 1) : i * 16 + r);
-                    p[0] = o[i][t][x] * vup;
-                    p[I8 ? 1 : 8] = o[i][t][x + 2] * vup;
+                    p[0] = none ? 0.f : o[i][t][x] * f;
+                    p[I8 ? 1 : 8] = none ? 0.f : o[i][t][x + 2] * f;
                 }
             }
         }
-        if (lane == 0) s_tile[warp] = (int)((uint8_t*)tile - ring_all);
-        team_sync();
-        const bool whole = it.u == 0 && it.end == it.n;
-        const int tt = solo ? lane : tid, nthr = solo ? 32 : THREADS;
-        const int w_lo = solo ? warp : 0, w_hi = solo ? warp + 1 : WARPS;
-        // an item's first part is its CTA's second one: that CTA may hold the last part of another
-        float* part = a.parts + (int64_t)(2 * blockIdx.x + (it.u == 0)) * Sh::PART;
         constexpr int Q4 = D / 4;
-        auto finish = [&](int row, int d, float mx, float sum, const float4& acc) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const int64_t h = (int64_t)it.b * a.hq + h0 + row;
-            *(uint2*)((uint16_t*)a.out + h * D + d) =
-                sum == 0.f ? make_uint2(0, 0)
-                           : make_uint2(Elem<TYPE>::down(acc.x * inv, acc.y * inv), Elem<TYPE>::down(acc.z * inv, acc.w * inv));
-            if (d == 0 && a.lse) a.lse[h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
-        };
-        for (int i = tt; i < rows * Q4; i += nthr) {
-            const int row = i / Q4, d = (i - row * Q4) * 4;
-            float mx = -INFINITY;
-            for (int w = w_lo; w < w_hi; w++) mx = fmaxf(mx, s_ml[w][row][0]);
-            float sum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = w_lo; w < w_hi; w++) {
-                const float f = weight(make_float2(s_ml[w][row][0], s_ml[w][row][1]), mx);
-                const float4 x = *(const float4*)((const float*)(ring_all + s_tile[w]) + row * Sh::OS + d);
-                if (f != 0.f) {
-                    sum += s_ml[w][row][1] * f;
-                    acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
-                }
+        uint16_t* out = (uint16_t*)a.out + ((int64_t)it.b * a.hq + h0) * D;
+        if (solo) {  // never cut: an item of so few units
+            __syncwarp();
+            for (int i = lane; i < rows * Q4; i += 32) {
+                const int row = i / Q4, d = (i - row * Q4) * 4;
+                const float4 x = *(const float4*)(tile + row * Sh::OS + d);
+                *(uint2*)(out + row * D + d) = make_uint2(Elem<TYPE>::down(x.x, x.y), Elem<TYPE>::down(x.z, x.w));
             }
-            if (whole) {
-                finish(row, d, mx, sum, acc);
-            } else {
-                *(float4*)(part + row * D + d) = acc;
-                if (d == 0) *(float2*)(part + Sh::ROWS * D + 2 * row) = make_float2(mx, sum);
-            }
+            __syncwarp();
+            continue;
         }
-        if (!whole) {  // never alone: an item of so few units is not cut
+        __syncthreads();
+        // an item's first part is its piece's second one: the piece may begin with the last part of another item
+        float* part = a.parts + (2 * piece + (it.u == 0)) * Sh::PART;
+        for (int i = tid; i < rows * Q4; i += THREADS) {
+            const int row = i / Q4, d = (i - row * Q4) * 4;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float4 x = *(const float4*)((const float*)(ring_all + s_tile[w]) + row * Sh::OS + d);
+                acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+            }
+            if (whole)
+                *(uint2*)(out + row * D + d) = make_uint2(Elem<TYPE>::down(acc.x, acc.y), Elem<TYPE>::down(acc.z, acc.w));
+            else
+                *(float4*)(part + row * D + d) = acc;
+        }
+        if (!whole) {
             __threadfence();
             __syncthreads();
-            // the cuts inside the item lie at multiples of per; parts - 1 of them, the first at t_lo * per
-            const int t_lo = (int)((it_begin + ITEM_COST + near + per - 1) / per);
-            const int parts = (int)((it_begin + ITEM_COST + it.n - near) / per) - t_lo + 2;
+            // the cuts inside the item: parts - 1 of them, the first at cut t_lo
+            const int t_lo = s_cuts.from(it_begin + ITEM_COST + near);
+            const int parts = s_cuts.upto(it_begin + ITEM_COST + it.n - near) - t_lo + 2;
             if (tid == 0) {
-                const int64_t item = (int64_t)it.b * per_seq + it.hh;
+                const int64_t item = (int64_t)it.b * per_seq + it.head * split + it.sub;
                 s_last = atomicAdd(a.arrived + item, 1) == parts - 1;
                 if (s_last) a.arrived[item] = 0;
             }
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                for (int i = tid; i < rows * Q4; i += THREADS) {
-                    const int row = i / Q4, d = (i - row * Q4) * 4;
-                    const float* from = a.parts + (int64_t)2 * (t_lo - 1) * Sh::PART;
-                    float mx = -INFINITY;
-                    for (int t = 0; t < parts; t++)
-                        mx = fmaxf(mx, __ldcg(from + (int64_t)(2 * t + (t == 0)) * Sh::PART + Sh::ROWS * D + 2 * row));
-                    float sum = 0.f;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int t = 0; t < parts; t++) {
-                        const float* p = from + (int64_t)(2 * t + (t == 0)) * Sh::PART;
-                        const float2 ml = __ldcg((const float2*)(p + Sh::ROWS * D + 2 * row));
-                        const float4 x = __ldcg((const float4*)(p + row * D + d));
-                        const float f = weight(ml, mx);
-                        if (f != 0.f) {
-                            sum += ml.y * f;
-                            acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
+                // a warp takes a row; lane t holds the weight of part t of 32, then four elements of the sum
+                const float* from = a.parts + (int64_t)2 * (t_lo - 1) * Sh::PART;
+                auto part_at = [&](int t) { return from + (2 * t + (t == 0)) * Sh::PART; };
+                for (int row = warp; row < rows; row += WARPS) {
+                    float mx = -INFINITY, sum = 0.f;
+                    for (int t = lane; t < parts; t += 32) mx = fmaxf(mx, __ldcg(part_at(t) + Sh::ROWS * D + 2 * row));
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                    constexpr int Q = (Q4 + 31) / 32;
+                    float4 acc[Q];
+#pragma unroll
+                    for (int i = 0; i < Q; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int t0 = 0; t0 < parts; t0 += 32) {
+                        float w = 0.f;
+                        if (t0 + lane < parts) {
+                            const float2 ml = __ldcg((const float2*)(part_at(t0 + lane) + Sh::ROWS * D + 2 * row));
+                            w = weight(ml, mx);
+                            sum += ml.y * w;
+                        }
+                        const int n = min(32, parts - t0);
+                        for (int j0 = 0; j0 < n; j0 += 8) {  // eight parts' loads together
+                            float4 x[8][Q];
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                const float* p = part_at(t0 + min(j0 + j, n - 1)) + row * D;
+#pragma unroll
+                                for (int i = 0; i < Q; i++)
+                                    if (i * 32 + lane < Q4) x[j][i] = __ldcg((const float4*)p + i * 32 + lane);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                const float f = j0 + j < n ? __shfl_sync(0xffffffffu, w, j0 + j) : 0.f;
+                                if (f != 0.f)
+#pragma unroll
+                                    for (int i = 0; i < Q; i++) {
+                                        acc[i].x += x[j][i].x * f, acc[i].y += x[j][i].y * f;
+                                        acc[i].z += x[j][i].z * f, acc[i].w += x[j][i].w * f;
+                                    }
+                            }
                         }
                     }
-                    finish(row, d, mx, sum, acc);
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                    for (int i = 0; i < Q; i++)
+                        if (i * 32 + lane < Q4)
+                            *((uint2*)(out + row * D) + i * 32 + lane) = make_uint2(Elem<TYPE>::down(acc[i].x * inv, acc[i].y * inv),
+                                                                                    Elem<TYPE>::down(acc[i].z * inv, acc[i].w * inv));
+                    if (a.lse && lane == 0) a.lse[(int64_t)it.b * a.hq + h0 + row] = log_sum(mx, sum);
                 }
             }
         }
-        team_sync();  // the tiles' slots may be filled again
+        __syncthreads();  // the tiles' slots may be filled again
     }
     copies_wait<0>();
+    __syncthreads();
+    if (!shared) break;
+    }
+    if (shared && tid == 0) {
+        int32_t* next = a.arrived + (int64_t)B * per_seq;
+        if (atomicAdd(next + 1, 1) == (int)gridDim.x - 1) next[0] = next[1] = 0;
+    }
 }
-
-// query heads of an item, in eights: 16 rows' accumulators and queries fit the registers up to D = 128
-template <int D>
-static int eights(int group) {
-    return group <= 8 || D > 128 ? 1 : 2;
-}
-static int rows_of(int dim, int group) { return 8 * (group <= 8 || dim > 128 ? 1 : 2); }
 
 template <int D, int TYPE, int STORE, int NT>
-static int launch_nt(fvs_stream_t stream, const AttendArgs& a) {
+static int launch_nt(fvs_stream_t stream, AttendArgs a) {
     using Sh = Shape<D, STORE, NT>;
     auto kernel = attend_kernel<D, TYPE, STORE, NT>;
     if (cudaError_t e = fvs_ensure_smem((const void*)kernel, Sh::SMEM)) return (int)e;
+    a.split = (a.group + Sh::ROWS - 1) / Sh::ROWS;
     // no more CTAs than the page tables' room can fill
     const int64_t room = (int64_t)a.tb.wide * a.c.page;
-    const int64_t units = ((room < 0x7fffffff ? room : 0x7fffffff) + UNIT - 1) / UNIT * a.tb.seqs * a.c.heads *
-                          ((a.group + Sh::ROWS - 1) / Sh::ROWS);
+    const int64_t units = ((room < INT_MAX ? room : INT_MAX) + Sh::UNIT - 1) / Sh::UNIT * a.tb.seqs * a.c.heads * a.split;
     int64_t grid = (units + WARPS - 1) / WARPS;
     const int64_t full = (int64_t)fvs_sm_count() * Sh::CTAS;
     if (grid > full) grid = full;
@@ -716,8 +937,8 @@ static int launch_nt(fvs_stream_t stream, const AttendArgs& a) {
 }
 template <int D, int TYPE, int STORE>
 static int launch(fvs_stream_t stream, const AttendArgs& a) {
-    if (eights<D>(a.group) == 1) return launch_nt<D, TYPE, STORE, 1>(stream, a);
-    return launch_nt<D, TYPE, STORE, D <= 128 ? 2 : 1>(stream, a);
+    if (a.group <= 8) return launch_nt<D, TYPE, STORE, 1>(stream, a);
+    return launch_nt<D, TYPE, STORE, 2>(stream, a);
 }
 template <int D>
 static int launch_types(fvs_stream_t stream, const AttendArgs& a, int type) {
@@ -731,11 +952,11 @@ static int launch_types(fvs_stream_t stream, const AttendArgs& a, int type) {
 
 using namespace fvs::kv;
 
-// two partial results for each of up to 3 CTAs on every SM
+// two partial results for each of the pieces: 3 for each of up to 4 CTAs on every SM
 extern "C" int fvs_kv_attend_work(int dim) {
     if (dim < 1) return FVS_EINVAL;
     if (dim > 256) return FVS_ERANGE;
-    return 2 * 3 * fvs_sm_count() * 16 * (dim + 2) * 4;
+    return 2 * 3 * 4 * fvs_sm_count() * 16 * (dim + 2) * 4;
 }
 
 extern "C" int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,
@@ -753,7 +974,12 @@ extern "C" int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int
                   arrived);
     if ((int64_t)seqs * hq > (1 << 28)) return FVS_ERANGE;
     AttendArgs a{*cache, {table, table_stride, seqs, wide}, q, q_seq, q_head, lens, out, lse, arrived,
-                 (float*)work, hq, hq / cache->heads, scale * 1.4426950408889634f};
+                 (float*)work, hq, hq / cache->heads, 1, scale * 1.4426950408889634f, 0, 0};
+    // exact for numerators below 2^31: 2^shift <= page_mul * page < 2^shift + 2^(shift - 31)
+    uint32_t bits = 0;
+    while ((1ull << bits) < (uint64_t)cache->page) bits++;
+    a.page_shift = 31 + bits;
+    a.page_mul = (uint32_t)(((1ull << a.page_shift) + cache->page - 1) / cache->page);
     switch (cache->dim) {
         case 64: return launch_types<64>(stream, a, type);
         case 96: return launch_types<96>(stream, a, type);
