@@ -51,6 +51,9 @@ struct AttendArgs {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int ITEM_COST = 3;   // of an item beside its units (loading q, adding up and writing), in units
+#ifndef V_SH
+#define V_SH 192
+#endif
 constexpr float SLACK = 8.f;   // how far (log2) a score may pass the running maximum before it moves
 
 template <int D, int STORE, int NT_>
@@ -291,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     // to an item's begin or end moves there: joining two parts costs more than that
     Cuts cuts;
     cuts.share = max((int64_t)16, (total + gridDim.x - 1) / gridDim.x);
-    const bool shared = cuts.share >= 192;  // with less, setting up another piece costs more than it evens out
+    const bool shared = cuts.share >= V_SH;  // with less, setting up another piece costs more than it evens out
     if (shared) {
         cuts.small = (int)((cuts.share + 7) / 8);
         cuts.lead = cuts.share - 2 * cuts.small;
@@ -855,49 +858,67 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                // a warp takes a row; lane t holds the weight of part t of 32, then four elements of the sum
+                // a warp takes a row; lane t holds the weights of parts t + 32 k, then four elements of the sum.  Loads that
+                // wait for the memory of a busy GPU cost 2000 cycles and more each time: all the weights in one wait, then
+                // 16 parts at a time
+                constexpr int Q = (Q4 + 31) / 32, WK = 4, BATCH = 16 / Q;
                 const float* from = a.parts + (int64_t)2 * (t_lo - 1) * Sh::PART;
                 auto part_at = [&](int t) { return from + (2 * t + (t == 0)) * Sh::PART; };
                 for (int row = warp; row < rows; row += WARPS) {
                     float mx = -INFINITY, sum = 0.f;
-                    for (int t = lane; t < parts; t += 32) mx = fmaxf(mx, __ldcg(part_at(t) + Sh::ROWS * D + 2 * row));
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                    constexpr int Q = (Q4 + 31) / 32;
                     float4 acc[Q];
 #pragma unroll
                     for (int i = 0; i < Q; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int t0 = 0; t0 < parts; t0 += 32) {
-                        float w = 0.f;
-                        if (t0 + lane < parts) {
-                            const float2 ml = __ldcg((const float2*)(part_at(t0 + lane) + Sh::ROWS * D + 2 * row));
-                            w = weight(ml, mx);
-                            sum += ml.y * w;
+                    for (int t0 = 0; t0 < parts; t0 += 32 * WK) {
+                        float2 ml[WK];
+#pragma unroll
+                        for (int k = 0; k < WK; k++) {
+                            const int t = t0 + 32 * k + lane;
+                            ml[k] = t < parts ? __ldcg((const float2*)(part_at(t) + Sh::ROWS * D + 2 * row)) : make_float2(-INFINITY, 0.f);
                         }
-                        const int n = min(32, parts - t0);
-                        for (int j0 = 0; j0 < n; j0 += 8) {  // eight parts' loads together
-                            float4 x[8][Q];
+                        float top = mx;
 #pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                const float* p = part_at(t0 + min(j0 + j, n - 1)) + row * D;
+                        for (int k = 0; k < WK; k++) top = fmaxf(top, ml[k].x);
 #pragma unroll
-                                for (int i = 0; i < Q; i++)
-                                    if (i * 32 + lane < Q4) x[j][i] = __ldcg((const float4*)p + i * 32 + lane);
-                            }
+                        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const float f0 = weight(make_float2(mx, sum), top);  // of what the parts before added up to
+                        mx = top;
+                        if (f0 != 1.f) {
+                            sum *= f0;
 #pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                const float f = j0 + j < n ? __shfl_sync(0xffffffffu, w, j0 + j) : 0.f;
-                                if (f != 0.f)
+                            for (int i = 0; i < Q; i++) acc[i].x *= f0, acc[i].y *= f0, acc[i].z *= f0, acc[i].w *= f0;
+                        }
 #pragma unroll
-                                    for (int i = 0; i < Q; i++) {
-                                        acc[i].x += x[j][i].x * f, acc[i].y += x[j][i].y * f;
-                                        acc[i].z += x[j][i].z * f, acc[i].w += x[j][i].w * f;
-                                    }
+                        for (int k = 0; k < WK; k++) {
+                            const int n = min(32, parts - t0 - 32 * k);
+                            if (n <= 0) break;
+                            const float w = weight(ml[k], mx);
+                            float part_sum = ml[k].y * w;
+#pragma unroll
+                            for (int d = 16; d; d >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, d);
+                            sum += part_sum;
+                            for (int j0 = 0; j0 < n; j0 += BATCH) {
+                                float4 x[BATCH][Q];
+#pragma unroll
+                                for (int j = 0; j < BATCH; j++) {
+                                    const float* p = part_at(t0 + 32 * k + min(j0 + j, n - 1)) + row * D;
+#pragma unroll
+                                    for (int i = 0; i < Q; i++)
+                                        if (i * 32 + lane < Q4) x[j][i] = __ldcg((const float4*)p + i * 32 + lane);
+                                }
+#pragma unroll
+                                for (int j = 0; j < BATCH; j++) {
+                                    const float f = __shfl_sync(0xffffffffu, w, min(j0 + j, 31));
+                                    if (j0 + j < n && f != 0.f)
+#pragma unroll
+                                        for (int i = 0; i < Q; i++) {
+                                            acc[i].x += x[j][i].x * f, acc[i].y += x[j][i].y * f;
+                                            acc[i].z += x[j][i].z * f, acc[i].w += x[j][i].w * f;
+                                        }
+                                }
                             }
                         }
                     }
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
                     for (int i = 0; i < Q; i++)
