@@ -23,6 +23,7 @@ from ._lib import check
 HEAD_DIMS = (64, 96, 128, 192, 256)
 _CODE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.int8: _lib.I8, torch.float32: _lib.F32T}
 _WIDE = (torch.float16, torch.bfloat16)
+_READ = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def _need(cond, what):
@@ -64,6 +65,8 @@ class PagedKV:
         self.k, self.v, self.k_scale, self.v_scale, self.fill = k, v, k_scale, v_scale, fill
         self.pages, self.heads, self.page, self.dim = k.shape
         self.device, self.dtype = k.device, k.dtype
+        self.scale = 1.0 / math.sqrt(self.dim)
+        self._index = k.device.index
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         p = lambda t: None if t is None else t.data_ptr()
         ss = k_scale.stride() if i8 else (0, 0, 0)
@@ -83,33 +86,45 @@ class PagedKV:
         return cls(k, v, *scales, fill=fill)
 
     # ---------------------------------------------------------------- arguments
+    # A decoding step makes these calls for every layer, so each check is one condition and messages are made on failure.
     def _table(self, table):
-        _need(table.dim() == 2 and table.dtype == torch.int32 and table.device == self.device
-              and (table.shape[1] <= 1 or table.stride(1) == 1) and table.shape[1] >= 1,
-              "the page table is an int32 [sequences, wide] with contiguous rows on the cache's GPU")
-        return table.data_ptr(), table.shape[0], table.shape[1], table.stride(0)
+        shape, stride = table.shape, table.stride()
+        if not (len(shape) == 2 and table.dtype is torch.int32 and table.device == self.device and shape[1] >= 1
+                and (shape[1] == 1 or stride[1] == 1)):
+            raise ValueError("the page table is an int32 [sequences, wide] with contiguous rows on the cache's GPU")
+        return table.data_ptr(), shape[0], shape[1], stride[0]
 
     def _ints(self, t, n, what):
         if t is None:
             return None
-        _need(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == self.device,
-              f"{what} is a contiguous int32 [{n}] on the cache's GPU")
+        if not (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == self.device):
+            raise ValueError(f"{what} is a contiguous int32 [{n}] on the cache's GPU")
         return t.data_ptr()
 
     def _heads(self, x, n, what, heads=None):
         """address, token stride and head stride of [n, heads, dim]"""
-        _need(x.dim() == 3 and x.shape[0] == n and x.shape[2] == self.dim and (heads is None or x.shape[1] == heads)
-              and x.device == self.device, f"{what} is [{n}, {heads or 'heads'}, {self.dim}] on the cache's GPU")
-        s = x.stride()
+        shape = x.shape
+        if not (len(shape) == 3 and shape[0] == n and shape[2] == self.dim and (heads is None or shape[1] == heads)
+                and x.device == self.device):
+            raise ValueError(f"{what} is [{n}, {heads or 'heads'}, {self.dim}] on the cache's GPU")
+        s0, s1, s2 = x.stride()
         at = x.data_ptr()
-        _need(s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and at % 16 == 0,
-              f"{what} needs contiguous, 16-byte aligned heads")
-        return at, s[0], s[1]
+        if s2 != 1 or s0 % 8 or s1 % 8 or at % 16:
+            raise ValueError(f"{what} needs contiguous, 16-byte aligned heads")
+        return at, s0, s1
 
     def _type(self, dtype, what):
-        _need(dtype in _WIDE and (self.dtype == torch.int8 or dtype == self.dtype),
-              f"{what} is {dtype}: fp16 or bf16, and the cache's own type unless that holds int8 codes")
+        if not (dtype in _WIDE and (self.dtype is torch.int8 or dtype is self.dtype)):
+            raise ValueError(f"{what} is {dtype}: fp16 or bf16, and the cache's own type unless that holds int8 codes")
         return _CODE[dtype]
+
+    def _like(self, out, x, what):
+        if not (out.dtype is x.dtype and out.shape == x.shape and out.is_contiguous() and out.device == self.device):
+            raise ValueError(f"{what} is a contiguous tensor like q")
+        return out.data_ptr()
+
+    def _stream(self):
+        return torch._C._cuda_getCurrentRawStream(self._index)  # torch.cuda.current_stream takes 2 us more
 
     # ---------------------------------------------------------------- the operators
     def append(self, k, v, table, idx, seq=None, pos=None, rope=None, pairs="halves", q=None, q_out=None):
@@ -120,30 +135,31 @@ class PagedKV:
         tokens that have no place), or None without q."""
         n = k.shape[0]
         ty = self._type(k.dtype, "k")
-        _need(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "k, v and q need one type")
+        if v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
+            raise ValueError("k, v and q need one type")
         ka, va = self._heads(k, n, "k", self.heads), self._heads(v, n, "v", self.heads)
         qa, hq, qo = (None, 0, 0), 0, None
         if q is not None:
             qa, hq = self._heads(q, n, "q"), q.shape[1]
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            _need(q_out.dtype == q.dtype and q_out.shape == q.shape and q_out.is_contiguous()
-                  and q_out.device == q.device, "q_out is a contiguous tensor like q")
-            qo = q_out.data_ptr()
+            qo = self._like(q_out, q, "q_out")
         cos = sin = None
         positions = rot = 0
         if rope is not None:
             cos, sin = rope
-            _need(cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
-                  and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == self.device,
-                  "rope is two contiguous fp32 [positions, rot / 2] on the cache's GPU")
+            if not (cos.dtype is sin.dtype is torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
+                    and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == self.device):
+                raise ValueError("rope is two contiguous fp32 [positions, rot / 2] on the cache's GPU")
             positions, rot = cos.shape[0], 2 * cos.shape[1]
-            _need(rot % 16 == 0 and 0 < rot <= self.dim and positions >= 1, f"rotation of {rot} elements: a multiple of 16, "
-                  f"at most {self.dim}")
+            if rot % 16 or not 0 < rot <= self.dim or positions < 1:
+                raise ValueError(f"rotation of {rot} elements: a multiple of 16, at most {self.dim}")
             cos, sin = cos.data_ptr(), sin.data_ptr()
-        _need(pairs in _lib.PAIRS, f"pairs {pairs!r}: one of {sorted(_lib.PAIRS)}")
-        _need(seq is not None or n <= table.shape[0], "without seq there is a table row for each token")
-        check(self.L.fvs_kv_append(_lib.stream_handle(), self._ref, ty, *ka, *va, *qa, hq, qo, *self._table(table),
+        if pairs not in _lib.PAIRS:
+            raise ValueError(f"pairs {pairs!r}: one of {sorted(_lib.PAIRS)}")
+        if seq is None and n > table.shape[0]:
+            raise ValueError("without seq there is a table row for each token")
+        check(self.L.fvs_kv_append(self._stream(), self._ref, ty, *ka, *va, *qa, hq, qo, *self._table(table),
                                    self._ints(seq, n, "seq"), self._ints(idx, n, "idx"), self._ints(pos, n, "pos"), n,
                                    cos, sin, positions, rot, _lib.PAIRS[pairs]), "kv_append")
         self.launches += 1
@@ -153,12 +169,14 @@ class PagedKV:
         """The stored rows of tokens idx [n] of sequences seq [n] (default: token i is sequence i's) as (k, v), each
         [n, heads, dim] of `dtype` (fp16, bf16 or fp32; default the cache's, fp32 for int8 codes); zeros for a hole."""
         n = idx.shape[0]
-        dtype = dtype or (torch.float32 if self.dtype == torch.int8 else self.dtype)
-        _need(dtype in (torch.float16, torch.bfloat16, torch.float32), f"read as {dtype}: fp16, bf16 or fp32")
-        _need(seq is not None or n <= table.shape[0], "without seq there is a table row for each token")
-        k = torch.empty(n, self.heads, self.dim, dtype=dtype, device=self.device)
-        v = torch.empty(n, self.heads, self.dim, dtype=dtype, device=self.device)
-        check(self.L.fvs_kv_read(_lib.stream_handle(), self._ref, _CODE[dtype], k.data_ptr(), v.data_ptr(),
+        dtype = dtype or (torch.float32 if self.dtype is torch.int8 else self.dtype)
+        if dtype not in _READ:
+            raise ValueError(f"read as {dtype}: fp16, bf16 or fp32")
+        if seq is None and n > table.shape[0]:
+            raise ValueError("without seq there is a table row for each token")
+        k = torch.empty((n, self.heads, self.dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        check(self.L.fvs_kv_read(self._stream(), self._ref, _CODE[dtype], k.data_ptr(), v.data_ptr(),
                                  *self._table(table), self._ints(seq, n, "seq"), self._ints(idx, n, "idx"), n), "kv_read")
         self.launches += 1
         return k, v
@@ -172,25 +190,26 @@ class PagedKV:
         ty = self._type(q.dtype, "q")
         qa = self._heads(q, n, "q")
         hq = q.shape[1]
-        _need(hq >= 1 and hq % self.heads == 0, f"{hq} query heads over {self.heads} key heads")
-        _need(table.shape[0] == n, f"the page table has {table.shape[0]} rows for {n} sequences")
+        if hq < 1 or hq % self.heads:
+            raise ValueError(f"{hq} query heads over {self.heads} key heads")
+        ta = self._table(table)
+        if ta[1] != n:
+            raise ValueError(f"the page table has {ta[1]} rows for {n} sequences")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        else:
-            _need(out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous() and out.device == q.device,
-                  "out is a contiguous tensor like q")
         if lse is None:
-            lse = torch.empty(n, hq, device=q.device)
-        else:
-            _need(lse.dtype == torch.float32 and lse.shape == (n, hq) and lse.is_contiguous()
-                  and lse.device == q.device, "lse is a contiguous fp32 [sequences, query heads]")
+            lse = torch.empty((n, hq), device=q.device)
+        elif not (lse.dtype is torch.float32 and lse.shape == (n, hq) and lse.is_contiguous()
+                  and lse.device == self.device):
+            raise ValueError("lse is a contiguous fp32 [sequences, query heads]")
+        oa, la = self._like(out, q, "out"), self._ints(lens, n, "lens")
         if n == 0:
             return out, lse
-        stream = _lib.stream_handle()
-        work, arrived = self._workspace(stream.value, n * hq)
-        check(self.L.fvs_kv_attend(stream, self._ref, ty, *qa, hq, *self._table(table), self._ints(lens, n, "lens"),
-                                   1.0 / math.sqrt(self.dim) if scale is None else scale, out.data_ptr(),
-                                   lse.data_ptr(), work, arrived), "kv_attend")
+        stream = self._stream()
+        work, arrived = self._workspace(stream, n * hq)
+        check(self.L.fvs_kv_attend(stream, self._ref, ty, *qa, hq, *ta, la,
+                                   self.scale if scale is None else scale, oa, lse.data_ptr(), work, arrived),
+              "kv_attend")
         self.launches += 1
         return out, lse
 
