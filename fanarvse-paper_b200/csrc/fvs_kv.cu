@@ -2,18 +2,20 @@
 // passages behind these ids have keys and values in pages).
 //
 // fvs_kv_append: rotates the query and key heads of new tokens by their positions and stores keys and values at their
-// places.  fvs_kv_read: copies rows out as floating point.  Both move every byte once and are bound by memory.  A warp
-// works for one token: its place and its cosines are looked up once, then it takes the token's heads (of q, k and v in
-// turn) a few at a time with the next heads' loads in flight.  A head of D elements is D / 16 lanes' (append: in a group of
-// 4, 8 or 16; each lane holds two chunks of 8 elements, those that a rotation by halves pairs) or D / 8 lanes' (read).
-// With few tokens a token's heads are spread over several warps.
+// places.  fvs_kv_read: copies rows out as floating point.  Both move every byte once and are bound by memory, so what
+// counts is bytes on the way: a warp loads up to 16 heads of one token's q, k or v (append: under way while the token's
+// place and its cosines are looked up) or the rows of several tokens (read: their places looked up side by side), then
+// stores them and ends; nothing is done one after another.  A head of D elements is D / 16 lanes' (append: in a group of 4,
+// 8 or 16; each lane holds two chunks of 8 elements, those that a rotation by halves pairs) or a lane's per 16 bytes (read).
 #include "fvs_kv.cuh"
 
 namespace fvs {
 namespace kv {
 
 constexpr int THREADS = 256;
-constexpr int BATCH = 4;  // heads of a lane whose loads are in flight together
+// loads of a lane that are on the way together: append takes 35 us with two at 9000 tokens of 48 heads of 64 (39 with one
+// or four: a lane's work after them, or its registers, grow), read 23 us with four at 31000 tokens of 8 int8 rows of 96 (25)
+constexpr int BATCH = 2, READ_BATCH = 4;
 
 struct Heads {  // token and head strides in elements
     const void* at;
@@ -28,7 +30,7 @@ struct AppendArgs {
     const int32_t *seq, *idx, *pos;
     const float *cos, *sin;
     int hq, tokens, positions, rot;
-    int spread;  // warps of a token
+    int q_warps, k_warps;  // of a token for q and for k (as many for v)
 };
 
 // lanes of a head of D elements
@@ -46,26 +48,40 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
     a = x;
 }
 
+// four values as rounded int8 (half to even; at most 127 in magnitude here, 0 for a not-a-number)
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(r) : "r"(__float2int_rn(d)), "r"(__float2int_rn(c)));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(__float2int_rn(b)), "r"(__float2int_rn(a)), "r"(r));
+    return r;
+}
+
+// the larger magnitude; not-a-numbers stay
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+
 // TYPE: of the new rows; STORE: of the cache (TYPE or int8); HALVES: pairs (i, i + rot/2), else neighbours (2i, 2i + 1)
 template <int D, int TYPE, int STORE, bool HALVES>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     using T = typename Elem<TYPE>::T;
     constexpr int L = Lanes<D>::group, AT_ONCE = 32 / L;
-    const unsigned w = blockIdx.x * (THREADS / 32) + threadIdx.x / 32;
-    const int token = (int)(w / (unsigned)a.spread);
+    const unsigned w = blockIdx.x * (THREADS / 32) + threadIdx.x / 32, warps = a.q_warps + 2 * a.k_warps;
+    const int token = (int)(w / warps);
     if (token >= a.tokens) return;
     const int lane = threadIdx.x & 31, j = lane % L, sub = lane / L;
-    const int rows = a.hq + 2 * a.c.heads;
-    // this warp's heads
-    const int per = ((rows + a.spread - 1) / a.spread + AT_ONCE - 1) / AT_ONCE * AT_ONCE;
-    const int begin = (int)(w % (unsigned)a.spread) * per, end = min(rows, begin + per);
-    int page = 0, slot = 0;
-    const int t = __ldg(a.idx + token), pos = a.pos ? __ldg(a.pos + token) : t;
-    bool there = place(a.c, a.tb, a.seq ? __ldg(a.seq + token) : token, t, page, slot);
-    if (there && a.rot && (unsigned)pos >= (unsigned)a.positions) {
-        atomicOr(a.c.status, BAD_INDEX);
-        there = false;
-    }
+    // this warp's heads of q, k or v
+    int part = (int)(w % warps);
+    const bool is_q = part < a.q_warps;
+    if (!is_q) part -= a.q_warps;
+    const bool is_k = !is_q && part < a.k_warps;
+    if (!is_q && !is_k) part -= a.k_warps;
+    const Heads src = is_q ? a.q : is_k ? a.k : a.v;
+    const int heads = is_q ? a.hq : a.c.heads, share = is_q ? a.q_warps : a.k_warps;
+    const int per = ((heads + share - 1) / share + AT_ONCE - 1) / AT_ONCE * AT_ONCE;
+    const int head0 = part * per + sub, end = min(heads, part * per + per), count = end - part * per;
     // the lane's two chunks, of neighbouring lanes side by side in memory
     int e0, e1;
     bool turn0, turn1;
@@ -81,94 +97,87 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
         turn1 = e1 < a.rot;
     }
     const bool used = j < Lanes<D>::used;
-    float c[8], s[8];
+    uint4 raw[BATCH][2];
+    const T* from = (const T*)src.at + token * src.token + head0 * src.head;
 #pragma unroll
-    for (int n = 0; n < 8; n++) c[n] = 1.f, s[n] = 0.f;
-    if (there && used && (turn0 || turn1)) {
+    for (int u = 0; u < BATCH; u++) {
+        raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+        if (u * AT_ONCE < count && used && head0 + u * AT_ONCE < end) {
+            raw[u][0] = *(const uint4*)(from + e0);
+            raw[u][1] = *(const uint4*)(from + e1);
+        }
+        from += AT_ONCE * src.head;
+    }
+    int page = 0, slot = 0;
+    const int t = __ldg(a.idx + token), pos = a.pos ? __ldg(a.pos + token) : t;
+    bool there = place(a.c, a.tb, a.seq ? __ldg(a.seq + token) : token, t, page, slot);
+    if (there && a.rot && (unsigned)pos >= (unsigned)a.positions) {
+        atomicOr(a.c.status, BAD_INDEX);
+        there = false;
+    }
+    float c[8], s[8];
+    const bool turns = (is_q || is_k) && there && used && (turn0 || turn1);
+    if (turns) {
         const float *pc = a.cos + (int64_t)pos * (a.rot / 2), *ps = a.sin + (int64_t)pos * (a.rot / 2);
-        const int o0 = HALVES ? e0 : e0 / 2, o1 = HALVES ? e0 + 4 : e1 / 2;
+        const int o0 = HALVES ? e0 : e0 / 2, o1 = HALVES ? e0 + 4 : turn1 ? e1 / 2 : o0;
         *(float4*)c = __ldg((const float4*)(pc + o0));
         *(float4*)s = __ldg((const float4*)(ps + o0));
-        if (HALVES || turn1) {
-            *(float4*)(c + 4) = __ldg((const float4*)(pc + o1));
-            *(float4*)(s + 4) = __ldg((const float4*)(ps + o1));
-        }
+        *(float4*)(c + 4) = __ldg((const float4*)(pc + o1));
+        *(float4*)(s + 4) = __ldg((const float4*)(ps + o1));
     }
-    const int64_t to = page * a.c.page_stride + slot * a.c.slot_stride;
-    const int64_t to_scale = page * a.c.scale_page_stride + slot * a.c.scale_slot_stride;
-    for (int row0 = begin; row0 < end; row0 += AT_ONCE * BATCH) {
-        uint4 raw[BATCH][2];
+    if (!there && !is_q) return;  // a whole warp
+    const int64_t to_scale = page * a.c.scale_page_stride + slot * a.c.scale_slot_stride + head0 * a.c.scale_head_stride;
+    const int64_t to = is_q ? ((int64_t)token * a.hq + head0) * D
+                            : page * a.c.page_stride + slot * a.c.slot_stride + head0 * a.c.head_stride;
+    const int64_t step = is_q ? AT_ONCE * D : AT_ONCE * a.c.head_stride;
+    void* dst = is_q ? a.q_out : is_k ? a.c.k : a.c.v;
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int row = row0 + u * AT_ONCE + sub;
-            raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
-            if (there && used && row < end) {
-                const bool is_q = row < a.hq, is_k = row < a.hq + a.c.heads;
-                const Heads& src = is_q ? a.q : is_k ? a.k : a.v;
-                const int head = is_q ? row : is_k ? row - a.hq : row - a.hq - a.c.heads;
-                const T* p = (const T*)src.at + token * src.token + head * src.head;
-                raw[u][0] = *(const uint4*)(p + e0);
-                raw[u][1] = *(const uint4*)(p + e1);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int row = row0 + u * AT_ONCE + sub;
-            const bool is_q = row < a.hq, is_k = !is_q && row < a.hq + a.c.heads;
-            const int head = is_q ? row : is_k ? row - a.hq : row - a.hq - a.c.heads;
-            float x0[8], x1[8];
+    for (int u = 0; u < BATCH; u++) {
+        if (u * AT_ONCE >= count) break;  // a whole warp
+        const bool live = used && head0 + u * AT_ONCE < end;
+        const bool codes = STORE == FVS_I8 && !is_q;
+        float x0[8], x1[8];
+        if (turns || codes) {
             up8<TYPE>(raw[u][0], x0);
             up8<TYPE>(raw[u][1], x1);
-            if (is_q || is_k) {
-                if (HALVES) {
-                    if (turn0) {
+        }
+        if (turns) {
+            if (HALVES) {
 #pragma unroll
-                        for (int n = 0; n < 8; n++) turn(x0[n], x1[n], c[n], s[n]);
-                    }
-                } else {
+                for (int n = 0; n < 8; n++) turn(x0[n], x1[n], c[n], s[n]);
+            } else {
 #pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        if (turn0) turn(x0[2 * n], x0[2 * n + 1], c[n], s[n]);
-                        if (turn1) turn(x1[2 * n], x1[2 * n + 1], c[4 + n], s[4 + n]);
-                    }
+                for (int n = 0; n < 4; n++) {
+                    turn(x0[2 * n], x0[2 * n + 1], c[n], s[n]);
+                    if (turn1) turn(x1[2 * n], x1[2 * n + 1], c[4 + n], s[4 + n]);
                 }
             }
-            if (STORE == FVS_I8) {
-                // the row's largest magnitude as ordered bits: a not-a-number is larger than infinity, so it is not lost
-                uint32_t top = 0;
+        }
+        if (codes) {
+            float m = 0.f;
 #pragma unroll
-                for (int n = 0; n < 8; n++)
-                    top = max(top, max(__float_as_uint(x0[n]) & 0x7fffffffu, __float_as_uint(x1[n]) & 0x7fffffffu));
+            for (int n = 0; n < 8; n++) m = max_abs(m, max_abs(x0[n], x1[n]));
 #pragma unroll
-                for (int o = L / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                if (!is_q) {
-                    if (!there || !used || row >= end) continue;
-                    const float m = __uint_as_float(top);
-                    const float inv = m > 0.f ? fminf(__fmul_rn(__frcp_rn(m), 127.f), 3.402823466e38f) : 0.f;
-                    uint32_t code[4];
+            for (int o = L / 2; o; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (!live) continue;
+            // no reciprocal of a subnormal: it would be infinite
+            const float inv = m > 0.f ? fminf(__fmul_rn(__frcp_rn(m), 127.f), 3.402823466e38f) : 0.f;
+            uint32_t code[4];
 #pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        const float* x = n < 2 ? x0 : x1;
-                        code[n] = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int y = max(-127, min(127, __float2int_rn(__fmul_rn(x[(n & 1) * 4 + i], inv))));
-                            code[n] |= (uint32_t)(y & 0xff) << (8 * i);
-                        }
-                    }
-                    int8_t* p = (int8_t*)(is_k ? a.c.k : a.c.v) + to + head * a.c.head_stride;
-                    *(uint2*)(p + e0) = make_uint2(code[0], code[1]);
-                    *(uint2*)(p + e1) = make_uint2(code[2], code[3]);
-                    if (j == 0)
-                        (is_k ? a.c.k_scale : a.c.v_scale)[to_scale + head * a.c.scale_head_stride] = __fmul_rn(m, 1.f / 127.f);
-                    continue;
-                }
+            for (int n = 0; n < 4; n++) {
+                const float* x = (n < 2 ? x0 : x1) + (n & 1) * 4;
+                code[n] = codes4(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv), __fmul_rn(x[2], inv), __fmul_rn(x[3], inv));
             }
-            if (!used || row >= end || (!is_q && !there)) continue;
-            T* p = is_q ? (T*)a.q_out + ((int64_t)token * a.hq + head) * D  // zeros where the token has no place
-                        : (T*)(is_k ? a.c.k : a.c.v) + to + head * a.c.head_stride;
-            *(uint4*)(p + e0) = down8<TYPE>(x0);
-            *(uint4*)(p + e1) = down8<TYPE>(x1);
+            int8_t* p = (int8_t*)dst + to + u * step;
+            *(uint2*)(p + e0) = make_uint2(code[0], code[1]);
+            *(uint2*)(p + e1) = make_uint2(code[2], code[3]);
+            if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[to_scale + u * AT_ONCE * a.c.scale_head_stride] = __fmul_rn(m, 1.f / 127.f);
+        } else if (live) {
+            if (turns) raw[u][0] = down8<TYPE>(x0), raw[u][1] = down8<TYPE>(x1);
+            if (!there) raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);  // a query without a place
+            T* p = (T*)dst + to + u * step;
+            *(uint4*)(p + e0) = raw[u][0];
+            *(uint4*)(p + e1) = raw[u][1];
         }
     }
 }
@@ -178,76 +187,85 @@ struct ReadArgs {
     Table tb;
     void *k, *v;
     const int32_t *seq, *idx;
-    int tokens, spread;
+    int tokens, per;  // tokens of a warp, at most 32
+    int spread;       // warps that share a token's rows
+    float inv_rows;
 };
 
-// rows of the cache as TYPE, zeros where a token has no place: a lane moves 8 elements of a row
+// rows of the cache as TYPE, zeros where a token has no place: a lane moves 16 bytes of a row.  A warp's lanes look up
+// the places of its tokens side by side; then all their rows are on the way together.
 template <int D, int STORE, int TYPE>
 __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
-    constexpr int L = D / 8, AT_ONCE = 32 / L, ESZ = STORE == FVS_I8 ? 1 : 2;
+    constexpr int EL = STORE == FVS_I8 ? 16 : 8, L = D / EL, AT_ONCE = 32 / L, ESZ = 16 / EL;
     const unsigned w = blockIdx.x * (THREADS / 32) + threadIdx.x / 32;
-    const int token = (int)(w / (unsigned)a.spread);
-    if (token >= a.tokens) return;
-    const int lane = threadIdx.x & 31, e = lane % L * 8, sub = lane / L;
+    const int first = (int)(w / (unsigned)a.spread * (unsigned)a.per);
+    if (first >= a.tokens) return;
+    const int n = min(a.per, a.tokens - first);
+    const int lane = threadIdx.x & 31, e = lane % L * EL, sub = lane / L;
     const int rows = 2 * a.c.heads;
-    const int per = ((rows + a.spread - 1) / a.spread + AT_ONCE - 1) / AT_ONCE * AT_ONCE;
-    const int begin = (int)(w % (unsigned)a.spread) * per, end = min(rows, begin + per);
     int page = 0, slot = 0;
-    const bool there = place(a.c, a.tb, a.seq ? __ldg(a.seq + token) : token, __ldg(a.idx + token), page, slot);
-    const int64_t from = page * a.c.page_stride + slot * a.c.slot_stride + e;
-    const int64_t from_scale = page * a.c.scale_page_stride + slot * a.c.scale_slot_stride;
-    for (int row0 = begin; row0 < end; row0 += AT_ONCE * BATCH) {
-        uint4 raw[BATCH];
-        float scale[BATCH];
+    bool there = false;
+    if (lane < n) there = place(a.c, a.tb, a.seq ? __ldg(a.seq + first + lane) : first + lane, __ldg(a.idx + first + lane), page, slot);
+    if (!there) page = -1;
+    // i / rows; exact while a warp has several tokens, of fewer than 2 * 32 * READ_BATCH rows then
+    auto token_of = [&](int i) { return n == 1 ? 0 : (int)(((float)i + 0.5f) * a.inv_rows); };
+    for (int i0 = (int)(w % (unsigned)a.spread) * AT_ONCE * READ_BATCH; i0 < n * rows; i0 += a.spread * AT_ONCE * READ_BATCH) {
+        uint4 raw[READ_BATCH];
+        float scale[READ_BATCH];
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int row = row0 + u * AT_ONCE + sub;
+        for (int u = 0; u < READ_BATCH; u++) {
+            const int i = i0 + u * AT_ONCE + sub, t = min(token_of(i), n - 1), row = i - t * rows;
             const bool is_k = row < a.c.heads;
             const int head = is_k ? row : row - a.c.heads;
+            const int pg = __shfl_sync(0xffffffffu, page, t), sl = __shfl_sync(0xffffffffu, slot, t);
             raw[u] = make_uint4(0, 0, 0, 0);
             scale[u] = 0.f;
-            if (there && sub < AT_ONCE && row < end) {
-                const uint8_t* p = (const uint8_t*)(is_k ? a.c.k : a.c.v) + (from + head * a.c.head_stride) * ESZ;
-                if (STORE == FVS_I8) {
-                    *(uint2*)&raw[u] = __ldg((const uint2*)p);
-                    scale[u] = __ldg((is_k ? a.c.k_scale : a.c.v_scale) + from_scale + head * a.c.scale_head_stride);
-                } else {
-                    raw[u] = __ldg((const uint4*)p);
-                }
+            if (pg >= 0 && sub < AT_ONCE && i < n * rows) {
+                const uint8_t* p = (const uint8_t*)(is_k ? a.c.k : a.c.v) +
+                                   ((int64_t)pg * a.c.page_stride + (int64_t)head * a.c.head_stride + (int64_t)sl * a.c.slot_stride + e) * ESZ;
+                raw[u] = __ldg((const uint4*)p);
+                if (STORE == FVS_I8)
+                    scale[u] = __ldg((is_k ? a.c.k_scale : a.c.v_scale) + (int64_t)pg * a.c.scale_page_stride +
+                                     (int64_t)head * a.c.scale_head_stride + (int64_t)sl * a.c.scale_slot_stride);
             }
         }
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int row = row0 + u * AT_ONCE + sub;
-            if (sub >= AT_ONCE || row >= end) continue;
+        for (int u = 0; u < READ_BATCH; u++) {
+            const int i = i0 + u * AT_ONCE + sub, t = token_of(i), row = i - t * rows;
+            if (sub >= AT_ONCE || i >= n * rows) continue;
             const bool is_k = row < a.c.heads;
-            const int head = is_k ? row : row - a.c.heads;
-            const int64_t o = ((int64_t)token * a.c.heads + head) * D + e;
+            const int64_t o = ((int64_t)(first + t) * a.c.heads + (is_k ? row : row - a.c.heads)) * D + e;
             void* out = is_k ? a.k : a.v;
-            float x[8];
-            if (STORE == FVS_I8) {
-                const uint32_t word[2] = {raw[u].x, raw[u].y};
-#pragma unroll
-                for (int n = 0; n < 8; n++) x[n] = there ? __fmul_rn((float)(int8_t)(word[n / 4] >> (8 * (n % 4))), scale[u]) : 0.f;
-            } else {
-                up8<STORE == FVS_I8 ? FVS_F16 : STORE>(raw[u], x);
+            if (TYPE == STORE) {
+                *(uint4*)((uint16_t*)out + o) = raw[u];
+                continue;
             }
-            if (TYPE == FVS_F32) {
-                *(float4*)((float*)out + o) = make_float4(x[0], x[1], x[2], x[3]);
-                *(float4*)((float*)out + o + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            } else {
-                *(uint4*)((uint16_t*)out + o) = TYPE == STORE ? raw[u] : down8<TYPE == FVS_F32 ? FVS_F16 : TYPE>(x);
+            const uint32_t word[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int m0 = 0; m0 < EL; m0 += 8) {
+                float x[8];
+#pragma unroll
+                for (int m = 0; m < 8; m += 2) {
+                    if (STORE == FVS_I8) {
+                        // the byte code + 128 in the mantissa of 2^23
+                        const uint32_t u4 = word[(m0 + m) / 4] ^ 0x80808080u;
+                        x[m] = __fmul_rn(__uint_as_float(__byte_perm(u4, 0x4b000000u, 0x7440 + m % 4)) - 8388736.f, scale[u]);
+                        x[m + 1] = __fmul_rn(__uint_as_float(__byte_perm(u4, 0x4b000000u, 0x7441 + m % 4)) - 8388736.f, scale[u]);
+                    } else {
+                        const float2 two = Elem<STORE == FVS_I8 ? FVS_F16 : STORE>::up(word[m / 2]);
+                        x[m] = two.x, x[m + 1] = two.y;
+                    }
+                }
+                if (TYPE == FVS_F32) {
+                    *(float4*)((float*)out + o + m0) = make_float4(x[0], x[1], x[2], x[3]);
+                    *(float4*)((float*)out + o + m0 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                } else {
+                    *(uint4*)((uint16_t*)out + o + m0) = down8<TYPE == FVS_F32 ? FVS_F16 : TYPE>(x);
+                }
             }
         }
     }
 }
-
-// warps of a token: one, more where that would leave SMs without work (`at_once`: heads that a warp takes at a time)
-static int spread_of(int tokens, int rows, int at_once) {
-    const int want = (32 * fvs_sm_count() + tokens - 1) / tokens, most = (rows + at_once - 1) / at_once;
-    return want < 1 ? 1 : want < most ? want : most;
-}
-static unsigned grid_of(int tokens, int spread) { return (unsigned)(((int64_t)tokens * spread + THREADS / 32 - 1) / (THREADS / 32)); }
 
 static bool heads_ok(const void* p, int64_t token, int64_t head, int d) {
     return p && ((uintptr_t)p & 15) == 0 && token % 8 == 0 && head % 8 == 0 && token >= 0 && (head >= d || head == 0);
@@ -255,8 +273,11 @@ static bool heads_ok(const void* p, int64_t token, int64_t head, int d) {
 
 template <int D>
 static void launch_append(fvs_stream_t stream, AppendArgs a, int type, bool halves) {
-    a.spread = spread_of(a.tokens, a.hq + 2 * a.c.heads, 32 / Lanes<D>::group);
-    const unsigned grid = grid_of(a.tokens, a.spread);
+    constexpr int most = 32 / Lanes<D>::group * BATCH;  // heads of a warp
+    a.q_warps = (a.hq + most - 1) / most;
+    a.k_warps = (a.c.heads + most - 1) / most;
+    const int64_t warps = (int64_t)a.tokens * (a.q_warps + 2 * a.k_warps);
+    const unsigned grid = (unsigned)((warps + THREADS / 32 - 1) / (THREADS / 32));
     const bool i8 = a.c.type == FVS_I8;
     if (type == FVS_F16) {
         if (i8)
@@ -277,8 +298,13 @@ static void launch_append(fvs_stream_t stream, AppendArgs a, int type, bool halv
 
 template <int D, int STORE>
 static void launch_read(fvs_stream_t stream, ReadArgs a, int type) {
-    a.spread = spread_of(a.tokens, 2 * a.c.heads, 32 / (D / 8));
-    const unsigned grid = grid_of(a.tokens, a.spread);
+    // as many tokens as a warp has on the way at once (more of them per warp, one after another, took half as long again)
+    const int at_once = 32 / (D / (STORE == FVS_I8 ? 16 : 8)) * READ_BATCH, per = at_once / (2 * a.c.heads);
+    a.per = per < 1 ? 1 : per < 32 ? per : 32;
+    a.spread = per < 1 ? (2 * a.c.heads + at_once - 1) / at_once : 1;
+    a.inv_rows = 1.f / (2 * a.c.heads);
+    const int64_t warps = (int64_t)((a.tokens + a.per - 1) / a.per) * a.spread;
+    const unsigned grid = (unsigned)((warps + THREADS / 32 - 1) / (THREADS / 32));
     if (type == FVS_F16)
         read_kernel<D, STORE, FVS_F16><<<grid, THREADS, 0, stream>>>(a);
     else if (type == FVS_BF16)
@@ -312,7 +338,7 @@ extern "C" int fvs_kv_append(fvs_stream_t stream, const fvs_kv_cache* cache, int
                       (((uintptr_t)cos | (uintptr_t)sin) & 15) == 0);
     if ((int64_t)tokens * (hq + 2 * (int64_t)cache->heads) > 0x7fffff00ll) return FVS_ERANGE;
     AppendArgs a{*cache, {table, table_stride, seqs, wide}, {k, k_token, k_head}, {v, v_token, v_head},
-                 {q, q_token, q_head}, q_out, seq, idx, pos, cos, sin, hq, tokens, positions, rot, 1};
+                 {q, q_token, q_head}, q_out, seq, idx, pos, cos, sin, hq, tokens, positions, rot, 0, 0};
     const bool halves = pairs == FVS_PAIRS_HALVES;
     switch (cache->dim) {
         case 64: launch_append<64>(stream, a, type, halves); break;
@@ -334,7 +360,7 @@ extern "C" int fvs_kv_read(fvs_stream_t stream, const fvs_kv_cache* cache, int t
     if (int rc = check_table(table, seqs, wide, table_stride)) return rc;
     FVS_CHECK_ARG(idx && (seq || tokens <= seqs) && k && v && (((uintptr_t)k | (uintptr_t)v) & 15) == 0);
     if ((int64_t)tokens * 2 * cache->heads > 0x7fffff00ll) return FVS_ERANGE;
-    ReadArgs a{*cache, {table, table_stride, seqs, wide}, k, v, seq, idx, tokens, 1};
+    ReadArgs a{*cache, {table, table_stride, seqs, wide}, k, v, seq, idx, tokens, 1, 1, 0.f};
 #define FVS_KV_READ(D)                                                                     \
     (cache->type == FVS_I8    ? launch_read<D, FVS_I8>(stream, a, type)                    \
      : cache->type == FVS_F16 ? launch_read<D, FVS_F16>(stream, a, type)                   \
