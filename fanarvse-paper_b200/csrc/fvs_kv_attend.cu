@@ -28,6 +28,7 @@
 // over int8 codes are brought to fp16 by a power of two for each head.
 #include <limits.h>
 
+
 #include "fvs_kv.cuh"
 
 namespace fvs {
@@ -41,7 +42,8 @@ struct AttendArgs {
     const int32_t* lens;
     void* out;
     float* lse;
-    int32_t* arrived;  // [items], then the next piece of work and the CTAs that are done; zero between calls
+    int32_t* counts;   // the next piece of work, the CTAs that are done; zero between calls
+    unsigned long long* arrived;  // [items] parts that are there, 16 bits for each of a CTA's warps; zero between calls
     float* parts;
     int hq, group;     // query heads, query heads of a key head
     int split;         // items of a key head
@@ -88,6 +90,8 @@ struct Shape {
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
     static constexpr int S = FIT > 4 ? 4 : FIT;      // ring stages
     static_assert(S >= 2, "ring");
+    static constexpr int TAKEN = 8;  // more items than a warp has on the way: units in the ring, lookups, one in reserve
+    static_assert(S + 4 <= TAKEN, "taken");
     static constexpr int RING = S * STAGE;           // bytes per warp
     static constexpr int SMEM = WARPS * RING + FIXED;
     static constexpr int PART = ROWS * (D + 2);      // floats of a partial result
@@ -216,12 +220,113 @@ struct Cuts {
     __device__ __forceinline__ int64_t taken(int n) const { return (int64_t)(n / (runs - 1)) * runs + 1 + n % (runs - 1); }
 };
 
+__device__ __forceinline__ float log_sum(float mx, float sum) {
+    return sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+}
+// An item of which a piece holds a part.
+struct CutItem {
+    int b, head, sub, t_lo, parts;
+};
+// Joins an item's parts: rows warp, warp + 4, ... (R of them at most) of `rows`.  Lane t holds the weights of parts t and t +
+// 32, then four elements of the sums.  Loads that wait for the memory of a busy GPU cost 2000 cycles and more each time, so
+// all weights are one wait and WAYS rows of parts another.
+template <int D, int TYPE, int ROWS, int R, int WAYS>
+__device__ __forceinline__ void join_parts(const float* from, int parts, int warp, int rows, uint16_t* out, float* lse) {
+    const int lane = threadIdx.x & 31;
+    constexpr int Q4 = D / 4, PART = ROWS * (D + 2), Q = (Q4 + 31) / 32, WK = 2, BATCH = WAYS / Q / R > 0 ? WAYS / Q / R : 1;
+    auto part_at = [&](int t) { return from + (2 * t + (t == 0)) * PART; };
+    float mx[R], sum[R];
+    float4 acc[R][Q];
+#pragma unroll
+    for (int w = 0; w < R; w++) {
+        mx[w] = -INFINITY, sum[w] = 0.f;
+#pragma unroll
+        for (int i = 0; i < Q; i++) acc[w][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    auto row_of = [&](int w) { return min(warp + w * WARPS, rows - 1); };
+    for (int t0 = 0; t0 < parts; t0 += 32 * WK) {
+        float2 ml[R][WK];
+#pragma unroll
+        for (int w = 0; w < R; w++)
+#pragma unroll
+            for (int k = 0; k < WK; k++) {
+                const int t = t0 + 32 * k + lane;
+                ml[w][k] = t < parts ? __ldcg((const float2*)(part_at(t) + ROWS * D + 2 * row_of(w))) : make_float2(-INFINITY, 0.f);
+            }
+#pragma unroll
+        for (int w = 0; w < R; w++) {
+            float top = mx[w];
+#pragma unroll
+            for (int k = 0; k < WK; k++) top = fmaxf(top, ml[w][k].x);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float f = weight(make_float2(mx[w], sum[w]), top);  // of what the parts before added up to
+            mx[w] = top;
+            if (f != 1.f) {
+                sum[w] *= f;
+#pragma unroll
+                for (int i = 0; i < Q; i++) acc[w][i].x *= f, acc[w][i].y *= f, acc[w][i].z *= f, acc[w][i].w *= f;
+            }
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < WK; k++) {
+                const float f1 = weight(ml[w][k], top);
+                s += ml[w][k].y * f1;
+                ml[w][k].x = f1;
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+            sum[w] += s;
+        }
+#pragma unroll
+        for (int k = 0; k < WK; k++) {
+            const int n = min(32, parts - t0 - 32 * k);
+            for (int j0 = 0; j0 < n; j0 += BATCH) {
+                float4 x[BATCH][R][Q];
+#pragma unroll
+                for (int j = 0; j < BATCH; j++) {
+                    const float* p = part_at(t0 + 32 * k + min(j0 + j, n - 1));
+#pragma unroll
+                    for (int w = 0; w < R; w++)
+#pragma unroll
+                        for (int i = 0; i < Q; i++)
+                            if (i * 32 + lane < Q4) x[j][w][i] = __ldcg((const float4*)(p + row_of(w) * D) + i * 32 + lane);
+                }
+#pragma unroll
+                for (int j = 0; j < BATCH; j++)
+#pragma unroll
+                    for (int w = 0; w < R; w++) {
+                        const float f = __shfl_sync(0xffffffffu, ml[w][k].x, min(j0 + j, 31));
+                        if (j0 + j < n && f != 0.f)
+#pragma unroll
+                            for (int i = 0; i < Q; i++) {
+                                acc[w][i].x += x[j][w][i].x * f, acc[w][i].y += x[j][w][i].y * f;
+                                acc[w][i].z += x[j][w][i].z * f, acc[w][i].w += x[j][w][i].w * f;
+                            }
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int w = 0; w < R; w++) {
+        const int row = warp + w * WARPS;
+        if (row >= rows) break;
+        const float inv = sum[w] == 0.f ? 0.f : 1.f / sum[w];
+#pragma unroll
+        for (int i = 0; i < Q; i++)
+            if (i * 32 + lane < Q4)
+                *((uint2*)(out + row * D) + i * 32 + lane) = make_uint2(Elem<TYPE>::down(acc[w][i].x * inv, acc[w][i].y * inv),
+                                                                        Elem<TYPE>::down(acc[w][i].z * inv, acc[w][i].w * inv));
+        if (lse && lane == 0) lse[row] = log_sum(mx[w], sum[w]);
+    }
+}
+
 template <int D, int TYPE, int STORE, int NT>
 __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_kernel(AttendArgs a) {
     using Sh = Shape<D, STORE, NT>;
     constexpr bool I8 = Sh::I8;
     constexpr int MT = I8 ? FVS_F16 : TYPE;  // type of the matrix instructions' operands
-    constexpr int S = Sh::S, UNIT = Sh::UNIT, TILES = Sh::TILES;
+    constexpr int S = Sh::S, UNIT = Sh::UNIT, TILES = Sh::TILES, TAKEN = Sh::TAKEN;
     extern __shared__ __align__(128) uint8_t ring_all[];
     __shared__ int64_t s_sum[WARPS];
     __shared__ int s_none[WARPS];
@@ -229,7 +334,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     __shared__ Place s_place[2];           // where a piece begins and ends
     __shared__ int64_t s_base;             // cost before the first sequence of the piece
     __shared__ float s_ml[WARPS][Sh::ROWS][2];
-    __shared__ int s_tile[WARPS], s_last, s_next;
+    __shared__ int s_tile[WARPS], s_next;
+    __shared__ int s_short, s_taken[WARPS][TAKEN];
+    __shared__ CutItem s_cut[2];
     __shared__ Cuts s_cuts;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -293,7 +400,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     // ---- the pieces.  Unit u of an item that begins at cost x lies at x + ITEM_COST + u.  A cut nearer than `near` units
     // to an item's begin or end moves there: joining two parts costs more than that
     Cuts cuts;
-    cuts.share = max((int64_t)16, (total + gridDim.x - 1) / gridDim.x);
+    // a share holds 16 units or, if these are smaller, an item
+    const int64_t items = (int64_t)(B - none) * per_seq;
+    cuts.share = max(max((int64_t)1, min((int64_t)16, items ? total / items : 1)), (total + gridDim.x - 1) / gridDim.x);
     const bool shared = cuts.share >= V_SH;  // with less, setting up another piece costs more than it evens out
     if (shared) {
         cuts.small = (int)((cuts.share + 7) / 8);
@@ -307,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     if (tid == 0) s_cuts = cuts;
     const int near = max(8, cuts.small / 8);
     // items of up to so many units are one warp's; fewer than 2 near, so that none of them is cut
-    const int alone = Sh::Q_SMEM ? 0 : (int)min((int64_t)15, cuts.share / 8);
+    const int alone = Sh::Q_SMEM ? 0 : (int)min((int64_t)15, cuts.share / 4);
     uint8_t* ring = ring_all + warp * Sh::RING;
     const uint32_t ring_at = smem_addr(ring);
     const bool aligned = a.c.page % 16 == 0;  // a tile's keys lie in one page
@@ -318,7 +427,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     for (;; piece = s_cuts.taken(s_next)) {
     __syncthreads();
     if (s_cuts.at(piece) >= total) break;
-    if (tid == THREADS - 1 && shared) s_next = atomicAdd(a.arrived + (int64_t)B * per_seq, 1);
+    if (tid == THREADS - 1 && shared) s_next = atomicAdd(a.counts, 1);
+    if (tid == 0) s_short = 0;
     if (warp < 2) {
         const int64_t g = s_cuts.at(piece + warp);
         if (g >= total) {
@@ -381,14 +491,35 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     // the units that this warp copies: every fourth of an item, all of one that it has alone
     Item ahead = now;
     bool any = more;
-    auto owner = [&](const Item& it) { return ((it.b * a.c.heads + it.head) * split + it.sub) % WARPS; };
+    // The piece's short items are numbered as they come.  A warp takes the next number when it is through with the one it
+    // had, so that the warps come out even, and remembers it for the computation that follows.
+    int next = 0, number_ahead = 0, taken = 0;
+    bool own = false;
     auto settle = [&]() {
         while (any && ahead.u >= ahead.end) {
             any = next_item<UNIT>(a, ahead, stop);
-            if (any) ahead.u = ahead.n > alone ? warp : owner(ahead) == warp ? 0 : ahead.end;
+            if (own) {
+                own = false;
+                if (lane == 0) s_taken[warp][taken % TAKEN] = number_ahead = atomicAdd(&s_short, 1);
+                number_ahead = __shfl_sync(0xffffffffu, number_ahead, 0);
+                taken++;
+            }
+            if (any && ahead.n <= alone) {
+                own = next++ == number_ahead;
+                ahead.u = own ? 0 : ahead.end;
+            } else {
+                ahead.u += warp;
+            }
         }
     };
-    if (any) ahead.u = ahead.n > alone ? ahead.u + warp : owner(ahead) == warp ? 0 : ahead.end;
+    if (lane == 0) s_taken[warp][0] = number_ahead = atomicAdd(&s_short, 1);
+    number_ahead = __shfl_sync(0xffffffffu, number_ahead, 0);
+    taken = 1;
+    own = any && ahead.n <= alone && next++ == number_ahead;
+    if (any && ahead.n <= alone)
+        ahead.u = own ? 0 : ahead.end;
+    else
+        ahead.u += warp;
     settle();
 
     // ---- copies, two lookups ahead
@@ -508,7 +639,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     };
 
     // ---- the piece's items
-    int slot = 0;
+    int slot = 0, cut = 0, number = 0, done = 0;
+    __syncwarp();
 #pragma unroll 1
     for (; more;) {
         const bool solo = now.n <= alone;
@@ -518,7 +650,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         const int64_t it_begin = base * per_seq + (int64_t)(now.head * split + now.sub) * (now.n + ITEM_COST);
         more = next_item<UNIT>(a, now, stop);
         if (now.b != it.b) base += it.n + ITEM_COST;
-        if (solo && owner(it) != warp) continue;
+        if (solo) {
+            if (number++ != s_taken[warp][done % TAKEN]) continue;
+            done++;
+        }
 
         // q as the B operand: head r of each 8, elements of the order in which the keys' rows come
         uint32_t qf[Sh::Q_SMEM ? 1 : NT][Sh::Q_SMEM ? 1 : D / 16][2];
@@ -780,7 +915,6 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         if (lane == 0) s_tile[warp] = (int)((uint8_t*)tile - ring_all);
         if (!solo) __syncthreads();
         const float vup = I8 ? __uint_as_float((uint32_t)(vexp + 1) << 23) * 0x1p24f : 1.f;
-        auto log_sum = [](float mx, float sum) { return sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f; };
 #pragma unroll
         for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -844,100 +978,50 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             else
                 *(float4*)(part + row * D + d) = acc;
         }
-        if (!whole) {
-            __threadfence();
-            __syncthreads();
-            // the cuts inside the item: parts - 1 of them, the first at cut t_lo
+        __syncthreads();  // the part is written, and the tiles' slots may be filled again
+        if (whole) continue;
+        // its place among the parts: the cuts inside the item are parts - 1, the first at cut t_lo
+        if (tid == 0) {
             const int t_lo = s_cuts.from(it_begin + ITEM_COST + near);
-            const int parts = s_cuts.upto(it_begin + ITEM_COST + it.n - near) - t_lo + 2;
-            if (tid == 0) {
-                const int64_t item = (int64_t)it.b * per_seq + it.head * split + it.sub;
-                s_last = atomicAdd(a.arrived + item, 1) == parts - 1;
-                if (s_last) a.arrived[item] = 0;
-            }
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                // a warp takes a row; lane t holds the weights of parts t + 32 k, then four elements of the sum.  Loads that
-                // wait for the memory of a busy GPU cost 2000 cycles and more each time: all the weights in one wait, then
-                // 16 parts at a time
-                constexpr int Q = (Q4 + 31) / 32, WK = 4, BATCH = 16 / Q;
-                const float* from = a.parts + (int64_t)2 * (t_lo - 1) * Sh::PART;
-                auto part_at = [&](int t) { return from + (2 * t + (t == 0)) * Sh::PART; };
-                for (int row = warp; row < rows; row += WARPS) {
-                    float mx = -INFINITY, sum = 0.f;
-                    float4 acc[Q];
-#pragma unroll
-                    for (int i = 0; i < Q; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int t0 = 0; t0 < parts; t0 += 32 * WK) {
-                        float2 ml[WK];
-#pragma unroll
-                        for (int k = 0; k < WK; k++) {
-                            const int t = t0 + 32 * k + lane;
-                            ml[k] = t < parts ? __ldcg((const float2*)(part_at(t) + Sh::ROWS * D + 2 * row)) : make_float2(-INFINITY, 0.f);
-                        }
-                        float top = mx;
-#pragma unroll
-                        for (int k = 0; k < WK; k++) top = fmaxf(top, ml[k].x);
-#pragma unroll
-                        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float f0 = weight(make_float2(mx, sum), top);  // of what the parts before added up to
-                        mx = top;
-                        if (f0 != 1.f) {
-                            sum *= f0;
-#pragma unroll
-                            for (int i = 0; i < Q; i++) acc[i].x *= f0, acc[i].y *= f0, acc[i].z *= f0, acc[i].w *= f0;
-                        }
-#pragma unroll
-                        for (int k = 0; k < WK; k++) {
-                            const int n = min(32, parts - t0 - 32 * k);
-                            if (n <= 0) break;
-                            const float w = weight(ml[k], mx);
-                            float part_sum = ml[k].y * w;
-#pragma unroll
-                            for (int d = 16; d; d >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, d);
-                            sum += part_sum;
-                            for (int j0 = 0; j0 < n; j0 += BATCH) {
-                                float4 x[BATCH][Q];
-#pragma unroll
-                                for (int j = 0; j < BATCH; j++) {
-                                    const float* p = part_at(t0 + 32 * k + min(j0 + j, n - 1)) + row * D;
-#pragma unroll
-                                    for (int i = 0; i < Q; i++)
-                                        if (i * 32 + lane < Q4) x[j][i] = __ldcg((const float4*)p + i * 32 + lane);
-                                }
-#pragma unroll
-                                for (int j = 0; j < BATCH; j++) {
-                                    const float f = __shfl_sync(0xffffffffu, w, min(j0 + j, 31));
-                                    if (j0 + j < n && f != 0.f)
-#pragma unroll
-                                        for (int i = 0; i < Q; i++) {
-                                            acc[i].x += x[j][i].x * f, acc[i].y += x[j][i].y * f;
-                                            acc[i].z += x[j][i].z * f, acc[i].w += x[j][i].w * f;
-                                        }
-                                }
-                            }
-                        }
-                    }
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-                    for (int i = 0; i < Q; i++)
-                        if (i * 32 + lane < Q4)
-                            *((uint2*)(out + row * D) + i * 32 + lane) = make_uint2(Elem<TYPE>::down(acc[i].x * inv, acc[i].y * inv),
-                                                                                    Elem<TYPE>::down(acc[i].z * inv, acc[i].w * inv));
-                    if (a.lse && lane == 0) a.lse[(int64_t)it.b * a.hq + h0 + row] = log_sum(mx, sum);
-                }
-            }
+            s_cut[cut] = CutItem{it.b, it.head, it.sub, t_lo, s_cuts.upto(it_begin + ITEM_COST + it.n - near) - t_lo + 2};
         }
-        __syncthreads();  // the tiles' slots may be filled again
+        cut++;
     }
     copies_wait<0>();
     __syncthreads();
+    // ---- parts of cut items (the piece's first and last): each warp counts for the rows that it would join, and whoever is
+    // last joins them.  At the piece's end, where the registers are free and both waits for the counts are one
+    constexpr int WAYS = Sh::CTAS > 2 || D < 128 ? 8 : 16;  // what the registers hold
+    unsigned joins = 0;
+    if (lane < cut) {
+        const CutItem& it = s_cut[lane];
+        unsigned long long* count = a.arrived + ((int64_t)it.b * per_seq + it.head * split + it.sub);
+        __threadfence();
+        if ((int)((atomicAdd(count, 1ull << (16 * warp)) >> (16 * warp)) & 0xffff) == it.parts - 1) {
+            atomicAdd(count, 0ull - ((unsigned long long)it.parts << (16 * warp)));
+            joins = 1;
+        }
+    }
+    joins = __ballot_sync(0xffffffffu, joins);
+    if (joins) __threadfence();
+#pragma unroll 1
+    for (; joins; joins &= joins - 1) {
+        const CutItem it = s_cut[__ffs(joins) - 1];
+        const int rows = min(Sh::ROWS, a.group - it.sub * Sh::ROWS);
+        const int64_t row0 = (int64_t)it.b * a.hq + it.head * a.group + it.sub * Sh::ROWS;
+        const float* from = a.parts + (int64_t)2 * (it.t_lo - 1) * Sh::PART;
+        uint16_t* out = (uint16_t*)a.out + row0 * D;
+        float* lse = a.lse ? a.lse + row0 : nullptr;
+        if (warp >= rows) continue;
+        if (rows <= WARPS)
+            join_parts<D, TYPE, Sh::ROWS, 1, WAYS>(from, it.parts, warp, rows, out, lse);
+        else
+            join_parts<D, TYPE, Sh::ROWS, Sh::ROWS / WARPS, WAYS>(from, it.parts, warp, rows, out, lse);
+    }
     if (!shared) break;
     }
     if (shared && tid == 0) {
-        int32_t* next = a.arrived + (int64_t)B * per_seq;
-        if (atomicAdd(next + 1, 1) == (int)gridDim.x - 1) next[0] = next[1] = 0;
+        if (atomicAdd(a.counts + 1, 1) == (int)gridDim.x - 1) a.counts[0] = a.counts[1] = 0;
     }
 }
 
@@ -992,10 +1076,10 @@ extern "C" int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int
     if (int rc = check_table(table, seqs, wide, table_stride)) return rc;
     FVS_CHECK_ARG(q && ((uintptr_t)q & 15) == 0 && q_seq % 8 == 0 && q_head % 8 == 0 && q_seq >= 0 && q_head >= 0);
     FVS_CHECK_ARG(lens && out && ((uintptr_t)out & 15) == 0 && work && ((uintptr_t)work & 15) == 0 &&
-                  arrived);
+                  arrived && ((uintptr_t)arrived & 7) == 0);
     if ((int64_t)seqs * hq > (1 << 28)) return FVS_ERANGE;
     AttendArgs a{*cache, {table, table_stride, seqs, wide}, q, q_seq, q_head, lens, out, lse, arrived,
-                 (float*)work, hq, hq / cache->heads, 1, scale * 1.4426950408889634f, 0, 0};
+                 (unsigned long long*)(arrived + 2), (float*)work, hq, hq / cache->heads, 1, scale * 1.4426950408889634f, 0, 0};
     // exact for numerators below 2^31: 2^shift <= page_mul * page < 2^shift + 2^(shift - 31)
     uint32_t bits = 0;
     while ((1ull << bits) < (uint64_t)cache->page) bits++;

@@ -224,7 +224,7 @@ class PagedKV:
             if need < 0:
                 check(need, "kv_attend_work")
             work = torch.empty(need, dtype=torch.uint8, device=self.device)
-            arrived = torch.zeros(n + 2, dtype=torch.int32, device=self.device)
+            arrived = torch.zeros(2 * n + 2, dtype=torch.int32, device=self.device)
             held = (work.data_ptr(), arrived.data_ptr(), n, work, arrived)
             if capturing:
                 self._captured.append(held)

@@ -506,8 +506,8 @@ int fvs_kv_read(fvs_stream_t stream, const fvs_kv_cache* cache, int type, void* 
  * [seqs, hq, dim] of `type`; lse[b, h] (nullable, fp32) = ln sum_t exp(scale * <q, k_t>).  No visible token: out 0,
  * lse -infinity.  Slots that are not visible are never multiplied, whatever they hold.
  * A length above the table's row (or below 0) is cut to it, with FVS_KV_BAD_INDEX for the former.
- * work: fvs_kv_attend_work(dim) bytes of device memory, 16-byte aligned, of any contents; arrived: seqs * hq + 2 words
- * that are zero (each call leaves them zero).  Calls that may run at the same time need their own.
+ * work: fvs_kv_attend_work(dim) bytes of device memory, 16-byte aligned, of any contents; arrived: 2 * seqs *
+ * hq + 2 words, 8-byte aligned, that are zero (each call leaves them zero).  Calls that may run at the same time need their own.
  */
 int fvs_kv_attend_work(int dim);
 int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,

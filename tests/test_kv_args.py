@@ -77,7 +77,7 @@ def test_read_refuses(L, change):
 @pytest.mark.parametrize("change", [dict(type=3), dict(type=1), dict(q=None), dict(q=4104), dict(qs=4), dict(qh=-8),
                                     dict(hq=0), dict(hq=5), dict(table=None), dict(seqs=-1), dict(wide=0), dict(lens=None),
                                     dict(out=None), dict(work=None), dict(work=8),
-                                    dict(arrived=None)])
+                                    dict(arrived=None), dict(arrived=68)])
 def test_attend_refuses(L, change):
     assert attend(L, cache(L), **change) == -1
 
