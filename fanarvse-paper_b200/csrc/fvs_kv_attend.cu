@@ -22,12 +22,13 @@
 // The maximum moves only when a score passes it by more than 8 (a factor of 2^8 keeps fp32 sums and 16-bit probabilities
 // in range), so most units need one vote instead of shuffles and a rescale.
 //
-// Rounding: probabilities enter the second product in 16 bits (the type of v; fp16 for int8 codes), like the output
-// itself; l sums them in fp32 before that.  int8 codes are exact in fp16; their key scale multiplies the fp32 score, their
-// value scale the probability, divided by the largest power of two met so far so that it stays in fp16's range; queries
-// over int8 codes are brought to fp16 by a power of two for each head.
+// Rounding: l sums the probabilities in fp32.  They enter the second product with 11 bits as fp16 (fp16 caches, int8 codes),
+// about the output's own rounding with fp16 outputs and 8 times finer with bf16 ones; over bf16 caches, where 8 bits would
+// add as much error as the output's rounding, as two bf16 numbers with 16 bits together (the product of both takes 0 to 3 %
+// longer).  int8 codes are exact in fp16 (see codes2); their key scale multiplies the fp32 score, their value scale the
+// probability, divided by the largest power of two met so far so that it stays in fp16's range; queries over int8 codes are
+// brought to fp16 by a power of two for each head.
 #include <limits.h>
-
 
 #include "fvs_kv.cuh"
 
@@ -53,9 +54,6 @@ struct AttendArgs {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int ITEM_COST = 3;   // of an item beside its units (loading q, adding up and writing), in units
-#ifndef V_SH
-#define V_SH 192
-#endif
 constexpr float SLACK = 8.f;   // how far (log2) a score may pass the running maximum before it moves
 
 template <int D, int STORE, int NT_>
@@ -85,7 +83,7 @@ struct Shape {
     static constexpr int QBYTES = Q_SMEM ? ROWS * D * 2 : 0;
     static constexpr int FIXED = (O_IN_RING ? 0 : WARPS * OBYTES) + QBYTES;
     // CTAs per SM: three (12 warps hide each other's latencies; 168 registers a thread) where two stages fit
-    static constexpr int CTAS = NT == 1 && D <= 128 ? 3 : RB <= 256 && !Q_SMEM ? 2 : 1;
+    static constexpr int CTAS = NT == 1 && D <= 128 && !(I8 && D == 96) ? 3 : RB <= 256 && !Q_SMEM ? 2 : 1;
     static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 2560 - FIXED;
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
     static constexpr int S = FIT > 4 ? 4 : FIT;      // ring stages
@@ -144,6 +142,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ float weight(float2 ml, float mx) {
     return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - mx);
 }
+// A probability as the sum of two bf16 numbers: its upper bits, and the rest, which stays above zero so that an infinite value
+// times it is no not-a-number
+__device__ __forceinline__ uint32_t upper2(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+__device__ __forceinline__ uint32_t rest2(float a, float b) {
+    const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    return Elem<FVS_BF16>::down(fmaxf(ra, 1.2e-38f), fmaxf(rb, 1.2e-38f));
+}
 // Codes as fp16 without arithmetic: the byte u = code + 128 with a zero byte above it is the subnormal u 2^-24.  The 128 is
 // taken out by the matrix instructions too (see below), so the codes' values stay exact.
 __device__ __forceinline__ uint32_t codes2(uint32_t u, uint32_t sel) { return __byte_perm(u, 0u, sel); }
@@ -198,8 +203,9 @@ struct Lookup {
 constexpr int NO_UNIT = INT_MIN;
 
 // Cuts of the cost of all items: equal shares, one for each CTA, each share cut into `runs` pieces, the first of them
-// long.  A CTA begins with its share's long piece; the short ones are taken as CTAs finish.  (SMs differ in how fast memory
-// serves them: with equal pieces alone the slowest of 296 CTAs ran 110 us where half were done after 80 us.)
+// long.  A CTA begins with its share's long piece; the short ones are taken as CTAs finish, since SMs differ in how fast
+// memory serves them and the warps of an SM in how often they issue (148 SMs, int8, 192 requests of 2048 to 16384 keys: 533
+// -> 487 us).  Below 512 units a share one piece each is faster (48 such requests: 159 -> 145 us).
 struct Cuts {
     int64_t share, lead;  // of the cost: a share, its first piece
     int runs, small;      // pieces of a share, the cost of each but the first (the last one may be shorter)
@@ -326,6 +332,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     using Sh = Shape<D, STORE, NT>;
     constexpr bool I8 = Sh::I8;
     constexpr int MT = I8 ? FVS_F16 : TYPE;  // type of the matrix instructions' operands
+    constexpr bool SPLIT = MT == FVS_BF16;   // probabilities in two parts
     constexpr int S = Sh::S, UNIT = Sh::UNIT, TILES = Sh::TILES, TAKEN = Sh::TAKEN;
     extern __shared__ __align__(128) uint8_t ring_all[];
     __shared__ int64_t s_sum[WARPS];
@@ -403,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     // a share holds 16 units or, if these are smaller, an item
     const int64_t items = (int64_t)(B - none) * per_seq;
     cuts.share = max(max((int64_t)1, min((int64_t)16, items ? total / items : 1)), (total + gridDim.x - 1) / gridDim.x);
-    const bool shared = cuts.share >= V_SH;  // with less, setting up another piece costs more than it evens out
+    const bool shared = cuts.share >= 512;  // setting up another piece and joining its part costs more than it evens out below
     if (shared) {
         cuts.small = (int)((cuts.share + 7) / 8);
         cuts.lead = cuts.share - 2 * cuts.small;
@@ -851,7 +858,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             for (int j = 0; j < TILES; j++) {
                 if (TILES > 1 && ((mask >> (16 * j)) & 0xffffu) == 0) continue;  // its rows were not copied
                 // p, and p as the B operand of the second product
-                uint32_t pf[NT][2];
+                uint32_t pf[NT][2], pl[NT][2];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     const float z0 = m[t][0] == -INFINITY ? 0.f : m[t][0], z1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
@@ -860,8 +867,15 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     l[t][0] += p0 + p2;
                     l[t][1] += p1 + p3;
                     if (I8) p0 *= vs[j][0], p1 *= vs[j][0], p2 *= vs[j][1], p3 *= vs[j][1];
-                    pf[t][0] = transpose8x8(Elem<MT>::down(p0, p1));
-                    pf[t][1] = transpose8x8(Elem<MT>::down(p2, p3));
+                    if (SPLIT) {
+                        pf[t][0] = transpose8x8(upper2(p0, p1));
+                        pf[t][1] = transpose8x8(upper2(p2, p3));
+                        pl[t][0] = transpose8x8(rest2(p0, p1));
+                        pl[t][1] = transpose8x8(rest2(p2, p3));
+                    } else {
+                        pf[t][0] = transpose8x8(Elem<MT>::down(p0, p1));
+                        pf[t][1] = transpose8x8(Elem<MT>::down(p2, p3));
+                    }
                 }
                 // O^T += V^T P^T
                 if (I8) {
@@ -891,7 +905,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         uint32_t f[4];
                         ldm4t(f, at + Sh::v_chunk(lane, 2 * i + ((lane >> 3) & 1)) * 16);
 #pragma unroll
-                        for (int t = 0; t < NT; t++) mma<MT>(o[i][t], f, pf[t][0], pf[t][1]);
+                        for (int t = 0; t < NT; t++) {
+                            mma<MT>(o[i][t], f, pf[t][0], pf[t][1]);
+                            if (SPLIT) mma<MT>(o[i][t], f, pl[t][0], pl[t][1]);
+                        }
                     }
                 }
             }
@@ -1042,8 +1059,10 @@ static int launch_nt(fvs_stream_t stream, AttendArgs a) {
 }
 template <int D, int TYPE, int STORE>
 static int launch(fvs_stream_t stream, const AttendArgs& a) {
-    if (a.group <= 8) return launch_nt<D, TYPE, STORE, 1>(stream, a);
-    return launch_nt<D, TYPE, STORE, 2>(stream, a);
+    // wide int8 heads: two items of 8 rows take 68 us where one of 16 takes 87 (64 requests of 500 to 16000 keys, D = 256);
+    // wide 16-bit heads: 128 and 95 us
+    if (a.group <= 8 || (STORE == FVS_I8 && D > 128)) return launch_nt<D, TYPE, STORE, 1>(stream, a);
+    return launch_nt<D, TYPE, STORE, (STORE == FVS_I8 && D > 128 ? 1 : 2)>(stream, a);
 }
 template <int D>
 static int launch_types(fvs_stream_t stream, const AttendArgs& a, int type) {
