@@ -598,3 +598,54 @@ def test_search_then_answer(kv):
         if step in (0, 15, 17):
             check_attend(cache, q, table, idx + 1, got=got)
     cache.check_status()
+
+
+def test_example_answers_from_passages():
+    """examples/answer_from_passages.py: the attention of its last step against plain products of what the cache holds:
+    within the rounding of bf16 outputs (2^-8) and as much again."""
+    import importlib.util
+    import os
+    from conftest import REPO
+    pkg("build").build()
+    spec = importlib.util.spec_from_file_location("answer", os.path.join(REPO, "examples", "answer_from_passages.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(steps=20) < 2 ** -7
+
+
+def test_attend_one_table_for_all_and_long_rows(kv):
+    """A page table whose rows are one row (stride 0), and more sequences than a grid axis holds."""
+    g = torch.Generator().manual_seed(21)
+    table, pages = full_table([70], 16, g)
+    cache = make_cache(kv, pages, 1, 16, 64, F16, g)
+    n = 70000
+    q = torch.randn(3, 2, 64, generator=g).to(DEV, F16)
+    shared = table.to(DEV).expand(n, -1)
+    lens = (torch.arange(n, device=DEV) % 71).int()
+    many = q[torch.arange(n, device=DEV) % 3]
+    out, lse = cache.attend(many, shared, lens)
+    some = torch.arange(0, n, 997, device=DEV)
+    a, b = out[some].contiguous(), lse[some].contiguous()
+    check_attend(cache, many[some].contiguous(), shared[some].contiguous(), lens[some].contiguous(), got=(a, b))
+
+
+def test_attend_two_streams_at_once(kv):
+    """Calls in flight on two streams have workspaces of their own."""
+    g = torch.Generator().manual_seed(22)
+    table, pages = full_table([9000, 8000], 64, g)
+    cache = make_cache(kv, pages, 4, 64, 128, BF16, g)
+    lens = torch.tensor([9000, 8000], dtype=torch.int32, device=DEV)
+    q = [torch.randn(2, 8, 128, generator=g).to(DEV, BF16) for _ in range(2)]
+    table = table.to(DEV)
+    want = [cache.attend(x, table, lens) for x in q]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(cache.attend(q[k], table, lens))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for o, l in got[k]:
+            assert torch.equal(o, want[k][0]) and torch.equal(l, want[k][1])
