@@ -54,6 +54,7 @@ struct AttendArgs {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int ITEM_COST = 3;   // of an item beside its units (loading q, adding up and writing), in units
+constexpr int SM_ROWS = 32;    // rows of partial results that an SM's CTAs may hold at a time
 constexpr float SLACK = 8.f;   // how far (log2) a score may pass the running maximum before it moves
 
 template <int D, int STORE, int NT_>
@@ -87,7 +88,7 @@ struct Shape {
     static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 2560 - FIXED;
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
     static constexpr int S = FIT > 4 ? 4 : FIT;      // ring stages
-    static_assert(S >= 2, "ring");
+    static_assert(S >= 2 && CTAS * ROWS <= SM_ROWS, "ring, workspace");
     static constexpr int TAKEN = 8;  // more items than a warp has on the way: units in the ring, lookups, one in reserve
     static_assert(S + 4 <= TAKEN, "taken");
     static constexpr int RING = S * STAGE;           // bytes per warp
@@ -1076,11 +1077,12 @@ static int launch_types(fvs_stream_t stream, const AttendArgs& a, int type) {
 
 using namespace fvs::kv;
 
-// two partial results for each of the pieces: 3 for each of up to 4 CTAs on every SM
+// two partial results for each of the pieces: 3 for each CTA; CTAs of an SM times rows of a
+// partial result are at most SM_ROWS
 extern "C" int fvs_kv_attend_work(int dim) {
     if (dim < 1) return FVS_EINVAL;
     if (dim > 256) return FVS_ERANGE;
-    return 2 * 3 * 4 * fvs_sm_count() * 16 * (dim + 2) * 4;
+    return 2 * 3 * fvs_sm_count() * SM_ROWS * (dim + 2) * 4;
 }
 
 extern "C" int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,

@@ -24,6 +24,7 @@ HEAD_DIMS = (64, 96, 128, 192, 256)
 _CODE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.int8: _lib.I8, torch.float32: _lib.F32T}
 _WIDE = (torch.float16, torch.bfloat16)
 _READ = (torch.float16, torch.bfloat16, torch.float32)
+_WORK = {}  # (GPU, stream) -> workspace of attend
 
 
 def _need(cond, what):
@@ -73,9 +74,9 @@ class PagedKV:
         self._c = _lib.KvCache(p(k), p(v), p(k_scale), p(v_scale), p(fill), p(self.status), *k.stride()[:3], *ss,
                                self.pages, self.heads, self.page, self.dim, _CODE[k.dtype])
         self._ref = C.byref(self._c)
-        self._work = {}      # stream -> workspace of attend: addresses, counters held, tensors
-        self._captured = []  # workspaces of captured calls
         self.L = _lib.lib()
+        self._work_bytes = self.L.fvs_kv_attend_work(self.dim)
+        check(min(self._work_bytes, 0), "kv_attend_work")
         self.launches = 0
 
     @classmethod
@@ -206,31 +207,27 @@ class PagedKV:
         if n == 0:
             return out, lse
         stream = self._stream()
-        work, arrived = self._workspace(stream, n * hq)
+        work, arrived = self._workspace(stream, 2 * n * hq + 2)
         check(self.L.fvs_kv_attend(stream, self._ref, ty, *qa, hq, *ta, la,
-                                   self.scale if scale is None else scale, oa, lse.data_ptr(), work, arrived),
+                                   self.scale if scale is None else scale, oa, lse.data_ptr(), work.data_ptr(),
+                                   arrived.data_ptr()),
               "kv_attend")
         self.launches += 1
         return out, lse
 
     def _workspace(self, stream, n):
-        """Addresses of the partial results and of n arrival counters (zeroed once, left zeroed by every call), one pair for
-        each stream; a captured call gets its own, whose counters its graph zeroes, because the graph may be replayed
-        beside calls on any stream."""
+        """Tensors of the partial results and of n arrival counters (zeroed once, left zeroed by every call): one pair for
+        each stream, whose calls come one after another, shared by all caches.  A captured call's pair lives in its graph's
+        memory, and the graph zeroes its counters: it may be replayed beside calls on any stream."""
         capturing = torch.cuda.is_current_stream_capturing()
-        held = None if capturing else self._work.get(stream)
-        if held is None or held[2] < n:
-            need = self.L.fvs_kv_attend_work(self.dim)
-            if need < 0:
-                check(need, "kv_attend_work")
-            work = torch.empty(need, dtype=torch.uint8, device=self.device)
-            arrived = torch.zeros(2 * n + 2, dtype=torch.int32, device=self.device)
-            held = (work.data_ptr(), arrived.data_ptr(), n, work, arrived)
-            if capturing:
-                self._captured.append(held)
-            else:
-                self._work[stream] = held
-        return held[:2]
+        held = None if capturing else _WORK.get((self._index, stream))
+        if held is None or held[0].numel() < self._work_bytes or held[1].numel() < n:
+            work, arrived = (0, 0) if held is None else (held[0].numel(), held[1].numel())
+            held = (torch.empty(max(self._work_bytes, work), dtype=torch.uint8, device=self.device),
+                    torch.zeros(max(n, arrived), dtype=torch.int32, device=self.device))
+            if not capturing:
+                _WORK[self._index, stream] = held
+        return held
 
     def check_status(self):
         """Raises if a call since the last check met an index outside its table (synchronises)."""

@@ -649,3 +649,31 @@ def test_attend_two_streams_at_once(kv):
     for k in range(2):
         for o, l in got[k]:
             assert torch.equal(o, want[k][0]) and torch.equal(l, want[k][1])
+
+
+def test_attend_graph_of_several_caches(kv):
+    """Layers captured together (their workspaces follow one another in the graph's memory), replayed beside eager calls on
+    another stream."""
+    g = torch.Generator().manual_seed(23)
+    table, pages = full_table([5000, 4000, 10], 32, g)
+    caches = [make_cache(kv, pages, 2, 32, d, BF16, g) for d in (64, 128, 64)]
+    lens = torch.tensor([5000, 4000, 10], dtype=torch.int32, device=DEV)
+    table = table.to(DEV)
+    q = [torch.randn(3, 8, c.dim, generator=g).to(DEV, BF16) for c in caches]
+    want = [c.attend(x, table, lens) for c, x in zip(caches, q)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [c.attend(x, table, lens) for c, x in zip(caches, q)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for o, l in got:
+            o.zero_()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = [c.attend(x, table, lens) for c, x in zip(caches, q)]
+        torch.cuda.synchronize()
+        for a in (got, beside):
+            for (o, l), (wo, wl) in zip(a, want):
+                assert torch.equal(o, wo) and torch.equal(l, wl)
