@@ -75,6 +75,7 @@ class PagedKV:
                                self.pages, self.heads, self.page, self.dim, _CODE[k.dtype])
         self._ref = C.byref(self._c)
         self.L = _lib.lib()
+        self._append, self._read, self._attend = self.L.fvs_kv_append, self.L.fvs_kv_read, self.L.fvs_kv_attend
         self._work_bytes = self.L.fvs_kv_attend_work(self.dim)
         check(min(self._work_bytes, 0), "kv_attend_work")
         self.launches = 0
@@ -90,7 +91,7 @@ class PagedKV:
     # A decoding step makes these calls for every layer, so each check is one condition and messages are made on failure.
     def _table(self, table):
         shape, stride = table.shape, table.stride()
-        if not (len(shape) == 2 and table.dtype is torch.int32 and table.device == self.device and shape[1] >= 1
+        if not (len(shape) == 2 and table.dtype is torch.int32 and table.get_device() == self._index and shape[1] >= 1
                 and (shape[1] == 1 or stride[1] == 1)):
             raise ValueError("the page table is an int32 [sequences, wide] with contiguous rows on the cache's GPU")
         return table.data_ptr(), shape[0], shape[1], stride[0]
@@ -98,7 +99,8 @@ class PagedKV:
     def _ints(self, t, n, what):
         if t is None:
             return None
-        if not (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == self.device):
+        if not (t.dtype is torch.int32 and t.dim() == 1 and t.numel() == n and t.is_contiguous()
+                and t.get_device() == self._index):
             raise ValueError(f"{what} is a contiguous int32 [{n}] on the cache's GPU")
         return t.data_ptr()
 
@@ -106,7 +108,7 @@ class PagedKV:
         """address, token stride and head stride of [n, heads, dim]"""
         shape = x.shape
         if not (len(shape) == 3 and shape[0] == n and shape[2] == self.dim and (heads is None or shape[1] == heads)
-                and x.device == self.device):
+                and x.get_device() == self._index):
             raise ValueError(f"{what} is [{n}, {heads or 'heads'}, {self.dim}] on the cache's GPU")
         s0, s1, s2 = x.stride()
         at = x.data_ptr()
@@ -120,11 +122,14 @@ class PagedKV:
         return _CODE[dtype]
 
     def _like(self, out, x, what):
-        if not (out.dtype is x.dtype and out.shape == x.shape and out.is_contiguous() and out.device == self.device):
+        if not (out.dtype is x.dtype and out.shape == x.shape and out.is_contiguous()
+                and out.get_device() == self._index):
             raise ValueError(f"{what} is a contiguous tensor like q")
         return out.data_ptr()
 
     def _stream(self):
+        if torch._C._cuda_getDevice() != self._index:
+            raise ValueError(f"the cache is on GPU {self._index}, which is not the current one (torch.cuda.device)")
         return torch._C._cuda_getCurrentRawStream(self._index)  # torch.cuda.current_stream takes 2 us more
 
     # ---------------------------------------------------------------- the operators
@@ -150,7 +155,7 @@ class PagedKV:
         if rope is not None:
             cos, sin = rope
             if not (cos.dtype is sin.dtype is torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
-                    and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == self.device):
+                    and cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == self._index):
                 raise ValueError("rope is two contiguous fp32 [positions, rot / 2] on the cache's GPU")
             positions, rot = cos.shape[0], 2 * cos.shape[1]
             if rot % 16 or not 0 < rot <= self.dim or positions < 1:
@@ -158,11 +163,12 @@ class PagedKV:
             cos, sin = cos.data_ptr(), sin.data_ptr()
         if pairs not in _lib.PAIRS:
             raise ValueError(f"pairs {pairs!r}: one of {sorted(_lib.PAIRS)}")
-        if seq is None and n > table.shape[0]:
+        ta = self._table(table)
+        if seq is None and n > ta[1]:
             raise ValueError("without seq there is a table row for each token")
-        check(self.L.fvs_kv_append(self._stream(), self._ref, ty, *ka, *va, *qa, hq, qo, *self._table(table),
-                                   self._ints(seq, n, "seq"), self._ints(idx, n, "idx"), self._ints(pos, n, "pos"), n,
-                                   cos, sin, positions, rot, _lib.PAIRS[pairs]), "kv_append")
+        check(self._append(self._stream(), self._ref, ty, *ka, *va, *qa, hq, qo, *ta, self._ints(seq, n, "seq"),
+                           self._ints(idx, n, "idx"), self._ints(pos, n, "pos"), n, cos, sin, positions, rot,
+                           _lib.PAIRS[pairs]), "kv_append")
         self.launches += 1
         return q_out if q is not None else None
 
@@ -173,12 +179,13 @@ class PagedKV:
         dtype = dtype or (torch.float32 if self.dtype is torch.int8 else self.dtype)
         if dtype not in _READ:
             raise ValueError(f"read as {dtype}: fp16, bf16 or fp32")
-        if seq is None and n > table.shape[0]:
+        ta = self._table(table)
+        if seq is None and n > ta[1]:
             raise ValueError("without seq there is a table row for each token")
         k = torch.empty((n, self.heads, self.dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        check(self.L.fvs_kv_read(self._stream(), self._ref, _CODE[dtype], k.data_ptr(), v.data_ptr(),
-                                 *self._table(table), self._ints(seq, n, "seq"), self._ints(idx, n, "idx"), n), "kv_read")
+        check(self._read(self._stream(), self._ref, _CODE[dtype], k.data_ptr(), v.data_ptr(),
+                         *ta, self._ints(seq, n, "seq"), self._ints(idx, n, "idx"), n), "kv_read")
         self.launches += 1
         return k, v
 
@@ -201,17 +208,15 @@ class PagedKV:
         if lse is None:
             lse = torch.empty((n, hq), device=q.device)
         elif not (lse.dtype is torch.float32 and lse.shape == (n, hq) and lse.is_contiguous()
-                  and lse.device == self.device):
+                  and lse.get_device() == self._index):
             raise ValueError("lse is a contiguous fp32 [sequences, query heads]")
         oa, la = self._like(out, q, "out"), self._ints(lens, n, "lens")
         if n == 0:
             return out, lse
         stream = self._stream()
         work, arrived = self._workspace(stream, 2 * n * hq + 2)
-        check(self.L.fvs_kv_attend(stream, self._ref, ty, *qa, hq, *ta, la,
-                                   self.scale if scale is None else scale, oa, lse.data_ptr(), work.data_ptr(),
-                                   arrived.data_ptr()),
-              "kv_attend")
+        check(self._attend(stream, self._ref, ty, *qa, hq, *ta, la, self.scale if scale is None else scale, oa,
+                           lse.data_ptr(), work.data_ptr(), arrived.data_ptr()), "kv_attend")
         self.launches += 1
         return out, lse
 
