@@ -13,7 +13,6 @@ struct Elem;
 template <>
 struct Elem<FVS_F16> {
     using T = __half;
-    using T2 = __half2;
     static __device__ __forceinline__ float2 up(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
     static __device__ __forceinline__ uint32_t down(float a, float b) {
         const __half2 r = __floats2half2_rn(a, b);
@@ -23,7 +22,6 @@ struct Elem<FVS_F16> {
 template <>
 struct Elem<FVS_BF16> {
     using T = __nv_bfloat16;
-    using T2 = __nv_bfloat162;
     static __device__ __forceinline__ float2 up(uint32_t x) {
         return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
     }
@@ -32,15 +30,6 @@ struct Elem<FVS_BF16> {
         return *reinterpret_cast<const uint32_t*>(&r);
     }
 };
-template <>
-struct Elem<FVS_I8> {
-    using T = int8_t;
-};
-template <>
-struct Elem<FVS_F32> {
-    using T = float;
-};
-
 // 16 consecutive bytes of 16-bit elements as fp32 and back (one rounding per element)
 template <int TYPE>
 __device__ __forceinline__ void up8(const uint4& x, float (&f)[8]) {
