@@ -30,10 +30,11 @@
 // probability, divided by the largest power of two met so far so that it stays in fp16's range; queries over int8 codes are
 // brought to fp16 by a power of two for each head.
 //
-// Measured on one B200 (6550 GB/s measured copy rate): 131071 bf16 keys of 8 heads of 128, 32 query heads, 103 us (5.2
-// TB/s), four such sequences 340 us (6.3 TB/s); 64 sequences of 1 to 8192 keys 65 us (4.8 TB/s); int8 codes, 48 sequences of
-// 2048 to 16384 keys, 64 query heads, 143 to 155 us (4.1 to 4.5 TB/s, bound by 350 warp instructions for 16 keys); 2000
-// sequences of 1 to 200 int8 keys 39 us (per item, not per byte); one sequence of 100 keys 10 us (waits for memory in a row).
+// Measured on one B200 (6550 GB/s measured copy rate): 131071 bf16 keys of 8 heads of 128, 32 query heads, 103 to 106 us
+// (5.1 TB/s), four such sequences 340 us (6.3 TB/s); 64 sequences of 1 to 8192 keys 66 us (4.7 TB/s); int8 codes, 48
+// sequences of 2048 to 16384 keys, 64 query heads, 135 to 150 us (4.3 to 4.8 TB/s, bound by 350 warp instructions for 16
+// keys); 2000 sequences of 1 to 200 int8 keys 37 us (per item, not per byte); one sequence of 100 keys 10 us (waits for
+// memory in a row).
 #include <limits.h>
 
 #include "fvs_kv.cuh"
@@ -584,19 +585,22 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                                          (int64_t)(slot0 + row) * a.c.slot_stride) * ESZ + ch * 16;
                     const uint8_t *pk = (const uint8_t*)a.c.k + off, *pv = (const uint8_t*)a.c.v + off;
                     const int64_t step = a.c.slot_stride * (RPI * ESZ);
-                    const bool dense = a.c.slot_stride == D && m == 0xffffu;  // fixed distances: no address arithmetic
+                    // full tiles of dense rows have fixed distances: no address arithmetic.  The rest is a loop: unrolled, it
+                    // pushed the loop over units out of the instruction cache (large int8 calls 135 -> 143 us)
+                    if (a.c.slot_stride == D && m == 0xffffu) {
 #pragma unroll
-                    for (int i = 0; i < 16 / RPI; i++) {
-                        const int key = 16 * j + i * RPI + row;
-                        const uint32_t dk = st + key * Sh::KS + Sh::k_chunk(key, ch) * 16;
-                        const uint32_t dv = st + Sh::VALUES + key * Sh::VS + Sh::v_chunk(key, ch) * 16;
-                        if (dense) {
-                            copy16(dk, pk + i * RPI * Sh::RB, true);
-                            copy16(dv, pv + i * RPI * Sh::RB, true);
-                        } else {
+                        for (int i = 0; i < 16 / RPI; i++) {
+                            const int key = 16 * j + i * RPI + row;
+                            copy16(st + key * Sh::KS + Sh::k_chunk(key, ch) * 16, pk + i * RPI * Sh::RB, true);
+                            copy16(st + Sh::VALUES + key * Sh::VS + Sh::v_chunk(key, ch) * 16, pv + i * RPI * Sh::RB, true);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < 16 / RPI; i++) {
+                            const int key = 16 * j + i * RPI + row;
                             const bool on = (m >> (i * RPI + row)) & 1;
-                            copy16(dk, on ? pk + i * step : (const uint8_t*)a.c.k, on);
-                            copy16(dv, on ? pv + i * step : (const uint8_t*)a.c.v, on);
+                            copy16(st + key * Sh::KS + Sh::k_chunk(key, ch) * 16, on ? pk + i * step : (const uint8_t*)a.c.k, on);
+                            copy16(st + Sh::VALUES + key * Sh::VS + Sh::v_chunk(key, ch) * 16, on ? pv + i * step : (const uint8_t*)a.c.v, on);
                         }
                     }
                 }
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             const int64_t at0 = live ? (int64_t)k.entry * a.c.page_stride + (int64_t)k.head * a.c.head_stride +
                                            (int64_t)k.slot * a.c.slot_stride
                                      : 0;
-#pragma unroll
+#pragma unroll (D > 128 ? 2 : UNIT * PER / 32)
             for (int i = 0; i < UNIT * PER / 32; i++) {
                 const int at = i * 32 + lane, key = at / PER, ch = at % PER;
                 const int64_t off = __shfl_sync(0xffffffffu, at0, key) * ESZ + ch * 16;
