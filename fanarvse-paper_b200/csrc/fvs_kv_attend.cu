@@ -158,11 +158,15 @@ __device__ __forceinline__ uint32_t rest2(float a, float b) {
     const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
     return Elem<FVS_BF16>::down(fmaxf(ra, 1.2e-38f), fmaxf(rb, 1.2e-38f));
 }
-// Codes as fp16 without arithmetic: the byte u = code + 128 with a zero byte above it is the subnormal u 2^-24.  The 128 is
-// taken out by the matrix instructions too (see below), so the codes' values stay exact.
-__device__ __forceinline__ uint32_t codes2(uint32_t u, uint32_t sel) { return __byte_perm(u, 0u, sel); }
+// Two codes as fp16: the byte u = code + 128 under 0x64 is 1024 + u, and 1152 less is the code, exactly.  (Leaving the 128 in
+// the products and taking it out of their sums spares the subtraction, but the sums then round at 128 sum |q|: a row with
+// one large element, or one stored with an infinity, is not what the codes say.)
+__device__ __forceinline__ uint32_t codes2(uint32_t u, uint32_t sel) {
+    const uint32_t x = __byte_perm(u, 0x64646464u, sel), off = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 constexpr uint32_t LOW = 0x4140, HIGH = 0x4342;  // the lower and the upper two codes of a word
-constexpr uint32_t MINUS_128 = 0x80808080u;      // two fp16: -128 2^-24
 
 __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
     const int len = __ldg(a.lens + b);
@@ -678,7 +682,6 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         uint32_t qf[Sh::Q_SMEM ? 1 : NT][Sh::Q_SMEM ? 1 : D / 16][2];
         uint2* q_all = (uint2*)(ring_all + Sh::SMEM - Sh::QBYTES);
         float mul[NT][2];   // what a raw product is multiplied with, for heads 2 c4 and 2 c4 + 1
-        float bias[NT][2];  // int8: what the codes' 128 adds to it
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int h = t * 8 + r;
@@ -696,13 +699,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int e = max(1, min(230, (int)(__float_as_uint(top) >> 23)));  // 2^(e - 127) <= top
                 const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-                float sum = 0.f;  // of the rounded values
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const float2 x = Elem<TYPE>::up(raw[k].x), y = Elem<TYPE>::up(raw[k].y);
                     const uint32_t f0 = Elem<FVS_F16>::down(x.x * down, x.y * down), f1 = Elem<FVS_F16>::down(y.x * down, y.y * down);
-                    const float2 u = Elem<FVS_F16>::up(f0), v = Elem<FVS_F16>::up(f1);
-                    sum += (u.x + u.y) + (v.x + v.y);
                     if (Sh::Q_SMEM) {
                         if (k % WARPS == warp) q_all[(t * (D / 16) + k) * 32 + lane] = make_uint2(f0, f1);
                     } else {
@@ -710,15 +710,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][1] = f1;
                     }
                 }
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                const float up = a.scale2 * __uint_as_float((uint32_t)(e + 24) << 23);
-                sum *= -0x1p-17f;
+                const float up = a.scale2 * __uint_as_float((uint32_t)e << 23);
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    mul[t][x] = __shfl_sync(0xffffffffu, up, c4 * 8 + 4 * x);
-                    bias[t][x] = __shfl_sync(0xffffffffu, sum, c4 * 8 + 4 * x);
-                }
+                for (int x = 0; x < 2; x++) mul[t][x] = __shfl_sync(0xffffffffu, up, c4 * 8 + 4 * x);
             } else {
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
@@ -733,7 +727,6 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     }
                 }
                 mul[t][0] = mul[t][1] = a.scale2;
-                bias[t][0] = bias[t][1] = 0.f;
             }
         }
         if (Sh::Q_SMEM) __syncthreads();
@@ -770,7 +763,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int x = 0; x < 4; x++) s[j][t][x] = I8 ? bias[t][x & 1] : 0.f, s2[t][x] = 0.f;
+                    for (int x = 0; x < 4; x++) s[j][t][x] = s2[t][x] = 0.f;
                 if (I8) {
 #pragma unroll
                     for (int k = 0; k < D / 32; k++) {
@@ -891,7 +884,6 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 }
                 // O^T += V^T P^T
                 if (I8) {
-                    const uint32_t minus[4] = {MINUS_128, MINUS_128, MINUS_128, MINUS_128};
 #pragma unroll
                     for (int k = 0; k < D / 32; k++) {
                         // rows 2 c4, 2 c4 + 1 and 8 further: their chunks are permuted alike
@@ -903,10 +895,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                             const uint32_t x = __byte_perm(v0, v1, h ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, h ? 0x7362 : 0x5140);
                             const uint32_t f[4] = {codes2(x, LOW), codes2(x, HIGH), codes2(y, LOW), codes2(y, HIGH)};
 #pragma unroll
-                            for (int t = 0; t < NT; t++) {
-                                mma<MT>(o[2 * k + h][t], f, pf[t][0], pf[t][1]);
-                                mma<MT>(o[2 * k + h][t], minus, pf[t][0], pf[t][1]);
-                            }
+                            for (int t = 0; t < NT; t++) mma<MT>(o[2 * k + h][t], f, pf[t][0], pf[t][1]);
                         }
                     }
                 } else {
@@ -943,7 +932,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                                     : (float*)(ring_all + WARPS * Sh::RING + warp * Sh::OBYTES);
         if (lane == 0) s_tile[warp] = (int)((uint8_t*)tile - ring_all);
         if (!solo) __syncthreads();
-        const float vup = I8 ? __uint_as_float((uint32_t)(vexp + 1) << 23) * 0x1p24f : 1.f;
+        const float vup = I8 ? __uint_as_float((uint32_t)(vexp + 1) << 23) : 1.f;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
 #pragma unroll

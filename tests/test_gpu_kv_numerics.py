@@ -1,0 +1,117 @@
+"""Attention over the paged cache where its arithmetic could lose something: weights far below the largest, value scales and
+keys of very different size, rows that hold infinities; and calls large enough to take the kernel's other ways of
+dividing the work.
+
+Bounds, from the arithmetic alone, with u the unit roundoff of the output type and n the keys of a sequence:
+* a score is a sum of exact products (codes, 16-bit numbers), 16 to an instruction, in D / 16 instructions, each of which may
+  cut up to 2^-23 of the largest term or partial sum, plus 20 such steps for the ends (scale, factors of the heads, the
+  difference to the running maximum): es = (D / 16 + 20) 2^-23 scale sum |q k|, which changes a weight by a factor e^(es);
+* a weight enters the second product with 21 bits or more over fp16 values and codes (two fp16 numbers) and with 16 over bf16
+  values (two bf16 numbers): ep = 2^-20, 2^-16 of sum p |v|; the fp16 pair ends at 2^-36 of the largest weight (of the
+  largest weight times value scale over codes), so a key that is smaller still may be off by 2^-35 of that;
+* sums of fp32 over at most n / 16 + 64 steps, each cutting 2^-23: (n / 16 + 64) 2^-23 of sum p |v|;
+* one rounding of the output, u of it (2^-25 where fp16 has no more bits, 2^-134 where bf16 has none).
+"""
+import numpy as np
+import pytest
+import torch
+
+from conftest import pkg
+from oracle import kv_oracle as O
+from test_gpu_kv import BF16, DEV, F16, I8, U, c, full_table, make_cache, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kv():
+    pkg("build").build()
+    return pkg("kvcache")
+
+
+def close(cache, q, table, lens, got=None):
+    """attend against the oracle within the bounds above."""
+    out, lse = got or cache.attend(q, table, lens)
+    torch.cuda.synchronize()
+    d, scale = cache.dim, 1 / np.sqrt(cache.dim)
+    k, v = values(cache)
+    fill = None if cache.fill is None else c(cache.fill)
+    eo, el, pv, av, mag = O.attend(c(q), k, v, c(table), c(lens), scale, fill)
+    out, lse = c(out), c(lse)
+    assert np.isfinite(out).all() and np.isfinite(lse[np.isfinite(el)]).all()
+    es = (d / 16 + 20) * 2.0 ** -23 * mag
+    ep = 2.0 ** -16 if cache.dtype == BF16 else 2.0 ** -20
+    sums = (c(lens) / 16 + 64)[:, None] * 2.0 ** -23
+    least = 2.0 ** -35 * av                              # av: sum |v| over the sum of the weights
+    if cache.dtype == I8:                                # in units of the largest weighted scale
+        top = np.zeros_like(el)
+        n = np.zeros_like(el)
+        for b in range(len(top)):
+            t = np.arange(int(lens[b]))
+            p, s = c(table)[b][t // cache.page], t % cache.page
+            g = q.shape[1] // cache.heads
+            for h in range(q.shape[1]):
+                w = np.exp(k[p, h // g, s] @ c(q)[b, h] * scale - el[b, h])
+                top[b, h], n[b, h] = (w * np.abs(c(cache.v_scale)[p, h // g, s])).max(initial=0), len(t)
+        least = (2.0 ** -35 * 127 * n * top)[..., None]
+    tol = U[q.dtype] * np.abs(eo) + (2 * es[..., None] + ep + sums[..., None]) * pv * 1.01 + least
+    tol += 2.0 ** -25 if q.dtype == F16 else 2.0 ** -134
+    worst = (np.abs(out - eo) / np.maximum(tol, 1e-300)).max()
+    assert worst <= 1, f"out is {worst:.2f} of its bound"
+    tol = es + sums + 2.0 ** -22 * (1 + np.abs(np.where(np.isfinite(el), el, 0)))
+    seen = np.isfinite(el)
+    worst = (np.abs(lse[seen] - el[seen]) / tol[seen]).max(initial=0)
+    assert worst <= 1, f"lse is {worst:.2f} of its bound"
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------------------------------------ scores over codes
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_scores_of_rows_with_one_large_element(kv, dtype, dim):
+    """One element takes a row's scale, and no query has it; a sequence of one key has its score as lse."""
+    g = torch.Generator().manual_seed(dim)
+    B, page = 64, 16
+    x = torch.rand(B, 1, page, dim, generator=g) + 0.5
+    x[..., 5] = 127
+    cache = kv.PagedKV(x.round().to(DEV, I8), x.round().to(DEV, I8), *(torch.ones(B, 1, page, device=DEV) for _ in range(2)))
+    q = torch.rand(B, 8, dim, generator=g) + 0.5
+    q[..., 5] = 0
+    close(cache, q.to(DEV, dtype), torch.arange(B).view(B, 1).to(DEV, torch.int32), ints([1] * B))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("odd", [float("inf"), float("nan")])
+def test_key_rows_of_codes_that_are_not_finite(kv, dtype, odd):
+    """A key row stored with an infinity or a not-a-number makes every head that sees it not-a-number, and nothing else."""
+    g = torch.Generator().manual_seed(37)
+    B, hq, page, dim = 16, 64, 16, 128
+    lens = [40 + b for b in range(B)]
+    table, pages = full_table(lens, page, g)
+    cache = make_cache(kv, pages, 1, page, dim, I8, g)
+    table = table.to(DEV)
+    k = torch.randn(B // 2, 1, dim, generator=g)
+    k[:, 0, 3] = odd
+    v = torch.randn(B // 2, 1, dim, generator=g).to(DEV, dtype)
+    cache.append(k.to(DEV, dtype), v, table, ints([b * 5 for b in range(B // 2)]))
+    q = torch.randn(B, hq, dim, generator=g).to(DEV, dtype)
+    out, lse = cache.attend(q, table, ints(lens))
+    assert torch.isnan(lse[:B // 2]).all() and torch.isnan(out[:B // 2]).all()
+    assert torch.isfinite(lse[B // 2:]).all() and torch.isfinite(out[B // 2:]).all()
+
+
+def test_value_rows_of_codes_that_are_not_finite(kv):
+    g = torch.Generator().manual_seed(38)
+    table, pages = full_table([200, 200], 16, g)
+    cache = make_cache(kv, pages, 1, 16, 64, I8, g)
+    table = table.to(DEV)
+    x = torch.randn(1, 1, 64, generator=g).to(DEV, F16)
+    odd = x.clone()
+    odd[0, 0, 7] = float("-inf")
+    cache.append(x, odd, table, ints([123]))
+    out, lse = cache.attend(torch.randn(2, 2, 64, generator=g).to(DEV, F16), table, ints([200, 200]))
+    assert torch.isnan(out[0]).all() and torch.isfinite(lse).all() and torch.isfinite(out[1]).all()
