@@ -20,8 +20,9 @@
 // most 16 query rows, so the bound is the cache's bytes (2 G / element size flops per byte), and tcgen05's 128-row
 // tiles would be padded eightfold and more.
 //
-// The maximum moves only when a score passes it by more than 8 (a factor of 2^8 keeps fp32 sums and 16-bit probabilities
-// in range), so most units need one vote instead of shuffles and a rescale.
+// The maximum moves only when a score passes it by more than SLACK, so most units need one vote instead of shuffles and a
+// rescale.  Weights that become fp16 are taken 2^BELOW larger than the softmax's, near fp16's upper end: without that a key at
+// 2^-25 of the largest weight vanished from the second product and not from l.
 //
 // Rounding: l sums the probabilities in fp32.  They enter the second product with 11 bits as fp16 (fp16 caches, int8 codes),
 // about the output's own rounding with fp16 outputs and 8 times finer with bf16 ones; over bf16 caches, where 8 bits would
@@ -62,7 +63,11 @@ struct AttendArgs {
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int ITEM_COST = 3;   // of an item beside its units (loading q, adding up, writing), in units; 3 to 10 make 2 % of difference
 constexpr int SM_ROWS = 32;    // rows of partial results that an SM's CTAs may hold at a time
-constexpr float SLACK = 8.f;   // how far (log2) a score may pass the running maximum before it moves
+// How far (log2) a score may pass the running maximum before it moves, and how far below it the reference m lies.
+// fp16 weights use its range: 2^(SLACK + BELOW) = 2^15 at most, and 2^-25 / 2^BELOW = 2^-36 of the largest is the least.
+// bf16 ones have fp32's range.
+template <int TYPE> constexpr float SLACK = TYPE == FVS_F16 ? 4.f : 8.f;
+template <int TYPE> constexpr float BELOW = TYPE == FVS_F16 ? 11.f : 0.f;
 
 template <int D, int STORE, int NT_>
 struct Shape {
@@ -816,7 +821,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         for (int h = 0; h < 2; h++) {
                             float& y = s[j][t][2 * x + h];
                             y = on ? (I8 ? y * ks : y) : -INFINITY;
-                            moved |= y > m[t][h] + SLACK;
+                            moved |= y > m[t][h] + (SLACK<MT> + BELOW<MT>);
                         }
                 }
             }
@@ -827,7 +832,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     for (int x = 0; x < 2; x++) {
                         float y = m[t][x];
 #pragma unroll
-                        for (int j = 0; j < TILES; j++) y = fmaxf(y, fmaxf(s[j][t][x], s[j][t][x + 2]));
+                        for (int j = 0; j < TILES; j++) y = fmaxf(y, fmaxf(s[j][t][x], s[j][t][x + 2]) - BELOW<MT>);
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
                         const float f = y == -INFINITY ? 1.f : exp2_fast(m[t][x] - y);

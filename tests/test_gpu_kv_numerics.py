@@ -68,6 +68,32 @@ def ints(x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
 
+# ------------------------------------------------------------------------------------------------ weights
+
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (BF16, BF16), (F16, I8), (BF16, I8)])
+@pytest.mark.parametrize("bits", [12, 17, 22, 25.2, 29])
+def test_weights_far_below_the_largest(kv, dtype, store, bits):
+    """Keys without a value take nearly all of the weight; the others, 2^-bits of one of them, make the output."""
+    g = torch.Generator().manual_seed(int(bits))
+    n, page, dim = 4000, 16, 64
+    table, pages = full_table([n], page, g)
+    first = torch.zeros(pages * page, dtype=torch.bool)
+    t = torch.arange(n)
+    place = table[0].long()[t // page] * page + t % page
+    first[place[t % 32 == 3]] = True                                # in every unit of work
+    first = first.view(pages, 1, page, 1).to(DEV)
+    score = np.log(2) * bits                                        # <q, k> / 8 = 8 k for q = 1
+    k = torch.where(first, score / 8, 0.0) * torch.ones(pages, 1, page, dim, device=DEV)
+    v = (torch.rand(pages, 1, page, dim, generator=g).to(DEV) + 0.5) * 1000
+    if store == I8:
+        one = torch.ones(pages, 1, page, device=DEV)
+        cache = kv.PagedKV((first * 64 * torch.ones_like(k)).to(I8), torch.where(first, 0.0, v / 12).round().to(I8),
+                           one * float(score) / 8 / 64, one * 12)
+    else:
+        cache = kv.PagedKV(k.to(store), torch.where(first, 0.0, v).to(store))
+    close(cache, torch.ones(1, 2, dim, dtype=dtype, device=DEV), table.to(DEV), ints([n]))
+
+
 # ------------------------------------------------------------------------------------------------ scores over codes
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
