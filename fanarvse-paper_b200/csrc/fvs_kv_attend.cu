@@ -28,7 +28,8 @@
 // about the output's own rounding with fp16 outputs and 8 times finer with bf16 ones; over bf16 caches, where 8 bits would
 // add as much error as the output's rounding, as two bf16 numbers with 16 bits together (the product of both takes 0 to 3 %
 // longer).  int8 codes are exact in fp16 (see codes2); their key scale multiplies the fp32 score, their value scale the
-// probability, divided by the largest power of two met so far so that it stays in fp16's range; queries over int8 codes are
+// probability, and a power of two for each head brings that product to fp16's range, by the largest product met so far (by
+// the largest scale, one large row of no weight would take the others' bits); queries over int8 codes are
 // brought to fp16 by a power of two for each head.
 //
 // Measured on one B200 (6550 GB/s measured copy rate): 131071 bf16 keys of 8 heads of 128, 32 query heads, 103 to 106 us
@@ -64,10 +65,12 @@ constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int ITEM_COST = 3;   // of an item beside its units (loading q, adding up, writing), in units; 3 to 10 make 2 % of difference
 constexpr int SM_ROWS = 32;    // rows of partial results that an SM's CTAs may hold at a time
 // How far (log2) a score may pass the running maximum before it moves, and how far below it the reference m lies.
-// fp16 weights use its range: 2^(SLACK + BELOW) = 2^15 at most, and 2^-25 / 2^BELOW = 2^-36 of the largest is the least.
-// bf16 ones have fp32's range.
-template <int TYPE> constexpr float SLACK = TYPE == FVS_F16 ? 4.f : 8.f;
-template <int TYPE> constexpr float BELOW = TYPE == FVS_F16 ? 11.f : 0.f;
+// fp16 weights use its range: 2^(SLACK + BELOW) = 2^TOP at most, and 2^-25 / 2^BELOW = 2^-36 of the largest is the least.
+// bf16 ones have fp32's range.  Weights over int8 codes are multiplied by the value scale first, and that product has a
+// reference of its own with the same two distances.
+template <int STORE> constexpr float SLACK = STORE == FVS_BF16 ? 8.f : 4.f;
+template <int STORE> constexpr float BELOW = STORE == FVS_F16 ? 11.f : 0.f;
+constexpr float TOP = 15.f;
 
 template <int D, int STORE, int NT_>
 struct Shape {
@@ -152,6 +155,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^x of a whole number, exactly; 0 below fp32's normal range
+__device__ __forceinline__ float power2(float x) { return __uint_as_float((uint32_t)(127 + max(-127, min(127, (int)x))) << 23); }
 // weight of a part with maximum and sum `ml` in a join whose maximum is mx (a part of not-a-numbers alone keeps them)
 __device__ __forceinline__ float weight(float2 ml, float mx) {
     return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - mx);
@@ -740,9 +750,15 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
             return make_uint2(qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][0], qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][1]);
         };
         float m[NT][2], l[NT][2], o[D / 16][NT][4];
-        int vexp = 1;  // int8: value scales are divided by 2^(vexp - 126)
+        // int8: m is a whole number, the product of a weight and its value scale is at most 2^lim (in log2 units like m, a
+        // whole number too) and enters the matrix instructions times down = 2^(m + TOP - lim)
+        float lim[NT][2], down[NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; t++) m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
+        for (int t = 0; t < NT; t++) {
+            m[t][0] = m[t][1] = lim[t][0] = lim[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.f;
+            down[t][0] = down[t][1] = 1.f;
+        }
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
 #pragma unroll
@@ -804,7 +820,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
 #pragma unroll
                     for (int x = 0; x < 4; x++) s[j][t][x] = (s[j][t][x] + s2[t][x]) * mul[t][x & 1];
             }
-            float vs[TILES][2];
+            float vs[TILES][2], lv[TILES][2];  // int8: value scales, their log2
             bool moved = false;
 #pragma unroll
             for (int j = 0; j < TILES; j++) {
@@ -814,6 +830,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     const float* sc = (const float*)(stp + Sh::SCALES);
                     const float ks = I8 ? sc[key] : 1.f;
                     vs[j][x] = I8 ? sc[UNIT + key] : 1.f;
+                    lv[j][x] = I8 ? log2_fast(fabsf(vs[j][x])) : 0.f;
                     const bool on = (mask >> key) & 1;
 #pragma unroll
                     for (int t = 0; t < NT; t++)
@@ -821,7 +838,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         for (int h = 0; h < 2; h++) {
                             float& y = s[j][t][2 * x + h];
                             y = on ? (I8 ? y * ks : y) : -INFINITY;
-                            moved |= y > m[t][h] + (SLACK<MT> + BELOW<MT>);
+                            moved |= y > m[t][h] + (SLACK<STORE> + BELOW<STORE>);
+                            if (I8) moved |= y + lv[j][x] > lim[t][h];
                         }
                 }
             }
@@ -832,37 +850,31 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     for (int x = 0; x < 2; x++) {
                         float y = m[t][x];
 #pragma unroll
-                        for (int j = 0; j < TILES; j++) y = fmaxf(y, fmaxf(s[j][t][x], s[j][t][x + 2]) - BELOW<MT>);
+                        for (int j = 0; j < TILES; j++) y = fmaxf(y, fmaxf(s[j][t][x], s[j][t][x + 2]) - BELOW<STORE>);
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
-                        const float f = y == -INFINITY ? 1.f : exp2_fast(m[t][x] - y);
+                        float f;
+                        if (I8) {
+                            float g = -INFINITY;
+#pragma unroll
+                            for (int j = 0; j < TILES; j++) g = fmaxf(g, fmaxf(s[j][t][x] + lv[j][0], s[j][t][x + 2] + lv[j][1]));
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
+                            y = ceilf(y);
+                            g = fmaxf(fmaxf(lim[t][x], ceilf(g) + SLACK<STORE>), y + (TOP - 126.f));  // down <= 2^126
+                            l[t][x] *= power2(m[t][x] - y);
+                            f = power2(lim[t][x] - g);
+                            lim[t][x] = g;
+                            down[t][x] = power2(y + TOP - g);
+                        } else {
+                            f = y == -INFINITY ? 1.f : exp2_fast(m[t][x] - y);
+                            l[t][x] *= f;
+                        }
                         m[t][x] = y;
-                        l[t][x] *= f;
 #pragma unroll
                         for (int i = 0; i < D / 16; i++) o[i][t][x] *= f, o[i][t][x + 2] *= f;
                     }
                 }
-            }
-            if (I8) {
-                uint32_t big = 0;
-#pragma unroll
-                for (int j = 0; j < TILES; j++)
-#pragma unroll
-                    for (int x = 0; x < 2; x++) big = max(big, __float_as_uint(vs[j][x]) & 0x7fffffffu);
-                const int e = min(252, (int)(__reduce_max_sync(0xffffffffu, big) >> 23));
-                if (e > vexp) {
-                    const float f = e - vexp >= 126 ? 0.f : __uint_as_float((uint32_t)(127 - (e - vexp)) << 23);
-                    vexp = e;
-#pragma unroll
-                    for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int x = 0; x < 4; x++) o[i][t][x] *= f;
-                }
-                const float down = __uint_as_float((uint32_t)(253 - vexp) << 23);
-#pragma unroll
-                for (int j = 0; j < TILES; j++) vs[j][0] *= down, vs[j][1] *= down;
             }
 #pragma unroll
             for (int j = 0; j < TILES; j++) {
@@ -876,7 +888,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     float p2 = exp2_fast(s[j][t][2] - z0), p3 = exp2_fast(s[j][t][3] - z1);
                     l[t][0] += p0 + p2;
                     l[t][1] += p1 + p3;
-                    if (I8) p0 *= vs[j][0], p1 *= vs[j][0], p2 *= vs[j][1], p3 *= vs[j][1];
+                    if (I8) {  // in this order: the scale times down could be infinite
+                        p0 = p0 * vs[j][0] * down[t][0], p1 = p1 * vs[j][0] * down[t][1];
+                        p2 = p2 * vs[j][1] * down[t][0], p3 = p3 * vs[j][1] * down[t][1];
+                    }
                     if (SPLIT) {
                         pf[t][0] = transpose8x8(upper2(p0, p1));
                         pf[t][1] = transpose8x8(upper2(p2, p3));
@@ -937,7 +952,6 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                                     : (float*)(ring_all + WARPS * Sh::RING + warp * Sh::OBYTES);
         if (lane == 0) s_tile[warp] = (int)((uint8_t*)tile - ring_all);
         if (!solo) __syncthreads();
-        const float vup = I8 ? __uint_as_float((uint32_t)(vexp + 1) << 23) : 1.f;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -964,12 +978,12 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                     *(float2*)(a.parts + (2 * piece + (it.u == 0)) * Sh::PART + Sh::ROWS * D + 2 * row) = make_float2(mx, sum);
                 }
                 const bool none = f == 0.f;
-                f *= vup;
+                const float up = I8 ? power2(lim[t][x] - m[t][x] - TOP) : 1.f;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
                     float* p = tile + row * Sh::OS + (I8 ? (i / 2) * 32 + 4 * r + 2 * (i & 1) : i * 16 + r);
-                    p[0] = none ? 0.f : o[i][t][x] * f;
-                    p[I8 ? 1 : 8] = none ? 0.f : o[i][t][x + 2] * f;
+                    p[0] = none ? 0.f : o[i][t][x] * f * up;
+                    p[I8 ? 1 : 8] = none ? 0.f : o[i][t][x + 2] * f * up;
                 }
             }
         }

@@ -94,6 +94,54 @@ def test_weights_far_below_the_largest(kv, dtype, store, bits):
     close(cache, torch.ones(1, 2, dim, dtype=dtype, device=DEV), table.to(DEV), ints([n]))
 
 
+# ------------------------------------------------------------------------------------------------ value scales of codes
+
+@pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 16, 2.0 ** 20, 2.0 ** 24, 2.0 ** 40])
+@pytest.mark.parametrize("below", [60, 100])
+def test_large_value_scales_that_weigh_nothing(kv, ratio, below):
+    """Rows of a scale far above the others', at 2^-below of their weight, leave the others' bits alone."""
+    g = torch.Generator().manual_seed(33)
+    n, page, dim = 1000, 16, 64
+    table, pages = full_table([n, n], page, g)
+    cache = make_cache(kv, pages, 1, page, dim, I8, g)
+    cache.k.fill_(64)
+    cache.k_scale.fill_(0)
+    cache.v_scale.fill_(1 / 64)
+    t = torch.arange(7, n, 32)                                      # one in every unit of work, in one sequence at the end
+    for b, t in ((0, t), (1, torch.tensor([n - 1]))):
+        p, s = table[b].long()[t // page], t % page
+        cache.k_scale[p, 0, s] = -below * float(np.log(2)) / 8 / 64
+        cache.v_scale[p, 0, s] = ratio / 64
+    close(cache, torch.ones(2, 2, dim, dtype=BF16, device=DEV), table.to(DEV), ints([n, n]))
+
+
+def test_heads_that_weigh_rows_of_different_scale(kv):
+    """Query heads that share codes and prefer rows of different scale each keep their bits."""
+    g = torch.Generator().manual_seed(34)
+    n, page, dim, hq = 600, 16, 64, 8
+    table, pages = full_table([n], page, g)
+    cache = make_cache(kv, pages, 1, page, dim, I8, g)
+    t = torch.arange(n)
+    p, s = table[0].long()[t // page], t % page
+    cache.k[p, 0, s] = 0
+    cache.k[p, 0, s, t % hq] = 64                                   # head h prefers the tokens t = h mod 8
+    cache.k_scale.fill_(1 / 64)
+    cache.v_scale[p, 0, s] = (2.0 ** (-6.0 * (t % hq)) / 64).to(DEV)
+    q = torch.zeros(1, hq, dim)
+    q[0, torch.arange(hq), torch.arange(hq)] = 8 * 40               # scores of 40 and 0: 2^-57
+    close(cache, q.to(DEV, BF16), table.to(DEV), ints([n]))
+
+
+@pytest.mark.parametrize("log", [-126, -110, -60, 0, 60, 100, 103, 110])
+def test_value_scales_near_the_ends_of_fp32(kv, log):
+    g = torch.Generator().manual_seed(35)
+    table, pages = full_table([300, 1], 16, g)
+    cache = make_cache(kv, pages, 2, 16, 64, I8, g)
+    cache.v_scale.mul_(2.0 ** 5).mul_(2.0 ** log)                   # about 2^log of a code
+    q = torch.randn(2, 4, 64, generator=g).to(DEV, BF16)
+    close(cache, q, table.to(DEV), ints([300, 1]))
+
+
 # ------------------------------------------------------------------------------------------------ scores over codes
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
