@@ -24,11 +24,11 @@
 // rescale.  Weights that become fp16 are taken 2^BELOW larger than the softmax's, near fp16's upper end: without that a key at
 // 2^-25 of the largest weight vanished from the second product and not from l.
 //
-// Rounding: l sums the probabilities in fp32.  They enter the second product with 11 bits as fp16 (fp16 caches, int8 codes),
-// about the output's own rounding with fp16 outputs and 8 times finer with bf16 ones; over bf16 caches, where 8 bits would
-// add as much error as the output's rounding, as two bf16 numbers with 16 bits together (the product of both takes 0 to 3 %
-// longer).  int8 codes are exact in fp16 (see codes2); their key scale multiplies the fp32 score, their value scale the
-// probability, and a power of two for each head brings that product to fp16's range, by the largest product met so far (by
+// Rounding: l sums the probabilities in fp32.  They enter the second product as two 16-bit numbers, two fp16 ones with 21 bits
+// together (fp16 caches, int8 codes) or two bf16 ones with 16: a single one would add as much error as the output's own
+// rounding (fp16 outputs: 1.4 times the error against 64 bits).  The product of both takes 0 to 3 % longer over 16-bit caches
+// and 9 % over long int8 ones (144 -> 156 us).  int8 codes are exact in fp16 (see codes2); their key scale multiplies the
+// fp32 score, their value scale the probability, and a power of two for each head brings that product to fp16's range, by the largest product met so far (by
 // the largest scale, one large row of no weight would take the others' bits); queries over int8 codes are
 // brought to fp16 by a power of two for each head.
 //
@@ -166,12 +166,23 @@ __device__ __forceinline__ float power2(float x) { return __uint_as_float((uint3
 __device__ __forceinline__ float weight(float2 ml, float mx) {
     return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - mx);
 }
-// A probability as the sum of two bf16 numbers: its upper bits, and the rest, which stays above zero so that an infinite value
-// times it is no not-a-number
-__device__ __forceinline__ uint32_t upper2(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+// A weight as the sum of two 16-bit numbers: its upper bits, and the rest.  Beside values that may be infinite (POS) the rest
+// stays above zero, so that an infinite value times it is no not-a-number.
+template <int TYPE>
+constexpr uint32_t UPPER = TYPE == FVS_F16 ? 0xffffe000u : 0xffff0000u;
+template <int TYPE>
+__device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & UPPER<TYPE>); }
+template <int TYPE>
+__device__ __forceinline__ uint32_t upper2(float a, float b) {
+    if (TYPE == FVS_F16) return Elem<TYPE>::down(upper<TYPE>(a), upper<TYPE>(b));
+    return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}
+template <int TYPE, bool POS>
 __device__ __forceinline__ uint32_t rest2(float a, float b) {
-    const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-    return Elem<FVS_BF16>::down(fmaxf(ra, 1.2e-38f), fmaxf(rb, 1.2e-38f));
+    float ra = a - upper<TYPE>(a), rb = b - upper<TYPE>(b);
+    constexpr float LEAST = TYPE == FVS_F16 ? 0x1p-24f : 1.2e-38f;  // the smallest number, the smallest normal one
+    if (POS) ra = fmaxf(ra, LEAST), rb = fmaxf(rb, LEAST);
+    return Elem<TYPE>::down(ra, rb);
 }
 // Two codes as fp16: the byte u = code + 128 under 0x64 is 1024 + u, and 1152 less is the code, exactly.  (Leaving the 128 in
 // the products and taking it out of their sums spares the subtraction, but the sums then round at 128 sum |q|: a row with
@@ -360,7 +371,6 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
     using Sh = Shape<D, STORE, NT>;
     constexpr bool I8 = Sh::I8;
     constexpr int MT = I8 ? FVS_F16 : TYPE;  // type of the matrix instructions' operands
-    constexpr bool SPLIT = MT == FVS_BF16;   // probabilities in two parts
     constexpr int S = Sh::S, UNIT = Sh::UNIT, TILES = Sh::TILES, TAKEN = Sh::TAKEN;
     extern __shared__ __align__(128) uint8_t ring_all[];
     __shared__ int64_t s_sum[WARPS];
@@ -879,7 +889,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
 #pragma unroll
             for (int j = 0; j < TILES; j++) {
                 if (TILES > 1 && ((mask >> (16 * j)) & 0xffffu) == 0) continue;  // its rows were not copied
-                // p, and p as the B operand of the second product
+                // p, and p's two parts as the B operands of the second product
                 uint32_t pf[NT][2], pl[NT][2];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
@@ -892,15 +902,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         p0 = p0 * vs[j][0] * down[t][0], p1 = p1 * vs[j][0] * down[t][1];
                         p2 = p2 * vs[j][1] * down[t][0], p3 = p3 * vs[j][1] * down[t][1];
                     }
-                    if (SPLIT) {
-                        pf[t][0] = transpose8x8(upper2(p0, p1));
-                        pf[t][1] = transpose8x8(upper2(p2, p3));
-                        pl[t][0] = transpose8x8(rest2(p0, p1));
-                        pl[t][1] = transpose8x8(rest2(p2, p3));
-                    } else {
-                        pf[t][0] = transpose8x8(Elem<MT>::down(p0, p1));
-                        pf[t][1] = transpose8x8(Elem<MT>::down(p2, p3));
-                    }
+                    pf[t][0] = transpose8x8(upper2<MT>(p0, p1));
+                    pf[t][1] = transpose8x8(upper2<MT>(p2, p3));
+                    pl[t][0] = transpose8x8(rest2<MT, !I8>(p0, p1));
+                    pl[t][1] = transpose8x8(rest2<MT, !I8>(p2, p3));
                 }
                 // O^T += V^T P^T
                 if (I8) {
@@ -915,7 +920,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                             const uint32_t x = __byte_perm(v0, v1, h ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, h ? 0x7362 : 0x5140);
                             const uint32_t f[4] = {codes2(x, LOW), codes2(x, HIGH), codes2(y, LOW), codes2(y, HIGH)};
 #pragma unroll
-                            for (int t = 0; t < NT; t++) mma<MT>(o[2 * k + h][t], f, pf[t][0], pf[t][1]);
+                            for (int t = 0; t < NT; t++) {
+                                mma<MT>(o[2 * k + h][t], f, pf[t][0], pf[t][1]);
+                                mma<MT>(o[2 * k + h][t], f, pl[t][0], pl[t][1]);
+                            }
                         }
                     }
                 } else {
@@ -928,7 +936,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
                             mma<MT>(o[i][t], f, pf[t][0], pf[t][1]);
-                            if (SPLIT) mma<MT>(o[i][t], f, pl[t][0], pl[t][1]);
+                            mma<MT>(o[i][t], f, pl[t][0], pl[t][1]);
                         }
                     }
                 }

@@ -94,6 +94,24 @@ def test_weights_far_below_the_largest(kv, dtype, store, bits):
     close(cache, torch.ones(1, 2, dim, dtype=dtype, device=DEV), table.to(DEV), ints([n]))
 
 
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (F16, I8), (BF16, I8), (BF16, BF16)])
+def test_weights_are_not_cut(kv, dtype, store):
+    """Two keys whose values nearly cancel show how many bits of their weights reach the output."""
+    g = torch.Generator().manual_seed(31)
+    B, dim, page = 256, 64, 16
+    table = torch.arange(B, dtype=torch.int32).view(B, 1)
+    size = torch.rand(B, 1, page, generator=g) * 0.25
+    v = torch.ones(B, 1, page, dim) * 96
+    v[:, :, 1] = -v[:, :, 0] * torch.exp(8 * (size[:, :, 0] - size[:, :, 1]))[..., None]
+    size, v = size.to(DEV), v.to(DEV)
+    if store == I8:
+        cache = kv.PagedKV(torch.full((B, 1, page, dim), 64, dtype=I8, device=DEV), (v / 8).round().to(I8), size / 64,
+                           torch.full_like(size, 8))
+    else:
+        cache = kv.PagedKV((size[..., None] * torch.ones(dim, device=DEV)).to(store), v.to(store))
+    close(cache, torch.ones(B, 1, dim, dtype=dtype, device=DEV), table.to(DEV), ints([2] * B))
+
+
 # ------------------------------------------------------------------------------------------------ value scales of codes
 
 @pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 16, 2.0 ** 20, 2.0 ** 24, 2.0 ** 40])
@@ -189,3 +207,17 @@ def test_value_rows_of_codes_that_are_not_finite(kv):
     cache.append(x, odd, table, ints([123]))
     out, lse = cache.attend(torch.randn(2, 2, 64, generator=g).to(DEV, F16), table, ints([200, 200]))
     assert torch.isnan(out[0]).all() and torch.isfinite(lse).all() and torch.isfinite(out[1]).all()
+
+
+def test_infinite_fp16_values(kv):
+    """A visible infinite value whose weight has no lower half gives an infinity, not a not-a-number."""
+    g = torch.Generator().manual_seed(39)
+    table, pages = full_table([50], 16, g)
+    cache = make_cache(kv, pages, 1, 16, 64, F16, g)
+    cache.k.zero_()                                                 # all weights are the same power of two before the end
+    p = table[0].long()
+    cache.v[p[1], 0, 4, 9] = float("inf")
+    cache.v[p[2], 0, 1, 3] = float("-inf")
+    out, _ = cache.attend(torch.ones(1, 2, 64, dtype=F16, device=DEV), table.to(DEV), ints([50]))
+    assert (out[0, :, 9] == float("inf")).all() and (out[0, :, 3] == float("-inf")).all()
+    assert torch.isfinite(out[0]).sum() == 2 * 62
