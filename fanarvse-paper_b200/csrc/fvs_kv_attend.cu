@@ -27,10 +27,10 @@
 // Rounding: l sums the probabilities in fp32.  They enter the second product as two 16-bit numbers, two fp16 ones with 21 bits
 // together (fp16 caches, int8 codes) or two bf16 ones with 16: a single one would add as much error as the output's own
 // rounding (fp16 outputs: 1.4 times the error against 64 bits).  The product of both takes 0 to 3 % longer over 16-bit caches
-// and 9 % over long int8 ones (144 -> 156 us).  int8 codes are exact in fp16 (see codes2); their key scale multiplies the
-// fp32 score, their value scale the probability, and a power of two for each head brings that product to fp16's range, by the largest product met so far (by
-// the largest scale, one large row of no weight would take the others' bits); queries over int8 codes are
-// brought to fp16 by a power of two for each head.
+// and 9 % over long int8 ones (144 -> 156 us).  int8 codes are exact in fp16 (see codes2).  Their key scale multiplies the
+// fp32 score, their value scale the probability, and a power of two for each head brings that product to fp16's range, by the
+// largest product met so far (by the largest scale, one large row of no weight would take the others' bits).  Queries over
+// int8 codes are brought to fp16 by a power of two for each head, their largest element to the upper end of its range.
 //
 // Measured on one B200 (6550 GB/s measured copy rate): 131071 bf16 keys of 8 heads of 128, 32 query heads, 103 to 106 us
 // (5.1 TB/s), four such sequences 340 us (6.3 TB/s); 64 sequences of 1 to 8192 keys 66 us (4.7 TB/s); int8 codes, 48
@@ -722,8 +722,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = max(1, min(230, (int)(__float_as_uint(top) >> 23)));  // 2^(e - 127) <= top
-                const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                // the largest element (2^(e - 127) at least) to 2^14: one 2^-39 of it still has a bit in fp16
+                const int e = max(15, min(254, (int)(__float_as_uint(top) >> 23)));
+                const float down = __uint_as_float((uint32_t)(268 - e) << 23);
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const float2 x = Elem<TYPE>::up(raw[k].x), y = Elem<TYPE>::up(raw[k].y);
@@ -735,7 +736,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][1] = f1;
                     }
                 }
-                const float up = a.scale2 * __uint_as_float((uint32_t)e << 23);
+                const float up = a.scale2 * __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
                 for (int x = 0; x < 2; x++) mul[t][x] = __shfl_sync(0xffffffffu, up, c4 * 8 + 4 * x);
             } else {

@@ -177,6 +177,18 @@ def test_scores_of_rows_with_one_large_element(kv, dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+def test_queries_with_one_large_element(kv, dtype):
+    """Elements far below the head's largest keep their bits."""
+    g = torch.Generator().manual_seed(36)
+    B, page, dim = 64, 16, 64
+    cache = make_cache(kv, B, 1, page, dim, I8, g)
+    cache.k[..., 9] = 0
+    q = torch.randn(B, 8, dim, generator=g) * 2.0 ** -6
+    q[..., 9] = 2.0 ** 15
+    close(cache, q.to(DEV, dtype), torch.arange(B).view(B, 1).to(DEV, torch.int32), ints([1] * B))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("odd", [float("inf"), float("nan")])
 def test_key_rows_of_codes_that_are_not_finite(kv, dtype, odd):
     """A key row stored with an infinity or a not-a-number makes every head that sees it not-a-number, and nothing else."""
