@@ -112,6 +112,24 @@ def test_weights_are_not_cut(kv, dtype, store):
     close(cache, torch.ones(B, 1, dim, dtype=dtype, device=DEV), table.to(DEV), ints([2] * B))
 
 
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (BF16, I8)])
+def test_scores_that_keep_rising(kv, dtype, store):
+    """Every unit of work passes the running maximum, by steps small and large."""
+    g = torch.Generator().manual_seed(32)
+    n, page, dim = 1500, 32, 64
+    table, pages = full_table([n] * 3, page, g)
+    cache = make_cache(kv, pages, 1, page, dim, store, g)
+    for b, step in enumerate((0.001, 0.02, 0.4)):
+        t = torch.arange(n)
+        p, s = table[b].long()[t // page], t % page
+        if store == I8:
+            cache.k[p, 0, s] = 32
+            cache.k_scale[p, 0, s] = (t * step / 8 / 32).to(DEV)
+        else:
+            cache.k[p, 0, s] = (t * step / 8)[:, None].to(DEV, store)
+    close(cache, torch.ones(3, 2, dim, dtype=dtype, device=DEV), table.to(DEV), ints([n] * 3))
+
+
 # ------------------------------------------------------------------------------------------------ value scales of codes
 
 @pytest.mark.parametrize("ratio", [2.0 ** 12, 2.0 ** 16, 2.0 ** 20, 2.0 ** 24, 2.0 ** 40])
@@ -233,3 +251,47 @@ def test_infinite_fp16_values(kv):
     out, _ = cache.attend(torch.ones(1, 2, 64, dtype=F16, device=DEV), table.to(DEV), ints([50]))
     assert (out[0, :, 9] == float("inf")).all() and (out[0, :, 3] == float("-inf")).all()
     assert torch.isfinite(out[0]).sum() == 2 * 62
+
+
+# ------------------------------------------------------------------------------------------------ large calls, wide heads
+
+@pytest.mark.parametrize("dtype,store,dim,group", [(BF16, I8, 128, 8), (F16, F16, 64, 4), (F16, I8, 64, 12)])
+def test_large_calls(kv, dtype, store, dim, group):
+    """Calls whose pieces are taken as blocks finish, with items cut at uneven places; then a small call on the same stream.
+    The sequences share the pages of one pool, each in an order of its own."""
+    g = torch.Generator().manual_seed(dim + group)
+    heads, page, pool, B = 8, 64, 256, 160
+    cache = make_cache(kv, pool, heads, page, dim, store, g)
+    table = torch.stack([torch.randperm(pool, generator=g) for _ in range(B)]).to(DEV, torch.int32)
+    lens = torch.randint(2000, pool * page + 1, (B,), generator=g, dtype=torch.int32)
+    lens[3], lens[40], lens[41], lens[B - 1] = 0, 1, 100, pool * page
+    units = int((lens.long() // (32 if store == I8 or dim == 64 else 16) + 3).sum()) * heads * -(-group // 16)
+    assert units >= 512 * 444, "too small a call to be divided that way"
+    q = torch.randn(B, heads * group, dim, generator=g).to(DEV, dtype)
+    lens = lens.to(DEV)
+    first = cache.attend(q, table, lens)
+    for _ in range(2):
+        again = cache.attend(q, table, lens)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    small = cache.attend(q[40:42].contiguous(), table[40:42].contiguous(), lens[40:42].contiguous())
+    some = torch.tensor([3, 40, 41, 7, 90, B - 1], device=DEV)
+    heads_seen = [0, heads * group // 2 + 1, heads * group - 1]
+    # the oracle takes the sampled heads one at a time, each over its own key head
+    for h in heads_seen:
+        kh = h // group
+        scales = [None if s is None else s[:, kh:kh + 1] for s in (cache.k_scale, cache.v_scale)]
+        part = kv.PagedKV(cache.k[:, kh:kh + 1], cache.v[:, kh:kh + 1], *scales)
+        pick = lambda x: x[some][:, h:h + 1].contiguous()  # noqa: E731
+        close(part, pick(q), table[some], lens[some], got=(pick(first[0]), pick(first[1])))
+    close(cache, q[40:42].contiguous(), table[40:42], lens[40:42], got=small)
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (BF16, BF16), (BF16, I8)])
+@pytest.mark.parametrize("dim,group", [(192, 4), (256, 16), (256, 5)])
+def test_wide_heads_over_long_sequences(kv, dtype, store, dim, group):
+    g = torch.Generator().manual_seed(dim + group)
+    lens = [5000, 3000, 1, 0, 4099]
+    table, pages = full_table(lens, 48, g)
+    cache = make_cache(kv, pages, 1, 48, dim, store, g)
+    q = torch.randn(len(lens), group, dim, generator=g).to(DEV, dtype)
+    close(cache, q, table.to(DEV), ints(lens))
