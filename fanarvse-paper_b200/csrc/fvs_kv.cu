@@ -160,8 +160,14 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
 #pragma unroll
             for (int o = L / 2; o; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
             if (!live) continue;
-            // no reciprocal of a subnormal: it would be infinite
-            const float inv = m > 0.f ? fminf(__fmul_rn(__frcp_rn(m), 127.f), 3.402823466e38f) : 0.f;
+            const float scale = m < 0x1p-126f ? 0.f : __fmul_rn(m, 1.f / 127.f);
+            if (m < 0x1p-100f) {  // 127 / m could be infinite: the row 2^64 larger has the same codes.  Subnormal rows: zeros
+                const float up = m < 0x1p-126f ? 0.f : 0x1p64f;
+                m *= up;
+#pragma unroll
+                for (int n = 0; n < 8; n++) x0[n] *= up, x1[n] *= up;
+            }
+            const float inv = m > 0.f ? __fmul_rn(__frcp_rn(m), 127.f) : 0.f;
             uint32_t code[4];
 #pragma unroll
             for (int n = 0; n < 4; n++) {
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
             int8_t* p = (int8_t*)dst + to + u * step;
             *(uint2*)(p + e0) = make_uint2(code[0], code[1]);
             *(uint2*)(p + e1) = make_uint2(code[2], code[3]);
-            if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[to_scale + u * AT_ONCE * a.c.scale_head_stride] = __fmul_rn(m, 1.f / 127.f);
+            if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[to_scale + u * AT_ONCE * a.c.scale_head_stride] = scale;
         } else if (live) {
             if (turns) raw[u][0] = down8<TYPE>(x0), raw[u][1] = down8<TYPE>(x1);
             if (!there) raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);  // a query without a place

@@ -480,7 +480,7 @@ typedef struct fvs_kv_cache {
  * pairs (i, i + rot / 2) or (2i, 2i + 1): (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once.  q_out is
  * contiguous [tokens, hq, dim] and may be q; zeros for a token without a place.
  * Codes of an FVS_I8 cache: scale = amax * (1 / 127), code = rint(x * ((1 / amax) * 127)) in fp32, codes and scale 0
- * for a row of zeros; a row with an infinity or a not-a-number reads back as not-a-numbers.
+ * for a row of zeros or of magnitudes below 2^-126; a row with an infinity or a not-a-number reads back as not-a-numbers.
  */
 #define FVS_PAIRS_HALVES 0
 #define FVS_PAIRS_NEIGHBOURS 1

@@ -1,6 +1,6 @@
-"""Attention over the paged cache where its arithmetic could lose something: weights far below the largest, value scales and
-keys of very different size, rows that hold infinities; and calls large enough to take the kernel's other ways of
-dividing the work.
+"""The paged cache where its arithmetic could lose something: attention weights far below the largest, value scales and keys
+of very different size, rows that hold infinities, codes of very small rows; and calls large enough to take the attention
+kernel's other ways of dividing the work.
 
 Bounds, from the arithmetic alone, with u the unit roundoff of the output type and n the keys of a sequence:
 * a score is a sum of exact products (codes, 16-bit numbers), 16 to an instruction, in D / 16 instructions, each of which may
@@ -295,3 +295,31 @@ def test_wide_heads_over_long_sequences(kv, dtype, store, dim, group):
     cache = make_cache(kv, pages, 1, 48, dim, store, g)
     q = torch.randn(len(lens), group, dim, generator=g).to(DEV, dtype)
     close(cache, q, table.to(DEV), ints(lens))
+
+
+# ------------------------------------------------------------------------------------------------ append of codes
+
+@pytest.mark.parametrize("top", [2.0 ** -126, 1.3e-38, 1e-37, 3e-37, 3.7e-37, 1e-36, 2.0 ** -100, 7.8e-31, 1e-30])
+@pytest.mark.parametrize("dim", [64, 96])
+def test_append_of_small_rows(kv, top, dim):
+    """Rows of a small largest magnitude: each code within half a step (and 2^-20 of 127 steps of fp32 rounding), the scale
+    within half of fp32's smallest number."""
+    g = torch.Generator().manual_seed(41)
+    cache = kv.PagedKV.empty(2, 2, 16, dim, dtype=I8)
+    x = ((torch.rand(20, 2, dim, generator=g) * 2 - 1) * top).to(DEV, BF16)
+    x[:, :, 5] = top
+    table, idx = torch.tensor([[1, 0]] * 20, dtype=torch.int32, device=DEV), torch.arange(20, dtype=torch.int32, device=DEV)
+    cache.append(x, x, table, idx)
+    want = c(x)
+    step = np.abs(want).max(-1, keepdims=True) / 127
+    bound = 0.5 * step + 2.0 ** -20 * 127 * step + 127 * 2.0 ** -149
+    for got in cache.read(table, idx):
+        assert (np.abs(c(got) - want) <= bound).all()
+
+
+def test_append_of_subnormal_rows_stores_zeros(kv):
+    cache = kv.PagedKV.empty(1, 1, 16, 64, dtype=I8)
+    x = torch.full((1, 1, 64), 2.0 ** -127, device=DEV, dtype=BF16)
+    table, idx = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([2], dtype=torch.int32, device=DEV)
+    cache.append(x, x, table, idx)
+    assert not cache.k.any() and not cache.k_scale.any() and not cache.v.any() and not cache.v_scale.any()
