@@ -135,7 +135,8 @@ class PagedKV:
     # ---------------------------------------------------------------- the operators
     def append(self, k, v, table, idx, seq=None, pos=None, rope=None, pairs="halves", q=None, q_out=None):
         """Stores k, v [n, heads, dim] of n new tokens at logical places idx [n] (negative: not stored) of sequences seq
-        [n] (default: token i is sequence i's).  rope: (cos, sin), fp32 [positions, rot / 2]: the first rot elements of the
+        [n] (default: token i is sequence i's).  The places of a call are distinct: where two tokens meet, the row is
+        undefined afterwards.  rope: (cos, sin), fp32 [positions, rot / 2]: the first rot elements of the
         heads of k and of q [n, any, dim] are rotated at positions pos [n] (default idx), pairs "halves" (i, i + rot / 2)
         or "neighbours" (2i, 2i + 1).  Returns q_out, the rotated q (contiguous, default a new tensor, may be q; zeros for
         tokens that have no place), or None without q."""

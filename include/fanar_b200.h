@@ -474,7 +474,9 @@ typedef struct fvs_kv_cache {
 /*
  * Appends the keys k and values v [tokens, heads, dim] (type: FVS_F16 or FVS_BF16, the cache's own unless that is
  * FVS_I8; token and head strides in elements) of new tokens: token n goes to logical place idx[n] of sequence seq[n]
- * (seq NULL: sequence n).  idx[n] < 0 or a hole: nothing is stored.  Two tokens at one place: either one is kept.
+ * (seq NULL: sequence n).  idx[n] < 0 or a hole: nothing is stored.  Two tokens of a call at one place write it side by
+ * side: what it holds afterwards is undefined (parts of each, codes of one under the scale of the other); every other
+ * place is as it should be.
  * Before that the first `rot` elements of each key head (rot a multiple of 16, <= dim; 0: none) and of each head of q
  * [tokens, hq, dim] (hq 0: none) are rotated by cos / sin [positions, rot / 2] at position pos[n] (pos NULL: idx[n]),
  * pairs (i, i + rot / 2) or (2i, 2i + 1): (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once.  q_out is
