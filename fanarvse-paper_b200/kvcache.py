@@ -246,9 +246,17 @@ class PagedKV:
 def passage_table(ids, pages_of, own=None):
     """Page table rows for found passages: ids [B, k] as `search` returns them (-1: none), pages_of int32 [N, m] the
     pages of each passage in order (-1 after its last), own int32 [B, w] the pages of each sequence's own tokens ->
-    int32 [B, k * m + w].  The own tokens begin at logical token k * m * page."""
-    B = ids.shape[0]
+    int32 [B, k * m + w].  The own tokens begin at logical token k * m * page.  An id that pages_of has no row for is a
+    passage that is not there, like -1: its pages are holes."""
+    _need(ids.dim() == 2 and not ids.is_floating_point(), "ids are whole numbers [sequences, passages of each]")
     _need(pages_of.dtype == torch.int32 and pages_of.dim() == 2, "pages_of is int32 [passages, pages of each]")
-    rows = pages_of[ids.clamp(min=0).long()]
-    rows = torch.where((ids >= 0)[..., None], rows, torch.full_like(rows, -1)).reshape(B, -1)
+    B, k = ids.shape
+    _need(own is None or (own.dtype == torch.int32 and own.dim() == 2 and own.shape[0] == B),
+          f"own is int32 [{B}, pages of each]")
+    N, m = pages_of.shape
+    if N == 0:
+        rows = pages_of.new_full((B, k * m), -1)
+    else:
+        there = (ids >= 0) & (ids < N)
+        rows = pages_of[ids.clamp(0, N - 1).long()].masked_fill(~there[..., None], -1).reshape(B, k * m)
     return rows if own is None else torch.cat([rows, own], 1)

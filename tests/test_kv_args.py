@@ -112,6 +112,30 @@ def test_passage_table():
         f(torch.tensor([[1]]), pages_of.long())
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_passage_table_ids_without_a_row(dtype):
+    """Ids outside pages_of are holes (nothing is indexed with them), whatever the batch or the number of passages."""
+    f = pkg("kvcache").passage_table
+    pages_of = torch.tensor([[0, 1], [2, -1]], dtype=torch.int32)
+    own = torch.tensor([[7], [8]], dtype=torch.int32)
+    ids = torch.tensor([[2, 1, -7], [0, 2 ** 31 - 1, -1]], dtype=dtype)
+    assert f(ids, pages_of, own).tolist() == [[-1, -1, 2, -1, -1, -1, 7], [0, 1, -1, -1, -1, -1, 8]]
+    for b, k, n, m, w in ((0, 3, 2, 2, 1), (2, 0, 2, 2, 1), (2, 3, 0, 2, 1), (2, 3, 2, 0, 1), (0, 0, 0, 0, 0)):
+        got = f(torch.zeros(b, k, dtype=dtype), torch.zeros(n, m, dtype=torch.int32), torch.zeros(b, w, dtype=torch.int32))
+        assert got.shape == (b, k * m + w) and got.dtype == torch.int32
+        if n == 0:
+            assert (got[:, :k * m] == -1).all()
+
+
+def test_passage_table_refusals():
+    f = pkg("kvcache").passage_table
+    ids, pages_of, own = torch.zeros(2, 1, dtype=torch.int64), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int32)
+    for args in ((ids, pages_of, own.long()), (ids, pages_of, own[:1]), (ids, pages_of, own[0]), (ids.float(), pages_of),
+                 (ids[0], pages_of), (ids, pages_of[0])):
+        with pytest.raises(ValueError):
+            f(*args)
+
+
 def test_oracle_attention_against_torch():
     g = torch.Generator().manual_seed(0)
     q = torch.randn(2, 4, 64, generator=g, dtype=torch.float64)
