@@ -236,9 +236,11 @@ class PagedKV:
         return held
 
     def check_status(self):
-        """Raises if a call since the last check met an index outside its table (synchronises)."""
+        """Raises if a call since the last check, on any stream, met an index outside its table (waits for the GPU)."""
+        torch.cuda.synchronize(self.device)
         if int(self.status.item()) != 0:
             self.status.zero_()
+            torch.cuda.synchronize(self.device)  # so that a call on any stream from here on is seen
             raise _lib.FvsError("paged cache: an index was outside its table (page, sequence, token or position); "
                                 "that access was skipped")
 
