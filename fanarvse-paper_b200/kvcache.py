@@ -7,8 +7,8 @@ token per sequence, `read` gives stored rows back as floating point.  The refere
 the ids.
 
 Every call runs on the current torch stream, neither synchronises nor reads device memory on the host, and can be
-captured into a CUDA graph.  Wrong arguments raise; an index outside its table is skipped on the device and reported by
-`check_status()`.
+captured into a CUDA graph.  The operators have no gradients and refuse inputs that require one.  Wrong arguments raise;
+an index outside its table is skipped on the device and reported by `check_status()`.
 """
 from __future__ import annotations
 
@@ -30,6 +30,11 @@ _WORK = {}  # (GPU, stream) -> workspace of attend
 def _need(cond, what):
     if not cond:
         raise ValueError(what)
+
+
+def _no_gradient(x, what):
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which the cache's operators do not have (torch.no_grad())")
 
 
 class PagedKV:
@@ -63,6 +68,9 @@ class PagedKV:
                   "k_scale and v_scale are fp32 [pages, heads, page] with equal strides")
         _need(fill is None or (fill.dtype == torch.int32 and fill.shape == k.shape[:1] and fill.is_contiguous()
                                and fill.device == k.device), "fill is a contiguous int32 [pages]")
+        for x, what in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            if x is not None:
+                _no_gradient(x, what)
         self.k, self.v, self.k_scale, self.v_scale, self.fill = k, v, k_scale, v_scale, fill
         self.pages, self.heads, self.page, self.dim = k.shape
         self.device, self.dtype = k.device, k.dtype
@@ -110,6 +118,8 @@ class PagedKV:
         if not (len(shape) == 3 and shape[0] == n and shape[2] == self.dim and (heads is None or shape[1] == heads)
                 and x.get_device() == self._index):
             raise ValueError(f"{what} is [{n}, {heads or 'heads'}, {self.dim}] on the cache's GPU")
+        if x.requires_grad:
+            _no_gradient(x, what)
         s0, s1, s2 = x.stride()
         at = x.data_ptr()
         if s2 != 1 or s0 % 8 or s1 % 8 or at % 16:
@@ -158,6 +168,9 @@ class PagedKV:
             if not (cos.dtype is sin.dtype is torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
                     and cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == self._index):
                 raise ValueError("rope is two contiguous fp32 [positions, rot / 2] on the cache's GPU")
+            if cos.requires_grad or sin.requires_grad:
+                for x in rope:
+                    _no_gradient(x, "rope")
             positions, rot = cos.shape[0], 2 * cos.shape[1]
             if rot % 16 or not 0 < rot <= self.dim or positions < 1:
                 raise ValueError(f"rotation of {rot} elements: a multiple of 16, at most {self.dim}")

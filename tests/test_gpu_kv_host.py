@@ -34,3 +34,27 @@ def test_check_status_sees_calls_of_other_streams(kv):
         cache.check_status()
     cache.read(table, idx)
     cache.check_status()
+
+
+def test_inputs_that_require_gradients_are_refused(kv):
+    """Where gradients are recorded; under no_grad the same calls run."""
+    g = torch.Generator().manual_seed(1)
+    table, pages = full_table([20, 30], 16, g)
+    cache = make_cache(kv, pages, 1, 16, 64, F16, g)
+    table, n = table.to(DEV), ints([20, 30])
+    plain = torch.randn(2, 1, 64, generator=g).to(DEV, F16)
+    x = plain.clone().requires_grad_()
+    cs = torch.ones(40, 32, device=DEV), torch.zeros(40, 32, device=DEV)
+    learnt = cs[0].clone().requires_grad_()
+    calls = [lambda: cache.attend(x, table, n), lambda: cache.append(x, plain, table, n - 1),
+             lambda: cache.append(plain, x * 2, table, n - 1), lambda: cache.append(plain, plain, table, n - 1, q=x),
+             lambda: cache.append(plain, plain, table, n - 1, rope=(learnt, cs[1])),
+             lambda: kv.PagedKV(cache.k.clone().requires_grad_(), cache.v)]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        for call in calls:
+            call()
+        out, _ = cache.attend(x, table, n)
+    assert torch.equal(out, cache.attend(plain, table, n)[0]) and not out.requires_grad
