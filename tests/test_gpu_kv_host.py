@@ -58,3 +58,34 @@ def test_inputs_that_require_gradients_are_refused(kv):
             call()
         out, _ = cache.attend(x, table, n)
     assert torch.equal(out, cache.attend(plain, table, n)[0]) and not out.requires_grad
+
+
+def test_release_workspaces(kv):
+    """Memory held for streams comes back, calls in flight finish, and the next call works as before."""
+    g = torch.Generator().manual_seed(2)
+    table, pages = full_table([9000, 7000], 64, g)
+    cache = make_cache(kv, pages, 2, 64, 128, BF16, g)
+    table, n = table.to(DEV), ints([9000, 7000])
+    q = torch.randn(2, 8, 128, generator=g).to(DEV, BF16)
+    want = cache.attend(q, table, n)
+    kv.release_workspaces()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    out, lse = torch.empty_like(want[0]), torch.empty_like(want[1])
+    for stream in (torch.cuda.current_stream(), s):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                cache.attend(q, table, n, out=out, lse=lse)
+        held = torch.cuda.memory_allocated()
+        assert held > before + 2 ** 23
+        kv.release_workspaces()
+        assert torch.cuda.memory_allocated() <= held - 2 ** 23
+        with torch.cuda.stream(stream):
+            torch.full((2 ** 23,), 255, dtype=torch.uint8, device=DEV)          # in the memory that was given back
+            got = cache.attend(q, table, n)
+        stream.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        kv.release_workspaces()
