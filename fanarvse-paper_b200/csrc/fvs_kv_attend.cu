@@ -93,22 +93,21 @@ struct Shape {
     static constexpr int MASK = SCALES + (I8 ? 8 * UNIT : 0);  // of the word of visible keys
     static constexpr int STAGE = MASK + 16;
     static constexpr int OS = D + 4;                 // row stride (floats) of a staged output tile
-    static constexpr int OBYTES = ROWS * OS * 4;
-    static constexpr bool O_IN_RING = OBYTES <= STAGE;
+    static_assert(ROWS * OS * 4 <= STAGE, "an output tile fits a ring slot");
     static constexpr bool Q_SMEM = D > 128 && NT > 1;         // q's fragments would not fit the registers
+    static_assert(!(I8 && Q_SMEM), "not built: see launch");
     static constexpr int QBYTES = Q_SMEM ? ROWS * D * 2 : 0;
-    static constexpr int FIXED = (O_IN_RING ? 0 : WARPS * OBYTES) + QBYTES;
     // CTAs per SM: three (12 warps hide each other's latencies; 168 registers a thread) where two stages fit: 64 ragged
     // sequences take 66 us against 74 with two CTAs of three stages, 131071 keys 108 against 136
     static constexpr int CTAS = NT == 1 && D <= 128 && !(I8 && D == 96) ? 3 : RB <= 256 && !Q_SMEM ? 2 : 1;
-    static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 2560 - FIXED;
+    static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 2560 - QBYTES;
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
     static constexpr int S = FIT > 4 ? 4 : FIT;      // ring stages
     static_assert(S >= 2 && CTAS * ROWS <= SM_ROWS, "ring, workspace");
     static constexpr int TAKEN = 8;  // more items than a warp has on the way: units in the ring, lookups, one in reserve
     static_assert(S + 4 <= TAKEN, "taken");
     static constexpr int RING = S * STAGE;           // bytes per warp
-    static constexpr int SMEM = WARPS * RING + FIXED;
+    static constexpr int SMEM = WARPS * RING + QBYTES;
     static constexpr int PART = ROWS * (D + 2);      // floats of a partial result
 };
 
@@ -711,7 +710,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
         for (int t = 0; t < NT; t++) {
             const int h = t * 8 + r;
             const uint16_t* qp = (const uint16_t*)a.q + it.b * a.q_seq + (int64_t)(h0 + h) * a.q_head;
-            if (I8) {
+            if constexpr (I8) {
                 uint2 raw[D / 16];
                 float top = 0.f;
 #pragma unroll
@@ -729,12 +728,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 for (int k = 0; k < D / 16; k++) {
                     const float2 x = Elem<TYPE>::up(raw[k].x), y = Elem<TYPE>::up(raw[k].y);
                     const uint32_t f0 = Elem<FVS_F16>::down(x.x * down, x.y * down), f1 = Elem<FVS_F16>::down(y.x * down, y.y * down);
-                    if (Sh::Q_SMEM) {
-                        if (k % WARPS == warp) q_all[(t * (D / 16) + k) * 32 + lane] = make_uint2(f0, f1);
-                    } else {
-                        qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][0] = f0;
-                        qf[Sh::Q_SMEM ? 0 : t][Sh::Q_SMEM ? 0 : k][1] = f1;
-                    }
+                    qf[t][k][0] = f0;
+                    qf[t][k][1] = f1;
                 }
                 const float up = a.scale2 * __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
@@ -957,8 +952,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                 if (r == 0) *(float2*)s_ml[warp][t * 8 + 2 * c4 + x] = make_float2(m[t][x], l[t][x]);
             }
         __syncwarp();
-        float* tile = Sh::O_IN_RING ? (float*)(ring + ready * Sh::STAGE)
-                                    : (float*)(ring_all + WARPS * Sh::RING + warp * Sh::OBYTES);
+        float* tile = (float*)(ring + ready * Sh::STAGE);
         if (lane == 0) s_tile[warp] = (int)((uint8_t*)tile - ring_all);
         if (!solo) __syncthreads();
 #pragma unroll
