@@ -1,0 +1,8 @@
+// The attention kernels over heads of 256 elements.
+#include "fvs_kv_attend.cuh"
+
+namespace fvs {
+namespace kv {
+template int launch_types<256>(fvs_stream_t, const AttendArgs&, int);
+}
+}  // namespace fvs
