@@ -14,7 +14,8 @@ namespace kv {
 
 constexpr int THREADS = 256;
 // loads of a lane that are on the way together: append takes 35 us with two at 9000 tokens of 48 heads of 64 (39 with one
-// or four: a lane's work after them, or its registers, grow), read 23 us with four at 31000 tokens of 8 int8 rows of 96 (25)
+// or four: a lane's work after them, or its registers, grow), read 23 us with four at 31000 tokens of 8 int8 rows of 96 (25
+// with two; each lane looking its places up by itself, without the exchange below, took 20.5 us there)
 constexpr int BATCH = 2, READ_BATCH = 4;
 
 struct Heads {  // token and head strides in elements

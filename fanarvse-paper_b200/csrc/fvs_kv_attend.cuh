@@ -32,11 +32,12 @@
 // largest product met so far (by the largest scale, one large row of no weight would take the others' bits).  Queries over
 // int8 codes are brought to fp16 by a power of two for each head, their largest element to the upper end of its range.
 //
-// Measured on one B200 (6550 GB/s measured copy rate): 131071 bf16 keys of 8 heads of 128, 32 query heads, 103 to 106 us
-// (5.1 TB/s), four such sequences 340 us (6.3 TB/s); 64 sequences of 1 to 8192 keys 66 us (4.7 TB/s); int8 codes, 48
-// sequences of 2048 to 16384 keys, 64 query heads, 135 to 150 us (4.3 to 4.8 TB/s, bound by 350 warp instructions for 16
-// keys); 2000 sequences of 1 to 200 int8 keys 37 us (per item, not per byte); one sequence of 100 keys 10 us (waits for
-// memory in a row).
+// Measured on one B200 (6550 GB/s measured copy rate), calls back to back: 131071 bf16 keys of 8 heads of 128, 32 query
+// heads, 102 to 105 us (5.2 TB/s), four such sequences 341 us (6.3 TB/s); 64 sequences of 1 to 8192 keys 65 us (4.8 TB/s);
+// int8 codes, 48 sequences of 2048 to 16384 keys, 64 query heads, 141 us with two inputs in turn and 155 with more (4.2 to
+// 4.6 TB/s, bound by 510 warp instructions for 16 keys of a head, copies, setup and joins included), 192 such sequences
+// 530 to 570 us (4.6 to 5.0 TB/s); 2000 sequences of 1 to 200 int8 keys 38 us (per item, not per byte); one sequence of 100
+// keys 10 us (waits for memory in a row).
 #pragma once
 #include <limits.h>
 
@@ -99,7 +100,9 @@ struct Shape {
     static_assert(!(I8 && Q_SMEM), "not built: see launch");
     static constexpr int QBYTES = Q_SMEM ? ROWS * D * 2 : 0;
     // CTAs per SM: three (12 warps hide each other's latencies; 168 registers a thread) where two stages fit: 64 ragged
-    // sequences take 66 us against 74 with two CTAs of three stages, 131071 keys 108 against 136
+    // sequences of 8 heads of 128 take 65 us against 73 with two CTAs of three stages, 48 long int8 ones 141 against 155.  Heads
+    // of 96 and 64 at 168 registers spill 60 to 100 bytes, which costs as much as the third CTA gives: 64 ragged sequences 62
+    // and 64 us (three, two CTAs) at 96, 44 and 41 at 64, 131071 keys 87 and 86, 63 and 64; 2000 short int8 ones at 64 35.5 and 31
     static constexpr int CTAS = NT == 1 && D <= 128 && !(I8 && D == 96) ? 3 : RB <= 256 && !Q_SMEM ? 2 : 1;
     static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 2560 - QBYTES;
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
@@ -243,8 +246,9 @@ constexpr int NO_UNIT = INT_MIN;
 
 // Cuts of the cost of all items: equal shares, one for each CTA, each share cut into `runs` pieces, the first of them
 // long.  A CTA begins with its share's long piece; the short ones are taken as CTAs finish, since SMs differ in how fast
-// memory serves them and the warps of an SM in how often they issue (148 SMs, int8, 192 requests of 2048 to 16384 keys: 533
-// -> 487 us).  Below 512 units a share one piece each is faster (48 such requests: 159 -> 145 us).
+// memory serves them and the warps of an SM in how often they issue (148 SMs, int8, 192 requests of 2048 to 16384 keys: 594
+// -> 570 us; 4 of 131071 bf16 keys 357 -> 342).  Below 512 units a share one piece each has the same time (48 such int8
+// requests: 141 us both ways) and less to join.
 struct Cuts {
     int64_t share, lead;  // of the cost: a share, its first piece
     int runs, small;      // pieces of a share, the cost of each but the first (the last one may be shorter)
@@ -614,8 +618,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                                          (int64_t)(slot0 + row) * a.c.slot_stride) * ESZ + ch * 16;
                     const uint8_t *pk = (const uint8_t*)a.c.k + off, *pv = (const uint8_t*)a.c.v + off;
                     const int64_t step = a.c.slot_stride * (RPI * ESZ);
-                    // full tiles of dense rows have fixed distances: no address arithmetic.  The rest is a loop: unrolled, it
-                    // pushed the loop over units out of the instruction cache (large int8 calls 135 -> 143 us)
+                    // full tiles of dense rows have fixed distances: no address arithmetic.  The rest is a loop, for the
+                    // instruction cache's sake (unrolled, large int8 calls take 140 and 577 us, as a loop 141 and 570)
                     if (a.c.slot_stride == D && m == 0xffffu) {
 #pragma unroll
                         for (int i = 0; i < 16 / RPI; i++) {
@@ -1084,7 +1088,7 @@ static int launch_nt(fvs_stream_t stream, AttendArgs a) {
 template <int D, int TYPE, int STORE>
 static int launch(fvs_stream_t stream, const AttendArgs& a) {
     // wide int8 heads: two items of 8 rows take 68 us where one of 16 takes 87 (64 requests of 500 to 16000 keys, D = 256);
-    // wide 16-bit heads: 128 and 95 us
+    // wide 16-bit heads: 128 and 95 us (all with weights in one part; with two 76 us, and 87 us for 16-bit heads)
     if (a.group <= 8 || (STORE == FVS_I8 && D > 128)) return launch_nt<D, TYPE, STORE, 1>(stream, a);
     return launch_nt<D, TYPE, STORE, (STORE == FVS_I8 && D > 128 ? 1 : 2)>(stream, a);
 }
