@@ -24,16 +24,18 @@
 // rescale.  Weights that become fp16 are taken 2^BELOW larger than the softmax's, near fp16's upper end: without that a key at
 // 2^-25 of the largest weight vanished from the second product and not from l.
 //
-// Rounding: l sums the probabilities in fp32.  They enter the second product as two 16-bit numbers, two fp16 ones with 21 bits
-// together (fp16 caches, int8 codes) or two bf16 ones with 16: a single one would add as much error as the output's own
-// rounding (fp16 outputs: 1.4 times the error against 64 bits).  The product of both takes 0 to 3 % longer over 16-bit caches
-// and 9 % over long int8 ones (144 -> 156 us).  int8 codes are exact in fp16 (see codes2).  Their key scale multiplies the
-// fp32 score, their value scale the probability, and a power of two for each head brings that product to fp16's range, by the
-// largest product met so far (by the largest scale, one large row of no weight would take the others' bits).  Queries over
-// int8 codes are brought to fp16 by a power of two for each head, their largest element to the upper end of its range.
+// Rounding: l sums the probabilities in fp32.  They enter the second product as the sum of 16-bit numbers, two fp16 ones with
+// 21 bits together (fp16 caches, int8 codes) or three bf16 ones with 24, so that outputs are as near as fp32's sums bring
+// them.  One fp16 number each made the error against 64 bits 1.4 times that (fp16 outputs); with two bf16 ones (16 bits) an
+// output in 300 was on the neighbouring bf16 number, with three one in 3000 (64 sequences of 1 to 8192 keys).  Two fp16 parts
+// take 2 to 4 % longer than one, 5 to 9 % over long int8 sequences, the third bf16 part 0.5 % (heads of 128) to 4 % (of 64).
+// int8 codes are exact in fp16 (see codes2).  Their key scale multiplies the fp32 score, their value scale the probability, and
+// a power of two for each head brings that product to fp16's range, by the largest product met so far (by the largest scale,
+// one large row of no weight would take the others' bits).  Queries over int8 codes are brought to fp16 by a power of two for
+// each head, their largest element to the upper end of its range.
 //
 // Measured on one B200 (6550 GB/s measured copy rate), calls back to back: 131071 bf16 keys of 8 heads of 128, 32 query
-// heads, 102 to 105 us (5.2 TB/s), four such sequences 341 us (6.3 TB/s); 64 sequences of 1 to 8192 keys 65 us (4.8 TB/s);
+// heads, 102 to 105 us (5.2 TB/s), four such sequences 347 us (6.2 TB/s); 64 sequences of 1 to 8192 keys 65 us (4.8 TB/s);
 // int8 codes, 48 sequences of 2048 to 16384 keys, 64 query heads, 141 us with two inputs in turn and 155 with more (4.2 to
 // 4.6 TB/s, bound by 510 warp instructions for 16 keys of a head, copies, setup and joins included), 192 such sequences
 // 530 to 570 us (4.6 to 5.0 TB/s); 2000 sequences of 1 to 200 int8 keys 38 us (per item, not per byte); one sequence of 100
@@ -169,23 +171,21 @@ __device__ __forceinline__ float power2(float x) { return __uint_as_float((uint3
 __device__ __forceinline__ float weight(float2 ml, float mx) {
     return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - mx);
 }
-// A weight as the sum of two 16-bit numbers: its upper bits, and the rest.  Beside values that may be infinite (POS) the rest
-// stays above zero, so that an infinite value times it is no not-a-number.
+// A weight as the sum of 16-bit numbers, two fp16 or three bf16 ones: its upper bits, those below them (`last` if these are the
+// end, which is rounded), and so on.  Beside values that may be infinite (POS) each part stays above zero, so that an infinite
+// value times it is no not-a-number.
 template <int TYPE>
-constexpr uint32_t UPPER = TYPE == FVS_F16 ? 0xffffe000u : 0xffff0000u;
-template <int TYPE>
-__device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & UPPER<TYPE>); }
-template <int TYPE>
-__device__ __forceinline__ uint32_t upper2(float a, float b) {
-    if (TYPE == FVS_F16) return Elem<TYPE>::down(upper<TYPE>(a), upper<TYPE>(b));
-    return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-}
-template <int TYPE, bool POS>
-__device__ __forceinline__ uint32_t rest2(float a, float b) {
-    float ra = a - upper<TYPE>(a), rb = b - upper<TYPE>(b);
+constexpr int PARTS = TYPE == FVS_F16 ? 2 : 3;
+template <int TYPE, bool POS, bool LAST>
+__device__ __forceinline__ uint32_t part2(float& a, float& b) {
     constexpr float LEAST = TYPE == FVS_F16 ? 0x1p-24f : 1.2e-38f;  // the smallest number, the smallest normal one
-    if (POS) ra = fmaxf(ra, LEAST), rb = fmaxf(rb, LEAST);
-    return Elem<TYPE>::down(ra, rb);
+    constexpr uint32_t UPPER = TYPE == FVS_F16 ? 0xffffe000u : 0xffff0000u;
+    if (LAST) return Elem<TYPE>::down(POS ? fmaxf(a, LEAST) : a, POS ? fmaxf(b, LEAST) : b);
+    const float ua = __uint_as_float(__float_as_uint(a) & UPPER), ub = __uint_as_float(__float_as_uint(b) & UPPER);
+    const uint32_t r = TYPE == FVS_F16 ? Elem<TYPE>::down(ua, ub) : __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    a -= ua, b -= ub;
+    if (POS) a = fmaxf(a, LEAST), b = fmaxf(b, LEAST);
+    return r;
 }
 // Two codes as fp16: the byte u = code + 128 under 0x64 is 1024 + u, and 1152 less is the code, exactly.  (Leaving the 128 in
 // the products and taking it out of their sums spares the subtraction, but the sums then round at 128 sum |q|: a row with
@@ -890,8 +890,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
 #pragma unroll
             for (int j = 0; j < TILES; j++) {
                 if (TILES > 1 && ((mask >> (16 * j)) & 0xffffu) == 0) continue;  // its rows were not copied
-                // p, and p's two parts as the B operands of the second product
-                uint32_t pf[NT][2], pl[NT][2];
+                // p, and p's parts as the B operands of the second product
+                uint32_t pf[PARTS<MT>][NT][2];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     const float z0 = m[t][0] == -INFINITY ? 0.f : m[t][0], z1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
@@ -903,10 +903,13 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         p0 = p0 * vs[j][0] * down[t][0], p1 = p1 * vs[j][0] * down[t][1];
                         p2 = p2 * vs[j][1] * down[t][0], p3 = p3 * vs[j][1] * down[t][1];
                     }
-                    pf[t][0] = transpose8x8(upper2<MT>(p0, p1));
-                    pf[t][1] = transpose8x8(upper2<MT>(p2, p3));
-                    pl[t][0] = transpose8x8(rest2<MT, !I8>(p0, p1));
-                    pl[t][1] = transpose8x8(rest2<MT, !I8>(p2, p3));
+#pragma unroll
+                    for (int n = 0; n + 1 < PARTS<MT>; n++) {
+                        pf[n][t][0] = transpose8x8(part2<MT, !I8, false>(p0, p1));
+                        pf[n][t][1] = transpose8x8(part2<MT, !I8, false>(p2, p3));
+                    }
+                    pf[PARTS<MT> - 1][t][0] = transpose8x8(part2<MT, false, true>(p0, p1));
+                    pf[PARTS<MT> - 1][t][1] = transpose8x8(part2<MT, false, true>(p2, p3));
                 }
                 // O^T += V^T P^T
                 if (I8) {
@@ -921,10 +924,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                             const uint32_t x = __byte_perm(v0, v1, h ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, h ? 0x7362 : 0x5140);
                             const uint32_t f[4] = {codes2(x, LOW), codes2(x, HIGH), codes2(y, LOW), codes2(y, HIGH)};
 #pragma unroll
-                            for (int t = 0; t < NT; t++) {
-                                mma<MT>(o[2 * k + h][t], f, pf[t][0], pf[t][1]);
-                                mma<MT>(o[2 * k + h][t], f, pl[t][0], pl[t][1]);
-                            }
+                            for (int t = 0; t < NT; t++)
+#pragma unroll
+                                for (int n = 0; n < PARTS<MT>; n++) mma<MT>(o[2 * k + h][t], f, pf[n][t][0], pf[n][t][1]);
                         }
                     }
                 } else {
@@ -935,10 +937,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, STORE, NT>::CTAS) attend_ker
                         uint32_t f[4];
                         ldm4t(f, at + Sh::v_chunk(lane, 2 * i + ((lane >> 3) & 1)) * 16);
 #pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            mma<MT>(o[i][t], f, pf[t][0], pf[t][1]);
-                            mma<MT>(o[i][t], f, pl[t][0], pl[t][1]);
-                        }
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int n = 0; n < PARTS<MT>; n++) mma<MT>(o[i][t], f, pf[n][t][0], pf[n][t][1]);
                     }
                 }
             }
