@@ -101,11 +101,12 @@ struct Shape {
     static constexpr bool Q_SMEM = D > 128 && NT > 1;         // q's fragments would not fit the registers
     static_assert(!(I8 && Q_SMEM), "not built: see launch");
     static constexpr int QBYTES = Q_SMEM ? ROWS * D * 2 : 0;
-    // CTAs per SM: three (12 warps hide each other's latencies; 168 registers a thread) where two stages fit: 64 ragged
-    // sequences of 8 heads of 128 take 65 us against 73 with two CTAs of three stages, 48 long int8 ones 141 against 155.  Heads
-    // of 96 and 64 at 168 registers spill 60 to 100 bytes, which costs as much as the third CTA gives: 64 ragged sequences 62
-    // and 64 us (three, two CTAs) at 96, 44 and 41 at 64, 131071 keys 87 and 86, 63 and 64; 2000 short int8 ones at 64 35.5 and 31
-    static constexpr int CTAS = NT == 1 && D <= 128 && !(I8 && D == 96) ? 3 : RB <= 256 && !Q_SMEM ? 2 : 1;
+    // CTAs per SM: three (12 warps hide each other's latencies; 168 registers a thread) where two stages fit: 64 ragged bf16
+    // sequences of 8 heads of 128 take 66 us against 73 with two CTAs of three stages, 48 long int8 ones 141 against 155.  Heads
+    // of 64 spill at 168 registers: two CTAs take 43 us there against 46 (131071 keys 62 and 63; 2000 short int8 sequences 31
+    // and 35, 48 long ones 115 and 116).  16-bit heads of 96 spill as well, and gain on some calls (ragged 62 us against 66 with
+    // two CTAs) what they lose on others (131071 keys 90 and 87).
+    static constexpr int CTAS = NT == 1 && (D == 128 || (D == 96 && !I8)) ? 3 : RB <= 256 && !Q_SMEM ? 2 : 1;
     static constexpr int BUDGET = (227 * 1024) / CTAS - 1024 - 2560 - QBYTES;
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
     static constexpr int S = FIT > 4 ? 4 : FIT;      // ring stages
