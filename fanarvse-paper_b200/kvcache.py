@@ -165,13 +165,14 @@ class PagedKV:
         positions = rot = 0
         if rope is not None:
             cos, sin = rope
-            if not (cos.dtype is sin.dtype is torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
+            shape = cos.shape
+            if not (cos.dtype is sin.dtype is torch.float32 and len(shape) == 2 and sin.shape == shape
                     and cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == self._index):
                 raise ValueError("rope is two contiguous fp32 [positions, rot / 2] on the cache's GPU")
             if cos.requires_grad or sin.requires_grad:
                 for x in rope:
                     _no_gradient(x, "rope")
-            positions, rot = cos.shape[0], 2 * cos.shape[1]
+            positions, rot = shape[0], 2 * shape[1]
             if rot % 16 or not 0 < rot <= self.dim or positions < 1:
                 raise ValueError(f"rotation of {rot} elements: a multiple of 16, at most {self.dim}")
             cos, sin = cos.data_ptr(), sin.data_ptr()
