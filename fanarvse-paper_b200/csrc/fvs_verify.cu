@@ -1,0 +1,270 @@
+// Verification of drafted tokens against a target model's probabilities, from given random numbers (new: what follows the
+// attention of a tree of drafted tokens; the reference ends with the found rows' ids).
+//
+// Behind the last node taken (at first the sequence's end) the target's probabilities are p and the draft's q.  The node's
+// children are tried in order: with r_0 = p and m_0 = 1, child c of token x is taken if u_c m_k q(x) < r_k(x), else
+// r_{k+1} = max(r_k - m_k q, 0) and m_{k+1} = sum r_{k+1}, unless that is 0.  Where none is taken the next token is drawn from
+// r_k: the first whose running sum passes u_last sum(r_k).  Taken this way the tokens are distributed as the target's own.
+//
+// All of it is in fp64: p and q are exact in it and so is a first difference, so that a decision depends on the order of a
+// sum only within 1e-16 of its border.
+//
+// Whether a node is taken without a refusal before it needs two numbers, gathered for all nodes at once; a whole row (and
+// the draft's) is read only for a node's refused child and for the last draw: 2 V elements of a sequence where the floor is
+// V (1 + draft), each pass after the first from L2.  A cluster of CTAs shares a row, since one SM reads it at 1/148 of the
+// memory's rate; the sums of its CTAs are exchanged through distributed shared memory and added in order of rank, so that
+// every CTA comes to the same numbers and walks the same path by itself.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+#include "fvs_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace fvs {
+namespace drafts {
+
+constexpr int THREADS = 512, WARPS = THREADS / 32, NODES = 256, CTAS = 8, AHEAD = 8;
+
+struct Rows {  // [seqs, nodes + 1, vocab], strides in elements; null: none
+    const void* at;
+    int64_t seq, row;
+};
+
+struct Args {
+    Rows target, draft;
+    const int32_t *parents, *tokens, *counts;
+    const float* u;
+    int64_t parent_stride;  // 0: one tree for all
+    int seqs, nodes, vocab;
+    int32_t *path, *kept, *token;
+};
+
+template <typename T>
+__device__ __forceinline__ double value(const T* p) {
+    const float x = (float)*p;
+    return x > 0.f && x < __int_as_float(0x7f800000) ? (double)x : 0.0;  // what is no probability counts as none
+}
+
+struct Shared {
+    double left[NODES];   // r_k of the node's token, while its parent is the last node taken
+    double qx[NODES];
+    float u[NODES + 1];
+    int parent[NODES], tok[NODES];
+    double mass[NODES + 1];  // m_0 .. m_k of the present row
+    int refused[NODES];      // tokens refused in it (drafts without probabilities)
+    double warp[WARPS], scan[WARPS];
+    double total[2][CTAS];   // of each CTA, two passes in turn
+    int found, positive;
+};
+
+// r_k of element v of the present row
+template <bool DRAFT>
+__device__ __forceinline__ double rest(double p, double q, int v, const Shared& s, int k) {
+    if (DRAFT) {
+        for (int j = 0; j < k; j++) p = fmax(__dsub_rn(p, __dmul_rn(s.mass[j], q)), 0.0);  // as written, not one operation
+    } else {
+        for (int j = 0; j < k; j++) p = v == s.refused[j] ? 0.0 : p;
+    }
+    return p;
+}
+
+template <typename T, bool DRAFT>
+__global__ void __launch_bounds__(THREADS) verify_kernel(Args a) {
+    __shared__ Shared s;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = blockIdx.x / ctas, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const T* target = (const T*)a.target.at + b * a.target.seq;
+    const T* draft = (const T*)a.draft.at + b * a.draft.seq;
+    const int nodes = a.counts ? min(max(__ldg(a.counts + b), 0), a.nodes) : a.nodes;
+    for (int i = tid; i < nodes; i += THREADS) {
+        const int up = __ldg(a.parents + b * a.parent_stride + i), x = __ldg(a.tokens + (int64_t)b * a.nodes + i);
+        const bool ok = up >= -1 && up < i && x >= 0 && x < a.vocab;
+        s.parent[i] = ok ? up : -2;  // never taken
+        s.tok[i] = x;
+        s.u[i] = __ldg(a.u + (int64_t)b * (a.nodes + 1) + i);
+        s.left[i] = ok ? value(target + (up + 1) * a.target.row + x) : 0.0;
+        s.qx[i] = !ok ? 0.0 : DRAFT ? value(draft + (up + 1) * a.draft.row + x) : 1.0;
+    }
+    // the part of a row that this warp sums: the cluster's warps side by side
+    const int span = ((a.vocab + ctas * WARPS - 1) / (ctas * WARPS) + 31) / 32 * 32;
+    const int lo = min(a.vocab, (rank * WARPS + warp) * span), hi = min(a.vocab, lo + span);
+    int last = -1, kept = 0, k = 0, turn = 0;
+    double total = 0.0;
+    bool summed = false;  // total and the warps' sums are those of r_k
+    // sums of r_n over the row behind `last`; ends with all of the cluster's threads having them
+    auto pass = [&](int n) {
+        const T *p = target + (last + 1) * a.target.row, *q = draft + (last + 1) * a.draft.row;
+        double sum = 0.0;
+        for (int v0 = lo + lane; v0 < hi; v0 += 32 * AHEAD) {
+            double pv[AHEAD], qv[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                const int v = v0 + 32 * j;
+                pv[j] = v < hi ? value(p + v) : 0.0;
+                qv[j] = DRAFT && n > 0 && v < hi ? value(q + v) : 0.0;
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) sum += rest<DRAFT>(pv[j], qv[j], v0 + 32 * j, s, n);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        __syncthreads();  // the sums before were read
+        if (lane == 0) s.warp[warp] = sum;
+        __syncthreads();
+        if (tid < ctas) {
+            double all = 0.0;
+            for (int w = 0; w < WARPS; w++) all += s.warp[w];
+            *cluster.map_shared_rank(&s.total[turn][rank], tid) = all;
+        }
+        cluster.sync();
+        double all = 0.0;
+        for (int r = 0; r < ctas; r++) all += s.total[turn][r];
+        return all;
+    };
+    cluster.sync();  // every CTA has begun and has its nodes
+    double mass = 1.0;
+    for (int i = 0; i < nodes; i++) {  // children come after their parents
+        if (s.parent[i] != last) continue;
+        if ((double)s.u[i] * mass * s.qx[i] < s.left[i]) {
+            if (rank == 0 && tid == 0) a.path[(int64_t)b * a.nodes + kept] = i;
+            last = i;
+            kept++;
+            k = 0;
+            mass = 1.0;
+            summed = false;
+            continue;
+        }
+        __syncthreads();  // mass and refused of the pass before were read
+        if (tid == 0) {
+            s.mass[k] = mass;
+            s.refused[k] = s.tok[i];
+        }
+        __syncthreads();
+        const double m = pass(k + 1);
+        turn ^= 1;
+        summed = m > 0.0;
+        if (m > 0.0) {
+            __syncthreads();
+            for (int c = tid; c < nodes; c += THREADS) {
+                if (s.parent[c] != last) continue;
+                if (DRAFT)
+                    s.left[c] = fmax(__dsub_rn(s.left[c], __dmul_rn(mass, s.qx[c])), 0.0);
+                else if (s.tok[c] == s.tok[i])
+                    s.left[c] = 0.0;
+            }
+            __syncthreads();
+            mass = m;
+            total = m;
+            k++;
+        }
+    }
+    if (!summed) {
+        __syncthreads();
+        total = pass(k);
+    }
+    // the draw: the first CTA, warp and element at which the running sum passes the limit
+    const double limit = (double)__ldg(a.u + (int64_t)b * (a.nodes + 1) + a.nodes) * total;
+    if (summed) turn ^= 1;  // the buffer of the last pass
+    int owner = -1, some = -1;
+    double before = 0.0;
+    for (int r = 0; r < ctas; r++) {
+        const double all = s.total[turn][r];
+        if (all > 0.0) some = r;
+        if (before + all > limit) {
+            owner = r;
+            break;
+        }
+        if (r < ctas - 1) before += all;
+    }
+    const bool none = owner < 0;  // a limit that no sum passes (u of 1, say): the last element with a probability
+    if (none) owner = some;
+    if (rank == 0 && tid == 0) {
+        a.kept[b] = kept;
+        if (owner < 0) a.token[b] = -1;
+    }
+    if (rank == 0)
+        for (int n = kept + tid; n < a.nodes; n += THREADS) a.path[(int64_t)b * a.nodes + n] = -1;
+    if (rank == owner) {
+        int w = 0, positive = -1;
+        bool over = false;
+        for (; w < WARPS; w++) {
+            if (s.warp[w] > 0.0) positive = w;
+            if (!none && before + s.warp[w] > limit) {
+                over = true;
+                break;
+            }
+            if (w < WARPS - 1) before += s.warp[w];
+        }
+        if (!over) w = positive;  // the sums' rounding, or none
+        const int from = min(a.vocab, (rank * WARPS + w) * span), to = min(a.vocab, from + span);
+        if (tid == 0) s.found = INT_MAX, s.positive = -1;
+        __syncthreads();
+        const T *p = target + (last + 1) * a.target.row, *q = draft + (last + 1) * a.draft.row;
+        for (int v0 = from; v0 < to; v0 += THREADS) {
+            const int v = v0 + tid;
+            double x = 0.0;
+            if (v < to) x = rest<DRAFT>(value(p + v), DRAFT && k > 0 ? value(q + v) : 0.0, v, s, k);
+            if (x > 0.0) atomicMax(&s.positive, v);
+            double sum = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += y;
+            }
+            if (lane == 31) s.scan[warp] = sum;
+            __syncthreads();
+            double add = before;
+            for (int j = 0; j < warp; j++) add += s.scan[j];
+            if (over && x > 0.0 && add + sum > limit) atomicMin(&s.found, v);
+            for (int j = warp; j < WARPS; j++) add += s.scan[j];
+            before = add;
+            __syncthreads();
+            if (s.found != INT_MAX) break;
+        }
+        if (tid == 0) a.token[b] = s.found != INT_MAX ? s.found : s.positive;
+    }
+    cluster.sync();  // no CTA ends while another may still write its sums
+}
+
+template <typename T>
+static int launch(fvs_stream_t stream, const Args& a) {
+    // CTAs of a row: two waves of them where there are few sequences, and at least 4096 elements each
+    int ctas = 1;
+    while (ctas < CTAS && ctas * 2 * a.seqs <= 4 * fvs_sm_count() && a.vocab >= ctas * 2 * 4096) ctas *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.seqs * ctas));
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = a.draft.at ? cudaLaunchKernelEx(&cfg, verify_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, verify_kernel<T, false>, a);
+    return e == cudaSuccess ? fvs_launch_status() : (int)e;
+}
+
+}  // namespace drafts
+}  // namespace fvs
+
+using namespace fvs::drafts;
+
+extern "C" int fvs_verify(fvs_stream_t stream, int type, const void* target, int64_t target_seq, int64_t target_row,
+                          const void* draft, int64_t draft_seq, int64_t draft_row, const int32_t* parents,
+                          int64_t parent_stride, const int32_t* tokens, const int32_t* counts, const float* u, int seqs,
+                          int nodes, int vocab, int32_t* path, int32_t* kept, int32_t* token) {
+    FVS_CHECK_ARG(type == FVS_F16 || type == FVS_BF16 || type == FVS_F32);
+    FVS_CHECK_ARG(seqs >= 0 && nodes >= 0 && vocab >= 1);
+    if (seqs == 0) return FVS_OK;
+    const uintptr_t odd = type == FVS_F32 ? 3 : 1;
+    FVS_CHECK_ARG(target && u && kept && token && (nodes == 0 || (parents && tokens && path)));
+    FVS_CHECK_ARG(((uintptr_t)target & odd) == 0 && ((uintptr_t)draft & odd) == 0);
+    FVS_CHECK_ARG(target_seq >= 0 && target_row >= 0 && draft_seq >= 0 && draft_row >= 0 && parent_stride >= 0);
+    if (nodes > NODES || vocab > (1 << 30) || seqs > (1 << 27)) return FVS_ERANGE;
+    const Args a{{target, target_seq, target_row}, {draft, draft_seq, draft_row}, parents, tokens, counts, u, parent_stride,
+                 seqs, nodes, vocab, path, kept, token};
+    return type == FVS_F32 ? launch<float>(stream, a) : type == FVS_F16 ? launch<__half>(stream, a) : launch<__nv_bfloat16>(stream, a);
+}

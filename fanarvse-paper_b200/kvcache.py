@@ -84,6 +84,7 @@ class PagedKV:
         self._ref = C.byref(self._c)
         self.L = _lib.lib()
         self._append, self._read, self._attend = self.L.fvs_kv_append, self.L.fvs_kv_read, self.L.fvs_kv_attend
+        self._append_norm, self._compact = self.L.fvs_kv_append_norm, self.L.fvs_kv_compact
         self._work_bytes = self.L.fvs_kv_attend_work(self.dim)
         check(min(self._work_bytes, 0), "kv_attend_work")
         self.launches = 0
@@ -131,6 +132,24 @@ class PagedKV:
             raise ValueError(f"{what} is {dtype}: fp16 or bf16, and the cache's own type unless that holds int8 codes")
         return _CODE[dtype]
 
+    def _weights(self, norm, dtype, has_q):
+        """addresses of the norms' weights and their type"""
+        wq, wk = norm
+        if wq is not None and not has_q:
+            raise ValueError("a norm of query heads without q")
+        kind = None
+        for w, what in ((wq, "the query norm's weight"), (wk, "the key norm's weight")):
+            if w is None:
+                continue
+            if not (w.dim() == 1 and w.numel() == self.dim and w.is_contiguous() and w.get_device() == self._index
+                    and w.data_ptr() % 16 == 0 and w.dtype in (dtype, torch.float32) and kind in (None, w.dtype)):
+                raise ValueError(f"{what} is a contiguous, 16-byte aligned [{self.dim}] of k's type or fp32 (both alike) "
+                                 "on the cache's GPU")
+            if w.requires_grad:
+                _no_gradient(w, what)
+            kind = w.dtype
+        return None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), _CODE[kind or dtype]
+
     def _like(self, out, x, what):
         if not (out.dtype is x.dtype and out.shape == x.shape and out.is_contiguous()
                 and out.get_device() == self._index):
@@ -143,13 +162,15 @@ class PagedKV:
         return torch._C._cuda_getCurrentRawStream(self._index)  # torch.cuda.current_stream takes 2 us more
 
     # ---------------------------------------------------------------- the operators
-    def append(self, k, v, table, idx, seq=None, pos=None, rope=None, pairs="halves", q=None, q_out=None):
+    def append(self, k, v, table, idx, seq=None, pos=None, rope=None, pairs="halves", q=None, q_out=None, norm=None,
+               eps=1e-6):
         """Stores k, v [n, heads, dim] of n new tokens at logical places idx [n] (negative: not stored) of sequences seq
         [n] (default: token i is sequence i's).  The places of a call are distinct: where two tokens meet, the row is
         undefined afterwards.  rope: (cos, sin), fp32 [positions, rot / 2]: the first rot elements of the
         heads of k and of q [n, any, dim] are rotated at positions pos [n] (default idx), pairs "halves" (i, i + rot / 2)
         or "neighbours" (2i, 2i + 1).  Returns q_out, the rotated q (contiguous, default a new tensor, may be q; zeros for
-        tokens that have no place), or None without q."""
+        tokens that have no place), or None without q.  norm: (q weight, k weight), each [dim] of k's type or both fp32, or
+        None: before the rotation those heads become x / sqrt(mean x^2 + eps) * weight."""
         n = k.shape[0]
         ty = self._type(k.dtype, "k")
         if v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
@@ -181,9 +202,12 @@ class PagedKV:
         ta = self._table(table)
         if seq is None and n > ta[1]:
             raise ValueError("without seq there is a table row for each token")
-        check(self._append(self._stream(), self._ref, ty, *ka, *va, *qa, hq, qo, *ta, self._ints(seq, n, "seq"),
-                           self._ints(idx, n, "idx"), self._ints(pos, n, "pos"), n, cos, sin, positions, rot,
-                           _lib.PAIRS[pairs]), "kv_append")
+        args = (self._stream(), self._ref, ty, *ka, *va, *qa, hq, qo, *ta, self._ints(seq, n, "seq"),
+                self._ints(idx, n, "idx"), self._ints(pos, n, "pos"), n, cos, sin, positions, rot, _lib.PAIRS[pairs])
+        if norm is None:
+            check(self._append(*args), "kv_append")
+        else:
+            check(self._append_norm(*args, *self._weights(norm, k.dtype, q is not None), eps), "kv_append_norm")
         self.launches += 1
         return q_out if q is not None else None
 
@@ -234,6 +258,20 @@ class PagedKV:
                            lse.data_ptr(), work.data_ptr(), arrived.data_ptr()), "kv_attend")
         self.launches += 1
         return out, lse
+
+    def compact(self, table, lens, path):
+        """Moves the rows of the drafted tokens that were taken together: the row at logical place lens[b] + path[b, n]
+        goes to lens[b] + n, path int32 [sequences, nodes] as `drafts.verify` returns it (rising, then -1).  The sequences
+        are then kept [b] tokens longer.  Places that no row goes to keep what they hold."""
+        ta = self._table(table)
+        n = ta[1]
+        shape = path.shape
+        if not (path.dtype is torch.int32 and len(shape) == 2 and shape[0] == n and path.is_contiguous()
+                and path.get_device() == self._index):
+            raise ValueError(f"path is a contiguous int32 [{n}, nodes] on the cache's GPU")
+        check(self._compact(self._stream(), self._ref, *ta, self._ints(lens, n, "lens"), path.data_ptr(), shape[1]),
+              "kv_compact")
+        self.launches += 1
 
     def _workspace(self, stream, n):
         """Tensors of the partial results and of n arrival counters (zeroed once, left zeroed by every call): one pair for

@@ -493,6 +493,19 @@ int fvs_kv_append(fvs_stream_t stream, const fvs_kv_cache* cache, int type, cons
                   const float* sin, int positions, int rot, int pairs);
 
 /*
+ * fvs_kv_append with norms of the heads in the same pass: before the rotation each head x of q (if q_weight is not NULL)
+ * and of k (if k_weight is not NULL) becomes x / sqrt(mean x^2 + eps) * weight, in fp32; norm and rotation are rounded
+ * once together.  Weights are [dim] of weight_type (`type` or FVS_F32), 16-byte aligned; 0 < eps < 1e30.  The squares are
+ * summed in fp32, so rows of bf16 magnitudes above 2^60 are outside its range (they become zeros).
+ */
+int fvs_kv_append_norm(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* k, int64_t k_token,
+                       int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* q, int64_t q_token,
+                       int64_t q_head, int hq, void* q_out, const int32_t* table, int seqs, int wide,
+                       int64_t table_stride, const int32_t* seq, const int32_t* idx, const int32_t* pos, int tokens,
+                       const float* cos, const float* sin, int positions, int rot, int pairs, const void* q_weight,
+                       const void* k_weight, int weight_type, float eps);
+
+/*
  * Reads the rows of tokens idx[n] of sequences seq[n] (NULL: sequence n) back: k and v contiguous [tokens, heads, dim]
  * of `type` FVS_F16, FVS_BF16 or FVS_F32, codes times their scale in fp32, rounded once.  Zeros where there is no place.
  * fill is not looked at.
@@ -515,6 +528,37 @@ int fvs_kv_attend_work(int dim);
 int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,
                   int64_t q_head, int hq, const int32_t* table, int seqs, int wide, int64_t table_stride,
                   const int32_t* lens, float scale, void* out, float* lse, void* work, int32_t* arrived);
+
+/*
+ * Moves the rows of drafted tokens together: of each sequence b, the row at logical place lens[b] + path[b, n] goes to
+ * lens[b] + n, for n up to the first negative entry of path [seqs, nodes] (contiguous).  A path rises (each entry above
+ * the one before it, all below nodes); rows from an entry on that does not are left where they are, with
+ * FVS_KV_BAD_INDEX.  Rows from or to a hole are left too.  Places that no row goes to keep what they hold.  The pages of
+ * the places that change belong to one sequence each.
+ */
+int fvs_kv_compact(fvs_stream_t stream, const fvs_kv_cache* cache, const int32_t* table, int seqs, int wide,
+                   int64_t table_stride, const int32_t* lens, const int32_t* path, int nodes);
+
+/*
+ * Verification of trees of drafted tokens from given random numbers (new).  target and draft [seqs, nodes + 1, vocab] of
+ * `type` FVS_F32, FVS_F16 or FVS_BF16 hold probabilities (sequence and row strides in elements, a row's elements side by
+ * side): row 0 behind the sequence, row i + 1 behind node i.  draft NULL: each token was drafted with certainty.  Node i
+ * of sequence b is token tokens[b, i] ([seqs, nodes], contiguous) behind node parents[b, i] (-1: behind the sequence;
+ * parent_stride elements between the sequences' parents, 0: the same tree for all); parents come before their children.
+ * counts (nullable) [seqs]: nodes that a sequence has.  u [seqs, nodes + 1] fp32 in [0, 1).
+ *
+ * Behind the last node taken (first the sequence itself), with r_0 its target row, q its draft row and m_0 = 1, the
+ * children are tried in order of their index: child i of token x is taken if u[i] m q(x) < r(x); otherwise r becomes
+ * max(r - m q, 0) and m its sum (not where that sum is 0).  Where no child is taken, token[b] = the first v with r(0) +
+ * .. + r(v) > u[nodes] sum r (the last with r(v) > 0 if rounding leaves none; -1 for a row without any probability).
+ * path[b] = the nodes taken in order, then -1; kept[b] = their number.  All of it in fp64.  Entries that are negative or
+ * not finite count as 0.  A node whose parent does not come before it, or whose token is outside the vocabulary, is never
+ * taken and changes nothing.  nodes <= 256 (FVS_ERANGE above).  Rows behind nodes that are not taken are not read.
+ */
+int fvs_verify(fvs_stream_t stream, int type, const void* target, int64_t target_seq, int64_t target_row,
+               const void* draft, int64_t draft_seq, int64_t draft_row, const int32_t* parents, int64_t parent_stride,
+               const int32_t* tokens, const int32_t* counts, const float* u, int seqs, int nodes, int vocab,
+               int32_t* path, int32_t* kept, int32_t* token);
 
 #ifdef __cplusplus
 }
