@@ -69,6 +69,8 @@ SIGNATURES = {
                              P, P, I32, I32, I32]),
     "fvs_kv_append_norm": (I32, [P, P, I32, P, I64, I64, P, I64, I64, P, I64, I64, I32, P, P, I32, I32, I64, P, P, P, I32,
                                   P, P, I32, I32, I32, P, P, I32, F32]),
+    "fvs_kv_attend_tree_work": (I32, [I32, I32]),
+    "fvs_kv_attend_tree": (I32, [P, P, I32, P, I64, I64, I64, I32, P, I32, I32, I64, P, P, I64, P, I32, F32, P, P, P]),
     "fvs_kv_compact": (I32, [P, P, P, I32, I32, I64, P, P, I32]),
     "fvs_verify": (I32, [P, I32, P, I64, I64, P, I64, I64, P, I64, P, P, P, I32, I32, I32, P, P, P]),
     "fvs_kv_read": (I32, [P, P, I32, P, P, P, I32, I32, I64, P, P, I32]),
@@ -87,6 +89,7 @@ class KvCache(C.Structure):
 
 
 F16, BF16, I8, F32T = 0, 1, 2, 3        # element type codes
+GAVE_UP, TREE_NODES = 2, 256            # status bit of attend_tree's waits; most nodes of a tree
 PAIRS = {"halves": 0, "neighbours": 1}  # which elements of a head the rotation pairs
 
 ERRORS = {-1: "FVS_EINVAL (bad argument)", -2: "FVS_ERANGE (size above the kernel's limit)"}

@@ -1,0 +1,10 @@
+// The tree attention kernels over heads of 192 elements.
+#include "fvs_kv_tree.cuh"
+
+namespace fvs {
+namespace kv {
+namespace tree {
+template int launch_types<192>(fvs_stream_t, const Args&, int);
+}
+}  // namespace kv
+}  // namespace fvs

@@ -16,7 +16,7 @@ import torch
 from . import _lib
 from ._lib import check
 
-MAX_NODES = 256
+MAX_NODES = _lib.TREE_NODES
 _CODE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32T}
 
 

@@ -25,6 +25,7 @@ _CODE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.int8: _lib.I8
 _WIDE = (torch.float16, torch.bfloat16)
 _READ = (torch.float16, torch.bfloat16, torch.float32)
 _WORK = {}  # (GPU, stream) -> workspace of attend
+_TREE_WORK = {}  # (GPU, stream) -> workspace of attend_tree
 
 
 def _need(cond, what):
@@ -85,6 +86,7 @@ class PagedKV:
         self.L = _lib.lib()
         self._append, self._read, self._attend = self.L.fvs_kv_append, self.L.fvs_kv_read, self.L.fvs_kv_attend
         self._append_norm, self._compact = self.L.fvs_kv_append_norm, self.L.fvs_kv_compact
+        self._attend_tree = self.L.fvs_kv_attend_tree
         self._work_bytes = self.L.fvs_kv_attend_work(self.dim)
         check(min(self._work_bytes, 0), "kv_attend_work")
         self.launches = 0
@@ -259,6 +261,64 @@ class PagedKV:
         self.launches += 1
         return out, lse
 
+    def attend_tree(self, q, table, lens, parents, counts=None, scale=None, out=None, lse=None):
+        """Attention of a tree of drafted tokens per sequence: q [sequences, nodes, query heads, dim], node i at logical
+        place lens[b] + i (appended there before) and behind node parents[b, i], or behind the sequence where that is -1
+        (int32 [nodes] for all or [sequences, nodes]; parents come before their children, at most drafts.MAX_NODES nodes).
+        A node sees the visible ones of the first lens [sequences] logical tokens, its ancestors and itself; counts int32
+        [sequences]: the nodes that a sequence has (default: all).  Returns (out like q, lse fp32 [sequences, nodes, query
+        heads]): zeros and -inf where nothing is visible and for nodes that a sequence does not have.  One node is
+        `attend` with a length of lens + 1."""
+        shape = q.shape
+        if not (len(shape) == 4 and shape[3] == self.dim and q.get_device() == self._index):
+            raise ValueError(f"q is [sequences, nodes, heads, {self.dim}] on the cache's GPU")
+        n, nodes, hq = shape[:3]
+        ty = self._type(q.dtype, "q")
+        if q.requires_grad:
+            _no_gradient(q, "q")
+        s0, s1, s2, s3 = q.stride()
+        at = q.data_ptr()
+        if s3 != 1 or s0 % 8 or s1 % 8 or s2 % 8 or at % 16:
+            raise ValueError("q needs contiguous, 16-byte aligned heads")
+        if hq < 1 or hq % self.heads:
+            raise ValueError(f"{hq} query heads over {self.heads} key heads")
+        if nodes > _lib.TREE_NODES:
+            raise ValueError(f"{nodes} nodes: at most {_lib.TREE_NODES}")
+        ta = self._table(table)
+        if ta[1] != n:
+            raise ValueError(f"the page table has {ta[1]} rows for {n} sequences")
+        if not (parents.dtype is torch.int32 and parents.shape in ((nodes,), (n, nodes)) and parents.is_contiguous()
+                and parents.get_device() == self._index):
+            raise ValueError(f"parents is a contiguous int32 [{nodes}] or [{n}, {nodes}] on the cache's GPU")
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        if lse is None:
+            lse = torch.empty(shape[:3], device=q.device)
+        elif not (lse.dtype is torch.float32 and lse.shape == shape[:3] and lse.is_contiguous()
+                  and lse.get_device() == self._index):
+            raise ValueError("lse is a contiguous fp32 [sequences, nodes, query heads]")
+        oa, la, ca = self._like(out, q, "out"), self._ints(lens, n, "lens"), self._ints(counts, n, "counts")
+        if n == 0 or nodes == 0:
+            return out, lse
+        stream = self._stream()
+        check(self._attend_tree(stream, self._ref, ty, at, s0, s1, s2, hq, *ta, la, parents.data_ptr(),
+                                nodes if parents.dim() == 2 else 0, ca, nodes, self.scale if scale is None else scale, oa,
+                                lse.data_ptr(), self._tree_workspace(stream, nodes * (hq // self.heads)).data_ptr()),
+              "kv_attend_tree")
+        self.launches += 2
+        return out, lse
+
+    def _tree_workspace(self, stream, rows):
+        """The partial results' tensor, for each stream as `_workspace`'s; a captured call's lives in its graph's memory."""
+        need = self.L.fvs_kv_attend_tree_work(self.dim, rows)
+        capturing = torch.cuda.is_current_stream_capturing()
+        held = None if capturing else _TREE_WORK.get((self._index, stream))
+        if held is None or held.numel() < need:
+            held = torch.empty(need, dtype=torch.uint8, device=self.device)
+            if not capturing:
+                _TREE_WORK[self._index, stream] = held
+        return held
+
     def compact(self, table, lens, path):
         """Moves the rows of the drafted tokens that were taken together: the row at logical place lens[b] + path[b, n]
         goes to lens[b] + n, path int32 [sequences, nodes] as `drafts.verify` returns it (rising, then -1).  The sequences
@@ -291,17 +351,22 @@ class PagedKV:
     def check_status(self):
         """Raises if a call since the last check, on any stream, met an index outside its table (waits for the GPU)."""
         torch.cuda.synchronize(self.device)
-        if int(self.status.item()) != 0:
+        status = int(self.status.item())
+        if status != 0:
             self.status.zero_()
             torch.cuda.synchronize(self.device)  # so that a call on any stream from here on is seen
+            if status & _lib.GAVE_UP:
+                raise _lib.FvsError("paged cache: a wait inside attend_tree ran out; its outputs are undefined")
             raise _lib.FvsError("paged cache: an index was outside its table (page, sequence, token or position); "
                                 "that access was skipped")
 
 
 def release_workspaces():
-    """Gives the workspaces of attend back to torch's allocator (8 to 29 MB for each stream that attended; a stream's next
-    call makes its own again).  Calls in flight keep what they have: the memory is used again on its own stream only."""
+    """Gives the workspaces of attend and attend_tree back to torch's allocator (8 to 29 MB for each stream that attended, 10
+    to 39 MB for trees; a stream's next call makes its own again).  Calls in flight keep what they have: the memory is used
+    again on its own stream only."""
     _WORK.clear()
+    _TREE_WORK.clear()
 
 
 def passage_table(ids, pages_of, own=None):

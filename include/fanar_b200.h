@@ -461,6 +461,8 @@ int fvs_merge_topk(fvs_stream_t stream, const int64_t* ids_g, const float* score
 #define FVS_I8 2
 #define FVS_F32 3
 #define FVS_KV_BAD_INDEX 1
+#define FVS_KV_GAVE_UP 2 /* a bounded wait of fvs_kv_attend_tree ran out (fvs_set_wait_limit); its outputs are undefined */
+#define FVS_TREE_NODES 256
 typedef struct fvs_kv_cache {
     void *k, *v;
     float *k_scale, *v_scale;
@@ -528,6 +530,27 @@ int fvs_kv_attend_work(int dim);
 int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,
                   int64_t q_head, int hq, const int32_t* table, int seqs, int wide, int64_t table_stride,
                   const int32_t* lens, float scale, void* out, float* lse, void* work, int32_t* arrived);
+
+/*
+ * Attention of trees of drafted tokens: q [seqs, nodes, hq, dim] (type FVS_F16 or FVS_BF16, the cache's own unless that is
+ * FVS_I8; strides in elements, multiples of 16 bytes), hq a multiple of the cache's heads, query head h reads key head h /
+ * (hq / heads).  Node i of sequence b lies at logical place lens[b] + i, behind node parents[i] of b's tree (-1, or no
+ * node before it: behind the sequence; parent_stride elements between the sequences' parents, 0: the same tree for all).
+ * It sees the tokens before lens[b], its ancestors and itself, as far as they are there: a page in the table, slot < fill.
+ * counts (nullable) [seqs]: the nodes that a sequence has, all without it.  out and lse as fvs_kv_attend's, contiguous
+ * [seqs, nodes, hq, dim] and [seqs, nodes, hq] (lse nullable); out 0 and lse -infinity for a node that sees nothing and for
+ * nodes from counts[b] on.  Places before lens[b] that are not there may hold anything, and so may every place behind the
+ * nodes; the nodes' own rows are finite (one that is not may reach nodes that do not see it).
+ * A length above the table's row (or below 0) is cut to it; where the nodes reach past the row those places are not
+ * there, with FVS_KV_BAD_INDEX.  nodes <= FVS_TREE_NODES (FVS_ERANGE above).
+ * work: fvs_kv_attend_tree_work(dim, nodes * (hq / heads)) bytes of device memory, 16-byte aligned, of any contents.  Calls that
+ * may run at the same time need their own.
+ */
+int fvs_kv_attend_tree_work(int dim, int rows);
+int fvs_kv_attend_tree(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,
+                       int64_t q_node, int64_t q_head, int hq, const int32_t* table, int seqs, int wide,
+                       int64_t table_stride, const int32_t* lens, const int32_t* parents, int64_t parent_stride,
+                       const int32_t* counts, int nodes, float scale, void* out, float* lse, void* work);
 
 /*
  * Moves the rows of drafted tokens together: of each sequence b, the row at logical place lens[b] + path[b, n] goes to

@@ -23,7 +23,7 @@ def sees(parents):
 
 def attend_tree(q, k, v, table, lens, parents, counts, scale, fill=None):
     """q [B, nodes, hq, d], k and v [pages, heads, page, d] (values), parents [B, nodes].  Returns out, lse, and for error
-    bounds sum p |v|, scale * max sum |q k|."""
+    bounds sum p |v|, |scale| * max sum |q k|."""
     B, nodes, hq, d = q.shape
     pages, heads, page, _ = k.shape
     g = hq // heads
@@ -59,7 +59,7 @@ def attend_tree(q, k, v, table, lens, parents, counts, scale, fill=None):
                     out[b, i, at] = np.where(tot == 0, 0, (w @ V) / safe)
                     pv[b, i, at] = (w @ np.abs(V)) / safe
                     lse[b, i, at] = np.where(tot == 0, -np.inf, top + np.log(safe))[:, 0]
-                    mag[b, i, at] = scale * (np.abs(qq[i]) @ np.abs(K).T).max(1)
+                    mag[b, i, at] = abs(scale) * (np.abs(qq[i]) @ np.abs(K).T).max(1)
     return out, lse, pv, mag
 
 

@@ -31,6 +31,13 @@ def compact(L, c, **change):
     return L.lib().fvs_kv_compact(None, c, *a.values())
 
 
+def attend_tree(L, c, **change):
+    a = dict(type=L.F16, q=4096, qs=5 * 256, qn=256, qh=64, hq=4, table=64, seqs=4, wide=2, stride=2, lens=64, parents=64, ps=5,
+             counts=None, nodes=5, scale=0.1, out=4096, lse=64, work=64)
+    a.update(change)
+    return L.lib().fvs_kv_attend_tree(None, c, *a.values())
+
+
 def verify(L, **change):
     a = dict(type=L.F32T, target=64, ts=6 * 100, tr=100, draft=64, ds=6 * 100, dr=100, parents=64, ps=5, tokens=64,
              counts=None, u=64, seqs=2, nodes=5, vocab=100, path=64, kept=64, token=64)
@@ -40,13 +47,28 @@ def verify(L, **change):
 
 @pytest.mark.parametrize("change", BAD_CACHES)
 def test_bad_caches(L, change):
-    for call in (append_norm, compact):
+    for call in (append_norm, compact, attend_tree):
         assert call(L, cache(L, **change)) == -1
 
 
 def test_unsupported_head_dim(L):
-    for call in (append_norm, compact):
+    for call in (append_norm, compact, attend_tree):
         assert call(L, cache(L, dim=80, slot_stride=80)) == -2
+
+
+@pytest.mark.parametrize("change,rc", [(dict(type=3), -1), (dict(type=1), -1), (dict(q=None), -1), (dict(q=4104), -1), (dict(qs=4), -1),
+                                       (dict(qn=-8), -1), (dict(qh=12), -1), (dict(hq=0), -1), (dict(hq=5), -1), (dict(table=None), -1),
+                                       (dict(seqs=-1), -1), (dict(wide=0), -1), (dict(lens=None), -1), (dict(parents=None), -1),
+                                       (dict(ps=-1), -1), (dict(nodes=-1), -1), (dict(out=None), -1), (dict(out=4104), -1),
+                                       (dict(work=None), -1), (dict(work=8), -1), (dict(nodes=257), -2), (dict(wide=2 ** 27 + 1), -2)])
+def test_attend_tree_refuses(L, change, rc):
+    assert attend_tree(L, cache(L), **change) == rc
+
+
+def test_tree_workspace_size(L):
+    f = L.lib().fvs_kv_attend_tree_work
+    assert f(0, 4) == -1 and f(64, -1) == -1 and f(512, 4) == -2
+    assert 0 < f(64, 1) == f(64, 128) < f(64, 129) == f(64, 4096) and f(256, 1) == f(256, 4096)
 
 
 @pytest.mark.parametrize("change", [dict(q_weight=68), dict(k_weight=8), dict(weight_type=1), dict(weight_type=2),
@@ -75,6 +97,7 @@ def test_empty_calls_do_nothing(L):
     assert append_norm(L, cache(L), tokens=0) == 0
     assert compact(L, cache(L), seqs=0) == 0 and compact(L, cache(L), nodes=0) == 0
     assert verify(L, seqs=0) == 0
+    assert attend_tree(L, cache(L), seqs=0) == 0 and attend_tree(L, cache(L), nodes=0) == 0
 
 
 def test_host_memory_is_refused():

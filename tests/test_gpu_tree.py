@@ -1,0 +1,342 @@
+"""Attention of trees of drafted tokens over a paged cache, against the 64-bit oracle.
+
+Bounds, from the arithmetic alone (u: unit roundoff of the output type):
+* a score is off by es <= (dim + 4) 2^-23 scale sum |q k| (fp32 sums; the tensor cores may cut instead of round), which
+  changes its weight by a factor e^(es);
+* a weight enters the second product as two parts of the 16-bit type: 2^-17 of it with bf16, 2^-21 with fp16, where weights
+  below 2^-25 of the largest lose more (2^-36 of the largest, absolute); the exponential is within 2^-21;
+* sums over L keys in fp32, cut or rounded: (L + 64) 2^-22 of sum p |v|; one rounding of the output.
+"""
+import numpy as np
+import pytest
+import torch
+
+from conftest import pkg
+from oracle import drafts_oracle as O
+from test_gpu_drafts import ints, some_trees
+from test_gpu_kv import BF16, DEV, F16, I8, U, c, full_table, kv, make_cache, values  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def check_tree(cache, q, table, lens, parents, counts=None, scale=None, got=None):
+    out, lse = got or cache.attend_tree(q, table, lens, parents, counts=counts, scale=scale)
+    torch.cuda.synchronize()
+    d = cache.dim
+    scale = 1 / np.sqrt(d) if scale is None else scale
+    k, v = values(cache)
+    up = np.broadcast_to(c(parents), q.shape[:2])
+    eo, el, pv, mag = O.attend_tree(c(q), k, v, c(table), c(lens), up, None if counts is None else c(counts), scale,
+                                    None if cache.fill is None else c(cache.fill))
+    out, lse = c(out), c(lse)
+    L = int(max(1, c(lens).max() + q.shape[1]))
+    es = (d + 4) * 2.0 ** -23 * mag
+    part = 2.0 ** -17 if BF16 in (q.dtype,) or cache.dtype == I8 else 2.0 ** -21
+    u = U[q.dtype]
+    tiny = 2.0 ** -25 if q.dtype == F16 else 0.0
+    tol = u * np.abs(eo) + (part + 2 * es[..., None] + 2.0 ** -20 + (L + 64) * 2.0 ** -22) * pv * 1.01 + tiny + 2.0 ** -36 * np.abs(np.nan_to_num(v)).max()
+    empty = np.isinf(el)
+    assert (out[empty] == 0).all() and np.array_equal(np.isneginf(lse), empty)
+    assert np.isfinite(out).all()
+    worst = (np.abs(out - eo) / tol).max()
+    assert worst <= 1, f"out is {worst:.2f} of its bound"
+    tol = 2 * es + (L + 64) * 2.0 ** -22 + 2.0 ** -20 * (1 + np.abs(np.where(empty, 0, el)))
+    worst = (np.abs(lse[~empty] - el[~empty]) / tol[~empty]).max(initial=0)
+    assert worst <= 1, f"lse is {worst:.2f} of its bound"
+    cache.check_status()
+
+
+def setup(kv, lens, nodes, heads, group, page, dim, dtype, store, g, **more):  # noqa: F811
+    table, pages = full_table([n + nodes for n in lens], page, g)
+    cache = make_cache(kv, pages, heads, page, dim, store, g, **more)
+    q = (torch.randn(len(lens), nodes, heads * group, dim, generator=g) * 1.5).to(DEV, dtype)
+    return cache, q, table.to(DEV), ints(lens)
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("dtype,store", [(BF16, BF16), (F16, F16), (BF16, I8), (F16, I8)])
+@pytest.mark.parametrize("heads,group,nodes", [(2, 1, 5), (1, 7, 20), (2, 4, 64)])
+def test_tree_types_and_dims(kv, dim, dtype, store, heads, group, nodes):  # noqa: F811
+    g, rng = torch.Generator().manual_seed(dim + heads), np.random.default_rng(dim)
+    lens = [0, 1, 17, 63, 64, 127, 128, 200, 391]
+    cache, q, table, n = setup(kv, lens, nodes, heads, group, 16, dim, dtype, store, g)
+    check_tree(cache, q, table, n, ints(some_trees(len(lens), nodes, rng)))
+
+
+@pytest.mark.parametrize("nodes,group", [(1, 1), (1, 16), (2, 3), (31, 1), (33, 2), (128, 1), (129, 1), (43, 3), (32, 8), (64, 16),
+                                         (256, 1), (256, 3), (255, 5), (100, 71)])
+@pytest.mark.parametrize("store", [BF16, I8])
+def test_tree_rows(kv, nodes, group, store):  # noqa: F811
+    """Fewer rows than a warp, one more than a tile, several tiles; one tree for all and a chain."""
+    g, rng = torch.Generator().manual_seed(nodes + group), np.random.default_rng(nodes)
+    lens = [300, 45, 0]
+    cache, q, table, n = setup(kv, lens, nodes, 2, group, 32, 64, BF16, store, g)
+    check_tree(cache, q, table, n, ints(some_trees(1, nodes, rng)[0]))
+    check_tree(cache, q, table, n, ints(np.arange(nodes) - 1))
+    check_tree(cache, q, table, n, ints(np.full(nodes, -1)), counts=ints([nodes // 2, 0, max(0, nodes - 1)]))
+
+
+@pytest.mark.parametrize("page", [1, 3, 7, 16, 20, 48, 100, 256])
+@pytest.mark.parametrize("store", [F16, I8])
+def test_tree_page_sizes(kv, page, store):  # noqa: F811
+    g, rng = torch.Generator().manual_seed(page), np.random.default_rng(page)
+    lens = [page - 1, page, page + 1, 5 * page, 333, 0, 1000]
+    cache, q, table, n = setup(kv, lens, 12, 2, 3, page, 128, F16, store, g, token_major=page == 16)
+    check_tree(cache, q, table, n, ints(some_trees(len(lens), 12, rng)), counts=ints([12, 3, 0, 1, 12, 12, 7]))
+
+
+@pytest.mark.parametrize("store", [BF16, I8])
+@pytest.mark.parametrize("page", [5, 16, 64])
+@pytest.mark.parametrize("dim", [64, 192])
+def test_tree_holes_fill_and_what_memory_holds(kv, page, store, dim):  # noqa: F811
+    g, rng = torch.Generator().manual_seed(page), np.random.default_rng(page)
+    B, nodes, w = 7, 9, 12
+    own = -(-nodes // page) + 1
+    pages = B * (w + own) + 2
+    perm = torch.randperm(pages - 2, generator=g).view(B, w + own).int()
+    table = perm.clone()
+    table[:, :w][torch.rand(B, w, generator=g) < 0.3] = -1
+    table[2, :w] = -1
+    fill = torch.randint(0, page + 1, (pages,), generator=g, dtype=torch.int32)
+    fill[perm[:, w:].reshape(-1).long()] = page
+    lens = torch.full((B,), w * page, dtype=torch.int32)
+    lens[3] += 1
+    cache = make_cache(kv, pages, 2, page, dim, store, g, fill=fill.to(DEV))
+    # every slot that nothing sees holds not-a-numbers
+    seen = torch.zeros(pages, page, dtype=torch.bool)
+    for b in range(B):
+        for t in range(int(lens[b]) + nodes):
+            p = int(table[b, t // page])
+            if p >= 0 and t % page < int(fill[p]):
+                seen[p, t % page] = True
+    seen = seen.to(DEV)
+    for x, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        (x if s is None else s).masked_fill_(~seen[:, None, :, None] if s is None else ~seen[:, None], float("nan"))
+    q = torch.randn(B, nodes, 6, dim, generator=g).to(DEV, BF16)
+    check_tree(cache, q, table.to(DEV), lens.to(DEV), ints(some_trees(B, nodes, rng)))
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (BF16, BF16), (BF16, I8)])
+@pytest.mark.parametrize("B,heads,group,dim,nodes,longest", [(1, 1, 1, 64, 1, 20000), (1, 8, 4, 128, 8, 9000), (1, 2, 4, 128, 64, 5000),
+                                                             (3, 2, 16, 96, 5, 4099), (2, 1, 4, 256, 30, 3001), (5, 3, 2, 192, 65, 700)])
+def test_tree_splits_over_the_length(kv, dtype, store, B, heads, group, dim, nodes, longest):  # noqa: F811
+    g, rng = torch.Generator().manual_seed(dim), np.random.default_rng(dim)
+    lens = [longest - i * (longest // 3) for i in range(B)] if B <= 3 else [longest] * B
+    cache, q, table, n = setup(kv, lens, nodes, heads, group, 64, dim, dtype, store, g)
+    check_tree(cache, q, table, n, ints(some_trees(B, nodes, rng)))
+
+
+@pytest.mark.parametrize("B,lens", [(300, (0, 300)), (900, (0, 40)), (1500, (0, 3)), (129, (0, 2000))])
+def test_tree_many_sequences(kv, B, lens):  # noqa: F811
+    g, rng = torch.Generator().manual_seed(B), np.random.default_rng(B)
+    n = list(rng.integers(*lens, B))
+    cache, q, table, n = setup(kv, n, 4, 1, 2, 16, 64, F16, F16, g)
+    check_tree(cache, q, table, n, ints(some_trees(B, 4, rng)), counts=ints(rng.integers(0, 5, B)))
+
+
+def test_tree_batches_of_changing_size(kv):  # noqa: F811
+    """Calls on one stream share a workspace."""
+    g, rng = torch.Generator().manual_seed(3), np.random.default_rng(3)
+    for B, nodes, longest in ((1, 64, 4000), (9, 5, 700), (1, 8, 6000), (40, 3, 100), (2, 200, 1000)):
+        cache, q, table, n = setup(kv, list(rng.integers(1, longest, B)), nodes, 2, 4, 16, 128, BF16, BF16, g)
+        check_tree(cache, q, table, n, ints(some_trees(B, nodes, rng)))
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (BF16, BF16), (F16, I8)])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0, 5.0])
+def test_tree_scores_far_apart(kv, dtype, store, scale):  # noqa: F811
+    """Scores that rise and fall by hundreds, a scale of its own, below zero or zero."""
+    g, rng = torch.Generator().manual_seed(4), np.random.default_rng(4)
+    cache, q, table, n = setup(kv, [900, 130], 10, 2, 2, 16, 64, dtype, store, g)
+    ramp = torch.linspace(-3, 3, cache.page * cache.pages, device=DEV)[torch.randperm(cache.page * cache.pages, generator=g).to(DEV)]
+    ramp = ramp.view(cache.pages, 1, cache.page)
+    if store == I8:
+        cache.k_scale *= ramp.abs() + 0.1
+    else:
+        cache.k *= ramp[..., None].to(dtype)
+    check_tree(cache, q, table, n, ints(some_trees(2, 10, rng)), scale=scale)
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (BF16, BF16), (BF16, I8)])
+def test_tree_scores_that_keep_rising(kv, dtype, store):  # noqa: F811
+    """Each tile's scores a little above those before, around the step at which outputs are scaled again."""
+    g = torch.Generator().manual_seed(5)
+    n, nodes, dim = 3000, 4, 64
+    table, pages = full_table([n + nodes], 16, g)
+    cache = make_cache(kv, pages, 1, 16, dim, F16 if store == F16 else BF16, g)
+    t = torch.arange(n + nodes).float() * (40.0 / n)
+    k = torch.zeros(pages, 1, 16, dim)
+    order = table[0].long().repeat_interleave(16)[:n + nodes]
+    k[order, 0, torch.arange(n + nodes) % 16, 0] = t
+    if store == I8:
+        scale = k.abs().amax(-1) / 127 + 1e-9
+        codes = (k / scale[..., None]).round().to(I8)
+        vs = c(cache.v)
+        vscale = torch.tensor(np.abs(vs).max(-1) / 127, dtype=torch.float32, device=DEV)
+        cache = kv.PagedKV(codes.to(DEV), (cache.v.float() / vscale[..., None]).round().to(I8), scale.to(DEV), vscale)
+    else:
+        cache.k.copy_(k)
+    q = torch.zeros(1, nodes, 2, dim)
+    q[..., 0] = torch.linspace(0.2, 8, 2 * nodes).view(1, nodes, 2)
+    check_tree(cache, q.to(DEV, dtype), table.to(DEV), ints([n]), ints([-1, 0, 0, 1]), scale=1.0)
+
+
+@pytest.mark.parametrize("dtype,store", [(F16, F16), (BF16, BF16)])
+def test_tree_weights_are_not_cut(kv, dtype, store):  # noqa: F811
+    """Equal scores over values that all but cancel: one part of a weight would be off by its own rounding."""
+    g = torch.Generator().manual_seed(6)
+    cache, q, table, n = setup(kv, [4000], 3, 1, 2, 16, 128, dtype, store, g)
+    check_tree(cache, q * 0.1, table, n, ints([-1, 0, 1]))
+
+
+def test_tree_non_finite_inputs(kv):  # noqa: F811
+    """A node's not-a-numbers stay in its own outputs; an infinite score is not-a-number as in the formula; rows whose
+    scores are all -infinity have no weight."""
+    g = torch.Generator().manual_seed(7)
+    cache, q, table, n = setup(kv, [40, 40], 4, 1, 2, 16, 64, F16, F16, g)
+    parents = ints([-1, 0, 0, -1])
+    want, _ = cache.attend_tree(q, table, n, parents)
+    q2 = q.clone()
+    q2[0, 1] = float("nan")
+    out, lse = cache.attend_tree(q2, table, n, parents)
+    assert torch.isnan(out[0, 1]).all() and torch.isnan(lse[0, 1]).all()
+    out[0, 1] = want[0, 1]
+    assert torch.equal(out, want)
+    cache.k[:] = 1.0
+    cache.k[..., 0] = float("-inf")
+    q[:] = 1.0
+    out, lse = cache.attend_tree(q, table, n, parents)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    cache.k[table[0, 0].item(), 0, 3, 0] = float("inf")
+    out, lse = cache.attend_tree(q, table, n, parents)
+    assert torch.isnan(out[0]).all() and (out[1] == 0).all()
+
+
+def test_tree_strides_streams_and_graphs(kv):  # noqa: F811
+    g, rng = torch.Generator().manual_seed(8), np.random.default_rng(8)
+    B, nodes = 3, 12
+    cache, q, table, n = setup(kv, [700, 90, 2500], nodes, 2, 4, 16, 128, BF16, BF16, g)
+    parents = ints(some_trees(B, nodes, rng))
+    want, wlse = cache.attend_tree(q, table, n, parents)
+    check_tree(cache, q, table, n, parents, got=(want, wlse))
+    room = torch.full((B, 8, nodes, 256), float("nan"), dtype=BF16, device=DEV)
+    view = room[..., 64:192].transpose(1, 2)
+    view.copy_(q)
+    out, lse = cache.attend_tree(view, table, n, parents)
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    wide = torch.full((B, table.shape[1] + 5), 10 ** 6, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    out, lse = cache.attend_tree(q, wide[:, :table.shape[1]], n, parents)
+    assert torch.equal(out, want)
+    one = q[:1].expand(B, nodes, 8, 128)
+    a, b = cache.attend_tree(one, table, n, parents), cache.attend_tree(one.contiguous(), table, n, parents)
+    assert torch.equal(a[0], b[0])
+    # two captured calls, replayed beside eager ones on another stream, and with new lengths and trees
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got = cache.attend_tree(q, table, n, parents)
+    with torch.cuda.graph(second, stream=side):
+        got2 = cache.attend_tree(q, table, n, parents)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        with torch.cuda.stream(side):
+            graph.replay()
+        with torch.cuda.stream(other):
+            second.replay()
+            beside = cache.attend_tree(q, table, n, parents)
+        torch.cuda.synchronize()
+        for x in (got, got2, beside):
+            assert torch.equal(x[0], want) and torch.equal(x[1], wlse)
+    n.copy_(ints([20, 90, 1234]))
+    parents.copy_(ints(some_trees(B, nodes, rng)))
+    graph.replay()
+    torch.cuda.synchronize()
+    check_tree(cache, q, table, n, parents, got=got)
+
+
+def test_tree_offsets_past_32_bits(kv):  # noqa: F811
+    g = torch.Generator().manual_seed(9)
+    pages, page, heads, dim = 9000, 64, 32, 128                   # 2.36e9 elements each of k and v
+    k, v = (torch.zeros(pages, heads, page, dim, dtype=F16, device=DEV) for _ in range(2))
+    cache = kv.PagedKV(k, v)
+    used = torch.tensor([pages - 1, pages - 3, 1, pages - 2])
+    for x in (k, v):
+        x[used.to(DEV)] = torch.randn(4, heads, page, dim, generator=g).to(DEV, F16)
+    q = torch.randn(1, 5, 32, dim, generator=g).to(DEV, F16)
+    out, lse = cache.attend_tree(q, ints(used[None]), ints([200]), ints([-1, 0, 0, 1, 2]))
+    small = kv.PagedKV(k[used.to(DEV)].contiguous(), v[used.to(DEV)].contiguous())
+    check_tree(small, q, ints([[0, 1, 2, 3]]), ints([200]), ints([-1, 0, 0, 1, 2]), got=(out, lse))
+
+
+def test_tree_of_one_node_is_attend(kv):  # noqa: F811
+    g = torch.Generator().manual_seed(10)
+    cache, q, table, n = setup(kv, [0, 5, 700, 64], 1, 2, 4, 16, 128, F16, F16, g)
+    out, lse = cache.attend_tree(q, table, n, ints([-1]))
+    one, olse = cache.attend(q[:, 0], table, n + 1)
+    assert (out[:, 0].float() - one.float()).abs().max() <= 2.0 ** -10 * one.float().abs().max()
+    assert (lse[:, 0] - olse).abs().max() <= 1e-5 * olse.abs().max()
+
+
+def test_tree_bad_indices_are_reported(kv):  # noqa: F811
+    """Lengths and nodes past the table, pages past the cache: cut or skipped, and reported; wrong parents are none."""
+    FvsError = pkg("_lib").FvsError
+    g = torch.Generator().manual_seed(11)
+    cache, q, table, n = setup(kv, [40, 40], 8, 1, 2, 16, 64, F16, F16, g)
+    parents = ints([-1, 0, 0, 1, 1, 2, 3, 3])
+    k, v = values(cache)
+
+    def reported(tab, lens, up=parents):
+        out, lse = cache.attend_tree(q, tab, lens, up)
+        with pytest.raises(FvsError):
+            cache.check_status()
+        room = tab.shape[1] * 16
+        eo, el, *_ = O.attend_tree(c(q), k, v, c(tab), np.clip(c(lens), 0, room), np.broadcast_to(c(up), (2, 8)), None, 0.125)
+        assert np.abs(c(out) - eo).max() < 2e-3 and np.array_equal(np.isinf(c(lse)), np.isinf(el))
+
+    reported(table, ints([44, 40]))
+    reported(table, ints([1000, 2 ** 31 - 1]))
+    bad = table.clone()
+    bad[0, 1] = cache.pages
+    reported(bad, n)
+    check_tree(cache, q, table, ints([-5, 40]), parents)
+    for wrong in ([0, 0, 5, 1, 4, -7, 3, 2 ** 31 - 1], [-(2 ** 31)] * 8, [7] * 8):
+        check_tree(cache, q, table, n, ints(wrong))
+
+
+def test_tree_refusals(kv):  # noqa: F811
+    g = torch.Generator().manual_seed(12)
+    z = lambda *s, dtype=F16: torch.zeros(*s, dtype=dtype, device=DEV)  # noqa: E731
+    cache = make_cache(kv, 4, 2, 16, 64, F16, g)
+    t, n, p, q = ints(np.zeros((3, 2))), ints(np.zeros(3)), ints([-1, 0]), z(3, 2, 4, 64)
+    learned = z(3, 2, 4, 64).requires_grad_()
+    for args, more in (((q.float(), t, n, p), {}), ((q.to(BF16), t, n, p), {}), ((z(3, 2, 5, 64), t, n, p), {}), ((z(3, 2, 4, 96), t, n, p), {}),
+                       ((z(3, 4, 64), t, n, p), {}), ((q, t.long(), n, p), {}), ((q, t[:2], n, p), {}), ((q, t, n.long(), p), {}),
+                       ((q, t, n, p[:1]), {}), ((q, t, n, p.long()), {}), ((q, t, n, ints(np.zeros((2, 2)))), {}), ((q.cpu(), t, n, p), {}),
+                       ((z(3, 2, 64, 4).transpose(2, 3), t, n, p), {}), ((learned, t, n, p), {}), ((z(3, 2, 4, 68)[..., :64], t, n, p), {}),
+                       ((z(3, 257, 2, 64), t, n, ints(np.arange(257) - 1)), {}), ((q, t, n, p), dict(counts=n[:2])),
+                       ((q, t, n, p), dict(out=q.float())), ((q, t, n, p), dict(lse=z(3, 2, 4))), ((q, t, n, p), dict(lse=z(3, 2, 2, dtype=torch.float32)))):
+        with pytest.raises(ValueError):
+            cache.attend_tree(*args, **more)
+    assert cache.launches == 0
+    out, lse = cache.attend_tree(z(0, 2, 4, 64), t[:0], n[:0], p)
+    assert out.shape == (0, 2, 4, 64) and lse.shape == (0, 2, 4)
+    out, lse = cache.attend_tree(z(3, 0, 4, 64), t, n, p[:0])
+    assert out.shape == (3, 0, 4, 64) and lse.shape == (3, 0, 4)
+
+
+def test_tree_waits_that_run_out(kv):  # noqa: F811
+    """With no polls allowed every wait inside the kernel gives up: the call reports it, and the next one works."""
+    L = pkg("_lib")
+    g = torch.Generator().manual_seed(13)
+    cache, q, table, n = setup(kv, [700, 90], 6, 2, 4, 16, 128, BF16, BF16, g)
+    parents = ints([-1, 0, 1, 2, 3, 4])
+    old = L.lib().fvs_set_wait_limit(0)
+    try:
+        cache.attend_tree(q, table, n, parents)
+        with pytest.raises(L.FvsError, match="ran out"):
+            cache.check_status()
+    finally:
+        L.lib().fvs_set_wait_limit(old)
+    check_tree(cache, q, table, n, parents)
