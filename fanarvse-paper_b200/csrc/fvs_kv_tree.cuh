@@ -34,6 +34,7 @@ using namespace fvs::tcg;
 
 constexpr int ROWS = 128;     // rows of a matrix instruction
 constexpr int INFO = 4;       // tiles whose keys' flags and scales are held
+constexpr int SEGS = 4;       // segments that the scheduler is ahead
 constexpr int ITEM_COST = 2;  // cost of an item in tiles: its queries' copy and its output
 constexpr int GAVE_UP = 2;    // status bit: a bounded wait ran out
 
@@ -60,12 +61,13 @@ struct Shape {
     static constexpr int W = D <= 128 ? 2 : 1;
     static constexpr int BLOCKS = (D + 63) / 64;  // 128-byte columns of a tile
     static constexpr int SLOT = KEYS * 128 * BLOCKS;
-    static constexpr int THREADS = 32 * (4 * W + 4 + 1);
+    static constexpr int THREADS = 32 * (4 * W + 4 + 2);  // softmax, producers, matrix instructions and scheduler
     static constexpr int O0 = 2 * KEYS;  // TMEM columns: two S, then W of O
     static_assert(O0 + W * D <= 512, "tensor memory columns");
 };
 constexpr int BARS = 64 * 8, INFO_BYTES = 16 + 2 * 128 * 4, MERGE_BYTES = 2 * 2 * ROWS * 8;
-constexpr int MISC = BARS + INFO * INFO_BYTES + MERGE_BYTES + 64;
+constexpr int SEG_BYTES = 48, MASK_BYTES = 2 * 4 * ROWS * 4;  // masks: a row's 128 bits for each softmax thread
+constexpr int MISC = BARS + INFO * INFO_BYTES + MERGE_BYTES + 64 + SEGS * SEG_BYTES + MASK_BYTES;
 template <int D, int MT>
 struct Plan {
     using S = Shape<D>;
@@ -95,49 +97,52 @@ __device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) {
     return (int64_t)s.rts * a.c.heads * (ITEM_COST + s.tiles);
 }
 
-struct Seg {  // tiles [t0, t1) of one item
-    int b, head, rt, rows, t0, t1;
-    Seq s;
+struct Seg {             // tiles [t0, t1) of one item; t0 == t1: no more
+    int b, head, rt, rows, t0, t1, n, keys, tiles, item;
 };
 
-// Walks over the segments of a CTA: every role does so by itself, over the same numbers.
+// Walks over the segments of a CTA (the scheduler's).
 template <int KEYS, int RT>
 struct Walk {
-    int64_t base, end;  // cost before the item, and where the CTA's share ends
-    int64_t start;
-    int item;           // of its sequence
-    Seg g;
-    __device__ __forceinline__ void begin(const Args& a, int b, int64_t b_base, int64_t from, int64_t to) {
+    int64_t base, start, end;  // cost before the item, and the CTA's share
+    int item, b;               // item of the sequence
+    Seq s;
+    __device__ __forceinline__ void begin(const Args& a, int first, int64_t first_base, int64_t from, int64_t to) {
         start = from;
         end = to;
-        g.b = b;
-        base = b_base;
+        b = first;
+        base = first_base;
         item = -1;
         if (from < to) {
-            g.s = sequence<KEYS, RT>(a, b);
-            const int each = ITEM_COST + g.s.tiles;
-            item = (int)((from - b_base) / each) - 1;
-            base = b_base + (int64_t)item * each;
+            s = sequence<KEYS, RT>(a, b);
+            const int each = ITEM_COST + s.tiles;
+            item = (int)((from - first_base) / each) - 1;
+            base = first_base + (int64_t)item * each;
         }
     }
-    __device__ __forceinline__ bool next(const Args& a) {
+    __device__ __forceinline__ bool next(const Args& a, Seg& g) {
         if (start >= end) return false;
         while (true) {
-            base += ITEM_COST + g.s.tiles;
+            base += ITEM_COST + s.tiles;
             item++;
-            while (item >= g.s.rts * a.c.heads) {
+            while (item >= s.rts * a.c.heads) {
                 item = 0;
-                if (base >= end || ++g.b >= a.tb.seqs) return false;
-                g.s = sequence<KEYS, RT>(a, g.b);
+                if (base >= end || ++b >= a.tb.seqs) return false;
+                s = sequence<KEYS, RT>(a, b);
             }
             if (base >= end) return false;
             const int64_t first = start - base - ITEM_COST, last = end - base - ITEM_COST;
             g.t0 = first > 0 ? (int)first : 0;
-            g.t1 = last < g.s.tiles ? (int)last : g.s.tiles;
+            g.t1 = last < s.tiles ? (int)last : s.tiles;
             if (g.t0 >= g.t1) continue;
-            g.head = item / g.s.rts;
-            g.rt = item - g.head * g.s.rts;
-            g.rows = min(RT, g.s.count * a.group - g.rt * RT);
+            g.b = b;
+            g.item = item;
+            g.head = item / s.rts;
+            g.rt = item - g.head * s.rts;
+            g.rows = min(RT, s.count * a.group - g.rt * RT);
+            g.n = s.n;
+            g.keys = s.keys;
+            g.tiles = s.tiles;
             return true;
         }
     }
@@ -176,6 +181,24 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
+// waits for the loads so far, those into r among them: what reads r comes behind
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
@@ -195,6 +218,35 @@ __device__ __forceinline__ float exp2_of(float x) {
     return r;
 }
 
+// two fp32 operations in one instruction
+struct Two {
+    uint64_t x;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.x) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 one(Two a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.x));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.x) : "l"(a.x), "l"(b.x), "l"(c.x));
+    return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
+    return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.x) : "l"(a.x), "l"(b.x));
+    return r;
+}
 // four int8 codes as 16-bit values, exactly: fp16 by 1024 + 128 + code in the mantissa; bf16 by the low seven bits behind
 // 128, less 128 or, for a negative code, 256
 template <int TYPE>
@@ -242,6 +294,9 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
     auto pv_done = [&](int w) { return bars + 8 * (36 + w); };
     const uint32_t q_full = bars + 8 * 38, q_empty = bars + 8 * 39, o_free = bars + 8 * 40, merge_bar = bars + 8 * 41,
                    drain = bars + 8 * 42;
+    auto seg_full = [&](int s) { return bars + 8 * (43 + s); };
+    auto seg_empty = [&](int s) { return bars + 8 * (43 + SEGS + s); };
+    volatile Seg* segs = reinterpret_cast<volatile Seg*>(misc + BARS + INFO * INFO_BYTES + MERGE_BYTES + 64);
     uint8_t* info = misc + BARS;
     float2* merge = reinterpret_cast<float2*>(misc + BARS + INFO * INFO_BYTES);  // [2][W][ROWS]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + BARS + INFO * INFO_BYTES + MERGE_BYTES);
@@ -271,6 +326,10 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
         mbar_init(o_free, 128 * W);
         mbar_init(merge_bar, 128 * W);
         mbar_init(drain, 1);
+        for (int s = 0; s < SEGS; s++) {
+            mbar_init(seg_full(s), 1);
+            mbar_init(seg_empty(s), 4 * W + 4 + 1);
+        }
         *abort = 0;
         s_place[0] = s_place[1] = s_place[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -338,62 +397,80 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    Walk<KEYS, RT> walk;
-    {
-        const int64_t total = s_place[0];
-        walk.begin(a, (int)s_place[1], s_place[2], total * (int64_t)blockIdx.x / gridDim.x, total * ((int64_t)blockIdx.x + 1) / gridDim.x);
-    }
-    Seg& g = walk.g;
+    const float scale2 = a.scale * 1.4426950408889634f;  // of scores in powers of two
 
     if (warp >= W_PROD && warp < W_MMA) {
         // ------------------------------------------------------------ producers
-        constexpr int PER = KEYS / 4;            // keys of a warp
+        constexpr int PER = KEYS / 4;              // keys of a warp
         constexpr int CH = (I8 ? D / 16 : D / 8);  // 16-byte chunks of a stored row
         constexpr int TURNS = PER * CH / 32;
         static_assert(PER * CH % 32 == 0, "whole turns");
-        constexpr int ESZ = I8 ? 1 : 2;
+        constexpr uint32_t NONE = 0xffffffffu;
         const int pw = warp - W_PROD, key = pw * PER + (lane % PER);
         const uint8_t *kbase = (const uint8_t*)a.c.k, *vbase = (const uint8_t*)a.c.v;
-        int slot = 0, phase = 1, tile = 0, seg = 0;  // the first pass over the ring finds it free
+        int slot = 0, phase = 1, tile = 0;  // the first pass over the ring finds it free
+        int b = 0, head = 0, keys = 0;      // of the segment
         bool ok = true;
-        // where key `key` of tile t lies: elements from the head's first, -1 for none
-        auto lookup = [&](int t, int64_t& at, int64_t& scale_at) {
+        // where key `key` of tile t lies, in 16 bytes from the tensor's first, and its scales
+        uint32_t at, next_at;
+        float ks = 0.f, vs = 0.f;
+        auto lookup = [&](int t) {
             const int x = t * KEYS + key;
-            at = -1;
-            scale_at = 0;
-            if (x < g.s.keys) {
+            next_at = NONE;
+            if (I8) ks = vs = 0.f;
+            if (x < keys) {
                 int page, s;
-                if (place(a.c, a.tb, g.b, x, page, s) && (!a.c.fill || s < __ldg(a.c.fill + page))) {
-                    at = (int64_t)page * a.c.page_stride + (int64_t)s * a.c.slot_stride + (int64_t)g.head * a.c.head_stride;
-                    if (I8) scale_at = (int64_t)page * a.c.scale_page_stride + (int64_t)s * a.c.scale_slot_stride + (int64_t)g.head * a.c.scale_head_stride;
+                if (place(a.c, a.tb, b, x, page, s) && (!a.c.fill || s < __ldg(a.c.fill + page))) {
+                    const int64_t e = (int64_t)page * a.c.page_stride + (int64_t)s * a.c.slot_stride + (int64_t)head * a.c.head_stride;
+                    next_at = (uint32_t)(e / (I8 ? 16 : 8));
+                    if (I8) {
+                        const int64_t se = (int64_t)page * a.c.scale_page_stride + (int64_t)s * a.c.scale_slot_stride + (int64_t)head * a.c.scale_head_stride;
+                        ks = __ldg(a.c.k_scale + se);
+                        vs = __ldg(a.c.v_scale + se);
+                    }
                 }
             }
         };
         auto advance = [&]() {
             if (++slot == SLOTS) slot = 0, phase ^= 1;
         };
-        // the warp's rows of one operand into the ring's next slot
-        auto copy = [&](const uint8_t* base, int64_t at) {
+        // chunk c of key k in a slot
+        auto chunk = [&](int k, int c) { return (uint32_t)((c >> 3) * (KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4)); };
+        // the rows that this lane copies chunks of, a turn each: the same for keys and values
+        uint32_t rows[TURNS];
+        auto exchange = [&](uint32_t x) {
+#pragma unroll
+            for (int i = 0; i < TURNS; i++) rows[i] = __shfl_sync(0xffffffffu, x, (i * 32 + lane) / CH);
+        };
+        auto copy = [&](const uint8_t* base, bool all) {
             const uint32_t dst = ring + slot * S::SLOT;
-#pragma unroll 4
-            for (int i = 0; i < TURNS; i++) {
-                const int id = i * 32 + lane, r = id / CH, c = id - r * CH;
-                const int64_t row = __shfl_sync(0xffffffffu, at, r);
-                const int k = pw * PER + r;
-                cp_async16(dst + (c >> 3) * (KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), base + (row < 0 ? 0 : (row * ESZ + c * 16)), row >= 0);
+            if (all) {
+#pragma unroll
+                for (int i = 0; i < TURNS; i++) {
+                    const int id = i * 32 + lane, r = id / CH, c = id - r * CH;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + chunk(pw * PER + r, c)), "l"(base + c * 16 + (uint64_t)rows[i] * 16) : "memory");
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < TURNS; i++) {
+                    const int id = i * 32 + lane, r = id / CH, c = id - r * CH;
+                    const bool there = rows[i] != NONE;
+                    cp_async16(dst + chunk(pw * PER + r, c), base + (there ? c * 16 + (uint64_t)rows[i] * 16 : 0), there);
+                }
             }
             copies_arrive(full(slot));
         };
-        uint4 raw[I8 ? TURNS : 1];
-        auto fetch = [&](const uint8_t* base, int64_t at) {
+        // int8 codes: keys and values of the next tile are on their way in registers
+        uint4 rk[I8 ? TURNS : 1], rv[I8 ? TURNS : 1];
+        auto fetch = [&](uint4* raw, const uint8_t* base) {
 #pragma unroll
             for (int i = 0; i < (I8 ? TURNS : 0); i++) {
                 const int id = i * 32 + lane, r = id / CH, c = id - r * CH;
-                const int64_t row = __shfl_sync(0xffffffffu, at, r);
-                raw[i] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg((const uint4*)(base + row + c * 16));
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (rows[i] != NONE) raw[i] = __ldg((const uint4*)(base + c * 16 + (uint64_t)rows[i] * 16));
             }
         };
-        auto widen = [&](auto type) {
+        auto widen = [&](uint4* raw, auto type) {
             constexpr int T = decltype(type)::value;
             const uint32_t dst = ring + slot * S::SLOT;
 #pragma unroll
@@ -404,21 +481,30 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                 widen4<T>(raw[i].y, w[2], w[3]);
                 widen4<T>(raw[i].z, w[4], w[5]);
                 widen4<T>(raw[i].w, w[6], w[7]);
-                const uint32_t at = dst + (c >> 3) * (KEYS * 128) + k * 128;
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((c & 7) ^ (k & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at + ((((c + 1) & 7) ^ (k & 7)) << 4)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + chunk(k, c)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + chunk(k, c + 1)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
             }
             proxy_fence();
             mbar_arrive(full(slot));
         };
-        while (ok && walk.next(a)) {
-            int64_t at, scale_at;
-            lookup(g.t0, at, scale_at);
-            for (int t = g.t0; t < g.t1 && ok; t++, tile++) {
+        for (int seg = 0; ok; seg++) {
+            if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
+            const volatile Seg& g = segs[seg % SEGS];
+            const int t0 = g.t0, t1 = g.t1;
+            b = g.b, head = g.head, keys = g.keys;
+            if (t0 >= t1) break;
+            lookup(t0);
+            at = next_at;
+            if (I8) {
+                exchange(at);
+                fetch(rk, kbase);
+                fetch(rv, vbase);
+            }
+            for (int t = t0; t < t1 && ok; t++, tile++) {
                 // flags and scales
                 const int is = tile % INFO;
                 if (!warp_wait(info_empty(is), ((tile / INFO) & 1) ^ 1, abort, WL)) { ok = false; break; }
-                const unsigned there = __ballot_sync(0xffffffffu, at >= 0);
+                const unsigned there = __ballot_sync(0xffffffffu, at != NONE);
                 uint8_t* mine = info + is * INFO_BYTES;
                 if (lane == 0) {
                     if (PER == 32)
@@ -428,50 +514,60 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                 }
                 if (I8 && lane < PER) {
                     float* sc = reinterpret_cast<float*>(mine + 16);
-                    sc[key] = at >= 0 ? __ldg(a.c.k_scale + scale_at) : 0.f;
-                    sc[128 + key] = at >= 0 ? __ldg(a.c.v_scale + scale_at) : 0.f;
+                    sc[key] = ks * scale2;  // scores in powers of two
+                    sc[128 + key] = vs;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(info_full(is));
-                const int64_t now = at;
-                if (I8) fetch(kbase, now);
-                if (t + 1 < g.t1) lookup(t + 1, at, scale_at);
+                if (!I8) exchange(at);
+                if (t + 1 < t1) {
+                    lookup(t + 1);
+                    at = next_at;
+                }
                 if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
-                if (I8)
-                    widen(std::integral_constant<int, TYPE>());
-                else
-                    copy(kbase, now);
+                if (I8) {
+                    widen(rk, std::integral_constant<int, TYPE>());
+                    if (t + 1 < t1) {
+                        exchange(at);
+                        fetch(rk, kbase);
+                    }
+                } else {
+                    copy(kbase, there == 0xffffffffu);
+                }
                 advance();
-                if (I8) fetch(vbase, now);
                 if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
-                if (I8)
-                    widen(std::integral_constant<int, FVS_BF16>());
-                else
-                    copy(vbase, now);
+                if (I8) {
+                    widen(rv, std::integral_constant<int, FVS_BF16>());
+                    if (t + 1 < t1) fetch(rv, vbase);
+                } else {
+                    copy(vbase, there == 0xffffffffu);
+                }
                 advance();
-                if (t == g.t0) {
+                if (t == t0) {
                     // the rows' queries, behind the first tile: their buffer is free when the segment before has its scores
                     if (!warp_wait(q_empty, (seg & 1) ^ 1, abort, WL)) { ok = false; break; }
                     constexpr int QCH = D / 8;
+                    const int rt = g.rt, live_rows = g.rows;
                     for (int id = pw * 32 + lane; id < RT * QCH; id += 128) {
-                        const int r = id / QCH, c = id - r * QCH, mt = r / ROWS, k = r - mt * ROWS, row = g.rt * RT + r;
-                        const bool live = r < g.rows;
+                        const int r = id / QCH, c = id - r * QCH, mt = r / ROWS, k = r - mt * ROWS, row = rt * RT + r;
+                        const bool live = r < live_rows;
                         const int node = live ? row / a.group : 0, h = live ? row - node * a.group : 0;
-                        const uint16_t* src = (const uint16_t*)a.q + (int64_t)g.b * a.q_seq + (int64_t)node * a.q_node + (int64_t)(g.head * a.group + h) * a.q_head + c * 8;
+                        const uint16_t* src = (const uint16_t*)a.q + (int64_t)b * a.q_seq + (int64_t)node * a.q_node + (int64_t)(head * a.group + h) * a.q_head + c * 8;
                         cp_async16(q_smem + mt * (ROWS * 128 * S::BLOCKS) + (c >> 3) * (ROWS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), src, live);
                     }
                     copies_arrive(q_full);
                 }
             }
-            seg++;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(seg_empty(seg % SEGS));
         }
         cp_async_wait_all();
-    } else if (warp == W_MMA) {
+    } else if (warp >= W_MMA) {
         // ------------------------------------------------------------ the matrix instructions' thread
-        if (lane == 0) {
+        if (warp == W_MMA && lane == 0) {
             const uint32_t id_s = idesc(KEYS, TYPE == FVS_BF16, false), id_o = idesc(D, VTYPE == FVS_BF16, true);
             int kslot = 0, kphase = 0, vslot = 1, vphase = 0;  // keys in even places of the stream, values in odd ones
-            int unit = 0, seg = 0;
+            int unit = 0;
             bool ok = true;
             auto scores = [&](int u, int mt) {
                 const uint32_t d = tmem + (u & 1) * KEYS, ab = q_smem + mt * (ROWS * 128 * S::BLOCKS), bb = ring + kslot * S::SLOT;
@@ -506,9 +602,11 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                 }
                 return true;
             };
-            while (ok && walk.next(a)) {
-                if (!mbar_wait(q_full, seg & 1, abort, WL)) break;
-                const int tiles = g.t1 - g.t0, units = tiles * MT;
+            for (int seg = 0;; seg++) {
+                if (!mbar_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
+                const int tiles = segs[seg % SEGS].t1 - segs[seg % SEGS].t0, units = tiles * MT;
+                mbar_arrive(seg_empty(seg % SEGS));
+                if (tiles == 0 || !mbar_wait(q_full, seg & 1, abort, WL)) break;
                 for (int x = 0; x < units && ok; x++, unit++) {
                     const int mt = MT == 2 ? x & 1 : 0;
                     if (mt == 0 && !mbar_wait(full(kslot), kphase, abort, WL)) { ok = false; break; }
@@ -528,20 +626,40 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                     }
                 }
                 if (!ok || !outputs(unit - 1, tiles - 1, MT - 1)) break;
-                seg++;
             }
             mma_commit(drain);  // what was issued has to end before the CTA does
             mbar_drain(drain, 0);
+        } else if (warp == W_MMA + 1 && lane == 0) {
+            // -------------------------------------------------------- the scheduler
+            Walk<KEYS, RT> walk;
+            const int64_t total = s_place[0];
+            walk.begin(a, (int)s_place[1], s_place[2], total * (int64_t)blockIdx.x / gridDim.x, total * ((int64_t)blockIdx.x + 1) / gridDim.x);
+            bool more = true;
+            for (int seg = 0; more; seg++) {
+                Seg g;
+                more = walk.next(a, g);
+                if (!more) g.t0 = g.t1 = 0;
+                if (!mbar_wait(seg_empty(seg % SEGS), ((seg / SEGS) & 1) ^ 1, abort, WL)) break;
+                volatile Seg& to = segs[seg % SEGS];
+                to.t0 = g.t0, to.t1 = g.t1;
+                if (more) to.b = g.b, to.head = g.head, to.rt = g.rt, to.rows = g.rows, to.n = g.n, to.keys = g.keys, to.tiles = g.tiles, to.item = g.item;
+                mbar_arrive(seg_full(seg % SEGS));
+            }
         }
         __syncwarp();
     } else if (warp < W_PROD) {
         // ------------------------------------------------------------ softmax, a thread per row
         const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // warpgroup, TMEM lane
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const float c = a.scale * 1.4426950408889634f;
-        int tile = 0, seg = 0;
+        uint32_t* mask = reinterpret_cast<uint32_t*>(misc + BARS + INFO * INFO_BYTES + MERGE_BYTES + 64 + SEGS * SEG_BYTES) + w * 4 * ROWS + r;
+        const float lift = scale2 == 0.f ? 1.f : fabsf(scale2);  // the sign, and a scale of 0, are in the scores
+        int tile = 0;
         bool ok = true;
-        while (ok && walk.next(a)) {
+        for (int seg = 0;; seg++) {
+            if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) { ok = false; break; }
+            const volatile Seg& g = segs[seg % SEGS];
+            const int t0 = g.t0, t1 = g.t1;
+            if (t0 >= t1) break;
             const int mine = MT == 2 ? w * ROWS + r : r;            // row of the item's row tile
             const bool warp_live = mine - lane < g.rows;
             const int row = g.rt * RT + mine;
@@ -549,7 +667,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
             float m = __int_as_float(0xff800000), l = 0.f;
             bool any = false;                                       // units of this warpgroup in this segment
             int last = -1;                                          // the last of them
-            for (int t = g.t0; t < g.t1; t++, tile++) {
+            for (int t = t0; t < t1; t++, tile++) {
                 int u = MT == 2 ? 2 * tile + w : tile;
                 if (MT == 1 && W == 2 && (u & 1) != w) continue;
                 const int n_th = W == 2 ? u >> 1 : u;               // of this warpgroup
@@ -563,7 +681,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                     bool all = true;
 #pragma unroll
                     for (int k = 0; k < CHUNKS; k++) see[k] = reinterpret_cast<const uint32_t*>(inf)[k];
-                    const int x0 = t * KEYS - g.s.n;                // of the tile's first key behind the sequence
+                    const int x0 = t * KEYS - g.n;                // of the tile's first key behind the sequence
                     if (x0 + KEYS > 0) {
                         uint32_t tree[CHUNKS];
 #pragma unroll
@@ -585,31 +703,53 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                     }
 #pragma unroll
                     for (int k = 0; k < CHUNKS; k++) all &= see[k] == 0xffffffffu;
-                    const bool plain = __all_sync(0xffffffffu, all);
+                    const bool odd = __any_sync(0xffffffffu, !all) || (!I8 && scale2 <= 0.f);
+                    if (odd) {
+#pragma unroll
+                        for (int k = 0; k < CHUNKS; k++) mask[k * ROWS] = see[k];
+                    }
                     const float* ks = reinterpret_cast<const float*>(inf + 16);
-                    // the largest score, in powers of two
-                    float top = __int_as_float(0xff800000);
+                    // Two passes over the row's scores in TMEM, 32 at a time: the largest, then the weights.  (All of a
+                    // tile's at once leave no registers, and unrolled code no place in the instruction cache: both took up
+                    // to half as long again.)
+                    uint32_t s[32];
+                    // what the scores are before `lift`: with the key's scale and in powers of two (int8), with their sign;
+                    // masked where the tile is not plain
+                    auto fetch = [&](int k) {
+                        tmem_ld32(s_tmem + 32 * k, s);
+                        tmem_wait32(s);
+                        if (I8) {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const float4 f = *reinterpret_cast<const float4*>(ks + 32 * k + j);
+                                const float2 y = one(mul2(two(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), two(f.x, f.y)));
+                                const float2 z = one(mul2(two(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])), two(f.z, f.w)));
+                                s[j] = __float_as_uint(y.x), s[j + 1] = __float_as_uint(y.y);
+                                s[j + 2] = __float_as_uint(z.x), s[j + 3] = __float_as_uint(z.y);
+                            }
+                        }
+                        if (odd) {
+                            const uint32_t word = reinterpret_cast<const volatile uint32_t*>(mask)[k * ROWS];
+                            const float sign = I8 ? 1.f : scale2 < 0.f ? -1.f : scale2 == 0.f ? 0.f : 1.f;
+#pragma unroll
+                            for (int j = 0; j < 32; j++) s[j] = word >> j & 1 ? __float_as_uint(__uint_as_float(s[j]) * sign) : 0xff800000u;
+                        }
+                    };
+                    float tops[4];
+#pragma unroll
+                    for (int y = 0; y < 4; y++) tops[y] = __int_as_float(0xff800000);
 #pragma unroll 1
                     for (int k = 0; k < CHUNKS; k++) {
-                        uint32_t s[32];
-                        tmem_ld32(s_tmem + 32 * k, s);
-                        const uint32_t word = plain ? 0xffffffffu : CHUNKS == 2 ? (k ? see[1] : see[0]) : k < 2 ? (k ? see[1] : see[0]) : (k == 2 ? see[CHUNKS - 2] : see[CHUNKS - 1]);
-                        tmem_ld_wait();
+                        fetch(k);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) {
-                            float x = __uint_as_float(s[j]) * c;
-                            if (I8) x *= ks[32 * k + j];
-                            s[j] = __float_as_uint(x);
-                        }
-                        if (plain) {
+                        for (int j = 0; j < 32; j += 8) {
 #pragma unroll
-                            for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(s[j]));
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (word >> j & 1) top = fmaxf(top, __uint_as_float(s[j]));
+                            for (int y = 0; y < 4; y++)
+                                tops[y] = fmaxf(tops[y], fmaxf(__uint_as_float(s[j + y]), __uint_as_float(s[j + y + 4])));
                         }
                     }
+                    float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    if (!I8) top *= lift;
                     const bool rises = any ? top > m + SLACK : true;
                     if (__any_sync(0xffffffffu, rises)) {
                         const float to = fmaxf(m, top);
@@ -622,7 +762,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                             for (int k = 0; k < D; k += 16) {
                                 uint32_t o[16];
                                 tmem_ld16(lanes + S::O0 + w * D + k, o);
-                                tmem_ld_wait();
+                                tmem_wait16(o);
 #pragma unroll
                                 for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
                                 tmem_st16(lanes + S::O0 + w * D + k, o);
@@ -631,37 +771,37 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                         m = to;
                     }
                     const float off = m == __int_as_float(0xff800000) ? 0.f : m;
+                    const Two minus = two(-off, -off), factor = two(lift, lift);
+                    Two sums[2] = {two(0.f, 0.f), two(0.f, 0.f)};
 #pragma unroll 1
                     for (int k = 0; k < CHUNKS; k++) {
-                        uint32_t s[32];
-                        tmem_ld32(s_tmem + 32 * k, s);
-                        const uint32_t word = plain ? 0xffffffffu : CHUNKS == 2 ? (k ? see[1] : see[0]) : k < 2 ? (k ? see[1] : see[0]) : (k == 2 ? see[CHUNKS - 2] : see[CHUNKS - 1]);
-                        tmem_ld_wait();
+                        fetch(k);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) {
-                            float x = __uint_as_float(s[j]) * c;
-                            if (I8) x *= ks[32 * k + j];
-                            s[j] = __float_as_uint(exp2_of(x - off));
-                        }
-                        if (!plain) {
+                        for (int h = 0; h < 32; h += 16) {
+                            uint32_t hi[8], lo[8];
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (!(word >> j & 1)) s[j] = 0;
+                            for (int j = 0; j < 16; j += 2) {
+                                const Two raw = two(__uint_as_float(s[h + j]), __uint_as_float(s[h + j + 1]));
+                                const float2 x = one(I8 ? add2(raw, minus) : fma2(raw, factor, minus));
+                                Two p = two(exp2_of(x.x), exp2_of(x.y));
+                                sums[(j / 2) & 1] = add2(sums[(j / 2) & 1], p);
+                                if (I8) {
+                                    const float2 f = *reinterpret_cast<const float2*>(ks + 128 + 32 * k + h + j);
+                                    p = mul2(p, two(f.x, f.y));
+                                }
+                                if (LIFT != 0.f) p = mul2(p, two(2048.f, 2048.f));
+                                const float2 w2 = one(p);
+                                hi[j / 2] = Elem<VTYPE>::down(w2.x, w2.y);
+                                const float2 got = Elem<VTYPE>::up(hi[j / 2]);
+                                const float2 rest = one(add2(p, two(-got.x, -got.y)));
+                                lo[j / 2] = Elem<VTYPE>::down(rest.x, rest.y);
+                            }
+                            tmem_st8(s_tmem + 32 * k + h / 2, hi);
+                            tmem_st8(s_tmem + 32 * k + 16 + h / 2, lo);
                         }
-                        uint32_t hi[16], lo[16];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            float p0 = __uint_as_float(s[j]), p1 = __uint_as_float(s[j + 1]);
-                            l += p0 + p1;
-                            if (I8) p0 *= ks[128 + 32 * k + j], p1 *= ks[128 + 32 * k + j + 1];
-                            if (LIFT != 0.f) p0 *= 2048.f, p1 *= 2048.f;
-                            hi[j / 2] = Elem<VTYPE>::down(p0, p1);
-                            const float2 got = Elem<VTYPE>::up(hi[j / 2]);
-                            lo[j / 2] = Elem<VTYPE>::down(p0 - got.x, p1 - got.y);
-                        }
-                        tmem_st16(s_tmem + 32 * k, hi);
-                        tmem_st16(s_tmem + 32 * k + 16, lo);
                     }
+                    const float2 sum = one(add2(sums[0], sums[1]));
+                    l += sum.x + sum.y;
                     tmem_st_wait();
                 }
                 any = true;
@@ -676,8 +816,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
             }
             if (!ok) break;
             // ---------------------------------------------------------------- the segment's result
-            const bool whole = g.t0 == 0 && g.t1 == g.s.tiles;
-            float* part = a.work + (int64_t)(2 * blockIdx.x + (g.t0 == 0 ? 1 : 0)) * RT * (D + 2);
+            const bool whole = t0 == 0 && t1 == g.tiles;
+            float* part = a.work + (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * RT * (D + 2);
             if (any && !warp_wait(pv_done(w), last & 1, abort, WL)) { ok = false; break; }
             float scale0, scale1 = 0.f;  // of this thread's O and, with two for a row, of the other
             int c0 = 0, c1 = D;
@@ -687,7 +827,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                 merge[((seg & 1) * 2 + w) * ROWS + r] = make_float2(m, l);
                 mbar_arrive(merge_bar);
                 if (!warp_wait(merge_bar, seg & 1, abort, WL)) { ok = false; break; }
-                has1 = g.t1 - g.t0 > 1 || !any;
+                has1 = t1 - t0 > 1 || !any;
                 if (has1) {
                     // the other's last unit: the segment's last tile, or the one before it
                     const int end_tile = tile - 1, other = (end_tile & 1) == w ? end_tile - 1 : end_tile;
@@ -717,7 +857,8 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                     uint32_t x[16], y[16];
                     if (has0) tmem_ld16(lanes + S::O0 + w * D + k, x);
                     if (has1) tmem_ld16(lanes + S::O0 + (w ^ 1) * D + k, y);
-                    tmem_ld_wait();
+                    if (has0) tmem_wait16(x);
+                    if (has1) tmem_wait16(y);
                     float o[16];
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
@@ -752,14 +893,15 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
             // what join_kernel reads: the item that begins here and goes on, and the one that came from the CTA before
             if (tid == 0 && !whole) {
                 int32_t* d = a.desc + 8 * blockIdx.x;
-                const int item = (g.head * g.s.rts + g.rt);
-                if (g.t0 == 0) {
+                const int item = g.item;
+                if (t0 == 0) {
                     d[0] = g.b, d[1] = item, d[2] = g.head, d[3] = g.rt, d[4] = g.rows;
                 } else {
                     d[5] = g.b, d[6] = item;
                 }
             }
-            seg++;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(seg_empty(seg % SEGS));
         }
         if (!ok && lane == 0) atomicOr(a.c.status, GAVE_UP);
     }
