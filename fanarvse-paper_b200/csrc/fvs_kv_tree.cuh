@@ -19,8 +19,8 @@
 // Rounding: scores, maxima, sums and O are fp32.  A weight enters the second product as two parts of the 16-bit type (its
 // rounded value and the rounded rest): 17 bits with bf16, 22 with fp16, where one part would double the error that the output's
 // own rounding makes; a third has no room in TMEM.  int8 codes are multiplied as bf16 with their key's scale in the weight.
-// The running maximum is moved only when it rises by more than 2^SLACK: O need not be rescaled at most tiles, and the
-// quotient is the same.
+// A row's weights are relative to a reference that rises only when they become large (LIMIT): O need not be rescaled at most
+// tiles, and the quotient is the same.
 #pragma once
 #include <type_traits>
 
@@ -33,10 +33,14 @@ namespace tree {
 using namespace fvs::tcg;
 
 constexpr int ROWS = 128;     // rows of a matrix instruction
-constexpr int INFO = 4;       // tiles whose keys' flags and scales are held
+constexpr int INFO = 8;       // tiles whose keys' flags and scales are held
 constexpr int SEGS = 4;       // segments that the scheduler is ahead
-constexpr int ITEM_COST = 2;  // cost of an item in tiles: its queries' copy and its output
+constexpr int ITEM_KEYS = 256; // cost of an item: its queries' copy and its output, as that of so many keys (64 ragged requests:
+                               // 119 us with 128, 112 with 384, 107 with 256)
+constexpr int LEAST_COST = 4;  // of a CTA's share, in tiles
 constexpr int GAVE_UP = 2;    // status bit: a bounded wait ran out
+
+constexpr int SEG_BYTES = 48;
 
 struct Args {
     fvs_kv_cache c;
@@ -55,26 +59,33 @@ struct Args {
 };
 
 
-template <int D>
+// How a kernel uses an SM, by head size and 128 * MT rows of an item.
+template <int D, int STORE, int MT>
 struct Shape {
-    static constexpr int KEYS = D <= 128 ? 128 : 64;
-    static constexpr int W = D <= 128 ? 2 : 1;
-    static constexpr int BLOCKS = (D + 63) / 64;  // 128-byte columns of a tile
+    static_assert(MT == 1 || D <= 128, "tensor memory holds one O of a wide head");
+    // CTAs of an SM: with 128 rows of heads up to 128 two, whose beginnings and ends overlap (one CTA whose two softmax
+    // warpgroups took turns at the tiles took 113 us where this takes 90, at 64 ragged requests of 64 rows)
+    static constexpr int CTAS = MT == 1 && D <= 128 ? 2 : 1;
+    static constexpr int W = MT;  // softmax warpgroups
+    // keys of a tile: 128 where the codes' widening is the slower part (403 us instead of 445 at 24 long int8 contexts under
+    // 32 nodes), else 64, whose scores are computed a tile ahead (229 instead of 254 at 131000 tokens under 64 nodes)
+    static constexpr int KEYS = MT == 2 && STORE == FVS_I8 ? 128 : 64;
+    static constexpr int COLUMNS = 512 / CTAS;                                       // of tensor memory
+    static constexpr int BUFFERS = MT == 2 ? 256 / KEYS : CTAS == 2 ? 2 : 4;         // of scores in it
+    static constexpr int LEAD = BUFFERS == W ? 0 : 1;  // units whose scores are issued before a unit's outputs wait
+    static constexpr int PRODUCERS = CTAS == 2 ? 2 : 4;  // warps
+    static constexpr int BLOCKS = (D + 63) / 64;         // 128-byte columns of a tile
     static constexpr int SLOT = KEYS * 128 * BLOCKS;
-    static constexpr int THREADS = 32 * (4 * W + 4 + 2);  // softmax, producers, matrix instructions and scheduler
-    static constexpr int O0 = 2 * KEYS;  // TMEM columns: two S, then W of O
-    static_assert(O0 + W * D <= 512, "tensor memory columns");
-};
-constexpr int BARS = 64 * 8, INFO_BYTES = 16 + 2 * 128 * 4, MERGE_BYTES = 2 * 2 * ROWS * 8;
-constexpr int SEG_BYTES = 48, MASK_BYTES = 2 * 4 * ROWS * 4;  // masks: a row's 128 bits for each softmax thread
-constexpr int MISC = BARS + INFO * INFO_BYTES + MERGE_BYTES + 64 + SEGS * SEG_BYTES + MASK_BYTES;
-template <int D, int MT>
-struct Plan {
-    using S = Shape<D>;
-    static constexpr int Q = MT * ROWS * 128 * S::BLOCKS;
-    static constexpr int FIT = (232448 - 1024 - MISC - Q) / S::SLOT;
+    static constexpr int THREADS = 32 * (4 * W + PRODUCERS + W + 1);  // softmax, producers, matrix instructions, scheduler
+    static constexpr int O0 = BUFFERS * KEYS;                         // columns of the scores, then W of O
+    static_assert(O0 + W * D <= COLUMNS, "tensor memory columns");
+    // shared memory: queries, the ring, then barriers, the tiles' flags and scales, segments and masks
+    static constexpr int Q = MT * ROWS * 128 * BLOCKS;
+    static constexpr int BARS = 88 * 8, INFO_BYTES = 16 + 2 * KEYS * 4, MASK_BYTES = W * ROWS * (KEYS / 32) * 4;
+    static constexpr int MISC = BARS + INFO * INFO_BYTES + 64 + SEGS * SEG_BYTES + MASK_BYTES;
+    static constexpr int FIT = ((CTAS == 2 ? 115712 : 232448) - 1024 - MISC - Q) / SLOT;
     static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
-    static constexpr int BYTES = 1024 + Q + SLOTS * S::SLOT + MISC;
+    static constexpr int BYTES = 1024 + Q + SLOTS * SLOT + MISC;
     static_assert(SLOTS >= 4, "two tiles of keys and of values");
 };
 
@@ -93,9 +104,14 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
     s.rts = (s.count * a.group + RT - 1) / RT;
     return s;
 }
+template <int KEYS>
 __device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) {
-    return (int64_t)s.rts * a.c.heads * (ITEM_COST + s.tiles);
+    return (int64_t)s.rts * a.c.heads * (ITEM_KEYS / KEYS + s.tiles);
 }
+
+// Where the share of CTA c begins: of equal cost, of as many CTAs as have LEAST_COST or more (what a cut costs)
+__device__ __forceinline__ int64_t shares(int64_t total) { return min((int64_t)gridDim.x, max((int64_t)1, total / LEAST_COST)); }
+__device__ __forceinline__ int64_t share(int64_t total, int64_t ctas, unsigned c) { return c >= ctas ? total : total * (int64_t)c / ctas; }
 
 struct Seg {             // tiles [t0, t1) of one item; t0 == t1: no more
     int b, head, rt, rows, t0, t1, n, keys, tiles, item;
@@ -104,6 +120,7 @@ struct Seg {             // tiles [t0, t1) of one item; t0 == t1: no more
 // Walks over the segments of a CTA (the scheduler's).
 template <int KEYS, int RT>
 struct Walk {
+    static constexpr int ITEM_COST = ITEM_KEYS / KEYS;
     int64_t base, start, end;  // cost before the item, and the CTA's share
     int item, b;               // item of the sequence
     Seq s;
@@ -194,6 +211,15 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait8(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
@@ -207,6 +233,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// whether the phase with the given parity is complete, without waiting
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done;
+}
 // the barrier counts this thread when all of its copies so far have landed
 __device__ __forceinline__ void copies_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -269,66 +307,70 @@ __device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
 }
 
 template <int D, int TYPE, int STORE, int MT>
-__global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
-    using S = Shape<D>;
-    using P = Plan<D, MT>;
+__global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, MT>::CTAS) tree_kernel(Args a) {
+    using S = Shape<D, STORE, MT>;
     constexpr bool I8 = STORE == FVS_I8;
-    constexpr int KEYS = S::KEYS, W = S::W, RT = ROWS * MT, SLOTS = P::SLOTS, CHUNKS = KEYS / 32;
+    constexpr int KEYS = S::KEYS, BUFFERS = S::BUFFERS, PARTS = KEYS / 64, W = S::W, RT = ROWS * MT, SLOTS = S::SLOTS, LEAD = S::LEAD;
+    constexpr int INFO_BYTES = S::INFO_BYTES, PRODUCERS = S::PRODUCERS;
     constexpr int VTYPE = I8 ? FVS_BF16 : TYPE;  // of weights and values
-    // weights: of fp16 values in the upper part of fp16's range, 2^(LIFT + SLACK) at most
-    constexpr float SLACK = VTYPE == FVS_F16 ? 4.f : 8.f, LIFT = VTYPE == FVS_F16 ? 11.f : 0.f;
-    static_assert(MT == 1 || W == 2, "256 rows need two softmax warpgroups");
+    // the most that 32 weights may add up to before their reference rises; over fp16 values they lie in the upper part of
+    // fp16's range, LIMIT * LIFT at most
+    constexpr float LIMIT = VTYPE == FVS_F16 ? 127.f : 4096.f, LIFT = VTYPE == FVS_F16 ? 512.f : 1.f;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = saddr(smem);
-    const uint32_t q_smem = sbase, ring = sbase + P::Q;
-    uint8_t* misc = smem + P::Q + SLOTS * S::SLOT;
+    const uint32_t q_smem = sbase, ring = sbase + S::Q;
+    uint8_t* misc = smem + S::Q + SLOTS * S::SLOT;
     const uint32_t bars = saddr(misc);
     auto full = [&](int s) { return bars + 8 * s; };
     auto empty = [&](int s) { return bars + 8 * (12 + s); };
     auto info_full = [&](int s) { return bars + 8 * (24 + s); };
-    auto info_empty = [&](int s) { return bars + 8 * (24 + INFO + s); };
-    auto s_full = [&](int s) { return bars + 8 * (32 + s); };
-    auto p_full = [&](int s) { return bars + 8 * (34 + s); };
-    auto pv_done = [&](int w) { return bars + 8 * (36 + w); };
-    const uint32_t q_full = bars + 8 * 38, q_empty = bars + 8 * 39, o_free = bars + 8 * 40, merge_bar = bars + 8 * 41,
-                   drain = bars + 8 * 42;
-    auto seg_full = [&](int s) { return bars + 8 * (43 + s); };
-    auto seg_empty = [&](int s) { return bars + 8 * (43 + SEGS + s); };
-    volatile Seg* segs = reinterpret_cast<volatile Seg*>(misc + BARS + INFO * INFO_BYTES + MERGE_BYTES + 64);
-    uint8_t* info = misc + BARS;
-    float2* merge = reinterpret_cast<float2*>(misc + BARS + INFO * INFO_BYTES);  // [2][W][ROWS]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + BARS + INFO * INFO_BYTES + MERGE_BYTES);
+    auto info_empty = [&](int s) { return bars + 8 * (32 + s); };
+    auto s_full = [&](int u) { return bars + 8 * (80 + u % BUFFERS); };
+    auto p_full = [&](int u, int part) { return bars + 8 * (44 + u % BUFFERS * PARTS + part); };  // 64 keys
+    auto pv_half = [&](int u) { return bars + 8 * (84 + u % BUFFERS); };                            // of a tile of 128
+    auto pv_done = [&](int u) { return bars + 8 * (48 + u % BUFFERS); };
+    auto round_of = [&](int u) { return (uint32_t)(u / BUFFERS) & 1u; };  // parity of unit u's phase of these
+    auto seg_full = [&](int s) { return bars + 8 * (52 + s); };
+    auto seg_empty = [&](int s) { return bars + 8 * (52 + SEGS + s); };
+    const uint32_t q_full = bars + 8 * 60, q_empty = bars + 8 * 61, o_free = bars + 8 * 62,
+                   drain = bars + 8 * 64, q_landed = bars + 8 * 65;
+    auto landed = [&](int s) { return bars + 8 * (66 + s); };
+    volatile Seg* segs = reinterpret_cast<volatile Seg*>(misc + S::BARS + INFO * INFO_BYTES + 64);
+    uint8_t* info = misc + S::BARS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + S::BARS + INFO * INFO_BYTES);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int64_t* s_place = reinterpret_cast<int64_t*>(tmem_slot + 2);  // total, sequence, cost before it
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int W_PROD = 4 * W, W_MMA = 4 * W + 4;
+    constexpr int W_PROD = 4 * W, W_MMA = 4 * W + PRODUCERS;
     const uint32_t WL = a.wait_limit;
 
     if (tid == 0) {
         for (int s = 0; s < SLOTS; s++) {
-            mbar_init(full(s), 128);
-            mbar_init(empty(s), 1);
+            mbar_init(landed(s), 32 * PRODUCERS);
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), MT);
         }
         for (int s = 0; s < INFO; s++) {
-            mbar_init(info_full(s), 4);
+            mbar_init(info_full(s), PRODUCERS);
             mbar_init(info_empty(s), 4 * MT);
         }
-        for (int s = 0; s < 2; s++) {
-            mbar_init(s_full(s), 1);
-            mbar_init(p_full(s), 128);
-            mbar_init(pv_done(s), 1);
+        for (int u = 0; u < BUFFERS; u++) {
+            mbar_init(s_full(u), 1);
+            for (int part = 0; part < PARTS; part++) mbar_init(p_full(u, part), 4);
+            if (PARTS == 2) mbar_init(pv_half(u), 1);
+            mbar_init(pv_done(u), 1);
         }
-        mbar_init(q_full, 128);
-        mbar_init(q_empty, 1);
+        mbar_init(q_landed, 32 * PRODUCERS);
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, W);
         mbar_init(o_free, 128 * W);
-        mbar_init(merge_bar, 128 * W);
-        mbar_init(drain, 1);
+        mbar_init(drain, W);
         for (int s = 0; s < SEGS; s++) {
             mbar_init(seg_full(s), 1);
-            mbar_init(seg_empty(s), 4 * W + 4 + 1);
+            mbar_init(seg_empty(s), 4 * W + PRODUCERS + W);
         }
         *abort = 0;
         s_place[0] = s_place[1] = s_place[2] = 0;
@@ -336,7 +378,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
         proxy_fence();
     }
     if (warp == W_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(tmem_slot)), "r"((uint32_t)S::COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     // ---------------------------------------------------------------- this CTA's share
@@ -347,7 +389,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
         int64_t mine = 0;
         for (int b = b0; b < b1; b++) {
             const Seq s = sequence<KEYS, RT>(a, b);
-            mine += cost_of(a, s);
+            mine += cost_of<KEYS>(a, s);
             if (blockIdx.x == 0 && s.count > 0 && (int64_t)__ldg(a.lens + b) + s.count > (int64_t)a.tb.wide * a.c.page)
                 atomicOr(a.c.status, BAD_INDEX);
         }
@@ -365,11 +407,11 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
             if (w < warp) before += sums[w];
             total += sums[w];
         }
-        const int64_t from = total * (int64_t)blockIdx.x / gridDim.x;
+        const int64_t ctas = shares(total), from = share(total, ctas, blockIdx.x);
         if (from >= before && from < before + mine) {
             int b = b0;
             for (;; b++) {
-                const int64_t cost = cost_of(a, sequence<KEYS, RT>(a, b));
+                const int64_t cost = cost_of<KEYS>(a, sequence<KEYS, RT>(a, b));
                 if (from < before + cost) break;
                 before += cost;
             }
@@ -380,7 +422,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
             s_place[0] = total;
             int32_t* d = a.desc + 8 * blockIdx.x;  // no share of a cut item yet; whether there is any share
             d[0] = d[5] = -1;
-            d[7] = from < total * ((int64_t)blockIdx.x + 1) / gridDim.x;
+            d[7] = from < share(total, ctas, blockIdx.x + 1);
         }
         // rows of nodes that a sequence does not have
         if (a.counts)
@@ -401,7 +443,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
 
     if (warp >= W_PROD && warp < W_MMA) {
         // ------------------------------------------------------------ producers
-        constexpr int PER = KEYS / 4;              // keys of a warp
+        constexpr int PER = KEYS / PRODUCERS;      // keys of a warp
         constexpr int CH = (I8 ? D / 16 : D / 8);  // 16-byte chunks of a stored row
         constexpr int TURNS = PER * CH / 32;
         static_assert(PER * CH % 32 == 0, "whole turns");
@@ -442,23 +484,15 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
 #pragma unroll
             for (int i = 0; i < TURNS; i++) rows[i] = __shfl_sync(0xffffffffu, x, (i * 32 + lane) / CH);
         };
-        auto copy = [&](const uint8_t* base, bool all) {
+        auto copy = [&](const uint8_t* base) {
             const uint32_t dst = ring + slot * S::SLOT;
-            if (all) {
 #pragma unroll
-                for (int i = 0; i < TURNS; i++) {
-                    const int id = i * 32 + lane, r = id / CH, c = id - r * CH;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + chunk(pw * PER + r, c)), "l"(base + c * 16 + (uint64_t)rows[i] * 16) : "memory");
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < TURNS; i++) {
-                    const int id = i * 32 + lane, r = id / CH, c = id - r * CH;
-                    const bool there = rows[i] != NONE;
-                    cp_async16(dst + chunk(pw * PER + r, c), base + (there ? c * 16 + (uint64_t)rows[i] * 16 : 0), there);
-                }
+            for (int i = 0; i < TURNS; i++) {
+                const int id = i * 32 + lane, r = id / CH, c = id - r * CH;
+                const bool there = rows[i] != NONE;
+                cp_async16(dst + chunk(pw * PER + r, c), base + (there ? c * 16 + (uint64_t)rows[i] * 16 : 0), there);
             }
-            copies_arrive(full(slot));
+            copies_arrive(landed(slot));
         };
         // int8 codes: keys and values of the next tile are on their way in registers
         uint4 rk[I8 ? TURNS : 1], rv[I8 ? TURNS : 1];
@@ -484,8 +518,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + chunk(k, c)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + chunk(k, c + 1)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
             }
-            proxy_fence();
-            mbar_arrive(full(slot));
+            mbar_arrive(landed(slot));
         };
         for (int seg = 0; ok; seg++) {
             if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
@@ -515,7 +548,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                 if (I8 && lane < PER) {
                     float* sc = reinterpret_cast<float*>(mine + 16);
                     sc[key] = ks * scale2;  // scores in powers of two
-                    sc[128 + key] = vs;
+                    sc[KEYS + key] = vs;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(info_full(is));
@@ -524,38 +557,37 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                     lookup(t + 1);
                     at = next_at;
                 }
-                if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
-                if (I8) {
-                    widen(rk, std::integral_constant<int, TYPE>());
-                    if (t + 1 < t1) {
-                        exchange(at);
-                        fetch(rk, kbase);
+#pragma unroll 1
+                for (int op = 0; op < 2; op++) {  // keys, then values
+                    if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
+                    if (!I8) {
+                        copy(op ? vbase : kbase);
+                    } else if (op == 0) {
+                        widen(rk, std::integral_constant<int, TYPE>());
+                        if (t + 1 < t1) {
+                            exchange(at);
+                            fetch(rk, kbase);
+                        }
+                    } else {
+                        widen(rv, std::integral_constant<int, FVS_BF16>());
+                        if (t + 1 < t1) fetch(rv, vbase);
                     }
-                } else {
-                    copy(kbase, there == 0xffffffffu);
+                    advance();
                 }
-                advance();
-                if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
-                if (I8) {
-                    widen(rv, std::integral_constant<int, FVS_BF16>());
-                    if (t + 1 < t1) fetch(rv, vbase);
-                } else {
-                    copy(vbase, there == 0xffffffffu);
-                }
-                advance();
+                if (!ok) break;
                 if (t == t0) {
                     // the rows' queries, behind the first tile: their buffer is free when the segment before has its scores
                     if (!warp_wait(q_empty, (seg & 1) ^ 1, abort, WL)) { ok = false; break; }
                     constexpr int QCH = D / 8;
                     const int rt = g.rt, live_rows = g.rows;
-                    for (int id = pw * 32 + lane; id < RT * QCH; id += 128) {
+                    for (int id = pw * 32 + lane; id < RT * QCH; id += 32 * PRODUCERS) {
                         const int r = id / QCH, c = id - r * QCH, mt = r / ROWS, k = r - mt * ROWS, row = rt * RT + r;
                         const bool live = r < live_rows;
                         const int node = live ? row / a.group : 0, h = live ? row - node * a.group : 0;
                         const uint16_t* src = (const uint16_t*)a.q + (int64_t)b * a.q_seq + (int64_t)node * a.q_node + (int64_t)(head * a.group + h) * a.q_head + c * 8;
                         cp_async16(q_smem + mt * (ROWS * 128 * S::BLOCKS) + (c >> 3) * (ROWS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), src, live);
                     }
-                    copies_arrive(q_full);
+                    copies_arrive(q_landed);
                 }
             }
             __syncwarp();
@@ -563,87 +595,129 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
         }
         cp_async_wait_all();
     } else if (warp >= W_MMA) {
-        // ------------------------------------------------------------ the matrix instructions' thread
-        if (warp == W_MMA && lane == 0) {
+        // A thread for each softmax warpgroup issues its matrix instructions: a unit's outputs (O += P V) 64 keys at a time as
+        // its weights come, and right behind the last ones the next unit's scores (S = Q K^T), which take the weights'
+        // place; instructions of one thread run in order.  An instruction is issued when the one before it has begun and a
+        // single thread is slow, so what it need not wait for between instructions it does before or behind them.
+        if (warp < W_MMA + W && lane == 0) {
+            const int w = warp - W_MMA;
             const uint32_t id_s = idesc(KEYS, TYPE == FVS_BF16, false), id_o = idesc(D, VTYPE == FVS_BF16, true);
-            int kslot = 0, kphase = 0, vslot = 1, vphase = 0;  // keys in even places of the stream, values in odd ones
-            int unit = 0;
+            int kslot = 0, kphase = 0, vslot = 1, vphase = 0;
+            int tile = 0;  // tiles of this CTA before the segment
             bool ok = true;
-            auto scores = [&](int u, int mt) {
-                const uint32_t d = tmem + (u & 1) * KEYS, ab = q_smem + mt * (ROWS * 128 * S::BLOCKS), bb = ring + kslot * S::SLOT;
+            const uint64_t q_desc = sw128_desc(q_smem + (MT == 2 ? w * (ROWS * 128 * S::BLOCKS) : 0)), k_desc = sw128_desc(ring),
+                           v_desc = values_desc(ring, KEYS * 128);
+            auto step = [&](int& slot, int& phase) {
+                slot += 2;
+                if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+            };
+            // S of unit u: keys in the next slot, which is full
+            auto scores = [&](int u) {
+                const uint32_t d = tmem + (u % BUFFERS) * KEYS;
+                const uint64_t bd = k_desc + (uint32_t)(kslot * (S::SLOT / 16));
 #pragma unroll
                 for (int k = 0; k < D / 16; k++)
-                    mma_ss(d, sw128_desc(ab + (k >> 2) * (ROWS * 128) + (k & 3) * 32), sw128_desc(bb + (k >> 2) * (KEYS * 128) + (k & 3) * 32), id_s, k > 0);
-                mma_commit(s_full(u & 1));
+                    mma_ss(d, q_desc + ((k >> 2) * (ROWS * 128 / 16) + (k & 3) * 2), bd + ((k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2), id_s, k > 0);
+                mma_commit(s_full(u));
+                mma_commit(empty(kslot));
+                step(kslot, kphase);
             };
-            auto step = [&](int& s, int& ph) {
-                s += 2;
-                if (s >= SLOTS) s -= SLOTS, ph ^= 1;
-            };
-            // O += P V of unit u (the tile k of its segment)
-            auto outputs = [&](int u, int k, int mt) {
-                if (mt == 0 && !mbar_wait(full(vslot), vphase, abort, WL)) return false;
-                if (!mbar_wait(p_full(u & 1), (u >> 1) & 1, abort, WL)) return false;
-                proxy_fence();
-                tc_fence_after();
-                const int w = W == 2 ? u & 1 : 0;
-                const uint32_t d = tmem + S::O0 + w * D, p = tmem + (u & 1) * KEYS, vb = ring + vslot * S::SLOT;
-                const bool first = k < (W == 2 && MT == 1 ? 2 : 1);
+            for (int seg = 0; ok; seg++) {
+                if (!mbar_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
+                const int tiles = segs[seg % SEGS].t1 - segs[seg % SEGS].t0;
+                mbar_arrive(seg_empty(seg % SEGS));
+                if (tiles == 0 || !mbar_wait(q_full, seg & 1, abort, WL)) break;
+                const int units = tiles;
+                auto unit = [&](int x) { return W * (tile + x) + w; };
+                int asked = 0;
+                // the next unit's scores, if its keys are there
+                auto ask = [&](int most) {
+                    if (asked < min(units, most) && mbar_test(full(kslot), kphase)) {
+                        tc_fence_after();
+                        scores(unit(asked));
+                        if (++asked == units) mma_commit(q_empty);
+                    }
+                };
+                // waits for a barrier and asks meanwhile (what is waited for may need the scores)
+                auto wait = [&](uint32_t bar, uint32_t parity, int most) {
+                    for (uint32_t it = 0; it < WL; it++) {
+                        ask(most);
+                        if (mbar_test(bar, parity)) return true;
+                        if ((it & 255u) == 255u && *abort) return false;
+                    }
+                    *abort = 1;
+                    return false;
+                };
+                // O's first products of this segment come behind the reads of the one before
+                if (seg > 0) ok = wait(o_free, (seg - 1) & 1, 1 + LEAD);
+#pragma unroll 1
+                for (int x = 0; x < units && ok; x++) {
+                    const int u = unit(x);
+                    const uint32_t d = tmem + S::O0 + w * D, p = tmem + (u % BUFFERS) * KEYS;
+                    const uint64_t v = v_desc + (uint32_t)(vslot * (S::SLOT / 16));
 #pragma unroll
-                for (int i = 0; i < KEYS / 16; i++) {
-                    const uint64_t v = values_desc(vb + i * 2048, KEYS * 128);
-                    mma_ts(d, p + 32 * (i >> 1) + 8 * (i & 1), v, id_o, !(first && i == 0));
-                    mma_ts(d, p + 32 * (i >> 1) + 8 * (i & 1) + 16, v, id_o, true);
-                }
-                mma_commit(pv_done(w));
-                if (mt == MT - 1) {
+                    for (int part = 0; part < PARTS; part++) {
+                        if (!(ok = wait(p_full(u, part), round_of(u), x + 1 + LEAD))) break;
+                        if (part == 0 && !(ok = mbar_wait(full(vslot), vphase, abort, WL))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = 4 * part; i < 4 * part + 4; i++) {
+                            mma_ts(d, p + 32 * (i >> 1) + 8 * (i & 1), v + i * 128, id_o, x + i > 0);
+                            mma_ts(d, p + 32 * (i >> 1) + 8 * (i & 1) + 16, v + i * 128, id_o, true);
+                        }
+                        if (part < PARTS - 1) mma_commit(pv_half(u));
+                    }
+                    if (!ok) break;
+                    if (LEAD == 0) ask(x + 2);  // right behind, in place of the weights
+                    mma_commit(pv_done(u));
                     mma_commit(empty(vslot));
                     step(vslot, vphase);
                 }
-                return true;
-            };
-            for (int seg = 0;; seg++) {
-                if (!mbar_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
-                const int tiles = segs[seg % SEGS].t1 - segs[seg % SEGS].t0, units = tiles * MT;
-                mbar_arrive(seg_empty(seg % SEGS));
-                if (tiles == 0 || !mbar_wait(q_full, seg & 1, abort, WL)) break;
-                for (int x = 0; x < units && ok; x++, unit++) {
-                    const int mt = MT == 2 ? x & 1 : 0;
-                    if (mt == 0 && !mbar_wait(full(kslot), kphase, abort, WL)) { ok = false; break; }
-                    proxy_fence();
-                    tc_fence_after();
-                    scores(unit, mt);
-                    if (mt == MT - 1) {
-                        mma_commit(empty(kslot));
-                        step(kslot, kphase);
-                    }
-                    if (x == units - 1) mma_commit(q_empty);
-                    if (x == 0) {
-                        // O's first products of this segment come behind the reads of the one before
-                        if (seg > 0 && !mbar_wait(o_free, (seg - 1) & 1, abort, WL)) ok = false;
-                    } else if (!outputs(unit - 1, MT == 2 ? (x - 1) >> 1 : x - 1, MT == 2 ? (x - 1) & 1 : 0)) {
-                        ok = false;
-                    }
-                }
-                if (!ok || !outputs(unit - 1, tiles - 1, MT - 1)) break;
+                tile += tiles;
             }
             mma_commit(drain);  // what was issued has to end before the CTA does
             mbar_drain(drain, 0);
-        } else if (warp == W_MMA + 1 && lane == 0) {
-            // -------------------------------------------------------- the scheduler
+        } else if (warp == W_MMA + W && lane == 0) {
+            // -------------------------------------------------------- the scheduler, which is also the relay
+            // What the producers wrote becomes visible to the matrix instructions by a fence between the two.  The
+            // instructions' own thread would wait at it until those it has issued are done (100 cycles for each
+            // instruction instead of 67).
             Walk<KEYS, RT> walk;
             const int64_t total = s_place[0];
-            walk.begin(a, (int)s_place[1], s_place[2], total * (int64_t)blockIdx.x / gridDim.x, total * ((int64_t)blockIdx.x + 1) / gridDim.x);
-            bool more = true;
-            for (int seg = 0; more; seg++) {
-                Seg g;
-                more = walk.next(a, g);
-                if (!more) g.t0 = g.t1 = 0;
-                if (!mbar_wait(seg_empty(seg % SEGS), ((seg / SEGS) & 1) ^ 1, abort, WL)) break;
-                volatile Seg& to = segs[seg % SEGS];
-                to.t0 = g.t0, to.t1 = g.t1;
-                if (more) to.b = g.b, to.head = g.head, to.rt = g.rt, to.rows = g.rows, to.n = g.n, to.keys = g.keys, to.tiles = g.tiles, to.item = g.item;
-                mbar_arrive(seg_full(seg % SEGS));
+            const int64_t ctas = shares(total);
+            walk.begin(a, (int)s_place[1], s_place[2], share(total, ctas, blockIdx.x), share(total, ctas, blockIdx.x + 1));
+            int slot = 0, phase = 0, told = 0;
+            bool ok = true, more = true;
+            auto pass = [&]() {
+                ok = ok && mbar_wait(landed(slot), phase, abort, WL);
+                if (!ok) return;
+                proxy_fence();
+                mbar_arrive(full(slot));
+                if (++slot == SLOTS) slot = 0, phase ^= 1;
+            };
+            for (int seg = 0; ok; seg++) {
+                for (; more && told <= seg + 1; told++) {  // a segment ahead
+                    Seg g;
+                    more = walk.next(a, g);
+                    if (!more) g.t0 = g.t1 = 0;
+                    if (!mbar_wait(seg_empty(told % SEGS), ((told / SEGS) & 1) ^ 1, abort, WL)) { ok = false; break; }
+                    volatile Seg& to = segs[told % SEGS];
+                    to.t0 = g.t0, to.t1 = g.t1;
+                    if (more) to.b = g.b, to.head = g.head, to.rt = g.rt, to.rows = g.rows, to.n = g.n, to.keys = g.keys, to.tiles = g.tiles, to.item = g.item;
+                    mbar_arrive(seg_full(told % SEGS));
+                }
+                if (!ok) break;
+                const int tiles = segs[seg % SEGS].t1 - segs[seg % SEGS].t0;
+                if (tiles == 0) break;
+                for (int t = 0; t < tiles && ok; t++) {
+                    pass();
+                    pass();
+                    if (t == 0 && ok) {
+                        ok = mbar_wait(q_landed, seg & 1, abort, WL);
+                        proxy_fence();
+                        mbar_arrive(q_full);
+                    }
+                }
             }
         }
         __syncwarp();
@@ -651,7 +725,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
         // ------------------------------------------------------------ softmax, a thread per row
         const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // warpgroup, TMEM lane
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        uint32_t* mask = reinterpret_cast<uint32_t*>(misc + BARS + INFO * INFO_BYTES + MERGE_BYTES + 64 + SEGS * SEG_BYTES) + w * 4 * ROWS + r;
+        uint32_t* mask = reinterpret_cast<uint32_t*>(misc + S::BARS + INFO * INFO_BYTES + 64 + SEGS * SEG_BYTES) + w * (KEYS / 32) * ROWS + r;
         const float lift = scale2 == 0.f ? 1.f : fabsf(scale2);  // the sign, and a scale of 0, are in the scores
         int tile = 0;
         bool ok = true;
@@ -664,28 +738,30 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
             const bool warp_live = mine - lane < g.rows;
             const int row = g.rt * RT + mine;
             const int node = mine < g.rows ? row / a.group : 0;
+            const int n = g.n;
             float m = __int_as_float(0xff800000), l = 0.f;
             bool any = false;                                       // units of this warpgroup in this segment
             int last = -1;                                          // the last of them
             for (int t = t0; t < t1; t++, tile++) {
-                int u = MT == 2 ? 2 * tile + w : tile;
-                if (MT == 1 && W == 2 && (u & 1) != w) continue;
-                const int n_th = W == 2 ? u >> 1 : u;               // of this warpgroup
+                const int u = W * tile + w;
                 const int is = tile % INFO;
-                if (!warp_wait(info_full(is), (tile / INFO) & 1, abort, WL) || !warp_wait(s_full(u & 1), (u >> 1) & 1, abort, WL)) { ok = false; break; }
+                if (!warp_wait(info_full(is), (tile / INFO) & 1, abort, WL) || !warp_wait(s_full(u), round_of(u), abort, WL)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t s_tmem = lanes + (u & 1) * KEYS;
+                const uint32_t s_tmem = lanes + (u % BUFFERS) * KEYS;
                 const uint8_t* inf = info + is * INFO_BYTES;
                 if (warp_live) {
-                    uint32_t see[CHUNKS];
-                    bool all = true;
+                    constexpr int WORDS = KEYS / 32;
+                    uint32_t see[WORDS];
+                    uint32_t all = 0xffffffffu;
 #pragma unroll
-                    for (int k = 0; k < CHUNKS; k++) see[k] = reinterpret_cast<const uint32_t*>(inf)[k];
-                    const int x0 = t * KEYS - g.n;                // of the tile's first key behind the sequence
+                    for (int k = 0; k < WORDS; k++) see[k] = reinterpret_cast<const uint32_t*>(inf)[k], all &= see[k];
+                    const int x0 = t * KEYS - n;  // of the tile's first key behind the sequence
+                    bool odd = all != 0xffffffffu || (!I8 && scale2 <= 0.f);
                     if (x0 + KEYS > 0) {
-                        uint32_t tree[CHUNKS];
+                        uint32_t tree[WORDS];
+                        all = 0xffffffffu;
 #pragma unroll
-                        for (int k = 0; k < CHUNKS; k++) {
+                        for (int k = 0; k < WORDS; k++) {
                             const int before = min(max(-x0 - 32 * k, 0), 32);  // keys of the sequence itself
                             tree[k] = before == 32 ? 0xffffffffu : (1u << before) - 1u;
                         }
@@ -693,29 +769,27 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                         for (int i = node; i >= 0 && i >= x0;) {
                             const int at = i - x0;
 #pragma unroll
-                            for (int k = 0; k < CHUNKS; k++)
+                            for (int k = 0; k < WORDS; k++)
                                 if (at >> 5 == k) tree[k] |= 1u << (at & 31);
                             const int p = __ldg(up + i);
                             i = p < i ? p : -1;
                         }
 #pragma unroll
-                        for (int k = 0; k < CHUNKS; k++) see[k] &= tree[k];
+                        for (int k = 0; k < WORDS; k++) see[k] &= tree[k], all &= see[k];
+                        odd = odd || __any_sync(0xffffffffu, all != 0xffffffffu);
                     }
-#pragma unroll
-                    for (int k = 0; k < CHUNKS; k++) all &= see[k] == 0xffffffffu;
-                    const bool odd = __any_sync(0xffffffffu, !all) || (!I8 && scale2 <= 0.f);
                     if (odd) {
 #pragma unroll
-                        for (int k = 0; k < CHUNKS; k++) mask[k * ROWS] = see[k];
+                        for (int k = 0; k < WORDS; k++) mask[k * ROWS] = see[k];
                     }
                     const float* ks = reinterpret_cast<const float*>(inf + 16);
-                    // Two passes over the row's scores in TMEM, 32 at a time: the largest, then the weights.  (All of a
-                    // tile's at once leave no registers, and unrolled code no place in the instruction cache: both took up
-                    // to half as long again.)
-                    uint32_t s[32];
-                    // what the scores are before `lift`: with the key's scale and in powers of two (int8), with their sign;
-                    // masked where the tile is not plain
-                    auto fetch = [&](int k) {
+                    // The row's scores 32 at a time: weights above the reference `m`, unless their sum says that one of them is
+                    // far above it, which is rare: then m rises and the 32 are taken again.  (A largest score
+                    // for every 32 took 90 of 730 cycles, all of a tile's scores at once left no registers, and unrolled
+                    // code no place in the instruction cache.)
+                    const Two factor = two(lift, lift);
+                    // 32 scores: with the key's scale, in powers of two (int8), masked, and with the scale's sign
+                    auto scores = [&](uint32_t (&s)[32], int k) {
                         tmem_ld32(s_tmem + 32 * k, s);
                         tmem_wait32(s);
                         if (I8) {
@@ -728,143 +802,141 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                                 s[j + 2] = __float_as_uint(z.x), s[j + 3] = __float_as_uint(z.y);
                             }
                         }
-                        if (odd) {
-                            const uint32_t word = reinterpret_cast<const volatile uint32_t*>(mask)[k * ROWS];
+                        if (__builtin_expect(odd, 0)) {
+                            const uint32_t word = mask[k * ROWS];
                             const float sign = I8 ? 1.f : scale2 < 0.f ? -1.f : scale2 == 0.f ? 0.f : 1.f;
 #pragma unroll
                             for (int j = 0; j < 32; j++) s[j] = word >> j & 1 ? __float_as_uint(__uint_as_float(s[j]) * sign) : 0xff800000u;
                         }
                     };
-                    float tops[4];
-#pragma unroll
-                    for (int y = 0; y < 4; y++) tops[y] = __int_as_float(0xff800000);
+                    bool raise = !any;  // no reference yet
 #pragma unroll 1
-                    for (int k = 0; k < CHUNKS; k++) {
-                        fetch(k);
+                    for (int k = 0; k < KEYS / 32;) {
+                        uint32_t s[32];
+                        scores(s, k);
+                        if (__builtin_expect(raise, 0)) {
+                            float top = __int_as_float(0xff800000);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-#pragma unroll
-                            for (int y = 0; y < 4; y++)
-                                tops[y] = fmaxf(tops[y], fmaxf(__uint_as_float(s[j + y]), __uint_as_float(s[j + y + 4])));
-                        }
-                    }
-                    float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                    if (!I8) top *= lift;
-                    const bool rises = any ? top > m + SLACK : true;
-                    if (__any_sync(0xffffffffu, rises)) {
-                        const float to = fmaxf(m, top);
-                        if (any) {
-                            const float by = m == to ? 1.f : exp2_of(m - to);
+                            for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(s[j]));
+                            if (!I8) top *= lift;
+                            const float to = fmaxf(m, top), by = m == to ? 1.f : exp2_of(m - to);
+                            m = to;
                             l *= by;
-                            if (!warp_wait(pv_done(w), (n_th - 1) & 1, abort, WL)) { ok = false; break; }
-                            tc_fence_after();
+                            const bool half = PARTS == 2 && k >= 2;  // the tile's first 64 weights may be in O
+                            if (any || half) {
+                                ok = ok && warp_wait(half ? pv_half(u) : pv_done(last), round_of(half ? u : last), abort, WL);
+                                tc_fence_after();
 #pragma unroll 1
-                            for (int k = 0; k < D; k += 16) {
-                                uint32_t o[16];
-                                tmem_ld16(lanes + S::O0 + w * D + k, o);
-                                tmem_wait16(o);
+                                for (int x = 0; x < D; x += 16) {
+                                    uint32_t o[16];
+                                    tmem_ld16(lanes + S::O0 + w * D + x, o);
+                                    tmem_wait16(o);
 #pragma unroll
-                                for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-                                tmem_st16(lanes + S::O0 + w * D + k, o);
+                                    for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+                                    tmem_st16(lanes + S::O0 + w * D + x, o);
+                                }
+                            }
+                            if (k & 1) {  // the 32 weights before are not in O yet
+#pragma unroll 1
+                                for (int x = 0; x < 16; x += 8) {
+                                    uint32_t hi[8], lo[8];
+                                    tmem_ld8(s_tmem + 32 * (k - 1) + x, hi);
+                                    tmem_ld8(s_tmem + 32 * (k - 1) + 16 + x, lo);
+                                    tmem_wait8(hi);
+                                    tmem_wait8(lo);
+#pragma unroll
+                                    for (int j = 0; j < 8; j++) {
+                                        const float2 y = Elem<VTYPE>::up(hi[j]), z = Elem<VTYPE>::up(lo[j]);
+                                        const float p = (y.x + z.x) * by, q = (y.y + z.y) * by;
+                                        hi[j] = Elem<VTYPE>::down(p, q);
+                                        const float2 got = Elem<VTYPE>::up(hi[j]);
+                                        lo[j] = Elem<VTYPE>::down(p - got.x, q - got.y);
+                                    }
+                                    tmem_st8(s_tmem + 32 * (k - 1) + x, hi);
+                                    tmem_st8(s_tmem + 32 * (k - 1) + 16 + x, lo);
+                                }
                             }
                         }
-                        m = to;
-                    }
-                    const float off = m == __int_as_float(0xff800000) ? 0.f : m;
-                    const Two minus = two(-off, -off), factor = two(lift, lift);
-                    Two sums[2] = {two(0.f, 0.f), two(0.f, 0.f)};
-#pragma unroll 1
-                    for (int k = 0; k < CHUNKS; k++) {
-                        fetch(k);
+                        const float off = m == __int_as_float(0xff800000) ? 0.f : m;
+                        const Two minus = two(-off, -off);
+                        Two sums[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const Two raw = two(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                            const float2 x = one(I8 ? add2(raw, minus) : fma2(raw, factor, minus));
+                            s[j] = __float_as_uint(exp2_of(x.x)), s[j + 1] = __float_as_uint(exp2_of(x.y));
+                            sums[(j / 2) & 1] = add2(sums[(j / 2) & 1], two(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+                        }
+                        const float2 pair = one(add2(sums[0], sums[1]));
+                        const float sum = pair.x + pair.y;
+                        // (not-a-numbers and rows that have seen nothing yet are taken again once)
+                        if (__any_sync(0xffffffffu, !(sum <= LIMIT) || m == __int_as_float(0xff800000)) && !raise) {
+                            raise = true;
+                            continue;
+                        }
+                        raise = false;
+                        l += sum;
 #pragma unroll
                         for (int h = 0; h < 32; h += 16) {
                             uint32_t hi[8], lo[8];
 #pragma unroll
-                            for (int j = 0; j < 16; j += 2) {
-                                const Two raw = two(__uint_as_float(s[h + j]), __uint_as_float(s[h + j + 1]));
-                                const float2 x = one(I8 ? add2(raw, minus) : fma2(raw, factor, minus));
-                                Two p = two(exp2_of(x.x), exp2_of(x.y));
-                                sums[(j / 2) & 1] = add2(sums[(j / 2) & 1], p);
-                                if (I8) {
-                                    const float2 f = *reinterpret_cast<const float2*>(ks + 128 + 32 * k + h + j);
-                                    p = mul2(p, two(f.x, f.y));
+                            for (int j = 0; j < 16; j += 4) {
+                                float4 f;
+                                if (I8) f = *reinterpret_cast<const float4*>(ks + KEYS + 32 * k + h + j);
+#pragma unroll
+                                for (int y = 0; y < 2; y++) {
+                                    Two p = two(__uint_as_float(s[h + j + 2 * y]), __uint_as_float(s[h + j + 2 * y + 1]));
+                                    if (I8) p = mul2(p, y ? two(f.z, f.w) : two(f.x, f.y));
+                                    if (LIFT != 1.f) p = mul2(p, two(LIFT, LIFT));
+                                    const float2 w2 = one(p);
+                                    hi[j / 2 + y] = Elem<VTYPE>::down(w2.x, w2.y);
+                                    const float2 got = Elem<VTYPE>::up(hi[j / 2 + y]);
+                                    const float2 rest = one(fma2(two(got.x, got.y), two(-1.f, -1.f), p));
+                                    lo[j / 2 + y] = Elem<VTYPE>::down(rest.x, rest.y);
                                 }
-                                if (LIFT != 0.f) p = mul2(p, two(2048.f, 2048.f));
-                                const float2 w2 = one(p);
-                                hi[j / 2] = Elem<VTYPE>::down(w2.x, w2.y);
-                                const float2 got = Elem<VTYPE>::up(hi[j / 2]);
-                                const float2 rest = one(add2(p, two(-got.x, -got.y)));
-                                lo[j / 2] = Elem<VTYPE>::down(rest.x, rest.y);
                             }
                             tmem_st8(s_tmem + 32 * k + h / 2, hi);
                             tmem_st8(s_tmem + 32 * k + 16 + h / 2, lo);
                         }
+                        if (k & 1) {
+                            tmem_st_wait();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(p_full(u, k >> 1));
+                        }
+                        k++;
                     }
-                    const float2 sum = one(add2(sums[0], sums[1]));
-                    l += sum.x + sum.y;
-                    tmem_st_wait();
+                    if (!ok) break;
+                } else {
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++)
+                        if (lane == 0) mbar_arrive(p_full(u, part));
                 }
                 any = true;
-                last = n_th;
-                // With one warpgroup its O may still be behind by two products here, which a parity cannot tell from none;
-                // with two, S(u) came behind the warpgroup's last product.
-                if (W == 1 && n_th > 0 && !warp_wait(pv_done(w), (n_th - 1) & 1, abort, WL)) { ok = false; break; }
-                tc_fence_before();
+                last = u;
                 __syncwarp();
-                mbar_arrive(p_full(u & 1));
                 if (lane == 0) mbar_arrive(info_empty(is));
             }
             if (!ok) break;
             // ---------------------------------------------------------------- the segment's result
             const bool whole = t0 == 0 && t1 == g.tiles;
             float* part = a.work + (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * RT * (D + 2);
-            if (any && !warp_wait(pv_done(w), last & 1, abort, WL)) { ok = false; break; }
-            float scale0, scale1 = 0.f;  // of this thread's O and, with two for a row, of the other
-            int c0 = 0, c1 = D;
-            bool has0 = any, has1 = false;
-            if (MT == 1 && W == 2) {
-                // both warpgroups have a share of each row: each adds up half of the columns
-                merge[((seg & 1) * 2 + w) * ROWS + r] = make_float2(m, l);
-                mbar_arrive(merge_bar);
-                if (!warp_wait(merge_bar, seg & 1, abort, WL)) { ok = false; break; }
-                has1 = t1 - t0 > 1 || !any;
-                if (has1) {
-                    // the other's last unit: the segment's last tile, or the one before it
-                    const int end_tile = tile - 1, other = (end_tile & 1) == w ? end_tile - 1 : end_tile;
-                    if (!warp_wait(pv_done(w ^ 1), (other >> 1) & 1, abort, WL)) { ok = false; break; }
-                }
-                const float2 o = merge[((seg & 1) * 2 + (w ^ 1)) * ROWS + r];
-                const float to = fmaxf(m, o.x);
-                scale0 = m == to ? 1.f : exp2_of(m - to);
-                scale1 = o.x == to ? 1.f : exp2_of(o.x - to);
-                l = l * scale0 + o.y * scale1;
-                m = to;
-                c0 = w == 0 ? 0 : D / 2;
-                c1 = c0 + D / 2;
-            } else {
-                scale0 = 1.f;
-            }
+            if (!warp_wait(pv_done(last), round_of(last), abort, WL)) { ok = false; break; }
             tc_fence_after();
             const bool live = mine < g.rows;
             if (warp_live) {
                 const int h = live ? row - node * a.group : 0;
                 const int64_t o_row = ((int64_t)g.b * a.nodes + node) * a.hq + g.head * a.group + h;
-                const float down = LIFT != 0.f ? 1.f / 2048.f : 1.f;
+                const float down = 1.f / LIFT;
                 const float by = whole ? (l == 0.f ? 0.f : down / l) : down;
-                const float f0 = scale0 * by, f1 = scale1 * by;
 #pragma unroll 1
-                for (int k = c0; k < c1; k += 16) {
-                    uint32_t x[16], y[16];
-                    if (has0) tmem_ld16(lanes + S::O0 + w * D + k, x);
-                    if (has1) tmem_ld16(lanes + S::O0 + (w ^ 1) * D + k, y);
-                    if (has0) tmem_wait16(x);
-                    if (has1) tmem_wait16(y);
+                for (int k = 0; k < D; k += 16) {
+                    uint32_t x[16];
+                    tmem_ld16(lanes + S::O0 + w * D + k, x);
+                    tmem_wait16(x);
                     float o[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        o[j] = has0 ? __uint_as_float(x[j]) * f0 : 0.f;
-                        if (has1) o[j] = fmaf(__uint_as_float(y[j]), f1, o[j]);
-                    }
+                    for (int j = 0; j < 16; j++) o[j] = __uint_as_float(x[j]) * by;
                     if (whole && live) {
                         uint16_t* out = (uint16_t*)a.out + o_row * D + k;
 #pragma unroll
@@ -879,7 +951,7 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
                         for (int j = 0; j < 16; j++) part[(k + j) * RT + mine] = o[j];
                     }
                 }
-                if (live && (MT == 2 || W == 1 || w == 0)) {
+                if (live) {
                     if (whole) {
                         if (a.lse) a.lse[o_row] = l == 0.f ? __int_as_float(0xff800000) : (m + log2f(l)) * 0.6931471805599453f;
                     } else {
@@ -908,30 +980,38 @@ __global__ void __launch_bounds__(Shape<D>::THREADS, 1) tree_kernel(Args a) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)S::COLUMNS));
     if (*abort && tid == 0) atomicOr(a.c.status, GAVE_UP);
 }
 
-// Adds the shares of the items that were cut.  Block (c, rows of 32): the item that begins in CTA c and goes on in the CTAs
-// behind it, each of which left one share.
+// Adds the shares of the items that were cut.  Block (c, 32 rows, 16 columns): the item that begins in CTA c and goes on in
+// the CTAs behind it, each of which left one share.  The shares are read once, from L2 mostly: many small blocks, with all
+// of a thread's loads on the way together (8 blocks of 20 shares each took 57 us where 4096 of them take 5).
+constexpr int JOIN_COLS = 16;
 template <int D, int TYPE, int RT>
 __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
     extern __shared__ float weight[];  // [shares][32]
     __shared__ float s_m[8][32], s_l[8][32];
+    __shared__ int s_upto;
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the shares are still computed
     const int32_t* d = a.desc + 8 * c;
     const int b = d[0], item = d[1], head = d[2], rt = d[3], rows = d[4];
     const int row = blockIdx.y * 32 + lane;
     if (b < 0 || (int)blockIdx.y * 32 >= rows) return;
-    // the CTAs behind that have a share of it: none between them has another item
-    int upto = c + 1;
-    while (upto < ctas && ((a.desc[8 * upto + 5] == b && a.desc[8 * upto + 6] == item) || a.desc[8 * upto + 7] == 0)) upto++;
+    // the CTAs behind that have a share of it: none between them has another item, some may have nothing at all
+    auto has = [&](int x) { return x == c || (a.desc[8 * x + 5] == b && a.desc[8 * x + 6] == item); };
+    if (threadIdx.x == 0) s_upto = ctas;
+    __syncthreads();
+    for (int x = c + 1 + (int)threadIdx.x; x < ctas; x += 256)
+        if (!has(x) && a.desc[8 * x + 7] != 0) atomicMin(&s_upto, x);
+    __syncthreads();
+    const int shares = s_upto - c;
     auto part = [&](int i) { return a.work + (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * RT * (D + 2); };
-    auto has = [&](int i) { return i == 0 || (a.desc[8 * (c + i) + 5] == b && a.desc[8 * (c + i) + 6] == item); };
-    const int shares = upto - c;
-    float m = __int_as_float(0xff800000);
+    constexpr float NONE = -__builtin_huge_valf();
+    float m = NONE;
     for (int i = warp; i < shares; i += 8) {
-        const float x = has(i) && row < rows ? part(i)[D * RT + row] : __int_as_float(0xff800000);
+        const float x = has(c + i) && row < rows ? part(i)[D * RT + row] : NONE;
         weight[i * 32 + lane] = x;
         m = fmaxf(m, x);
     }
@@ -942,7 +1022,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
     float l = 0.f;
     for (int i = warp; i < shares; i += 8) {
         const float x = weight[i * 32 + lane], by = x == m ? 1.f : exp2_of(x - m);
-        const bool there = has(i) && row < rows;
+        const bool there = has(c + i) && row < rows;
         weight[i * 32 + lane] = there ? by : 0.f;
         if (there) l = fmaf(part(i)[(D + 1) * RT + row], by, l);
     }
@@ -954,52 +1034,54 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
     if (row >= rows) return;
     const int at = rt * RT + row, node = at / a.group, h = at - node * a.group;
     const int64_t o_row = ((int64_t)b * a.nodes + node) * a.hq + head * a.group + h;
-    constexpr int COLS = D / 8;
-    float o[COLS];
-#pragma unroll
-    for (int j = 0; j < COLS; j++) o[j] = 0.f;
+    const int col = blockIdx.z * JOIN_COLS + warp * 2;
+    float o0 = 0.f, o1 = 0.f;
+#pragma unroll 8
     for (int i = 0; i < shares; i++) {
-        if (!has(i)) continue;
         const float by = weight[i * 32 + lane];
-        const float* p = part(i) + (int64_t)warp * COLS * RT + row;
-#pragma unroll
-        for (int j = 0; j < COLS; j++) o[j] = fmaf(p[j * RT], by, o[j]);
+        const float* p = part(i) + col * RT + row;
+        const float x = p[0], y = p[RT];  // of a CTA without a share: anything, and not added
+        if (by != 0.f) o0 = fmaf(x, by, o0), o1 = fmaf(y, by, o1);
     }
     const float by = l == 0.f ? 0.f : 1.f / l;
-    uint16_t* out = (uint16_t*)a.out + o_row * D + warp * COLS;
-#pragma unroll
-    for (int j = 0; j < COLS; j += 4) {
-        float e[4];
-#pragma unroll
-        for (int z = 0; z < 4; z++) e[z] = l == 0.f ? 0.f : o[j + z] * by;
-        *reinterpret_cast<uint2*>(out + j) = make_uint2(Elem<TYPE>::down(e[0], e[1]), Elem<TYPE>::down(e[2], e[3]));
-    }
-    if (warp == 0 && a.lse) a.lse[o_row] = l == 0.f ? __int_as_float(0xff800000) : (m + log2f(l)) * 0.6931471805599453f;
+    *reinterpret_cast<uint32_t*>((uint16_t*)a.out + o_row * D + col) = l == 0.f ? 0u : Elem<TYPE>::down(o0 * by, o1 * by);
+    if (blockIdx.z == 0 && warp == 0 && a.lse) a.lse[o_row] = l == 0.f ? NONE : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 template <int D, int TYPE, int STORE, int MT>
 static int launch(fvs_stream_t stream, Args a) {
-    using P = Plan<D, MT>;
+    using S = Shape<D, STORE, MT>;
     constexpr int RT = ROWS * MT;
-    const int ctas = fvs_sm_count();
+    const int ctas = fvs_sm_count() * S::CTAS;
     const void* f = (const void*)tree_kernel<D, TYPE, STORE, MT>;
-    cudaError_t e = fvs_ensure_smem(f, P::BYTES);
+    cudaError_t e = fvs_ensure_smem(f, S::BYTES);
     if (e != cudaSuccess) return (int)e;
     a.wait_limit = pipeline_wait_limit();
     a.desc = (int32_t*)a.work;
     a.work = a.work + 8 * ctas;
-    tree_kernel<D, TYPE, STORE, MT><<<ctas, Shape<D>::THREADS, P::BYTES, stream>>>(a);
+    tree_kernel<D, TYPE, STORE, MT><<<ctas, S::THREADS, S::BYTES, stream>>>(a);
     if (int rc = fvs_launch_status()) return rc;
     const int rows = a.nodes * a.group;
-    join_kernel<D, TYPE, RT><<<dim3(ctas, ((rows < RT ? rows : RT) + 31) / 32), 256, ctas * 32 * 4, stream>>>(a, ctas);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, ((rows < RT ? rows : RT) + 31) / 32, D / JOIN_COLS);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = ctas * 32 * 4;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, join_kernel<D, TYPE, RT>, a, ctas);
+    if (e != cudaSuccess) return (int)e;
     return fvs_launch_status();
 }
 
 // kernels over heads of D elements; MT: 256 rows of an item where there are more than 128
 template <int D>
 int launch_types(fvs_stream_t stream, const Args& a, int type) {
-    const bool i8 = a.c.type == FVS_I8, two = Shape<D>::W == 2 && a.nodes * a.group > ROWS;
-#define FVS_TREE(T, ST) (two ? launch<D, T, ST, Shape<D>::W>(stream, a) : launch<D, T, ST, 1>(stream, a))
+    const bool i8 = a.c.type == FVS_I8, two = D <= 128 && a.nodes * a.group > ROWS;
+#define FVS_TREE(T, ST) (two ? launch<D, T, ST, (D <= 128 ? 2 : 1)>(stream, a) : launch<D, T, ST, 1>(stream, a))
     if (type == FVS_F16) return i8 ? FVS_TREE(FVS_F16, FVS_I8) : FVS_TREE(FVS_F16, FVS_F16);
     return i8 ? FVS_TREE(FVS_BF16, FVS_I8) : FVS_TREE(FVS_BF16, FVS_BF16);
 #undef FVS_TREE

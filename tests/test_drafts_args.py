@@ -68,7 +68,7 @@ def test_attend_tree_refuses(L, change, rc):
 def test_tree_workspace_size(L):
     f = L.lib().fvs_kv_attend_tree_work
     assert f(0, 4) == -1 and f(64, -1) == -1 and f(512, 4) == -2
-    assert 0 < f(64, 1) == f(64, 128) < f(64, 129) == f(64, 4096) and f(256, 1) == f(256, 4096)
+    assert f(64, 1) > 0 and f(64, 1) % 16 == 0 and f(64, 129) >= f(64, 1) and f(256, 4096) >= f(256, 1) > f(192, 1)
 
 
 @pytest.mark.parametrize("change", [dict(q_weight=68), dict(k_weight=8), dict(weight_type=1), dict(weight_type=2),
