@@ -24,7 +24,9 @@ namespace cg = cooperative_groups;
 namespace fvs {
 namespace drafts {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, NODES = 256, CTAS = 8, AHEAD = 8;
+constexpr int THREADS = 256, WARPS = THREADS / 32, NODES = 256, CTAS = 8;
+constexpr int AHEAD = 4;  // loads of 16 bytes of a row that a lane has on the way
+constexpr int RUN = 8;    // elements of a thread in the draw
 
 struct Rows {  // [seqs, nodes + 1, vocab], strides in elements; null: none
     const void* at;
@@ -40,10 +42,22 @@ struct Args {
     int32_t *path, *kept, *token;
 };
 
+__device__ __forceinline__ float sane(float x) { return x > 0.f && x < __int_as_float(0x7f800000) ? x : 0.f; }  // else no probability
 template <typename T>
-__device__ __forceinline__ double value(const T* p) {
-    const float x = (float)*p;
-    return x > 0.f && x < __int_as_float(0x7f800000) ? (double)x : 0.0;  // what is no probability counts as none
+__device__ __forceinline__ float value(const T* p) { return sane((float)*p); }
+
+// 16 bytes of a row from element `at` on: one load where all of them are the row's (and its skew is the vectors'), else
+// those elements that are, and zeros
+template <typename T>
+__device__ __forceinline__ uint4 load(const T* row, int at, int vocab, bool aligned) {
+    constexpr int VEC = 16 / sizeof(T);
+    if (aligned && at >= 0 && at + VEC <= vocab) return __ldg((const uint4*)(row + at));
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; i++)
+        if (at + i >= 0 && at + i < vocab) e[i] = row[at + i];
+    return raw;
 }
 
 struct Shared {
@@ -58,19 +72,22 @@ struct Shared {
     int found, positive;
 };
 
-// r_k of element v of the present row
+// r_k of element v of the present row; m_0 = 1, and a difference of two fp32 numbers is exact in fp64
 template <bool DRAFT>
-__device__ __forceinline__ double rest(double p, double q, int v, const Shared& s, int k) {
-    if (DRAFT) {
-        for (int j = 0; j < k; j++) p = fmax(__dsub_rn(p, __dmul_rn(s.mass[j], q)), 0.0);  // as written, not one operation
+__device__ __forceinline__ double rest(float p, float q, int v, const Shared& s, int k) {
+    if constexpr (DRAFT) {
+        double r = k == 0 ? (double)p : p > q ? (double)p - (double)q : 0.0;
+        for (int j = 1; j < k; j++) r = fmax(__dsub_rn(r, __dmul_rn(s.mass[j], (double)q)), 0.0);  // as written, not one operation
+        return r;
     } else {
-        for (int j = 0; j < k; j++) p = v == s.refused[j] ? 0.0 : p;
+        for (int j = 0; j < k; j++) p = v == s.refused[j] ? 0.f : p;
+        return p;
     }
-    return p;
 }
 
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(THREADS) verify_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
+    constexpr int VEC = 16 / sizeof(T);
     __shared__ Shared s;
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -84,37 +101,48 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(Args a) {
         s.parent[i] = ok ? up : -2;  // never taken
         s.tok[i] = x;
         s.u[i] = __ldg(a.u + (int64_t)b * (a.nodes + 1) + i);
-        s.left[i] = ok ? value(target + (up + 1) * a.target.row + x) : 0.0;
-        s.qx[i] = !ok ? 0.0 : DRAFT ? value(draft + (up + 1) * a.draft.row + x) : 1.0;
+        s.left[i] = ok ? (double)value(target + (up + 1) * a.target.row + x) : 0.0;
+        s.qx[i] = !ok ? 0.0 : DRAFT ? (double)value(draft + (up + 1) * a.draft.row + x) : 1.0;
     }
-    // the part of a row that this warp sums: the cluster's warps side by side
-    const int span = ((a.vocab + ctas * WARPS - 1) / (ctas * WARPS) + 31) / 32 * 32;
-    const int lo = min(a.vocab, (rank * WARPS + warp) * span), hi = min(a.vocab, lo + span);
     int last = -1, kept = 0, k = 0, turn = 0;
     double total = 0.0;
     bool summed = false;  // total and the warps' sums are those of r_k
+    // The parts of a row that the cluster's warps sum lie side by side: vectors of 16 bytes, the first of them beginning
+    // `skew` elements before the row where that is not aligned.
+    auto skew_of = [&](const T* row) { return (int)((uintptr_t)row / sizeof(T) % VEC); };
+    auto span_of = [&](int skew) { return ((a.vocab + skew + VEC - 1) / VEC + ctas * WARPS - 1) / (ctas * WARPS); };
     // sums of r_n over the row behind `last`; ends with all of the cluster's threads having them
     auto pass = [&](int n) {
         const T *p = target + (last + 1) * a.target.row, *q = draft + (last + 1) * a.draft.row;
+        const int skew = skew_of(p), span = span_of(skew), lo = (rank * WARPS + warp) * span;
+        const int hi = min((a.vocab + skew + VEC - 1) / VEC, lo + span);
+        const bool alike = DRAFT && skew_of(q) == skew, both = DRAFT && n > 0;
         double sum = 0.0;
-        for (int v0 = lo + lane; v0 < hi; v0 += 32 * AHEAD) {
-            double pv[AHEAD], qv[AHEAD];
+        for (int j0 = lo + lane; j0 < hi; j0 += 32 * AHEAD) {
+            uint4 pv[AHEAD], qv[AHEAD];
 #pragma unroll
-            for (int j = 0; j < AHEAD; j++) {
-                const int v = v0 + 32 * j;
-                pv[j] = v < hi ? value(p + v) : 0.0;
-                qv[j] = DRAFT && n > 0 && v < hi ? value(q + v) : 0.0;
+            for (int i = 0; i < AHEAD; i++) {
+                const int j = j0 + 32 * i;
+                const int at = j < hi ? j * VEC - skew : a.vocab;  // none behind the part
+                pv[i] = load(p, at, a.vocab, true);
+                qv[i] = both ? load(q, at, a.vocab, alike) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int j = 0; j < AHEAD; j++) sum += rest<DRAFT>(pv[j], qv[j], v0 + 32 * j, s, n);
+            for (int i = 0; i < AHEAD; i++) {
+                const T *pe = reinterpret_cast<const T*>(&pv[i]), *qe = reinterpret_cast<const T*>(&qv[i]);
+                double some = 0.0;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) some += rest<DRAFT>(sane((float)pe[e]), sane((float)qe[e]), (j0 + 32 * i) * VEC - skew + e, s, n);
+                sum += some;
+            }
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        __syncthreads();  // the sums before were read
         if (lane == 0) s.warp[warp] = sum;
         __syncthreads();
         if (tid < ctas) {
             double all = 0.0;
+#pragma unroll
             for (int w = 0; w < WARPS; w++) all += s.warp[w];
             *cluster.map_shared_rank(&s.total[turn][rank], tid) = all;
         }
@@ -163,10 +191,11 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(Args a) {
     if (!summed) {
         __syncthreads();
         total = pass(k);
+    } else {
+        turn ^= 1;  // the buffer of the last pass
     }
     // the draw: the first CTA, warp and element at which the running sum passes the limit
     const double limit = (double)__ldg(a.u + (int64_t)b * (a.nodes + 1) + a.nodes) * total;
-    if (summed) turn ^= 1;  // the buffer of the last pass
     int owner = -1, some = -1;
     double before = 0.0;
     for (int r = 0; r < ctas; r++) {
@@ -198,28 +227,43 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(Args a) {
             if (w < WARPS - 1) before += s.warp[w];
         }
         if (!over) w = positive;  // the sums' rounding, or none
-        const int from = min(a.vocab, (rank * WARPS + w) * span), to = min(a.vocab, from + span);
+        const T *p = target + (last + 1) * a.target.row, *q = draft + (last + 1) * a.draft.row;
+        const int skew = skew_of(p), span = span_of(skew);
+        const int from = max(0, (rank * WARPS + w) * span * VEC - skew), to = min(a.vocab, (rank * WARPS + w + 1) * span * VEC - skew);
         if (tid == 0) s.found = INT_MAX, s.positive = -1;
         __syncthreads();
-        const T *p = target + (last + 1) * a.target.row, *q = draft + (last + 1) * a.draft.row;
-        for (int v0 = from; v0 < to; v0 += THREADS) {
-            const int v = v0 + tid;
-            double x = 0.0;
-            if (v < to) x = rest<DRAFT>(value(p + v), DRAFT && k > 0 ? value(q + v) : 0.0, v, s, k);
-            if (x > 0.0) atomicMax(&s.positive, v);
-            double sum = x;
+        for (int v0 = from; v0 < to; v0 += THREADS * RUN) {
+            const int v = v0 + tid * RUN;
+            double x[RUN], sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < RUN; j++) {
+                x[j] = v + j < to ? rest<DRAFT>(value(p + v + j), DRAFT && k > 0 ? value(q + v + j) : 0.f, v + j, s, k) : 0.0;
+                sum += x[j];
+            }
+            double upto = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += y;
+                const double y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
             }
-            if (lane == 31) s.scan[warp] = sum;
+            if (lane == 31) s.scan[warp] = upto;
             __syncthreads();
-            double add = before;
-            for (int j = 0; j < warp; j++) add += s.scan[j];
-            if (over && x > 0.0 && add + sum > limit) atomicMin(&s.found, v);
-            for (int j = warp; j < WARPS; j++) add += s.scan[j];
-            before = add;
+            double add = before, all = before;
+#pragma unroll
+            for (int j = 0; j < WARPS; j++) {
+                if (j < warp) add += s.scan[j];
+                all += s.scan[j];
+            }
+            add += upto - sum;
+#pragma unroll
+            for (int j = 0; j < RUN; j++) {
+                add += x[j];
+                if (x[j] > 0.0) {
+                    if (over && add > limit) atomicMin(&s.found, v + j);
+                    atomicMax(&s.positive, v + j);
+                }
+            }
+            before = all;
             __syncthreads();
             if (s.found != INT_MAX) break;
         }
@@ -230,9 +274,9 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(Args a) {
 
 template <typename T>
 static int launch(fvs_stream_t stream, const Args& a) {
-    // CTAs of a row: two waves of them where there are few sequences, and at least 4096 elements each
+    // CTAs of a row: as many as run at once, four an SM, and at least 2048 elements each
     int ctas = 1;
-    while (ctas < CTAS && ctas * 2 * a.seqs <= 4 * fvs_sm_count() && a.vocab >= ctas * 2 * 4096) ctas *= 2;
+    while (ctas < CTAS && ctas * 2 * a.seqs <= 4 * fvs_sm_count() && a.vocab >= ctas * 2 * 2048) ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.seqs * ctas));
     cfg.blockDim = dim3(THREADS);
