@@ -25,7 +25,7 @@ namespace fvs {
 namespace drafts {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, NODES = 256, CTAS = 8;
-constexpr int AHEAD = 4;  // loads of 16 bytes of a row that a lane has on the way
+constexpr int AHEAD = 2;  // loads of 16 bytes of a row that a lane has on the way (four: a third slower, their code is fetched again and again)
 constexpr int RUN = 8;    // elements of a thread in the draw
 
 struct Rows {  // [seqs, nodes + 1, vocab], strides in elements; null: none
@@ -85,6 +85,58 @@ __device__ __forceinline__ double rest(float p, float q, int v, const Shared& s,
     }
 }
 
+// sum of r_n over the 16 bytes from element v on
+template <typename T, bool DRAFT>
+__device__ __forceinline__ double sum_of(const uint4& praw, const uint4& qraw, int v, const Shared& s, int n) {
+    constexpr int VEC = 16 / sizeof(T);
+    const T *pe = reinterpret_cast<const T*>(&praw), *qe = reinterpret_cast<const T*>(&qraw);
+    float p[VEC], q[VEC];
+    uint32_t most = 0;  // above every number's bits where something is negative or not finite
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        p[e] = (float)pe[e];
+        most = max(most, __float_as_uint(p[e]));
+        if (DRAFT) {
+            q[e] = (float)qe[e];
+            most = max(most, __float_as_uint(q[e]));
+        }
+    }
+    if (__builtin_expect(most >= 0x7f800000u, 0)) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            p[e] = sane(p[e]);
+            if (DRAFT) q[e] = sane(q[e]);
+        }
+    }
+    double r[VEC];
+    if (DRAFT && n > 0) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) r[e] = p[e] > q[e] ? (double)p[e] - (double)q[e] : 0.0;
+#pragma unroll 1
+        for (int j = 1; j < n; j++) {
+            const double mass = s.mass[j];
+#pragma unroll
+            for (int e = 0; e < VEC; e++) r[e] = fmax(__dsub_rn(r[e], __dmul_rn(mass, (double)q[e])), 0.0);
+        }
+    } else {
+        if (!DRAFT) {
+#pragma unroll 1
+            for (int j = 0; j < n; j++) {
+                const int at = s.refused[j] - v;
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    if (at == e) p[e] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e++) r[e] = p[e];
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) sum += r[e] + r[e + 1];
+    return sum;
+}
+
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
     constexpr int VEC = 16 / sizeof(T);
@@ -128,13 +180,7 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
                 qv[i] = both ? load(q, at, a.vocab, alike) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                const T *pe = reinterpret_cast<const T*>(&pv[i]), *qe = reinterpret_cast<const T*>(&qv[i]);
-                double some = 0.0;
-#pragma unroll
-                for (int e = 0; e < VEC; e++) some += rest<DRAFT>(sane((float)pe[e]), sane((float)qe[e]), (j0 + 32 * i) * VEC - skew + e, s, n);
-                sum += some;
-            }
+            for (int i = 0; i < AHEAD; i++) sum += sum_of<T, DRAFT>(pv[i], qv[i], (j0 + 32 * i) * VEC - skew, s, n);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
