@@ -60,9 +60,10 @@ struct Args {
 
 
 // How a kernel uses an SM, by head size and 128 * MT rows of an item.
-template <int D, int STORE, int MT>
+template <int D, int STORE, int MT, int QR>
 struct Shape {
     static_assert(MT == 1 || D <= 128, "tensor memory holds one O of a wide head");
+    static_assert(QR == ROWS || (MT == 1 && D <= 128), "fewer rows of queries");
     // CTAs of an SM: with 128 rows of heads up to 128 two, whose beginnings and ends overlap (one CTA whose two softmax
     // warpgroups took turns at the tiles took 113 us where this takes 90, at 64 ragged requests of 64 rows)
     static constexpr int CTAS = MT == 1 && D <= 128 ? 2 : 1;
@@ -80,7 +81,7 @@ struct Shape {
     static constexpr int O0 = BUFFERS * KEYS;                         // columns of the scores, then W of O
     static_assert(O0 + W * D <= COLUMNS, "tensor memory columns");
     // shared memory: queries, the ring, then barriers, the tiles' flags and scales, segments and masks
-    static constexpr int Q = MT * ROWS * 128 * BLOCKS;
+    static constexpr int Q = MT * QR * 128 * BLOCKS;
     static constexpr int BARS = 88 * 8, INFO_BYTES = 16 + 2 * KEYS * 4, MASK_BYTES = W * ROWS * (KEYS / 32) * 4;
     static constexpr int MISC = BARS + INFO * INFO_BYTES + 64 + SEGS * SEG_BYTES + MASK_BYTES;
     static constexpr int FIT = ((CTAS == 2 ? 115712 : 232448) - 1024 - MISC - Q) / SLOT;
@@ -306,9 +307,11 @@ __device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
     }
 }
 
-template <int D, int TYPE, int STORE, int MT>
-__global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, MT>::CTAS) tree_kernel(Args a) {
-    using S = Shape<D, STORE, MT>;
+// QR: rows of queries that shared memory holds, 64 where an item has no more: the matrix instructions read 128, the others of
+// whatever lies behind (their scores and outputs go to rows that nobody reads), and the ring has a slot more
+template <int D, int TYPE, int STORE, int MT, int QR>
+__global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STORE, MT, QR>::CTAS) tree_kernel(Args a) {
+    using S = Shape<D, STORE, MT, QR>;
     constexpr bool I8 = STORE == FVS_I8;
     constexpr int KEYS = S::KEYS, BUFFERS = S::BUFFERS, PARTS = KEYS / 64, W = S::W, RT = ROWS * MT, SLOTS = S::SLOTS, LEAD = S::LEAD;
     constexpr int INFO_BYTES = S::INFO_BYTES, PRODUCERS = S::PRODUCERS;
@@ -520,12 +523,38 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, 
             }
             mbar_arrive(landed(slot));
         };
+        // the segment's queries, when their buffer is free: a warp's rows 32 at a time, addresses by a lane each
+        auto queries = [&](const volatile Seg& g) {
+            constexpr int QCH = D / 8;
+            const int rt = g.rt, live_rows = g.rows;
+#pragma unroll 1
+            for (int r0 = pw * 32; r0 < MT * QR; r0 += 32 * PRODUCERS) {
+                const int row = rt * RT + r0 + lane;
+                uint32_t from = NONE;
+                if (r0 + lane < live_rows) {
+                    const int node = row / a.group, h = head * a.group + row - node * a.group;
+                    from = (uint32_t)(((int64_t)b * a.q_seq + (int64_t)node * a.q_node + (int64_t)h * a.q_head) / 8);
+                }
+                const int mt = r0 / ROWS, k0 = r0 - mt * ROWS;
+                const uint32_t dst = q_smem + mt * (ROWS * 128 * S::BLOCKS);
+#pragma unroll 4
+                for (int i = 0; i < QCH; i++) {
+                    const int id = i * 32 + lane, r = id / QCH, c = id - r * QCH, k = k0 + r;
+                    const uint32_t at = __shfl_sync(0xffffffffu, from, r);
+                    cp_async16(dst + (c >> 3) * (QR * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), (const uint8_t*)a.q + (at == NONE ? 0 : c * 16 + (uint64_t)at * 16), at != NONE);
+                }
+            }
+            copies_arrive(q_landed);
+        };
         for (int seg = 0; ok; seg++) {
             if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
             const volatile Seg& g = segs[seg % SEGS];
             const int t0 = g.t0, t1 = g.t1;
             b = g.b, head = g.head, keys = g.keys;
             if (t0 >= t1) break;
+            // before the first tile if the segment before has all its scores, else behind it
+            const bool asked = __all_sync(0xffffffffu, mbar_test(q_empty, (seg & 1) ^ 1));
+            if (asked) queries(g);
             lookup(t0);
             at = next_at;
             if (I8) {
@@ -575,20 +604,8 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, 
                     advance();
                 }
                 if (!ok) break;
-                if (t == t0) {
-                    // the rows' queries, behind the first tile: their buffer is free when the segment before has its scores
-                    if (!warp_wait(q_empty, (seg & 1) ^ 1, abort, WL)) { ok = false; break; }
-                    constexpr int QCH = D / 8;
-                    const int rt = g.rt, live_rows = g.rows;
-                    for (int id = pw * 32 + lane; id < RT * QCH; id += 32 * PRODUCERS) {
-                        const int r = id / QCH, c = id - r * QCH, mt = r / ROWS, k = r - mt * ROWS, row = rt * RT + r;
-                        const bool live = r < live_rows;
-                        const int node = live ? row / a.group : 0, h = live ? row - node * a.group : 0;
-                        const uint16_t* src = (const uint16_t*)a.q + (int64_t)b * a.q_seq + (int64_t)node * a.q_node + (int64_t)(head * a.group + h) * a.q_head + c * 8;
-                        cp_async16(q_smem + mt * (ROWS * 128 * S::BLOCKS) + (c >> 3) * (ROWS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), src, live);
-                    }
-                    copies_arrive(q_landed);
-                }
+                if (t == t0 && !asked && !(ok = warp_wait(q_empty, (seg & 1) ^ 1, abort, WL))) break;
+                if (t == t0 && !asked) queries(g);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(seg_empty(seg % SEGS));
@@ -617,7 +634,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, 
                 const uint64_t bd = k_desc + (uint32_t)(kslot * (S::SLOT / 16));
 #pragma unroll
                 for (int k = 0; k < D / 16; k++)
-                    mma_ss(d, q_desc + ((k >> 2) * (ROWS * 128 / 16) + (k & 3) * 2), bd + ((k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2), id_s, k > 0);
+                    mma_ss(d, q_desc + ((k >> 2) * (QR * 128 / 16) + (k & 3) * 2), bd + ((k >> 2) * (KEYS * 128 / 16) + (k & 3) * 2), id_s, k > 0);
                 mma_commit(s_full(u));
                 mma_commit(empty(kslot));
                 step(kslot, kphase);
@@ -809,7 +826,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, 
                             for (int j = 0; j < 32; j++) s[j] = word >> j & 1 ? __float_as_uint(__uint_as_float(s[j]) * sign) : 0xff800000u;
                         }
                     };
-                    bool raise = !any;  // no reference yet
+                    bool raise = !any, need = raise;  // no reference yet; of the warp, of this row
 #pragma unroll 1
                     for (int k = 0; k < KEYS / 32;) {
                         uint32_t s[32];
@@ -819,7 +836,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, 
 #pragma unroll
                             for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(s[j]));
                             if (!I8) top *= lift;
-                            const float to = fmaxf(m, top), by = m == to ? 1.f : exp2_of(m - to);
+                            const float to = need ? fmaxf(m, top) : m, by = m == to ? 1.f : exp2_of(m - to);
                             m = to;
                             l *= by;
                             const bool half = PARTS == 2 && k >= 2;  // the tile's first 64 weights may be in O
@@ -870,7 +887,8 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT>::THREADS, Shape<D, STORE, 
                         const float2 pair = one(add2(sums[0], sums[1]));
                         const float sum = pair.x + pair.y;
                         // (not-a-numbers and rows that have seen nothing yet are taken again once)
-                        if (__any_sync(0xffffffffu, !(sum <= LIMIT) || m == __int_as_float(0xff800000)) && !raise) {
+                        need = !(sum <= LIMIT) || m == __int_as_float(0xff800000);
+                        if (__any_sync(0xffffffffu, need) && !raise) {
                             raise = true;
                             continue;
                         }
@@ -1048,18 +1066,18 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
     if (blockIdx.z == 0 && warp == 0 && a.lse) a.lse[o_row] = l == 0.f ? NONE : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-template <int D, int TYPE, int STORE, int MT>
+template <int D, int TYPE, int STORE, int MT, int QR>
 static int launch(fvs_stream_t stream, Args a) {
-    using S = Shape<D, STORE, MT>;
+    using S = Shape<D, STORE, MT, QR>;
     constexpr int RT = ROWS * MT;
     const int ctas = fvs_sm_count() * S::CTAS;
-    const void* f = (const void*)tree_kernel<D, TYPE, STORE, MT>;
+    const void* f = (const void*)tree_kernel<D, TYPE, STORE, MT, QR>;
     cudaError_t e = fvs_ensure_smem(f, S::BYTES);
     if (e != cudaSuccess) return (int)e;
     a.wait_limit = pipeline_wait_limit();
     a.desc = (int32_t*)a.work;
     a.work = a.work + 8 * ctas;
-    tree_kernel<D, TYPE, STORE, MT><<<ctas, S::THREADS, S::BYTES, stream>>>(a);
+    tree_kernel<D, TYPE, STORE, MT, QR><<<ctas, S::THREADS, S::BYTES, stream>>>(a);
     if (int rc = fvs_launch_status()) return rc;
     const int rows = a.nodes * a.group;
     cudaLaunchConfig_t cfg = {};
@@ -1077,11 +1095,17 @@ static int launch(fvs_stream_t stream, Args a) {
     return fvs_launch_status();
 }
 
-// kernels over heads of D elements; MT: 256 rows of an item where there are more than 128
+// kernels over heads of D elements, by the rows of an item: 256 at a time where there are more than 128, queries of 64 where
+// there are no more (heads wider than 128: always 128)
 template <int D>
 int launch_types(fvs_stream_t stream, const Args& a, int type) {
-    const bool i8 = a.c.type == FVS_I8, two = D <= 128 && a.nodes * a.group > ROWS;
-#define FVS_TREE(T, ST) (two ? launch<D, T, ST, (D <= 128 ? 2 : 1)>(stream, a) : launch<D, T, ST, 1>(stream, a))
+    constexpr bool narrow = D <= 128;
+    const bool i8 = a.c.type == FVS_I8;
+    const int rows = a.nodes * a.group;
+#define FVS_TREE(T, ST)                                                               \
+    (narrow && rows > ROWS ? launch<D, T, ST, narrow ? 2 : 1, ROWS>(stream, a)        \
+     : narrow && rows <= 64 ? launch<D, T, ST, 1, narrow ? 64 : ROWS>(stream, a)      \
+                            : launch<D, T, ST, 1, ROWS>(stream, a))
     if (type == FVS_F16) return i8 ? FVS_TREE(FVS_F16, FVS_I8) : FVS_TREE(FVS_F16, FVS_F16);
     return i8 ? FVS_TREE(FVS_BF16, FVS_I8) : FVS_TREE(FVS_BF16, FVS_BF16);
 #undef FVS_TREE
