@@ -5,11 +5,11 @@
 namespace fvs {
 namespace kv {
 namespace tree {
-extern template int launch_types<64>(fvs_stream_t, const Args&, int);
-extern template int launch_types<96>(fvs_stream_t, const Args&, int);
-extern template int launch_types<128>(fvs_stream_t, const Args&, int);
-extern template int launch_types<192>(fvs_stream_t, const Args&, int);
-extern template int launch_types<256>(fvs_stream_t, const Args&, int);
+extern template int launch_types<64>(fvs_stream_t, Args, int);
+extern template int launch_types<96>(fvs_stream_t, Args, int);
+extern template int launch_types<128>(fvs_stream_t, Args, int);
+extern template int launch_types<192>(fvs_stream_t, Args, int);
+extern template int launch_types<256>(fvs_stream_t, Args, int);
 }
 }  // namespace kv
 }  // namespace fvs
@@ -42,7 +42,7 @@ extern "C" int fvs_kv_attend_tree(fvs_stream_t stream, const fvs_kv_cache* cache
     if (nodes > FVS_TREE_NODES || (int64_t)nodes * group > (1 << 24) || (int64_t)wide * cache->page > 0x7fffff00ll - FVS_TREE_NODES)
         return FVS_ERANGE;
     tree::Args a{*cache, {table, table_stride, seqs, wide}, q, q_seq, q_node, q_head, lens, parents, counts, parent_stride,
-                 nodes, hq, group, scale, out, lse, (float*)work, nullptr, 0};
+                 nodes, hq, group, scale, out, lse, (float*)work, nullptr, 0, 0};
     switch (cache->dim) {
         case 64: return tree::launch_types<64>(stream, a, type);
         case 96: return tree::launch_types<96>(stream, a, type);

@@ -56,7 +56,12 @@ struct Args {
     float* work;     // two partial results of each CTA: [dim][rows] O, then [rows] maxima (log2), [rows] sums
     int32_t* desc;   // 8 words of each CTA: what join_kernel reads
     uint32_t wait_limit;
+    int box;         // keys of a tensor copy, a power of two that divides the page
 };
+struct Maps {  // of keys and values: element, slot, head, page
+    CUtensorMap k, v;
+};
+
 
 
 // How a kernel uses an SM, by head size and 128 * MT rows of an item.
@@ -309,8 +314,11 @@ __device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
 
 // QR: rows of queries that shared memory holds, 64 where an item has no more: the matrix instructions read 128, the others of
 // whatever lies behind (their scores and outputs go to rows that nobody reads), and the ring has a slot more
-template <int D, int TYPE, int STORE, int MT, int QR>
-__global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STORE, MT, QR>::CTAS) tree_kernel(Args a) {
+// BOXES: 16-bit rows come by tensor copies (pages of a multiple of 8 slots); else by the producers' lanes, 16 bytes each, whose
+// traffic delays every wait on a barrier (104 us instead of 70 at 64 ragged requests)
+template <int D, int TYPE, int STORE, int MT, int QR, bool BOXES>
+__global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STORE, MT, QR>::CTAS)
+    tree_kernel(Args a, const __grid_constant__ Maps maps) {
     using S = Shape<D, STORE, MT, QR>;
     constexpr bool I8 = STORE == FVS_I8;
     constexpr int KEYS = S::KEYS, BUFFERS = S::BUFFERS, PARTS = KEYS / 64, W = S::W, RT = ROWS * MT, SLOTS = S::SLOTS, LEAD = S::LEAD;
@@ -352,12 +360,12 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
 
     if (tid == 0) {
         for (int s = 0; s < SLOTS; s++) {
-            mbar_init(landed(s), 32 * PRODUCERS);
+            mbar_init(landed(s), BOXES ? 1 : 32 * PRODUCERS);
             mbar_init(full(s), 1);
             mbar_init(empty(s), MT);
         }
         for (int s = 0; s < INFO; s++) {
-            mbar_init(info_full(s), PRODUCERS);
+            mbar_init(info_full(s), BOXES ? 1 : PRODUCERS);
             mbar_init(info_empty(s), 4 * MT);
         }
         for (int u = 0; u < BUFFERS; u++) {
@@ -366,7 +374,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             if (PARTS == 2) mbar_init(pv_half(u), 1);
             mbar_init(pv_done(u), 1);
         }
-        mbar_init(q_landed, 32 * PRODUCERS);
+        mbar_init(q_landed, 32 * (BOXES ? PRODUCERS - 1 : PRODUCERS));
         mbar_init(q_full, 1);
         mbar_init(q_empty, W);
         mbar_init(o_free, 128 * W);
@@ -444,8 +452,111 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     const uint32_t tmem = *tmem_slot;
     const float scale2 = a.scale * 1.4426950408889634f;  // of scores in powers of two
 
-    if (warp >= W_PROD && warp < W_MMA) {
-        // ------------------------------------------------------------ producers
+    // chunk c of 16 bytes of row k of a 128-byte swizzled tile of `rows` rows
+    auto swizzled = [](int rows, int k, int c) { return (uint32_t)((c >> 3) * (rows * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4)); };
+    // a segment's queries into their buffer by warp qw of qn: 32 rows at a time, addresses by a lane each
+    auto queries = [&](const volatile Seg& g, int qw, int qn) {
+        constexpr int QCH = D / 8;
+        constexpr uint32_t NONE = 0xffffffffu;
+        const int b = g.b, head = g.head, rt = g.rt, live_rows = g.rows;
+#pragma unroll 1
+        for (int r0 = qw * 32; r0 < MT * QR; r0 += 32 * qn) {
+            const int row = rt * RT + r0 + lane;
+            uint32_t from = NONE;
+            if (r0 + lane < live_rows) {
+                const int node = row / a.group, h = head * a.group + row - node * a.group;
+                from = (uint32_t)(((int64_t)b * a.q_seq + (int64_t)node * a.q_node + (int64_t)h * a.q_head) / 8);
+            }
+            const int mt = r0 / ROWS, k0 = r0 - mt * ROWS;
+            const uint32_t dst = q_smem + mt * (ROWS * 128 * S::BLOCKS);
+#pragma unroll 4
+            for (int i = 0; i < QCH; i++) {
+                const int id = i * 32 + lane, r = id / QCH, c = id - r * QCH;
+                const uint32_t at = __shfl_sync(0xffffffffu, from, r);
+                cp_async16(dst + swizzled(QR, k0 + r, c), (const uint8_t*)a.q + (at == NONE ? 0 : c * 16 + (uint64_t)at * 16), at != NONE);
+            }
+        }
+        copies_arrive(q_landed);
+    };
+    if (BOXES && warp >= W_PROD && warp < W_MMA) {
+        // ------------------------------------------------------------ producers by tensor copies
+        if (warp == W_PROD) {
+            // Lane g looks up box g of a tile.  A box comes whole if it has any keys; the scores of what it holds beside them
+            // are masked, and the relay puts zeros in place of those values.
+            const int box = a.box, boxes = KEYS / box;
+            int slot = 0, phase = 1, tile = 0, issued = 0;
+            bool ok = true;
+            int page = 0, at = 0, have = 0, next_page, next_at, next_have;
+            for (int seg = 0; ok; seg++) {
+                if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
+                const volatile Seg& g = segs[seg % SEGS];
+                const int t0 = g.t0, t1 = g.t1, b = g.b, head = g.head, keys = g.keys;
+                if (t0 >= t1) break;
+                auto lookup = [&](int t) {
+                    const int x = t * KEYS + lane * box;
+                    next_have = 0;
+                    if (lane < boxes && x < keys && place(a.c, a.tb, b, x, next_page, next_at)) {
+                        next_have = min(box, keys - x);
+                        if (a.c.fill) next_have = max(0, min(next_have, __ldg(a.c.fill + next_page) - next_at));
+                    }
+                };
+                // the boxes of `mine` lanes into the next slot
+                auto copy = [&](const CUtensorMap* map, bool mine) {
+                    const int n = __popc(__ballot_sync(0xffffffffu, mine));
+                    if (lane == 0) mbar_expect_tx(landed(slot), n * box * 128 * S::BLOCKS);
+                    __syncwarp();
+                    if (mine) {
+#pragma unroll
+                        for (int c = 0; c < S::BLOCKS; c++)
+                            asm volatile(
+                                "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                                    ring + slot * S::SLOT + c * (KEYS * 128) + lane * box * 128),
+                                "l"(map), "r"(c * 64), "r"(at), "r"(head), "r"(page), "r"(landed(slot))
+                                : "memory");
+                    }
+                    if (++slot == SLOTS) slot = 0, phase ^= 1;
+                    issued++;
+                };
+                lookup(t0);
+                for (int t = t0; t < t1; t++, tile++) {
+                    page = next_page, at = next_at, have = next_have;
+                    const int is = tile % INFO, first = lane * box;
+                    uint32_t lo = 0, hi = 0;  // flags of the tile's keys
+                    if (have > 0) {
+                        const uint64_t mine = (have == 64 ? ~0ull : (1ull << have) - 1) << first;
+                        lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+                    }
+                    lo = __reduce_or_sync(0xffffffffu, lo);
+                    hi = __reduce_or_sync(0xffffffffu, hi);
+                    if (!warp_wait(info_empty(is), ((tile / INFO) & 1) ^ 1, abort, WL)) { ok = false; break; }
+                    if (lane == 0) {
+                        *reinterpret_cast<uint2*>(info + is * INFO_BYTES) = make_uint2(lo, hi);
+                        mbar_arrive(info_full(is));
+                    }
+                    if (t + 1 < t1) lookup(t + 1);
+                    if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
+                    copy(&maps.k, have > 0);
+                    if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
+                    copy(&maps.v, have > 0);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(seg_empty(seg % SEGS));
+            }
+            // no copy is under way when the CTA ends, whatever became of its waits
+            for (int i = max(0, issued - SLOTS); i < issued; i++) mbar_drain(landed(i % SLOTS), (i / SLOTS) & 1);
+        } else {
+            for (int seg = 0;; seg++) {
+                if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
+                const volatile Seg& g = segs[seg % SEGS];
+                if (g.t0 >= g.t1 || !warp_wait(q_empty, (seg & 1) ^ 1, abort, WL)) break;
+                queries(g, warp - W_PROD - 1, PRODUCERS - 1);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(seg_empty(seg % SEGS));
+            }
+            cp_async_wait_all();
+        }
+    } else if (!BOXES && warp >= W_PROD && warp < W_MMA) {
+        // ------------------------------------------------------------ producers by their lanes
         constexpr int PER = KEYS / PRODUCERS;      // keys of a warp
         constexpr int CH = (I8 ? D / 16 : D / 8);  // 16-byte chunks of a stored row
         constexpr int TURNS = PER * CH / 32;
@@ -480,7 +591,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             if (++slot == SLOTS) slot = 0, phase ^= 1;
         };
         // chunk c of key k in a slot
-        auto chunk = [&](int k, int c) { return (uint32_t)((c >> 3) * (KEYS * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4)); };
+        auto chunk = [&](int k, int c) { return swizzled(KEYS, k, c); };
         // the rows that this lane copies chunks of, a turn each: the same for keys and values
         uint32_t rows[TURNS];
         auto exchange = [&](uint32_t x) {
@@ -523,29 +634,6 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             }
             mbar_arrive(landed(slot));
         };
-        // the segment's queries, when their buffer is free: a warp's rows 32 at a time, addresses by a lane each
-        auto queries = [&](const volatile Seg& g) {
-            constexpr int QCH = D / 8;
-            const int rt = g.rt, live_rows = g.rows;
-#pragma unroll 1
-            for (int r0 = pw * 32; r0 < MT * QR; r0 += 32 * PRODUCERS) {
-                const int row = rt * RT + r0 + lane;
-                uint32_t from = NONE;
-                if (r0 + lane < live_rows) {
-                    const int node = row / a.group, h = head * a.group + row - node * a.group;
-                    from = (uint32_t)(((int64_t)b * a.q_seq + (int64_t)node * a.q_node + (int64_t)h * a.q_head) / 8);
-                }
-                const int mt = r0 / ROWS, k0 = r0 - mt * ROWS;
-                const uint32_t dst = q_smem + mt * (ROWS * 128 * S::BLOCKS);
-#pragma unroll 4
-                for (int i = 0; i < QCH; i++) {
-                    const int id = i * 32 + lane, r = id / QCH, c = id - r * QCH, k = k0 + r;
-                    const uint32_t at = __shfl_sync(0xffffffffu, from, r);
-                    cp_async16(dst + (c >> 3) * (QR * 128) + k * 128 + (((c & 7) ^ (k & 7)) << 4), (const uint8_t*)a.q + (at == NONE ? 0 : c * 16 + (uint64_t)at * 16), at != NONE);
-                }
-            }
-            copies_arrive(q_landed);
-        };
         for (int seg = 0; ok; seg++) {
             if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
             const volatile Seg& g = segs[seg % SEGS];
@@ -554,7 +642,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             if (t0 >= t1) break;
             // before the first tile if the segment before has all its scores, else behind it
             const bool asked = __all_sync(0xffffffffu, mbar_test(q_empty, (seg & 1) ^ 1));
-            if (asked) queries(g);
+            if (asked) queries(g, pw, PRODUCERS);
             lookup(t0);
             at = next_at;
             if (I8) {
@@ -605,7 +693,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                 }
                 if (!ok) break;
                 if (t == t0 && !asked && !(ok = warp_wait(q_empty, (seg & 1) ^ 1, abort, WL))) break;
-                if (t == t0 && !asked) queries(g);
+                if (t == t0 && !asked) queries(g, pw, PRODUCERS);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(seg_empty(seg % SEGS));
@@ -694,7 +782,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             }
             mma_commit(drain);  // what was issued has to end before the CTA does
             mbar_drain(drain, 0);
-        } else if (warp == W_MMA + W && lane == 0) {
+        } else if (warp == W_MMA + W) {
             // -------------------------------------------------------- the scheduler, which is also the relay
             // What the producers wrote becomes visible to the matrix instructions by a fence between the two.  The
             // instructions' own thread would wait at it until those it has issued are done (100 cycles for each
@@ -703,36 +791,53 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             const int64_t total = s_place[0];
             const int64_t ctas = shares(total);
             walk.begin(a, (int)s_place[1], s_place[2], share(total, ctas, blockIdx.x), share(total, ctas, blockIdx.x + 1));
-            int slot = 0, phase = 0, told = 0;
-            bool ok = true, more = true;
-            auto pass = [&]() {
-                ok = ok && mbar_wait(landed(slot), phase, abort, WL);
-                if (!ok) return;
+            int slot = 0, phase = 0, told = 0, tile = 0;
+            bool more = true, ok = true;
+            auto pass = [&](bool values) {
+                if (!warp_wait(landed(slot), phase, abort, WL)) return false;
+                if (BOXES && values) {  // zeros for keys that are not there: a weight of 0 times anything is not 0
+                    const int is = tile % INFO;
+                    if (!warp_wait(info_full(is), (tile / INFO) & 1, abort, WL)) return false;
+                    const uint2 there = *reinterpret_cast<const uint2*>(info + is * INFO_BYTES);
+                    if ((there.x & there.y) != 0xffffffffu) {
+                        constexpr int CH = D / 8;
+                        for (int id = lane; id < KEYS * CH; id += 32) {
+                            const int k = id / CH, c = id - k * CH;
+                            if (!((k < 32 ? there.x >> k : there.y >> (k - 32)) & 1))
+                                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring + slot * S::SLOT + swizzled(KEYS, k, c)), "r"(0) : "memory");
+                        }
+                    }
+                }
                 proxy_fence();
-                mbar_arrive(full(slot));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full(slot));
                 if (++slot == SLOTS) slot = 0, phase ^= 1;
+                return true;
             };
             for (int seg = 0; ok; seg++) {
                 for (; more && told <= seg + 1; told++) {  // a segment ahead
                     Seg g;
                     more = walk.next(a, g);
                     if (!more) g.t0 = g.t1 = 0;
-                    if (!mbar_wait(seg_empty(told % SEGS), ((told / SEGS) & 1) ^ 1, abort, WL)) { ok = false; break; }
-                    volatile Seg& to = segs[told % SEGS];
-                    to.t0 = g.t0, to.t1 = g.t1;
-                    if (more) to.b = g.b, to.head = g.head, to.rt = g.rt, to.rows = g.rows, to.n = g.n, to.keys = g.keys, to.tiles = g.tiles, to.item = g.item;
-                    mbar_arrive(seg_full(told % SEGS));
+                    if (!warp_wait(seg_empty(told % SEGS), ((told / SEGS) & 1) ^ 1, abort, WL)) { ok = false; break; }
+                    if (lane == 0) {
+                        volatile Seg& to = segs[told % SEGS];
+                        to.t0 = g.t0, to.t1 = g.t1;
+                        if (more) to.b = g.b, to.head = g.head, to.rt = g.rt, to.rows = g.rows, to.n = g.n, to.keys = g.keys, to.tiles = g.tiles, to.item = g.item;
+                        mbar_arrive(seg_full(told % SEGS));
+                    }
+                    __syncwarp();
                 }
                 if (!ok) break;
                 const int tiles = segs[seg % SEGS].t1 - segs[seg % SEGS].t0;
                 if (tiles == 0) break;
-                for (int t = 0; t < tiles && ok; t++) {
-                    pass();
-                    pass();
-                    if (t == 0 && ok) {
-                        ok = mbar_wait(q_landed, seg & 1, abort, WL);
+                for (int t = 0; t < tiles; t++, tile++) {
+                    if (!(ok = pass(false)) || !(ok = pass(true))) break;
+                    if (t == 0) {
+                        if (!(ok = warp_wait(q_landed, seg & 1, abort, WL))) break;
                         proxy_fence();
-                        mbar_arrive(q_full);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(q_full);
                     }
                 }
             }
@@ -1066,18 +1171,35 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
     if (blockIdx.z == 0 && warp == 0 && a.lse) a.lse[o_row] = l == 0.f ? NONE : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-template <int D, int TYPE, int STORE, int MT, int QR>
-static int launch(fvs_stream_t stream, Args a) {
+// the tensor maps of a 16-bit cache; false where tensor copies cannot take it
+static bool make_maps(const fvs_kv_cache& c, Maps& maps, int& box) {
+    box = 64;
+    while (c.page % box) box /= 2;
+    const EncodeTiledFn encode = encode_fn();
+    if (box < 8 || !encode || c.slot_stride < 1 || c.head_stride < 1 || c.page_stride < 1) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.dim, (cuuint64_t)c.page, (cuuint64_t)c.heads, (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.slot_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t tile[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = c.type == FVS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    for (int i = 0; i < 2; i++)
+        if (encode(i ? &maps.v : &maps.k, type, 4, i ? c.v : c.k, dims, strides, tile, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    return true;
+}
+
+template <int D, int TYPE, int STORE, int MT, int QR, bool BOXES>
+static int launch(fvs_stream_t stream, Args a, const Maps& maps) {
     using S = Shape<D, STORE, MT, QR>;
     constexpr int RT = ROWS * MT;
     const int ctas = fvs_sm_count() * S::CTAS;
-    const void* f = (const void*)tree_kernel<D, TYPE, STORE, MT, QR>;
+    const void* f = (const void*)tree_kernel<D, TYPE, STORE, MT, QR, BOXES>;
     cudaError_t e = fvs_ensure_smem(f, S::BYTES);
     if (e != cudaSuccess) return (int)e;
     a.wait_limit = pipeline_wait_limit();
     a.desc = (int32_t*)a.work;
     a.work = a.work + 8 * ctas;
-    tree_kernel<D, TYPE, STORE, MT, QR><<<ctas, S::THREADS, S::BYTES, stream>>>(a);
+    tree_kernel<D, TYPE, STORE, MT, QR, BOXES><<<ctas, S::THREADS, S::BYTES, stream>>>(a, maps);
     if (int rc = fvs_launch_status()) return rc;
     const int rows = a.nodes * a.group;
     cudaLaunchConfig_t cfg = {};
@@ -1097,18 +1219,20 @@ static int launch(fvs_stream_t stream, Args a) {
 
 // kernels over heads of D elements, by the rows of an item: 256 at a time where there are more than 128, queries of 64 where
 // there are no more (heads wider than 128: always 128)
-template <int D>
-int launch_types(fvs_stream_t stream, const Args& a, int type) {
+template <int D, int TYPE, int STORE, bool BOXES>
+static int launch_rows(fvs_stream_t stream, const Args& a, const Maps& maps) {
     constexpr bool narrow = D <= 128;
-    const bool i8 = a.c.type == FVS_I8;
     const int rows = a.nodes * a.group;
-#define FVS_TREE(T, ST)                                                               \
-    (narrow && rows > ROWS ? launch<D, T, ST, narrow ? 2 : 1, ROWS>(stream, a)        \
-     : narrow && rows <= 64 ? launch<D, T, ST, 1, narrow ? 64 : ROWS>(stream, a)      \
-                            : launch<D, T, ST, 1, ROWS>(stream, a))
-    if (type == FVS_F16) return i8 ? FVS_TREE(FVS_F16, FVS_I8) : FVS_TREE(FVS_F16, FVS_F16);
-    return i8 ? FVS_TREE(FVS_BF16, FVS_I8) : FVS_TREE(FVS_BF16, FVS_BF16);
-#undef FVS_TREE
+    if (narrow && rows > ROWS) return launch<D, TYPE, STORE, narrow ? 2 : 1, ROWS, BOXES>(stream, a, maps);
+    if (narrow && rows <= 64) return launch<D, TYPE, STORE, 1, narrow ? 64 : ROWS, BOXES>(stream, a, maps);
+    return launch<D, TYPE, STORE, 1, ROWS, BOXES>(stream, a, maps);
+}
+template <int D>
+int launch_types(fvs_stream_t stream, Args a, int type) {
+    Maps maps = {};
+    if (a.c.type == FVS_I8) return type == FVS_F16 ? launch_rows<D, FVS_F16, FVS_I8, false>(stream, a, maps) : launch_rows<D, FVS_BF16, FVS_I8, false>(stream, a, maps);
+    if (make_maps(a.c, maps, a.box)) return type == FVS_F16 ? launch_rows<D, FVS_F16, FVS_F16, true>(stream, a, maps) : launch_rows<D, FVS_BF16, FVS_BF16, true>(stream, a, maps);
+    return type == FVS_F16 ? launch_rows<D, FVS_F16, FVS_F16, false>(stream, a, maps) : launch_rows<D, FVS_BF16, FVS_BF16, false>(stream, a, maps);
 }
 
 }  // namespace tree

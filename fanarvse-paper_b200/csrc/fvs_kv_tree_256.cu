@@ -4,7 +4,7 @@
 namespace fvs {
 namespace kv {
 namespace tree {
-template int launch_types<256>(fvs_stream_t, const Args&, int);
+template int launch_types<256>(fvs_stream_t, Args, int);
 }
 }  // namespace kv
 }  // namespace fvs
