@@ -375,3 +375,90 @@ def test_compact_refusals_and_empty_calls(kv):  # noqa: F811
     cache.compact(t, n, ints(np.zeros((3, 0))))
     cache.compact(t[:0], n[:0], p[:0])
     assert torch.equal(cache.k, k0)
+
+
+# ------------------------------------------------------------------------------------------------ together
+
+def test_a_step_as_it_is_used(kv, drafts):  # noqa: F811
+    """Two steps of append with norm, tree attention, verification and compaction, eagerly and in one captured graph, against the
+    oracles one after the other."""
+    g, rng = torch.Generator().manual_seed(20), np.random.default_rng(20)
+    B, heads, group, dim, page, nodes, vocab = 5, 2, 4, 128, 16, 9, 301
+    hq = heads * group
+    shape = [int(rng.integers(-1, i)) if i else -1 for i in range(nodes)]
+    lens0 = [30, 0, 77, 16, 5]
+    table, pages = full_table([n + 3 * nodes for n in lens0], page, g)
+    start = make_cache(kv, pages, heads, page, dim, BF16, g)
+    norm = tuple((1 + 0.2 * torch.randn(dim, generator=g)).to(DEV, BF16) for _ in range(2))
+    cs = rope(200, dim, g)
+    parents, depth = ints(shape), [0] * nodes
+    for i, p in enumerate(shape):
+        depth[i] = depth[p] + 1 if p >= 0 else 0
+    table, depth, seq = table.to(DEV), ints(depth), ints(np.repeat(np.arange(B), nodes))
+    fused = [(torch.randn(B * nodes, hq + 2 * heads, dim, generator=g)).to(DEV, BF16) for _ in range(2)]
+    logits = torch.randn(B, nodes + 1, vocab, generator=g).to(DEV)
+    draft = torch.softmax(logits + 0.5 * torch.randn(B, nodes + 1, vocab, generator=g).to(DEV), -1)
+    tokens = [drawn(draft, np.tile(shape, (B, 1)), g) for _ in range(2)]
+    u = [torch.rand(B, nodes + 1, generator=g).to(DEV) for _ in range(2)]
+    mix = torch.randn(hq * dim, vocab, generator=g).to(DEV) / 8
+
+    def step(cache, lens, i):
+        x = fused[i]
+        at = (lens[:, None] + torch.arange(nodes, dtype=torch.int32, device=DEV)).view(-1)
+        q = cache.append(x[:, hq:hq + heads], x[:, hq + heads:], table, at, seq=seq, pos=(lens[:, None] + depth).view(-1), rope=cs,
+                         q=x[:, :hq], norm=norm)
+        out, lse = cache.attend_tree(q.view(B, nodes, hq, dim), table, lens, parents)
+        behind = torch.cat([logits[:, :1], logits[:, 1:] + out.reshape(B, nodes, -1).float() @ mix], 1)
+        target = torch.softmax(behind, -1)
+        path, kept, token = drafts.verify(target, parents, tokens[i], u[i], draft=draft)
+        before = cache.k.clone(), cache.v.clone()
+        cache.compact(table, lens, path)
+        return dict(q=q, out=out, lse=lse, target=target, path=path, kept=kept, token=token, k=before[0], v=before[1], lens=lens + kept)
+
+    fresh = lambda: kv.PagedKV(start.k.clone(), start.v.clone())  # noqa: E731
+    eager, captured = fresh(), fresh()
+    lens, got = ints(lens0), []
+    for i in range(2):
+        got.append(step(eager, lens, i))
+        lens = got[-1]["lens"]
+    torch.cuda.synchronize()
+    first = ints(lens0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one = step(captured, first, 0)
+        two = step(captured, one["lens"], 1)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, (one, two)):
+        assert all(torch.equal(a[name], b[name]) for name in a)
+    assert torch.equal(eager.k, captured.k) and torch.equal(eager.v, captured.v)
+    eager.check_status()
+    lens = np.array(lens0)
+    for i, s in enumerate(got):
+        k, v = c(s["k"]), c(s["v"])
+        eo, el, pv, _ = O.attend_tree(c(s["q"]).reshape(B, nodes, hq, dim), k, v, c(table), lens, np.tile(shape, (B, 1)), None, dim ** -0.5)
+        assert np.abs(c(s["out"]) - eo).max() <= 2.0 ** -8 * np.abs(eo).max() + 2.0 ** -14 * pv.max()
+        ep, ek, et = O.verify(c(s["target"]), np.tile(shape, (B, 1)), c(tokens[i]), c(u[i]), c(draft))
+        np.testing.assert_array_equal(c(s["path"]), ep)
+        np.testing.assert_array_equal(c(s["token"]), et)
+        want = O.compact(k, c(table), lens, ep, page)
+        after = c(got[i + 1]["k"]) if i == 0 else c(eager.k)
+        stay = np.ones(k.shape, bool)
+        if i == 0:                                          # the next step has appended behind its own start
+            for b in range(B):
+                for t in range(int(lens[b] + ek[b]), int(lens[b] + ek[b] + nodes)):
+                    stay[c(table)[b][t // page], :, t % page] = False
+        np.testing.assert_array_equal(after[stay], want[stay])
+        lens = lens + ek
+
+
+def test_example_answers_with_drafts():
+    import importlib.util
+    import os
+
+    from conftest import REPO
+    spec = importlib.util.spec_from_file_location("answer_with_drafts", os.path.join(REPO, "examples", "answer_with_drafts.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    worst, taken = m.main(steps=4)
+    assert worst < 2 ** -7 and taken > 0

@@ -340,3 +340,47 @@ def test_tree_waits_that_run_out(kv):  # noqa: F811
     finally:
         L.lib().fvs_set_wait_limit(old)
     check_tree(cache, q, table, n, parents)
+
+
+def test_tree_two_streams_at_once(kv):  # noqa: F811
+    """Calls of different shapes side by side, and workspaces given back between calls."""
+    g, rng = torch.Generator().manual_seed(14), np.random.default_rng(14)
+    sides = []
+    for B, nodes, group, longest in ((1, 64, 4, 9000), (7, 6, 2, 900)):
+        cache, q, table, n = setup(kv, list(rng.integers(1, longest, B)), nodes, 2, group, 16, 128, BF16, BF16, g)
+        sides.append((cache, q, table, n, ints(some_trees(B, nodes, rng)), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for i in range(10):
+        for cache, q, table, n, parents, stream in sides:
+            with torch.cuda.stream(stream):
+                got.append(cache.attend_tree(q, table, n, parents))
+        if i == 5:
+            kv.release_workspaces()
+    torch.cuda.synchronize()
+    for i, (cache, q, table, n, parents, _) in enumerate(sides):
+        check_tree(cache, q, table, n, parents, got=got[i])
+        assert all(torch.equal(x[0], got[i][0]) and torch.equal(x[1], got[i][1]) for x in got[i::2])
+
+
+@pytest.mark.parametrize("page", [8, 24, 64, 192])
+@pytest.mark.parametrize("dim", [64, 96, 192])
+def test_tree_boxes_of_a_page(kv, page, dim):  # noqa: F811
+    """Tensor copies of 8 to 64 keys, token-major memory, pages behind one another in a larger tensor, a hole in each box's place."""
+    g, rng = torch.Generator().manual_seed(page), np.random.default_rng(page)
+    lens, nodes = [200, 63, 65, 1, 511], 7
+    cache, q, table, n = setup(kv, lens, nodes, 2, 3, page, dim, BF16, BF16, g, token_major=True)
+    room = torch.full((cache.pages, 5, page + 3, dim + 8), float("nan"), dtype=BF16, device=DEV)
+    wide = []
+    for x in (cache.k, cache.v):
+        view = room.clone()[:, 1:3, 2:2 + page, 8:]
+        view.copy_(x)
+        wide.append(view)
+    holes = table.clone()
+    holes[0, ::3] = -1
+    holes[0, 200 // page:] = table[0, 200 // page:]
+    parents = ints(some_trees(len(lens), nodes, rng))
+    check_tree(cache, q, holes, n, parents)
+    a = cache.attend_tree(q, holes, n, parents)
+    b = kv.PagedKV(*wide).attend_tree(q, holes, n, parents)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
