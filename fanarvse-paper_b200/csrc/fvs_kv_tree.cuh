@@ -5,16 +5,19 @@
 // nodes * (hq / heads), so that keys and values are read once for all of them.  With 4 rows * dim flops per 4 * dim bytes of a
 // 16-bit key and value, memory bounds a call up to about 250 rows and the matrix instructions above that.
 //
-// A CTA per SM, a share of equal cost each of all items (sequence, key head, up to 128 * MT rows), cut anywhere between
-// tiles of KEYS keys; what is cut goes through the workspace and join_kernel.  Inside a CTA, a stream of tiles:
-//   producer warps (4): look up each key's page and copy its row of k and of v into a ring of slots, in the layout of a
-//     128-byte swizzled tile whatever the page size; a key that is not there becomes zeros.  int8 codes are widened to 16 bits
-//     on the way (exact), their scales go beside the tile.
-//   one thread of a warp issues the products: S = Q K^T into one of two TMEM buffers, and, when the rows' weights lie there
-//     in place of S, O += P V; the next tile's S is issued before this tile's O, so that the exponentials overlap both.
-//   softmax warpgroups (W), a thread per row: maximum, weights, sum.  With 128 rows (MT = 1) two of them take turns at the
-//     tiles, each with an O of its own, added at the end; with 256 rows (MT = 2) each has its rows; heads wider than 128
-//     leave TMEM for one O only.
+// One or two CTAs an SM (Shape), each with a share of equal cost of all items (sequence, key head, up to 256 rows), cut anywhere
+// between tiles of KEYS keys; what is cut goes through the workspace and join_kernel.  Inside a CTA, a stream of tiles:
+//   producers: keys and values into a ring of slots in the layout of a 128-byte swizzled tile.  16-bit rows come by tensor
+//     copies, a box for each piece of a page; pages of other than a multiple of 8 slots by 16-byte copies; int8 codes are
+//     widened to 16 bits on the way (exact), their scales go beside the tile.  Flags of the keys that are there go beside it.
+//   scheduler and relay (a warp): writes the CTA's segments ahead, and passes filled slots on behind a proxy fence.
+//   matrix instructions (a thread for each softmax warpgroup): S = Q K^T into TMEM, and, when the rows' weights lie there in
+//     place of S, O += P V; where TMEM has room a tile's S is issued before the O of the tile before.
+//   softmax warpgroups, a thread per row: weights and their sum; at a segment's end the output or the share of one.
+// What bounds it: up to 128 rows the copies' latency and a segment's beginning and end (64 ragged requests of 64 rows: 89 us
+// where the bytes take 48, a rate of 3.6 TB/s); with 256 rows the softmax warps, whose 11 instructions and 2 exponentials
+// for each pair of scores take 660 cycles for 32 columns of two warps of a quarter SM when they run alone (131000 tokens
+// under 64 nodes: 219 us where memory takes 84 and the matrix instructions with two parts of each weight 126).
 //
 // Rounding: scores, maxima, sums and O are fp32.  A weight enters the second product as two parts of the 16-bit type (its
 // rounded value and the rounded rest): 17 bits with bf16, 22 with fp16, where one part would double the error that the output's
@@ -35,11 +38,9 @@ using namespace fvs::tcg;
 constexpr int ROWS = 128;     // rows of a matrix instruction
 constexpr int INFO = 8;       // tiles whose keys' flags and scales are held
 constexpr int SEGS = 4;       // segments that the scheduler is ahead
-constexpr int ITEM_KEYS = 256; // cost of an item: its queries' copy and its output, as that of so many keys (64 ragged requests:
-                               // 119 us with 128, 112 with 384, 107 with 256)
+constexpr int ITEM_KEYS = 256;  // cost of an item, its queries' copy and its output, in keys (64 ragged requests: 90 us, with 384 91)
 constexpr int LEAST_COST = 4;  // of a CTA's share, in tiles
-constexpr int GAVE_UP = 2;    // status bit: a bounded wait ran out
-
+constexpr int GAVE_UP = 2;     // status bit: a bounded wait ran out
 constexpr int SEG_BYTES = 48;
 
 struct Args {
@@ -62,19 +63,17 @@ struct Maps {  // of keys and values: element, slot, head, page
     CUtensorMap k, v;
 };
 
-
-
 // How a kernel uses an SM, by head size and 128 * MT rows of an item.
 template <int D, int STORE, int MT, int QR>
 struct Shape {
     static_assert(MT == 1 || D <= 128, "tensor memory holds one O of a wide head");
     static_assert(QR == ROWS || (MT == 1 && D <= 128), "fewer rows of queries");
     // CTAs of an SM: with 128 rows of heads up to 128 two, whose beginnings and ends overlap (one CTA whose two softmax
-    // warpgroups took turns at the tiles took 113 us where this takes 90, at 64 ragged requests of 64 rows)
+    // warpgroups took turns at the tiles took 115 us where this took 107, at 64 ragged requests of 64 rows)
     static constexpr int CTAS = MT == 1 && D <= 128 ? 2 : 1;
     static constexpr int W = MT;  // softmax warpgroups
-    // keys of a tile: 128 where the codes' widening is the slower part (403 us instead of 445 at 24 long int8 contexts under
-    // 32 nodes), else 64, whose scores are computed a tile ahead (229 instead of 254 at 131000 tokens under 64 nodes)
+    // keys of a tile: 128 where the codes' widening is the slower part (403 us where 64 took 445, at 24 long int8 contexts under
+    // 32 nodes), else 64, whose scores are computed a tile ahead (229 where 128 took 254, at 131000 tokens under 64 nodes)
     static constexpr int KEYS = MT == 2 && STORE == FVS_I8 ? 128 : 64;
     static constexpr int COLUMNS = 512 / CTAS;                                       // of tensor memory
     static constexpr int BUFFERS = MT == 2 ? 256 / KEYS : CTAS == 2 ? 2 : 4;         // of scores in it
@@ -313,9 +312,10 @@ __device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
 }
 
 // QR: rows of queries that shared memory holds, 64 where an item has no more: the matrix instructions read 128, the others of
-// whatever lies behind (their scores and outputs go to rows that nobody reads), and the ring has a slot more
+// whatever lies behind (their scores and outputs go to rows that nobody reads), and the ring has a slot more (64 ragged requests:
+// 90 us instead of 93)
 // BOXES: 16-bit rows come by tensor copies (pages of a multiple of 8 slots); else by the producers' lanes, 16 bytes each, whose
-// traffic delays every wait on a barrier (104 us instead of 70 at 64 ragged requests)
+// traffic delays every wait on a barrier (104 us instead of 88 at 64 ragged requests)
 template <int D, int TYPE, int STORE, int MT, int QR, bool BOXES>
 __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STORE, MT, QR>::CTAS)
     tree_kernel(Args a, const __grid_constant__ Maps maps) {
@@ -1109,7 +1109,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
 
 // Adds the shares of the items that were cut.  Block (c, 32 rows, 16 columns): the item that begins in CTA c and goes on in
 // the CTAs behind it, each of which left one share.  The shares are read once, from L2 mostly: many small blocks, with all
-// of a thread's loads on the way together (8 blocks of 20 shares each took 57 us where 4096 of them take 5).
+// of a thread's loads on the way together (a block of all columns for each 32 rows took 57 us at 20 shares of 8 items).
 constexpr int JOIN_COLS = 16;
 template <int D, int TYPE, int RT>
 __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
@@ -1230,8 +1230,14 @@ static int launch_rows(fvs_stream_t stream, const Args& a, const Maps& maps) {
 template <int D>
 int launch_types(fvs_stream_t stream, Args a, int type) {
     Maps maps = {};
+    // what the other copies and the queries hold of an address: 32 bits of 16 bytes
+    const int64_t last = (a.c.pages - 1) * a.c.page_stride + (a.c.heads - 1) * a.c.head_stride + (a.c.page - 1) * a.c.slot_stride;
+    const int64_t last_q = (a.tb.seqs - 1) * a.q_seq + (a.nodes - 1) * a.q_node + (a.hq - 1) * a.q_head, most = 0xfffffff0ll;
+    const bool small = last / (a.c.type == FVS_I8 ? 16 : 8) < most;
+    if (last_q / 8 >= most || (a.c.type == FVS_I8 && !small)) return FVS_ERANGE;
     if (a.c.type == FVS_I8) return type == FVS_F16 ? launch_rows<D, FVS_F16, FVS_I8, false>(stream, a, maps) : launch_rows<D, FVS_BF16, FVS_I8, false>(stream, a, maps);
     if (make_maps(a.c, maps, a.box)) return type == FVS_F16 ? launch_rows<D, FVS_F16, FVS_F16, true>(stream, a, maps) : launch_rows<D, FVS_BF16, FVS_BF16, true>(stream, a, maps);
+    if (!small) return FVS_ERANGE;
     return type == FVS_F16 ? launch_rows<D, FVS_F16, FVS_F16, false>(stream, a, maps) : launch_rows<D, FVS_BF16, FVS_BF16, false>(stream, a, maps);
 }
 

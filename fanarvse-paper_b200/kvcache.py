@@ -3,8 +3,8 @@
 The ids that `search` returns name passages; with each passage's keys and values in pages of a `PagedKV`, they become
 rows of a page table (`passage_table`), and the model's next token attends over these pages, then over its own.
 `append` stores new tokens' keys and values with the position rotation on the way, `attend` is the attention of one new
-token per sequence, `read` gives stored rows back as floating point.  The reference has no counterpart: it ends with
-the ids.
+token per sequence, `read` gives stored rows back as floating point.  Drafted tokens: `append` with the norms of the heads,
+`attend_tree` and `compact`, with `drafts.verify` between them.  The reference has no counterpart: it ends with the ids.
 
 Every call runs on the current torch stream, neither synchronises nor reads device memory on the host, and can be
 captured into a CUDA graph.  The operators have no gradients and refuse inputs that require one.  Wrong arguments raise;
@@ -268,7 +268,8 @@ class PagedKV:
         A node sees the visible ones of the first lens [sequences] logical tokens, its ancestors and itself; counts int32
         [sequences]: the nodes that a sequence has (default: all).  Returns (out like q, lse fp32 [sequences, nodes, query
         heads]): zeros and -inf where nothing is visible and for nodes that a sequence does not have.  One node is
-        `attend` with a length of lens + 1."""
+        `attend` with a length of lens + 1.  Hidden slots may hold anything; the nodes' own keys and values are finite (one
+        that is not may reach nodes that do not see it)."""
         shape = q.shape
         if not (len(shape) == 4 and shape[3] == self.dim and q.get_device() == self._index):
             raise ValueError(f"q is [sequences, nodes, heads, {self.dim}] on the cache's GPU")
@@ -362,7 +363,7 @@ class PagedKV:
 
 
 def release_workspaces():
-    """Gives the workspaces of attend and attend_tree back to torch's allocator (8 to 29 MB for each stream that attended, 10
+    """Gives the workspaces of attend and attend_tree back to torch's allocator (8 to 29 MB for each stream that attended, 20
     to 39 MB for trees; a stream's next call makes its own again).  Calls in flight keep what they have: the memory is used
     again on its own stream only."""
     _WORK.clear()

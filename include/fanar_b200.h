@@ -542,7 +542,8 @@ int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, cons
  * nodes from counts[b] on.  Places before lens[b] that are not there may hold anything, and so may every place behind the
  * nodes; the nodes' own rows are finite (one that is not may reach nodes that do not see it).
  * A length above the table's row (or below 0) is cut to it; where the nodes reach past the row those places are not
- * there, with FVS_KV_BAD_INDEX.  nodes <= FVS_TREE_NODES (FVS_ERANGE above).
+ * there, with FVS_KV_BAD_INDEX.  nodes <= FVS_TREE_NODES (FVS_ERANGE above).  k, v and q span at most 64 GB each
+ * (FVS_ERANGE; 16-bit caches whose pages are a multiple of 8 slots any size).
  * work: fvs_kv_attend_tree_work(dim, nodes * (hq / heads)) bytes of device memory, 16-byte aligned, of any contents.  Calls that
  * may run at the same time need their own.
  */

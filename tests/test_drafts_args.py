@@ -65,6 +65,14 @@ def test_attend_tree_refuses(L, change, rc):
     assert attend_tree(L, cache(L), **change) == rc
 
 
+def test_attend_tree_spans(L):
+    """What 32 bits of 16 bytes cannot address is refused before any launch."""
+    far = dict(pages=2 ** 31 - 1, page_stride=2 * 16 * 64)
+    assert attend_tree(L, cache(L, type=L.I8, k_scale=64, v_scale=64, scale_page_stride=32, scale_head_stride=16, scale_slot_stride=1, **far)) == -2
+    assert attend_tree(L, cache(L, page=7, **far)) == -2
+    assert attend_tree(L, cache(L), qs=2 ** 36) == -2
+
+
 def test_tree_workspace_size(L):
     f = L.lib().fvs_kv_attend_tree_work
     assert f(0, 4) == -1 and f(64, -1) == -1 and f(512, 4) == -2
