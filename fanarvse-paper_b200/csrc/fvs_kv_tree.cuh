@@ -1107,67 +1107,78 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     if (*abort && tid == 0) atomicOr(a.c.status, GAVE_UP);
 }
 
-// Adds the shares of the items that were cut.  Block (c, 32 rows, 16 columns): the item that begins in CTA c and goes on in
-// the CTAs behind it, each of which left one share.  The shares are read once, from L2 mostly: many small blocks, with all
-// of a thread's loads on the way together (a block of all columns for each 32 rows took 57 us at 20 shares of 8 items).
-constexpr int JOIN_COLS = 16;
+// Adds the shares of the items that were cut.  Block (c, 32 rows, 32 columns): the item that begins in CTA c and goes on in
+// the CTAs behind it, each of which left one share.  The shares are read once, from L2 mostly, and what bounds it is the
+// latency of its loads behind one another (descriptors, maxima and sums, O).
+constexpr int JOIN_COLS = 32;
 template <int D, int TYPE, int RT>
 __global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
-    extern __shared__ float weight[];  // [shares][32]
+    constexpr int COLS = JOIN_COLS / 8;  // of a thread
+    extern __shared__ float tops[];      // maxima [shares][32], no share's -infinity
     __shared__ float s_m[8][32], s_l[8][32];
     __shared__ int s_upto;
+    __shared__ uint8_t s_has[512];
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) s_upto = ctas;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the shares are still computed
-    const int32_t* d = a.desc + 8 * c;
-    const int b = d[0], item = d[1], head = d[2], rt = d[3], rows = d[4];
+    const int4 d = *reinterpret_cast<const int4*>(a.desc + 8 * c);
+    const int b = d.x, item = d.y, head = d.z, rt = d.w, rows = a.desc[8 * c + 4];
     const int row = blockIdx.y * 32 + lane;
+    __syncthreads();
     if (b < 0 || (int)blockIdx.y * 32 >= rows) return;
     // the CTAs behind that have a share of it: none between them has another item, some may have nothing at all
-    auto has = [&](int x) { return x == c || (a.desc[8 * x + 5] == b && a.desc[8 * x + 6] == item); };
-    if (threadIdx.x == 0) s_upto = ctas;
-    __syncthreads();
-    for (int x = c + 1 + (int)threadIdx.x; x < ctas; x += 256)
-        if (!has(x) && a.desc[8 * x + 7] != 0) atomicMin(&s_upto, x);
+    for (int x = c + (int)threadIdx.x; x < ctas; x += 256) {
+        const int4 e = *reinterpret_cast<const int4*>(a.desc + 8 * x + 4);
+        const bool has = x == c || (e.y == b && e.z == item);
+        s_has[x - c] = has;
+        if (!has && e.w != 0) atomicMin(&s_upto, x);
+    }
     __syncthreads();
     const int shares = s_upto - c;
     auto part = [&](int i) { return a.work + (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * RT * (D + 2); };
     constexpr float NONE = -__builtin_huge_valf();
-    float m = NONE;
+    float m = NONE, l = 0.f;
+#pragma unroll 2
     for (int i = warp; i < shares; i += 8) {
-        const float x = has(c + i) && row < rows ? part(i)[D * RT + row] : NONE;
-        weight[i * 32 + lane] = x;
-        m = fmaxf(m, x);
+        const bool there = s_has[i] && row < rows;
+        const float x = there ? part(i)[D * RT + row] : NONE, y = there ? part(i)[(D + 1) * RT + row] : 0.f;
+        tops[i * 32 + lane] = x;
+        const float top = fmaxf(m, x);
+        l = l * (m == top ? 1.f : exp2_of(m - top)) + y * (x == top ? 1.f : exp2_of(x - top));
+        m = top;
     }
     s_m[warp][lane] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++) m = fmaxf(m, s_m[w][lane]);
-    float l = 0.f;
-    for (int i = warp; i < shares; i += 8) {
-        const float x = weight[i * 32 + lane], by = x == m ? 1.f : exp2_of(x - m);
-        const bool there = has(c + i) && row < rows;
-        weight[i * 32 + lane] = there ? by : 0.f;
-        if (there) l = fmaf(part(i)[(D + 1) * RT + row], by, l);
-    }
     s_l[warp][lane] = l;
     __syncthreads();
+    m = NONE;
+#pragma unroll
+    for (int w = 0; w < 8; w++) m = fmaxf(m, s_m[w][lane]);
     l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; w++) l += s_l[w][lane];
+    for (int w = 0; w < 8; w++) l = fmaf(s_l[w][lane], s_m[w][lane] == m ? 1.f : exp2_of(s_m[w][lane] - m), l);
     if (row >= rows) return;
     const int at = rt * RT + row, node = at / a.group, h = at - node * a.group;
     const int64_t o_row = ((int64_t)b * a.nodes + node) * a.hq + head * a.group + h;
-    const int col = blockIdx.z * JOIN_COLS + warp * 2;
-    float o0 = 0.f, o1 = 0.f;
-#pragma unroll 8
+    const int col = blockIdx.z * JOIN_COLS + warp * COLS;
+    float o[COLS] = {};
+#pragma unroll 4
     for (int i = 0; i < shares; i++) {
-        const float by = weight[i * 32 + lane];
+        const float top = tops[i * 32 + lane], by = top == m ? 1.f : exp2_of(top - m);
         const float* p = part(i) + col * RT + row;
-        const float x = p[0], y = p[RT];  // of a CTA without a share: anything, and not added
-        if (by != 0.f) o0 = fmaf(x, by, o0), o1 = fmaf(y, by, o1);
+        float x[COLS];
+#pragma unroll
+        for (int j = 0; j < COLS; j++) x[j] = p[j * RT];  // of a CTA without a share: anything, and not added
+#pragma unroll
+        for (int j = 0; j < COLS; j++)
+            if (top != NONE && by != 0.f) o[j] = fmaf(x[j], by, o[j]);
     }
     const float by = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint32_t*>((uint16_t*)a.out + o_row * D + col) = l == 0.f ? 0u : Elem<TYPE>::down(o0 * by, o1 * by);
+    uint32_t packed[COLS / 2];
+#pragma unroll
+    for (int j = 0; j < COLS; j += 2) packed[j / 2] = l == 0.f ? 0u : Elem<TYPE>::down(o[j] * by, o[j + 1] * by);
+    uint16_t* out = (uint16_t*)a.out + o_row * D + col;
+#pragma unroll
+    for (int j = 0; j < COLS / 2; j++) reinterpret_cast<uint32_t*>(out)[j] = packed[j];
     if (blockIdx.z == 0 && warp == 0 && a.lse) a.lse[o_row] = l == 0.f ? NONE : (m + log2f(l)) * 0.6931471805599453f;
 }
 
