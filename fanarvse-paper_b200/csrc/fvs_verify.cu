@@ -65,75 +65,60 @@ struct Shared {
     double qx[NODES];
     float u[NODES + 1];
     int parent[NODES], tok[NODES];
-    double mass[NODES + 1];  // m_0 .. m_k of the present row
     int refused[NODES];      // tokens refused in it (drafts without probabilities)
     double warp[WARPS], scan[WARPS];
     double total[2][CTAS];   // of each CTA, two passes in turn
     int found, positive;
 };
 
-// r_k of element v of the present row; m_0 = 1, and a difference of two fp32 numbers is exact in fp64
+// r_k of element v of the present row: as every m_j and q is at least 0, max(.. max(p - m_0 q, 0) .. - m_{k-1} q, 0) is max(p -
+// M q, 0) with M their sum.  M is 1 for k = 1, and a difference of two fp32 numbers is exact in fp64.
+__device__ __forceinline__ double rest_of(float p, float q, double M) {
+    const double r = fma(-M, (double)q, (double)p);
+    return r > 0.0 ? r : 0.0;
+}
 template <bool DRAFT>
-__device__ __forceinline__ double rest(float p, float q, int v, const Shared& s, int k) {
-    if constexpr (DRAFT) {
-        double r = k == 0 ? (double)p : p > q ? (double)p - (double)q : 0.0;
-        for (int j = 1; j < k; j++) r = fmax(__dsub_rn(r, __dmul_rn(s.mass[j], (double)q)), 0.0);  // as written, not one operation
-        return r;
-    } else {
-        for (int j = 0; j < k; j++) p = v == s.refused[j] ? 0.f : p;
-        return p;
-    }
+__device__ __forceinline__ double rest(float p, float q, int v, const Shared& s, int k, double M) {
+    if (DRAFT) return rest_of(p, q, M);
+    for (int j = 0; j < k; j++) p = v == s.refused[j] ? 0.f : p;
+    return p;
 }
 
-// sum of r_n over the 16 bytes from element v on
-template <typename T, bool DRAFT>
-__device__ __forceinline__ double sum_of(const uint4& praw, const uint4& qraw, int v, const Shared& s, int n) {
+// sum of r_n over N times 16 bytes, the first of them from element v on, 32 lanes' vectors apart
+template <typename T, bool DRAFT, int N>
+__device__ __forceinline__ double sum_of(const uint4 (&praw)[N], const uint4 (&qraw)[N], int v, const Shared& s, int n, double M) {
     constexpr int VEC = 16 / sizeof(T);
-    const T *pe = reinterpret_cast<const T*>(&praw), *qe = reinterpret_cast<const T*>(&qraw);
-    float p[VEC], q[VEC];
+    float p[N * VEC], q[N * VEC];
     uint32_t most = 0;  // above every number's bits where something is negative or not finite
 #pragma unroll
-    for (int e = 0; e < VEC; e++) {
-        p[e] = (float)pe[e];
-        most = max(most, __float_as_uint(p[e]));
+    for (int i = 0; i < N * VEC; i++) {
+        p[i] = (float)reinterpret_cast<const T*>(&praw[i / VEC])[i % VEC];
+        most = max(most, __float_as_uint(p[i]));
         if (DRAFT) {
-            q[e] = (float)qe[e];
-            most = max(most, __float_as_uint(q[e]));
+            q[i] = (float)reinterpret_cast<const T*>(&qraw[i / VEC])[i % VEC];
+            most = max(most, __float_as_uint(q[i]));
         }
     }
     if (__builtin_expect(most >= 0x7f800000u, 0)) {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            p[e] = sane(p[e]);
-            if (DRAFT) q[e] = sane(q[e]);
+        for (int i = 0; i < N * VEC; i++) {
+            p[i] = sane(p[i]);
+            if (DRAFT) q[i] = sane(q[i]);
         }
     }
-    double r[VEC];
-    if (DRAFT && n > 0) {
-#pragma unroll
-        for (int e = 0; e < VEC; e++) r[e] = p[e] > q[e] ? (double)p[e] - (double)q[e] : 0.0;
+    if (!DRAFT) {
 #pragma unroll 1
-        for (int j = 1; j < n; j++) {
-            const double mass = s.mass[j];
+        for (int j = 0; j < n; j++) {
+            const int at = s.refused[j] - v;
 #pragma unroll
-            for (int e = 0; e < VEC; e++) r[e] = fmax(__dsub_rn(r[e], __dmul_rn(mass, (double)q[e])), 0.0);
+            for (int i = 0; i < N * VEC; i++)
+                if (at == i / VEC * 32 * VEC + i % VEC) p[i] = 0.f;
         }
-    } else {
-        if (!DRAFT) {
-#pragma unroll 1
-            for (int j = 0; j < n; j++) {
-                const int at = s.refused[j] - v;
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (at == e) p[e] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; e++) r[e] = p[e];
     }
     double sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < VEC; e += 2) sum += r[e] + r[e + 1];
+    for (int i = 0; i < N * VEC; i += 2)
+        sum += DRAFT ? rest_of(p[i], q[i], M) + rest_of(p[i + 1], q[i + 1], M) : (double)p[i] + (double)p[i + 1];
     return sum;
 }
 
@@ -164,7 +149,7 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
     auto skew_of = [&](const T* row) { return (int)((uintptr_t)row / sizeof(T) % VEC); };
     auto span_of = [&](int skew) { return ((a.vocab + skew + VEC - 1) / VEC + ctas * WARPS - 1) / (ctas * WARPS); };
     // sums of r_n over the row behind `last`; ends with all of the cluster's threads having them
-    auto pass = [&](int n) {
+    auto pass = [&](int n, double M) {
         const T *p = target + (last + 1) * a.target.row, *q = draft + (last + 1) * a.draft.row;
         const int skew = skew_of(p), span = span_of(skew), lo = (rank * WARPS + warp) * span;
         const int hi = min((a.vocab + skew + VEC - 1) / VEC, lo + span);
@@ -179,8 +164,7 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
                 pv[i] = load(p, at, a.vocab, true);
                 qv[i] = both ? load(q, at, a.vocab, alike) : make_uint4(0, 0, 0, 0);
             }
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++) sum += sum_of<T, DRAFT>(pv[i], qv[i], (j0 + 32 * i) * VEC - skew, s, n);
+            sum += sum_of<T, DRAFT, AHEAD>(pv, qv, j0 * VEC - skew, s, n, M);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -198,7 +182,7 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
         return all;
     };
     cluster.sync();  // every CTA has begun and has its nodes
-    double mass = 1.0;
+    double mass = 1.0, M = 0.0;  // m_k, m_0 + .. + m_{k-1}
     for (int i = 0; i < nodes; i++) {  // children come after their parents
         if (s.parent[i] != last) continue;
         if ((double)s.u[i] * mass * s.qx[i] < s.left[i]) {
@@ -207,20 +191,18 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
             kept++;
             k = 0;
             mass = 1.0;
+            M = 0.0;
             summed = false;
             continue;
         }
-        __syncthreads();  // mass and refused of the pass before were read
-        if (tid == 0) {
-            s.mass[k] = mass;
-            s.refused[k] = s.tok[i];
+        if (!DRAFT) {
+            if (tid == 0) s.refused[k] = s.tok[i];
+            __syncthreads();
         }
-        __syncthreads();
-        const double m = pass(k + 1);
+        const double m = pass(k + 1, M + mass);
         turn ^= 1;
         summed = m > 0.0;
         if (m > 0.0) {
-            __syncthreads();
             for (int c = tid; c < nodes; c += THREADS) {
                 if (s.parent[c] != last) continue;
                 if (DRAFT)
@@ -229,6 +211,7 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
                     s.left[c] = 0.0;
             }
             __syncthreads();
+            M += mass;
             mass = m;
             total = m;
             k++;
@@ -236,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
     }
     if (!summed) {
         __syncthreads();
-        total = pass(k);
+        total = pass(k, M);
     } else {
         turn ^= 1;  // the buffer of the last pass
     }
@@ -283,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(Args a) {
             double x[RUN], sum = 0.0;
 #pragma unroll
             for (int j = 0; j < RUN; j++) {
-                x[j] = v + j < to ? rest<DRAFT>(value(p + v + j), DRAFT && k > 0 ? value(q + v + j) : 0.f, v + j, s, k) : 0.0;
+                x[j] = v + j < to ? rest<DRAFT>(value(p + v + j), DRAFT && k > 0 ? value(q + v + j) : 0.f, v + j, s, k, M) : 0.0;
                 sum += x[j];
             }
             double upto = sum;
