@@ -244,7 +244,6 @@ static void launch_append(fvs_stream_t stream, AppendArgs a, int type, bool halv
     }
 }
 
-
 // host: the checks that both entry points make; fills a (tokens 0: nothing to do)
 static inline int append_args(AppendArgs& a, const fvs_kv_cache* cache, int type, const void* k, int64_t k_token,
                               int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* q,

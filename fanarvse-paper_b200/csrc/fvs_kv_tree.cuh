@@ -14,8 +14,8 @@
 //   matrix instructions (a thread for each softmax warpgroup): S = Q K^T into TMEM, and, when the rows' weights lie there in
 //     place of S, O += P V; where TMEM has room a tile's S is issued before the O of the tile before.
 //   softmax warpgroups, a thread per row: weights and their sum; at a segment's end the output or the share of one.
-// What bounds it: up to 128 rows the copies' latency and a segment's beginning and end (64 ragged requests of 64 rows: 89 us
-// where the bytes take 48, a rate of 3.6 TB/s); with 256 rows the softmax warps, whose 11 instructions and 2 exponentials
+// What bounds it: up to 128 rows the copies' latency and a segment's beginning and end (64 ragged requests of 64 rows: 82 us
+// where the bytes take 48, a rate of 3.9 TB/s); with 256 rows the softmax warps, whose 11 instructions and 2 exponentials
 // for each pair of scores take 660 cycles for 32 columns of two warps of a quarter SM when they run alone (131000 tokens
 // under 64 nodes: 219 us where memory takes 84 and the matrix instructions with two parts of each weight 126).
 //
@@ -38,7 +38,7 @@ using namespace fvs::tcg;
 constexpr int ROWS = 128;     // rows of a matrix instruction
 constexpr int INFO = 8;       // tiles whose keys' flags and scales are held
 constexpr int SEGS = 4;       // segments that the scheduler is ahead
-constexpr int ITEM_KEYS = 256;  // cost of an item, its queries' copy and its output, in keys (64 ragged requests: 90 us, with 384 91)
+constexpr int ITEM_KEYS = 256;  // cost of an item, its queries' copy and its output, in keys (384: 64 ragged requests take 2 % longer)
 constexpr int LEAST_COST = 4;  // of a CTA's share, in tiles
 constexpr int GAVE_UP = 2;     // status bit: a bounded wait ran out
 constexpr int SEG_BYTES = 48;
@@ -75,6 +75,9 @@ struct Shape {
     // keys of a tile: 128 where the codes' widening is the slower part (403 us where 64 took 445, at 24 long int8 contexts under
     // 32 nodes), else 64, whose scores are computed a tile ahead (229 where 128 took 254, at 131000 tokens under 64 nodes)
     static constexpr int KEYS = MT == 2 && STORE == FVS_I8 ? 128 : 64;
+    // keys whose weights enter O together, while the softmax warps are at the next ones: half a tile (131000 tokens under 64
+    // nodes: 217 us, 220 with whole tiles), whole tiles with two CTAs an SM (64 ragged requests: 83 us, 89 with halves)
+    static constexpr int PART = CTAS == 2 ? KEYS : KEYS / 2;
     static constexpr int COLUMNS = 512 / CTAS;                                       // of tensor memory
     static constexpr int BUFFERS = MT == 2 ? 256 / KEYS : CTAS == 2 ? 2 : 4;         // of scores in it
     static constexpr int LEAD = BUFFERS == W ? 0 : 1;  // units whose scores are issued before a unit's outputs wait
@@ -86,7 +89,7 @@ struct Shape {
     static_assert(O0 + W * D <= COLUMNS, "tensor memory columns");
     // shared memory: queries, the ring, then barriers, the tiles' flags and scales, segments and masks
     static constexpr int Q = MT * QR * 128 * BLOCKS;
-    static constexpr int BARS = 88 * 8, INFO_BYTES = 16 + 2 * KEYS * 4, MASK_BYTES = W * ROWS * (KEYS / 32) * 4;
+    static constexpr int BARS = 96 * 8, INFO_BYTES = 16 + 2 * KEYS * 4, MASK_BYTES = W * ROWS * (KEYS / 32) * 4;
     static constexpr int MISC = BARS + INFO * INFO_BYTES + 64 + SEGS * SEG_BYTES + MASK_BYTES;
     static constexpr int FIT = ((CTAS == 2 ? 115712 : 232448) - 1024 - MISC - Q) / SLOT;
     static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
@@ -312,8 +315,8 @@ __device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
 }
 
 // QR: rows of queries that shared memory holds, 64 where an item has no more: the matrix instructions read 128, the others of
-// whatever lies behind (their scores and outputs go to rows that nobody reads), and the ring has a slot more (64 ragged requests:
-// 90 us instead of 93)
+// whatever lies behind (their scores and outputs go to rows that nobody reads), and the ring has a slot more (64 ragged requests
+// are 3 % faster)
 // BOXES: 16-bit rows come by tensor copies (pages of a multiple of 8 slots); else by the producers' lanes, 16 bytes each, whose
 // traffic delays every wait on a barrier (104 us instead of 88 at 64 ragged requests)
 template <int D, int TYPE, int STORE, int MT, int QR, bool BOXES>
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     tree_kernel(Args a, const __grid_constant__ Maps maps) {
     using S = Shape<D, STORE, MT, QR>;
     constexpr bool I8 = STORE == FVS_I8;
-    constexpr int KEYS = S::KEYS, BUFFERS = S::BUFFERS, PARTS = KEYS / 64, W = S::W, RT = ROWS * MT, SLOTS = S::SLOTS, LEAD = S::LEAD;
+    constexpr int KEYS = S::KEYS, BUFFERS = S::BUFFERS, PART = S::PART, PARTS = KEYS / PART, W = S::W, RT = ROWS * MT, SLOTS = S::SLOTS, LEAD = S::LEAD;
     constexpr int INFO_BYTES = S::INFO_BYTES, PRODUCERS = S::PRODUCERS;
     constexpr int VTYPE = I8 ? FVS_BF16 : TYPE;  // of weights and values
     // the most that 32 weights may add up to before their reference rises; over fp16 values they lie in the upper part of
@@ -339,8 +342,8 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     auto info_full = [&](int s) { return bars + 8 * (24 + s); };
     auto info_empty = [&](int s) { return bars + 8 * (32 + s); };
     auto s_full = [&](int u) { return bars + 8 * (80 + u % BUFFERS); };
-    auto p_full = [&](int u, int part) { return bars + 8 * (44 + u % BUFFERS * PARTS + part); };  // 64 keys
-    auto pv_half = [&](int u) { return bars + 8 * (84 + u % BUFFERS); };                            // of a tile of 128
+    auto p_full = [&](int u, int part) { return bars + 8 * (88 + u % BUFFERS * PARTS + part); };  // PART keys
+    auto pv_half = [&](int u) { return bars + 8 * (84 + u % BUFFERS); };
     auto pv_done = [&](int u) { return bars + 8 * (48 + u % BUFFERS); };
     auto round_of = [&](int u) { return (uint32_t)(u / BUFFERS) & 1u; };  // parity of unit u's phase of these
     auto seg_full = [&](int s) { return bars + 8 * (52 + s); };
@@ -700,7 +703,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
         }
         cp_async_wait_all();
     } else if (warp >= W_MMA) {
-        // A thread for each softmax warpgroup issues its matrix instructions: a unit's outputs (O += P V) 64 keys at a time as
+        // A thread for each softmax warpgroup issues its matrix instructions: a unit's outputs (O += P V) PART keys at a time as
         // its weights come, and right behind the last ones the next unit's scores (S = Q K^T), which take the weights'
         // place; instructions of one thread run in order.  An instruction is issued when the one before it has begun and a
         // single thread is slow, so what it need not wait for between instructions it does before or behind them.
@@ -766,7 +769,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                         if (part == 0 && !(ok = mbar_wait(full(vslot), vphase, abort, WL))) break;
                         tc_fence_after();
 #pragma unroll
-                        for (int i = 4 * part; i < 4 * part + 4; i++) {
+                        for (int i = PART / 16 * part; i < PART / 16 * (part + 1); i++) {
                             mma_ts(d, p + 32 * (i >> 1) + 8 * (i & 1), v + i * 128, id_o, x + i > 0);
                             mma_ts(d, p + 32 * (i >> 1) + 8 * (i & 1) + 16, v + i * 128, id_o, true);
                         }
@@ -944,7 +947,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                             const float to = need ? fmaxf(m, top) : m, by = m == to ? 1.f : exp2_of(m - to);
                             m = to;
                             l *= by;
-                            const bool half = PARTS == 2 && k >= 2;  // the tile's first 64 weights may be in O
+                            const bool half = PARTS == 2 && k >= PART / 32;  // the tile's first weights may be in O
                             if (any || half) {
                                 ok = ok && warp_wait(half ? pv_half(u) : pv_done(last), round_of(half ? u : last), abort, WL);
                                 tc_fence_after();
@@ -958,7 +961,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                                     tmem_st16(lanes + S::O0 + w * D + x, o);
                                 }
                             }
-                            if (k & 1) {  // the 32 weights before are not in O yet
+                            if (PART == 64 && (k & 1)) {  // the 32 weights before are not in O yet
 #pragma unroll 1
                                 for (int x = 0; x < 16; x += 8) {
                                     uint32_t hi[8], lo[8];
@@ -1021,11 +1024,11 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                             tmem_st8(s_tmem + 32 * k + h / 2, hi);
                             tmem_st8(s_tmem + 32 * k + 16 + h / 2, lo);
                         }
-                        if (k & 1) {
+                        if ((k + 1) % (PART / 32) == 0) {
                             tmem_st_wait();
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(p_full(u, k >> 1));
+                            if (lane == 0) mbar_arrive(p_full(u, k / (PART / 32)));
                         }
                         k++;
                     }

@@ -172,7 +172,8 @@ class PagedKV:
         heads of k and of q [n, any, dim] are rotated at positions pos [n] (default idx), pairs "halves" (i, i + rot / 2)
         or "neighbours" (2i, 2i + 1).  Returns q_out, the rotated q (contiguous, default a new tensor, may be q; zeros for
         tokens that have no place), or None without q.  norm: (q weight, k weight), each [dim] of k's type or both fp32, or
-        None: before the rotation those heads become x / sqrt(mean x^2 + eps) * weight."""
+        None: before the rotation those heads become x / sqrt(mean x^2 + eps) * weight, with squares summed in fp32 (heads of
+        magnitudes above 2^60 become zeros)."""
         n = k.shape[0]
         ty = self._type(k.dtype, "k")
         if v.dtype is not k.dtype or (q is not None and q.dtype is not k.dtype):
