@@ -1,4 +1,4 @@
-"""Trees of drafted tokens in 64 bits (numpy): the checker of the CUDA kernels, never on a product path."""
+"""Trees of drafted tokens in 64 bits (numpy): the oracle of the CUDA kernels, never on a product path."""
 from __future__ import annotations
 
 import numpy as np
