@@ -577,7 +577,8 @@ int fvs_kv_compact(fvs_stream_t stream, const fvs_kv_cache* cache, const int32_t
  * .. + r(v) > u[nodes] sum r (the last with r(v) > 0 if rounding leaves none; -1 for a row without any probability).
  * path[b] = the nodes taken in order, then -1; kept[b] = their number.  All of it in fp64.  Entries that are negative or
  * not finite count as 0.  A node whose parent does not come before it, or whose token is outside the vocabulary, is never
- * taken and changes nothing.  nodes <= 256 (FVS_ERANGE above).  Rows behind nodes that are not taken are not read.
+ * taken and changes nothing.  nodes <= 256 (FVS_ERANGE above).  What the rows behind nodes that are not taken hold changes
+ * nothing.
  */
 int fvs_verify(fvs_stream_t stream, int type, const void* target, int64_t target_seq, int64_t target_row,
                const void* draft, int64_t draft_seq, int64_t draft_row, const int32_t* parents, int64_t parent_stride,

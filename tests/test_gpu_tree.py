@@ -126,6 +126,15 @@ def test_tree_splits_over_the_length(kv, dtype, store, B, heads, group, dim, nod
     check_tree(cache, q, table, n, ints(some_trees(B, nodes, rng)))
 
 
+@pytest.mark.parametrize("dtype,store,group,dim,nodes", [(BF16, BF16, 2, 64, 3), (F16, I8, 1, 128, 40), (F16, F16, 8, 64, 33)])
+def test_tree_one_item_over_every_sm(kv, dtype, store, group, dim, nodes):  # noqa: F811
+    """One key head of a long context: as many shares as the GPU has places, some of them behind a page that is not there."""
+    g, rng = torch.Generator().manual_seed(11), np.random.default_rng(11)
+    cache, q, table, n = setup(kv, [90001], nodes, 1, group, 64, dim, dtype, store, g)
+    table[0, 200:900] = -1
+    check_tree(cache, q, table, n, ints(some_trees(1, nodes, rng)))
+
+
 @pytest.mark.parametrize("B,lens", [(300, (0, 300)), (900, (0, 40)), (1500, (0, 3)), (129, (0, 2000))])
 def test_tree_many_sequences(kv, B, lens):  # noqa: F811
     g, rng = torch.Generator().manual_seed(B), np.random.default_rng(B)
