@@ -484,12 +484,14 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     if (BOXES && warp >= W_PROD && warp < W_MMA) {
         // ------------------------------------------------------------ producers by tensor copies
         if (warp == W_PROD) {
-            // Lane g looks up box g of a tile.  A box comes whole if it has any keys; the scores of what it holds beside them
-            // are masked, and the relay puts zeros in place of those values.
-            const int box = a.box, boxes = KEYS / box;
+            // A lane looks up a box: those of as many tiles at once as the lanes go to (a lookup is two or three loads behind one
+            // another).  A box comes whole if it has any keys; the scores of what it holds beside them are masked, and the
+            // relay puts zeros in place of those values.
+            const int box = a.box, boxes = KEYS / box, ahead = 32 / boxes;
             int slot = 0, phase = 1, tile = 0, issued = 0;
             bool ok = true;
-            int page = 0, at = 0, have = 0, next_page, next_at, next_have;
+            int page, at, have, next_page = 0, next_at = 0, next_have = 0;
+            int b_page = 0, b_at = 0, b_have = 0;  // of the lane's box of the tiles that were looked up
             for (int seg = 0; ok; seg++) {
                 if (!warp_wait(seg_full(seg % SEGS), (seg / SEGS) & 1, abort, WL)) break;
                 const volatile Seg& g = segs[seg % SEGS];
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                 auto lookup = [&](int t) {
                     const int x = t * KEYS + lane * box;
                     next_have = 0;
-                    if (lane < boxes && x < keys && place(a.c, a.tb, b, x, next_page, next_at)) {
+                    if ((unsigned)x < (unsigned)keys && place(a.c, a.tb, b, x, next_page, next_at)) {
                         next_have = min(box, keys - x);
                         if (a.c.fill) next_have = max(0, min(next_have, __ldg(a.c.fill + next_page) - next_at));
                     }
@@ -521,8 +523,14 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                     issued++;
                 };
                 lookup(t0);
-                for (int t = t0; t < t1; t++, tile++) {
-                    page = next_page, at = next_at, have = next_have;
+                for (int t = t0, i = ahead; t < t1; t++, tile++) {
+                    if (i == ahead) b_page = next_page, b_at = next_at, b_have = next_have, i = 0;
+                    const int from = (i * boxes + lane) & 31;
+                    page = __shfl_sync(0xffffffffu, b_page, from);
+                    at = __shfl_sync(0xffffffffu, b_at, from);
+                    have = __shfl_sync(0xffffffffu, b_have, from);
+                    if (lane >= boxes) have = 0;
+                    i++;
                     const int is = tile % INFO, first = lane * box;
                     uint32_t lo = 0, hi = 0;  // flags of the tile's keys
                     if (have > 0) {
@@ -536,11 +544,11 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                         *reinterpret_cast<uint2*>(info + is * INFO_BYTES) = make_uint2(lo, hi);
                         mbar_arrive(info_full(is));
                     }
-                    if (t + 1 < t1) lookup(t + 1);
                     if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
                     copy(&maps.k, have > 0);
                     if (!warp_wait(empty(slot), phase, abort, WL)) { ok = false; break; }
                     copy(&maps.v, have > 0);
+                    if (i == 1 && t + ahead < t1) lookup(t + ahead);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(seg_empty(seg % SEGS));
