@@ -956,6 +956,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                             m = to;
                             l *= by;
                             const bool half = PARTS == 2 && k >= PART / 32;  // the tile's first weights may be in O
+                            tmem_st_wait();  // weights, or an O that rose before, that are read again below
                             if (any || half) {
                                 ok = ok && warp_wait(half ? pv_half(u) : pv_done(last), round_of(half ? u : last), abort, WL);
                                 tc_fence_after();

@@ -393,3 +393,31 @@ def test_tree_boxes_of_a_page(kv, page, dim):  # noqa: F811
     a = cache.attend_tree(q, holes, n, parents)
     b = kv.PagedKV(*wide).attend_tree(q, holes, n, parents)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype,store,dim,group,nodes", [(BF16, BF16, 64, 2, 8), (BF16, BF16, 128, 4, 32), (F16, F16, 96, 1, 100),
+                                                         (BF16, I8, 128, 8, 32), (F16, I8, 64, 4, 64), (BF16, I8, 96, 2, 40),
+                                                         (BF16, BF16, 128, 4, 64), (BF16, BF16, 192, 2, 16)])
+@pytest.mark.parametrize("rise", [4, 8, 10])
+def test_tree_references_that_rise_in_every_half(kv, dtype, store, dim, group, nodes, rise):  # noqa: F811
+    """Every 32 keys weigh 2^rise times those before them, so that a row's reference rises twice in a tile of 64, the first and
+    the later ones, and what was stored for its first half is read again at once.  Keys before a rise keep 2^-rise of the
+    output, which is far above its bound."""
+    g, rng = torch.Generator().manual_seed(rise), np.random.default_rng(rise)
+    lens, heads, page = [160, 225, 31, 64, 97, 128] * 4, 2, 32
+    cache, q, table, n = setup(kv, lens, nodes, heads, group, page, dim, dtype, store, g)
+    q *= 0.1
+    q[..., 0] = 1.0
+    step = torch.zeros(cache.pages, device=DEV)  # a page is one step
+    for b, m in enumerate(lens):
+        row = table[b][table[b] >= 0].long()
+        step[row] = torch.arange(len(row), device=DEV).float()
+    if store == I8:
+        cache.k_scale.copy_((0.01 * (1 + step))[:, None, None].expand_as(cache.k_scale))
+        cache.k[..., 0] = 127
+        scale = rise * np.log(2) / 1.27  # 0.01 * 127 * scale a step, beside what the other elements add
+    else:
+        cache.k[..., 0] = step[:, None, None].to(store)
+        scale = rise * np.log(2)
+    cache.k[..., 1:] = 0
+    check_tree(cache, q, table, n, ints(some_trees(len(lens), nodes, rng)), scale=float(scale))
