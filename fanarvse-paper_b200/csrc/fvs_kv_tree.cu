@@ -1,5 +1,7 @@
 // Entry points of the attention of a tree of drafted tokens over a paged key-value cache; the kernels are in
 // fvs_kv_tree.cuh.
+#include <mutex>
+
 #include "fvs_kv_tree.cuh"
 
 namespace fvs {
@@ -43,6 +45,10 @@ extern "C" int fvs_kv_attend_tree(fvs_stream_t stream, const fvs_kv_cache* cache
         return FVS_ERANGE;
     tree::Args a{*cache, {table, table_stride, seqs, wide}, q, q_seq, q_node, q_head, lens, parents, counts, parent_stride,
                  nodes, hq, group, scale, out, lse, (float*)work, nullptr, 0, 0};
+    // The second launch reads what the first leaves in the workspace.  Threads that launch on one stream share a workspace, so
+    // no call's launches come between another's (ctypes gives up Python's lock meanwhile).
+    static std::mutex both;
+    const std::lock_guard<std::mutex> hold(both);
     switch (cache->dim) {
         case 64: return tree::launch_types<64>(stream, a, type);
         case 96: return tree::launch_types<96>(stream, a, type);

@@ -7,6 +7,8 @@ Bounds, from the arithmetic alone (u: unit roundoff of the output type):
   below 2^-25 of the largest lose more (2^-36 of the largest, absolute); the exponential is within 2^-21;
 * sums over L keys in fp32, cut or rounded: (L + 64) 2^-22 of sum p |v|; one rounding of the output.
 """
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -421,3 +423,31 @@ def test_tree_references_that_rise_in_every_half(kv, dtype, store, dim, group, n
         scale = rise * np.log(2)
     cache.k[..., 1:] = 0
     check_tree(cache, q, table, n, ints(some_trees(len(lens), nodes, rng)), scale=float(scale))
+
+
+def test_tree_two_threads_on_one_stream(kv):  # noqa: F811
+    """Threads share torch's default stream and its workspace: a call's two launches stay together."""
+    g, rng = torch.Generator().manual_seed(15), np.random.default_rng(15)
+    calls, want = [], []
+    for B, nodes, group, longest in ((1, 64, 4, 9000), (20, 6, 2, 900)):
+        cache, q, table, n = setup(kv, list(rng.integers(longest // 2, longest, B)), nodes, 2, group, 16, 128, BF16, BF16, g)
+        calls.append((cache, q, table, n, ints(some_trees(B, nodes, rng))))
+        want.append(calls[-1][0].attend_tree(*calls[-1][1:]))
+        check_tree(*calls[-1], got=want[-1])
+    start, got = threading.Barrier(4), [[] for _ in range(4)]
+
+    def work(i):
+        cache, *args = calls[i % 2]
+        start.wait()
+        for _ in range(100):
+            got[i].append(cache.attend_tree(*args))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        assert len(outs) == 100
+        assert all(torch.equal(x[0], want[i % 2][0]) and torch.equal(x[1], want[i % 2][1]) for x in outs)
