@@ -18,12 +18,12 @@ extern template int launch_types<256>(fvs_stream_t, Args, int);
 
 using namespace fvs::kv;
 
-// two partial results of each CTA, of as many rows as an item has, behind 8 words of each CTA: two CTAs of 128 rows an SM
+// two partial results of each CTA, of as many rows as an item has, behind DESC words of each CTA: two CTAs of 128 rows an SM
 // with heads up to 128, else one
 extern "C" int fvs_kv_attend_tree_work(int dim, int rows) {
     if (dim < 1 || rows < 0) return FVS_EINVAL;
     if (dim > 256) return FVS_ERANGE;
-    return fvs_sm_count() * (2 * 32 + (dim <= 128 ? 2 : 1) * 2 * tree::ROWS * (dim + 2) * 4);
+    return fvs_sm_count() * (2 * tree::DESC * 4 + (dim <= 128 ? 2 : 1) * 2 * tree::ROWS * (dim + 2) * 4);
 }
 
 extern "C" int fvs_kv_attend_tree(fvs_stream_t stream, const fvs_kv_cache* cache, int type, const void* q, int64_t q_seq,

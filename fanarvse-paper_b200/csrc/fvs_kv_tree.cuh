@@ -42,6 +42,11 @@ constexpr int ITEM_KEYS = 256;  // cost of an item, its queries' copy and its ou
 constexpr int LEAST_COST = 4;  // of a CTA's share, in tiles
 constexpr int GAVE_UP = 2;     // status bit: a bounded wait ran out
 constexpr int SEG_BYTES = 48;
+constexpr int DESC = 16;
+// Words of a CTA's descriptor: the item that begins in it and goes on in others (sequence or -1, item, key head, row tile, rows),
+// the item that it continues (sequence or -1, item), HAS_SHARE and NOT_FINITE, then where its share begins (sequence; cost
+// before that and of all, 64 bits each).
+constexpr int HAS_SHARE = 1, NOT_FINITE = 2;  // NOT_FINITE: an O of an item that it computed whole is not finite
 
 struct Args {
     fvs_kv_cache c;
@@ -55,7 +60,7 @@ struct Args {
     void* out;
     float* lse;
     float* work;     // two partial results of each CTA: [dim][rows] O, then [rows] maxima (log2), [rows] sums
-    int32_t* desc;   // 8 words of each CTA: what join_kernel reads
+    int32_t* desc;   // DESC words of each CTA: what join_kernel reads
     uint32_t wait_limit;
     int box;         // keys of a tensor copy, a power of two that divides the page
 };
@@ -118,7 +123,7 @@ __device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) {
 }
 
 // Where the share of CTA c begins: of equal cost, of as many CTAs as have LEAST_COST or more (what a cut costs)
-__device__ __forceinline__ int64_t shares(int64_t total) { return min((int64_t)gridDim.x, max((int64_t)1, total / LEAST_COST)); }
+__device__ __forceinline__ int64_t shares(int64_t total, int ctas) { return min((int64_t)ctas, max((int64_t)1, total / LEAST_COST)); }
 __device__ __forceinline__ int64_t share(int64_t total, int64_t ctas, unsigned c) { return c >= ctas ? total : total * (int64_t)c / ctas; }
 
 struct Seg {             // tiles [t0, t1) of one item; t0 == t1: no more
@@ -421,7 +426,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             if (w < warp) before += sums[w];
             total += sums[w];
         }
-        const int64_t ctas = shares(total), from = share(total, ctas, blockIdx.x);
+        const int64_t ctas = shares(total, gridDim.x), from = share(total, ctas, blockIdx.x);
         if (from >= before && from < before + mine) {
             int b = b0;
             for (;; b++) {
@@ -434,9 +439,9 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
         }
         if (tid == 0) {
             s_place[0] = total;
-            int32_t* d = a.desc + 8 * blockIdx.x;  // no share of a cut item yet; whether there is any share
+            int32_t* d = a.desc + DESC * blockIdx.x;  // no share of a cut item yet
             d[0] = d[5] = -1;
-            d[7] = from < share(total, ctas, blockIdx.x + 1);
+            d[7] = from < share(total, ctas, blockIdx.x + 1) ? HAS_SHARE : 0;
         }
         // rows of nodes that a sequence does not have
         if (a.counts)
@@ -452,6 +457,12 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (tid == 0) {
+        int32_t* d = a.desc + DESC * blockIdx.x;
+        d[8] = (int32_t)s_place[1];
+        *reinterpret_cast<int64_t*>(d + 10) = s_place[2];
+        *reinterpret_cast<int64_t*>(d + 12) = s_place[0];
+    }
     const uint32_t tmem = *tmem_slot;
     const float scale2 = a.scale * 1.4426950408889634f;  // of scores in powers of two
 
@@ -800,7 +811,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             // instruction instead of 67).
             Walk<KEYS, RT> walk;
             const int64_t total = s_place[0];
-            const int64_t ctas = shares(total);
+            const int64_t ctas = shares(total, gridDim.x);
             walk.begin(a, (int)s_place[1], s_place[2], share(total, ctas, blockIdx.x), share(total, ctas, blockIdx.x + 1));
             int slot = 0, phase = 0, told = 0, tile = 0;
             bool more = true, ok = true;
@@ -1064,12 +1075,15 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                 const int64_t o_row = ((int64_t)g.b * a.nodes + node) * a.hq + g.head * a.group + h;
                 const float down = 1.f / LIFT;
                 const float by = whole ? (l == 0.f ? 0.f : down / l) : down;
+                Two finite = two(0.f, 0.f);  // not-a-number if an element of O is not finite
 #pragma unroll 1
                 for (int k = 0; k < D; k += 16) {
                     uint32_t x[16];
                     tmem_ld16(lanes + S::O0 + w * D + k, x);
                     tmem_wait16(x);
                     float o[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) finite = fma2(two(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), two(0.f, 0.f), finite);
 #pragma unroll
                     for (int j = 0; j < 16; j++) o[j] = __uint_as_float(x[j]) * by;
                     if (whole && live) {
@@ -1088,6 +1102,9 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                 }
                 if (live) {
                     if (whole) {
+                        const float2 sure = one(finite);
+                        // (a sum of weights that is not finite either is not-a-number in the formula too)
+                        if (!(sure.x + sure.y == 0.f) && l > 0.f && l < -__int_as_float(0xff800000)) a.desc[DESC * blockIdx.x + 7] = HAS_SHARE | NOT_FINITE;
                         if (a.lse) a.lse[o_row] = l == 0.f ? __int_as_float(0xff800000) : (m + log2f(l)) * 0.6931471805599453f;
                     } else {
                         part[D * RT + mine] = m;
@@ -1099,7 +1116,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
             mbar_arrive(o_free);
             // what join_kernel reads: the item that begins here and goes on, and the one that came from the CTA before
             if (tid == 0 && !whole) {
-                int32_t* d = a.desc + 8 * blockIdx.x;
+                int32_t* d = a.desc + DESC * blockIdx.x;
                 const int item = g.item;
                 if (t0 == 0) {
                     d[0] = g.b, d[1] = item, d[2] = g.head, d[3] = g.rt, d[4] = g.rows;
@@ -1119,79 +1136,372 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     if (*abort && tid == 0) atomicOr(a.c.status, GAVE_UP);
 }
 
+// ---------------------------------------------------------------- outputs that are not finite
+// The products multiply every value of a tile by every row's weights, those of keys that a row does not see by zeros, and a
+// weight's second part may be negative: a value that is not finite makes not-a-numbers of outputs that the formula gives as an
+// infinity, or that it has no part in.  Large weights of large finite values may add up to an infinity.  Such outputs (an O that
+// is not finite where the sum of weights is) are computed again from the formula, behind everything else, by the block that
+// holds them: a column is what its values that are not finite make of it (weights are above zero), or, where a row sees none,
+// the mean of its values by weights of at most one.  Finite inputs pay for a look at O and for the blocks of this code: 24 long
+// int8 contexts under 32 nodes 386 us (381 without), 32 x 10 passages 64.2 (63.7), 131000 tokens under 64 nodes nothing.  Others
+// pay for what is computed again: of those 131000 tokens 2 ms for an infinite value in one key head, 92 for a not-a-number
+// in a node, whose siblings' scores are taken again; one short passage 60 and 120 us.
+constexpr int JOIN_COLS = 32, JOIN_THREADS = 256, JOIN_LEAST = 96;  // JOIN_LEAST: CTAs whose maxima leave room for a Redo
+constexpr int AGAIN = 4;                                            // rows at once
+
+// a key's row, and its scales
+struct Stored {
+    const uint8_t *k, *v;
+    float ks, vs;
+};
+template <int STORE>
+__device__ __forceinline__ bool stored(const Args& a, int b, int head, int x, Stored& r) {
+    int page, slot;
+    if (!place(a.c, a.tb, b, x, page, slot) || (a.c.fill && slot >= __ldg(a.c.fill + page))) return false;
+    const int64_t e = (int64_t)page * a.c.page_stride + (int64_t)slot * a.c.slot_stride + (int64_t)head * a.c.head_stride;
+    constexpr int ESZ = STORE == FVS_I8 ? 1 : 2;
+    r.k = (const uint8_t*)a.c.k + e * ESZ;
+    r.v = (const uint8_t*)a.c.v + e * ESZ;
+    r.ks = r.vs = 1.f;
+    if (STORE == FVS_I8) {
+        const int64_t se = (int64_t)page * a.c.scale_page_stride + (int64_t)slot * a.c.scale_slot_stride + (int64_t)head * a.c.scale_head_stride;
+        r.ks = __ldg(a.c.k_scale + se);
+        r.vs = __ldg(a.c.v_scale + se);
+    }
+    return true;
+}
+// 8 elements of a stored row
+template <int STORE>
+__device__ __forceinline__ void elements(const uint8_t* at, int first, float (&f)[8]) {
+    if (STORE == FVS_I8) {
+        const uint2 x = __ldg((const uint2*)(at + first));
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = (float)(int8_t)((i < 4 ? x.x : x.y) >> (8 * (i & 3)));
+    } else {
+        up8<STORE == FVS_I8 ? FVS_F16 : STORE>(__ldg((const uint4*)(at + 2 * first)), f);
+    }
+}
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < __int_as_float(0x7f800000); }
+
+struct Kinds {  // a bit for each of 32 columns
+    uint32_t nan, up, down;
+    __device__ __forceinline__ void add(const Kinds& x) {
+        if (x.nan) atomicOr(&nan, x.nan);
+        if (x.up) atomicOr(&up, x.up);
+        if (x.down) atomicOr(&down, x.down);
+    }
+};
+// what redo() keeps in shared memory
+struct Redo {
+    float q[AGAIN][256];
+    float m[JOIN_THREADS / 32][AGAIN], l[JOIN_THREADS / 32][AGAIN];
+    float o[JOIN_THREADS / 32][AGAIN][JOIN_COLS];
+    uint32_t sees[AGAIN][FVS_TREE_NODES / 32];
+    Kinds all, tree[AGAIN];
+};
+
+// Rows [row0, row0 + 32) of an item's row tile, those of `which`, columns [col, col + 32): outputs that are not finite, by the
+// whole block, four lanes a key.  refs: a number near each row's largest score (log2), or null: a.lse has it, or, without one,
+// the scores are looked at first (a row whose sum of weights is not finite is not-a-number in the formula too, and is left).
+template <int D, int TYPE, int STORE, int RT>
+__device__ __noinline__ void redo(const Args& a, Redo& s, int b, int head, int rt, int rows, int n, int keys, int row0, int col, uint32_t which,
+                                  const float* refs) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & 3;
+    constexpr int STEP = JOIN_THREADS / 4;  // keys at once
+    const float scale2 = a.scale * 1.4426950408889634f;
+    const int before = min(n, keys);  // keys of the sequence, which all rows see
+    bool known = false;               // what the values of the sequence's keys are, in s.all
+    // (out and lse are read past the cache that other kernels' results may not be in)
+    for (int r0 = 0; r0 < min(32, rows - row0); r0 += AGAIN) {
+        uint32_t wrong[AGAIN], any = 0;
+        int64_t at[AGAIN];
+        float ref[AGAIN];
+#pragma unroll
+        for (int r = 0; r < AGAIN; r++) {
+            wrong[r] = 0;
+            if (row0 + r0 + r >= rows || !(which >> (r0 + r) & 1)) continue;
+            const int row = rt * RT + row0 + r0 + r, node = row / a.group, h = head * a.group + row - node * a.group;
+            at[r] = ((int64_t)b * a.nodes + node) * a.hq + h;
+            const float was = Elem<TYPE>::up((uint32_t)__ldcg((const uint16_t*)a.out + at[r] * D + col + lane)).x;
+            ref[r] = refs ? refs[r0 + r] : a.lse ? __ldcg(a.lse + at[r]) * 1.4426950408889634f : 0.f;
+            if (is_finite(ref[r])) wrong[r] = __ballot_sync(0xffffffffu, !is_finite(was));  // the same in every warp
+            any |= wrong[r];
+        }
+        __syncthreads();  // every warp has looked
+        if (any == 0) continue;
+        if (!known) {
+            if (tid == 0) s.all = Kinds{0, 0, 0};
+            __syncthreads();
+        }
+        // what is not finite in this lane's columns
+        auto kinds = [&](const Stored& k) {
+            Kinds x = {0, 0, 0};
+            float f[8];
+            elements<STORE>(k.v, col + 8 * sub, f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = f[j] * k.vs;
+                if (!is_finite(y)) (y > 0.f ? x.up : y < 0.f ? x.down : x.nan) |= 1u << (8 * sub + j);
+            }
+            return x;
+        };
+        if (!known) {
+            known = true;
+            for (int x = tid >> 2; x < before; x += STEP) {
+                Stored k;
+                if (stored<STORE>(a, b, head, x, k)) s.all.add(kinds(k));
+            }
+        }
+        if (tid < AGAIN) {
+            s.tree[tid] = Kinds{0, 0, 0};
+            for (int i = 0; i < FVS_TREE_NODES / 32; i++) s.sees[tid][i] = 0;
+            const int32_t* up = a.parents + (int64_t)b * a.parent_stride;
+            const int row = row0 + r0 + tid;
+            for (int i = row < rows ? (rt * RT + row) / a.group : -1; i >= 0;) {
+                s.sees[tid][i >> 5] |= 1u << (i & 31);
+                const int p = __ldg(up + i);
+                i = p < i ? p : -1;
+            }
+        }
+        for (int i = tid; i < AGAIN * D; i += JOIN_THREADS) {
+            const int r = i / D, e = i - r * D, row = rt * RT + row0 + r0 + r, node = row / a.group, h = head * a.group + row - node * a.group;
+            s.q[r][e] = row0 + r0 + r >= rows ? 0.f
+                            : Elem<TYPE>::up((uint32_t)((const uint16_t*)a.q)[(int64_t)b * a.q_seq + (int64_t)node * a.q_node + (int64_t)h * a.q_head + e]).x;
+        }
+        __syncthreads();
+        auto seen = [&](int r, int x) { return x < n || (s.sees[r][(x - n) >> 5] >> ((x - n) & 31) & 1); };
+        for (int x = before + (tid >> 2); x < keys; x += STEP) {
+            Stored k;
+            if (!stored<STORE>(a, b, head, x, k)) continue;
+            const Kinds of_node = kinds(k);
+            for (int r = 0; r < AGAIN; r++)
+                if (seen(r, x)) s.tree[r].add(of_node);
+        }
+        __syncthreads();
+        bool scores = !refs && !a.lse;
+#pragma unroll
+        for (int r = 0; r < AGAIN; r++)
+            scores = scores || (wrong[r] & ~(s.all.nan | s.all.up | s.all.down | s.tree[r].nan | s.tree[r].up | s.tree[r].down));
+        float l[AGAIN] = {}, o[AGAIN][8] = {};
+        if (scores) {
+            // the rows' scores of a key, by its four lanes together
+            auto score = [&](const Stored& k, bool there, float (&y)[AGAIN]) {
+#pragma unroll
+                for (int r = 0; r < AGAIN; r++) y[r] = 0.f;
+                if (there) {
+#pragma unroll 1
+                    for (int e = 8 * sub; e < D; e += 32) {
+                        float f[8];
+                        elements<STORE>(k.k, e, f);
+#pragma unroll
+                        for (int r = 0; r < AGAIN; r++) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++) y[r] = fmaf(s.q[r][e + j], f[j], y[r]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < AGAIN; r++) {
+                    y[r] += __shfl_xor_sync(0xffffffffu, y[r], 1);
+                    y[r] += __shfl_xor_sync(0xffffffffu, y[r], 2);
+                    y[r] *= k.ks * scale2;
+                }
+            };
+            if (!refs && !a.lse) {
+                float m[AGAIN];
+#pragma unroll
+                for (int r = 0; r < AGAIN; r++) m[r] = __int_as_float(0xff800000);
+                auto join = [&](int r, float om, float ol) {
+                    const float top = fmaxf(m[r], om);
+                    l[r] = l[r] * (m[r] == top ? 1.f : exp2_of(m[r] - top)) + ol * (om == top ? 1.f : exp2_of(om - top));
+                    m[r] = top;
+                };
+                for (int x0 = 0; x0 < keys; x0 += STEP) {
+                    const int x = x0 + (tid >> 2);
+                    Stored k = {nullptr, nullptr, 0.f, 0.f};
+                    const bool there = x < keys && stored<STORE>(a, b, head, x, k);
+                    float y[AGAIN];
+                    score(k, there, y);
+#pragma unroll
+                    for (int r = 0; r < AGAIN; r++)
+                        if (there && seen(r, x)) join(r, y[r], 1.f);
+                }
+#pragma unroll
+                for (int r = 0; r < AGAIN; r++) {
+#pragma unroll
+                    for (int i = 16; i >= 4; i >>= 1) {
+                        const float om = __shfl_xor_sync(0xffffffffu, m[r], i), ol = __shfl_xor_sync(0xffffffffu, l[r], i);
+                        join(r, om, ol);
+                    }
+                    if (lane == 0) s.m[warp][r] = m[r], s.l[warp][r] = l[r];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < AGAIN; r++) {
+                    m[r] = __int_as_float(0xff800000), l[r] = 0.f;
+                    for (int w = 0; w < JOIN_THREADS / 32; w++) join(r, s.m[w][r], s.l[w][r]);
+                    ref[r] = m[r];
+                    if (!is_finite(l[r])) wrong[r] = 0;
+                    l[r] = 0.f;
+                }
+                __syncthreads();
+            }
+            for (int x0 = 0; x0 < keys; x0 += STEP) {
+                const int x = x0 + (tid >> 2);
+                Stored k = {nullptr, nullptr, 0.f, 0.f};
+                const bool there = x < keys && stored<STORE>(a, b, head, x, k);
+                float y[AGAIN], f[8];
+                score(k, there, y);
+                if (!there) continue;
+                elements<STORE>(k.v, col + 8 * sub, f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = is_finite(f[j] * k.vs) ? f[j] * k.vs : 0.f;
+#pragma unroll
+                for (int r = 0; r < AGAIN; r++) {
+                    if (!seen(r, x)) continue;
+                    const float p = exp2_of(y[r] - ref[r]);
+                    l[r] += p;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) o[r][j] = fmaf(p, f[j], o[r][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < AGAIN; r++) {
+#pragma unroll
+            for (int i = 16; i >= 4; i >>= 1) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], i);
+#pragma unroll
+                for (int j = 0; j < 8; j++) o[r][j] += __shfl_xor_sync(0xffffffffu, o[r][j], i);
+            }
+            if (lane < 4) {
+                if (lane == 0) s.l[warp][r] = l[r];
+#pragma unroll
+                for (int j = 0; j < 8; j++) s.o[warp][r][8 * sub + j] = o[r][j];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < AGAIN; r++)
+            if (warp == r && (wrong[r] >> lane & 1)) {
+                float x = 0.f, sum = 0.f;
+                for (int w = 0; w < JOIN_THREADS / 32; w++) x += s.o[w][r][lane], sum += s.l[w][r];
+                const bool nan = (s.all.nan | s.tree[r].nan) >> lane & 1, up = (s.all.up | s.tree[r].up) >> lane & 1, down = (s.all.down | s.tree[r].down) >> lane & 1;
+                x = nan || (up && down) ? __int_as_float(0x7fc00000) : up ? __int_as_float(0x7f800000) : down ? __int_as_float(0xff800000) : x / sum;
+                ((uint16_t*)a.out)[at[r] * D + col + lane] = (uint16_t)Elem<TYPE>::down(x, 0.f);
+            }
+        __syncthreads();
+    }
+}
+
+// what join_kernel's block has of such rows: those of the cut item in `which`, and items that its CTA computed whole
+template <int D, int TYPE, int STORE, int RT, int KEYS>
+__device__ __noinline__ void redo_block(const Args& a, Redo& s, int ctas, uint32_t which, const float* refs) {
+    const int c = blockIdx.x, row0 = blockIdx.y * 32, col = blockIdx.z * JOIN_COLS;
+    const int32_t* desc = a.desc + DESC * c;
+    __syncthreads();
+    if (which) {
+        const Seq q = sequence<KEYS, RT>(a, desc[0]);
+        redo<D, TYPE, STORE, RT>(a, s, desc[0], desc[2], desc[3], desc[4], q.n, q.keys, row0, col, which, refs);
+    }
+    if (!(desc[7] & NOT_FINITE)) return;
+    Walk<KEYS, RT> walk;
+    const int64_t total = *reinterpret_cast<const int64_t*>(desc + 12), have = shares(total, ctas);
+    walk.begin(a, desc[8], *reinterpret_cast<const int64_t*>(desc + 10), share(total, have, c), share(total, have, c + 1));
+    Seg g;
+    while (walk.next(a, g))
+        if (g.t0 == 0 && g.t1 == g.tiles && row0 < g.rows)
+            redo<D, TYPE, STORE, RT>(a, s, g.b, g.head, g.rt, g.rows, g.n, g.keys, row0, col, 0xffffffffu, nullptr);
+}
+
 // Adds the shares of the items that were cut.  Block (c, 32 rows, 32 columns): the item that begins in CTA c and goes on in
 // the CTAs behind it, each of which left one share.  The shares are read once, from L2 mostly, and what bounds it is the
-// latency of its loads behind one another (descriptors, maxima and sums, O).
-constexpr int JOIN_COLS = 32;
-template <int D, int TYPE, int RT>
-__global__ void __launch_bounds__(256) join_kernel(Args a, int ctas) {
+// latency of its loads behind one another (descriptors, maxima and sums, O).  Then, where there are any, the outputs that are
+// not finite, of this item and of those that CTA c computed whole.  Blocks of an SM, which redo_block's registers would cut to
+// two: as many as the maxima leave room for with 296 CTAs, five; over int8 codes of 256 rows eight (24 long int8 contexts under
+// 32 nodes: 386 us, 389 with five), over 16-bit ones five as well (131000 tokens under 64 nodes: 246 us, 250 with eight).
+template <int D, int TYPE, int STORE, int RT, int KEYS>
+__global__ void __launch_bounds__(JOIN_THREADS, RT == 256 && STORE == FVS_I8 ? 8 : 5) join_kernel(const __grid_constant__ Args a, int ctas) {
     constexpr int COLS = JOIN_COLS / 8;  // of a thread
     extern __shared__ float tops[];      // maxima [shares][32], no share's -infinity
     __shared__ float s_m[8][32], s_l[8][32];
     __shared__ int s_upto;
     __shared__ uint8_t s_has[512];
+    __shared__ uint32_t s_wrong;         // rows with an O that is not finite
+    __shared__ float s_ref[32];          // their sums' logarithms
+    static_assert(sizeof(Redo) <= JOIN_LEAST * 32 * 4, "redo's memory takes that of the maxima");
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) s_upto = ctas;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the shares are still computed
-    const int4 d = *reinterpret_cast<const int4*>(a.desc + 8 * c);
-    const int b = d.x, item = d.y, head = d.z, rt = d.w, rows = a.desc[8 * c + 4];
-    const int row = blockIdx.y * 32 + lane;
+    if (threadIdx.x == 0) s_upto = ctas, s_wrong = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // all of the shares are there
+    const int32_t* desc = a.desc + DESC * c;
+    const int4 d = *reinterpret_cast<const int4*>(desc);
+    const int b = d.x, item = d.y, head = d.z, rt = d.w, rows = desc[4], flags = desc[7];
+    const int row = blockIdx.y * 32 + lane, col0 = blockIdx.z * JOIN_COLS;
     __syncthreads();
-    if (b < 0 || (int)blockIdx.y * 32 >= rows) return;
-    // the CTAs behind that have a share of it: none between them has another item, some may have nothing at all
-    for (int x = c + (int)threadIdx.x; x < ctas; x += 256) {
-        const int4 e = *reinterpret_cast<const int4*>(a.desc + 8 * x + 4);
-        const bool has = x == c || (e.y == b && e.z == item);
-        s_has[x - c] = has;
-        if (!has && e.w != 0) atomicMin(&s_upto, x);
-    }
-    __syncthreads();
-    const int shares = s_upto - c;
-    auto part = [&](int i) { return a.work + (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * RT * (D + 2); };
-    constexpr float NONE = -__builtin_huge_valf();
-    float m = NONE, l = 0.f;
+    if (b >= 0 && (int)blockIdx.y * 32 < rows) {
+        // the CTAs behind that have a share of it: none between them has another item, some may have nothing at all
+        for (int x = c + (int)threadIdx.x; x < ctas; x += JOIN_THREADS) {
+            const int4 e = *reinterpret_cast<const int4*>(a.desc + DESC * x + 4);
+            const bool has = x == c || (e.y == b && e.z == item);
+            s_has[x - c] = has;
+            if (!has && e.w != 0) atomicMin(&s_upto, x);
+        }
+        __syncthreads();
+        const int shares = s_upto - c;
+        auto part = [&](int i) { return a.work + (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * RT * (D + 2); };
+        constexpr float NONE = -__builtin_huge_valf();
+        float m = NONE, l = 0.f;
 #pragma unroll 2
-    for (int i = warp; i < shares; i += 8) {
-        const bool there = s_has[i] && row < rows;
-        const float x = there ? part(i)[D * RT + row] : NONE, y = there ? part(i)[(D + 1) * RT + row] : 0.f;
-        tops[i * 32 + lane] = x;
-        const float top = fmaxf(m, x);
-        l = l * (m == top ? 1.f : exp2_of(m - top)) + y * (x == top ? 1.f : exp2_of(x - top));
-        m = top;
-    }
-    s_m[warp][lane] = m;
-    s_l[warp][lane] = l;
-    __syncthreads();
-    m = NONE;
+        for (int i = warp; i < shares; i += 8) {
+            const bool there = s_has[i] && row < rows;
+            const float x = there ? part(i)[D * RT + row] : NONE, y = there ? part(i)[(D + 1) * RT + row] : 0.f;
+            tops[i * 32 + lane] = x;
+            const float top = fmaxf(m, x);
+            l = l * (m == top ? 1.f : exp2_of(m - top)) + y * (x == top ? 1.f : exp2_of(x - top));
+            m = top;
+        }
+        s_m[warp][lane] = m;
+        s_l[warp][lane] = l;
+        __syncthreads();
+        m = NONE;
 #pragma unroll
-    for (int w = 0; w < 8; w++) m = fmaxf(m, s_m[w][lane]);
-    l = 0.f;
+        for (int w = 0; w < 8; w++) m = fmaxf(m, s_m[w][lane]);
+        l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; w++) l = fmaf(s_l[w][lane], s_m[w][lane] == m ? 1.f : exp2_of(s_m[w][lane] - m), l);
-    if (row >= rows) return;
-    const int at = rt * RT + row, node = at / a.group, h = at - node * a.group;
-    const int64_t o_row = ((int64_t)b * a.nodes + node) * a.hq + head * a.group + h;
-    const int col = blockIdx.z * JOIN_COLS + warp * COLS;
-    float o[COLS] = {};
+        for (int w = 0; w < 8; w++) l = fmaf(s_l[w][lane], s_m[w][lane] == m ? 1.f : exp2_of(s_m[w][lane] - m), l);
+        if (row < rows) {
+            const int at = rt * RT + row, node = at / a.group, h = at - node * a.group;
+            const int64_t o_row = ((int64_t)b * a.nodes + node) * a.hq + head * a.group + h;
+            const int col = col0 + warp * COLS;
+            float o[COLS] = {};
 #pragma unroll 4
-    for (int i = 0; i < shares; i++) {
-        const float top = tops[i * 32 + lane], by = top == m ? 1.f : exp2_of(top - m);
-        const float* p = part(i) + col * RT + row;
-        float x[COLS];
+            for (int i = 0; i < shares; i++) {
+                const float top = tops[i * 32 + lane], by = top == m ? 1.f : exp2_of(top - m);
+                const float* p = part(i) + col * RT + row;
+                float x[COLS];
 #pragma unroll
-        for (int j = 0; j < COLS; j++) x[j] = p[j * RT];  // of a CTA without a share: anything, and not added
+                for (int j = 0; j < COLS; j++) x[j] = p[j * RT];  // of a CTA without a share: anything, and not added
 #pragma unroll
-        for (int j = 0; j < COLS; j++)
-            if (top != NONE && by != 0.f) o[j] = fmaf(x[j], by, o[j]);
+                for (int j = 0; j < COLS; j++)
+                    if (top != NONE && by != 0.f) o[j] = fmaf(x[j], by, o[j]);
+            }
+            const float by = l == 0.f ? 0.f : 1.f / l;
+            uint32_t packed[COLS / 2];
+            float finite = 0.f;  // not-a-number if an element of O is not finite
+#pragma unroll
+            for (int j = 0; j < COLS; j += 2) {
+                packed[j / 2] = l == 0.f ? 0u : Elem<TYPE>::down(o[j] * by, o[j + 1] * by);
+                finite = fmaf(o[j], 0.f, fmaf(o[j + 1], 0.f, finite));
+            }
+            uint16_t* out = (uint16_t*)a.out + o_row * D + col;
+#pragma unroll
+            for (int j = 0; j < COLS / 2; j++) reinterpret_cast<uint32_t*>(out)[j] = packed[j];
+            if (blockIdx.z == 0 && warp == 0 && a.lse) a.lse[o_row] = l == 0.f ? NONE : (m + log2f(l)) * 0.6931471805599453f;
+            if (finite != 0.f && l > 0.f && is_finite(l)) atomicOr(&s_wrong, 1u << lane), s_ref[lane] = m + log2f(l);
+        }
+        __syncthreads();
     }
-    const float by = l == 0.f ? 0.f : 1.f / l;
-    uint32_t packed[COLS / 2];
-#pragma unroll
-    for (int j = 0; j < COLS; j += 2) packed[j / 2] = l == 0.f ? 0u : Elem<TYPE>::down(o[j] * by, o[j + 1] * by);
-    uint16_t* out = (uint16_t*)a.out + o_row * D + col;
-#pragma unroll
-    for (int j = 0; j < COLS / 2; j++) reinterpret_cast<uint32_t*>(out)[j] = packed[j];
-    if (blockIdx.z == 0 && warp == 0 && a.lse) a.lse[o_row] = l == 0.f ? NONE : (m + log2f(l)) * 0.6931471805599453f;
+    if (s_wrong || (flags & NOT_FINITE)) redo_block<D, TYPE, STORE, RT, KEYS>(a, *reinterpret_cast<Redo*>(tops), ctas, s_wrong, s_ref);
 }
 
 // the tensor maps of a 16-bit cache; false where tensor copies cannot take it
@@ -1221,21 +1531,21 @@ static int launch(fvs_stream_t stream, Args a, const Maps& maps) {
     if (e != cudaSuccess) return (int)e;
     a.wait_limit = pipeline_wait_limit();
     a.desc = (int32_t*)a.work;
-    a.work = a.work + 8 * ctas;
+    a.work = a.work + DESC * ctas;
     tree_kernel<D, TYPE, STORE, MT, QR, BOXES><<<ctas, S::THREADS, S::BYTES, stream>>>(a, maps);
     if (int rc = fvs_launch_status()) return rc;
     const int rows = a.nodes * a.group;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, ((rows < RT ? rows : RT) + 31) / 32, D / JOIN_COLS);
     cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = ctas * 32 * 4;
+    cfg.dynamicSmemBytes = (ctas > JOIN_LEAST ? ctas : JOIN_LEAST) * 32 * 4;
     cfg.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, join_kernel<D, TYPE, RT>, a, ctas);
+    e = cudaLaunchKernelEx(&cfg, join_kernel<D, TYPE, STORE, RT, S::KEYS>, a, ctas);
     if (e != cudaSuccess) return (int)e;
     return fvs_launch_status();
 }

@@ -270,7 +270,8 @@ class PagedKV:
         [sequences]: the nodes that a sequence has (default: all).  Returns (out like q, lse fp32 [sequences, nodes, query
         heads]): zeros and -inf where nothing is visible and for nodes that a sequence does not have.  One node is
         `attend` with a length of lens + 1.  Hidden slots may hold anything; the nodes' own keys and values are finite (one
-        that is not may reach nodes that do not see it)."""
+        that is not may reach nodes that do not see it).  Visible values that are not finite do what the formula does; their
+        rows are computed again, which takes longer."""
         shape = q.shape
         if not (len(shape) == 4 and shape[3] == self.dim and q.get_device() == self._index):
             raise ValueError(f"q is [sequences, nodes, heads, {self.dim}] on the cache's GPU")

@@ -451,3 +451,118 @@ def test_tree_two_threads_on_one_stream(kv):  # noqa: F811
     for i, outs in enumerate(got):
         assert len(outs) == 100
         assert all(torch.equal(x[0], want[i % 2][0]) and torch.equal(x[1], want[i % 2][1]) for x in outs)
+
+
+def check_special(cache, q, table, lens, parents, counts=None, scale=None, got=None):
+    """check_tree for values that are not finite: a column is what the formula makes of its infinities and not-a-numbers, and
+    the others lie within their bound."""
+    out, lse = got or cache.attend_tree(q, table, lens, parents, counts=counts, scale=scale)
+    torch.cuda.synchronize()
+    d = cache.dim
+    scale = 1 / np.sqrt(d) if scale is None else scale
+    k, v = values(cache)
+    with np.errstate(invalid="ignore", over="ignore"):
+        eo, el, pv, mag = O.attend_tree(c(q), k, v, c(table), c(lens), np.broadcast_to(c(parents), q.shape[:2]),
+                                        None if counts is None else c(counts), scale, None if cache.fill is None else c(cache.fill))
+    out, lse = c(out), c(lse)
+    assert np.array_equal(np.isnan(out), np.isnan(eo))
+    inf = np.isinf(eo)
+    assert np.array_equal(np.isinf(out), inf) and np.array_equal(out[inf], eo[inf])
+    fine = np.isfinite(eo)
+    L = int(max(1, c(lens).max() + q.shape[1]))
+    es = (d + 4) * 2.0 ** -23 * np.broadcast_to(mag[..., None], eo.shape)
+    part = 2.0 ** -17 if q.dtype == BF16 or cache.dtype == I8 else 2.0 ** -21
+    tol = U[q.dtype] * np.abs(eo[fine]) + (part + 2 * es[fine] + 2.0 ** -20 + (L + 64) * 2.0 ** -22) * pv[fine] * 1.01 + (2.0 ** -25 if q.dtype == F16 else 0.0)
+    tol += 2.0 ** -36 * np.abs(v[np.isfinite(v)]).max()
+    worst = (np.abs(out[fine] - eo[fine]) / tol).max(initial=0)
+    assert worst <= 1, f"out is {worst:.2f} of its bound"
+    empty = np.isneginf(el)
+    assert np.array_equal(np.isneginf(lse), empty) and (out[empty] == 0).all()
+    assert np.array_equal(np.isnan(lse), np.isnan(el))
+    fine = np.isfinite(el)
+    tol = 2 * (d + 4) * 2.0 ** -23 * mag[fine] + (L + 64) * 2.0 ** -22 + 2.0 ** -20 * (1 + np.abs(el[fine]))
+    worst = (np.abs(lse[fine] - el[fine]) / tol).max(initial=0)
+    assert worst <= 1, f"lse is {worst:.2f} of its bound"
+    cache.check_status()
+
+
+def put(cache, table, b, t, h, col, x):
+    """Value `x` in column `col` of token t of sequence b (codes: a scale makes it of the row)."""
+    page, slot = int(table[b, t // cache.page]), t % cache.page
+    if cache.v_scale is None:
+        cache.v[page, h, slot, col] = x
+    else:
+        cache.v[page, h, slot] = 1
+        cache.v[page, h, slot, col] = 1 if x > 0 else -1 if x < 0 else 0
+        cache.v_scale[page, h, slot] = abs(x)
+
+
+KINDS = [(BF16, BF16, 64, 2, 9), (BF16, BF16, 128, 4, 20), (F16, F16, 96, 8, 25), (BF16, I8, 128, 8, 32), (F16, I8, 64, 2, 10), (BF16, BF16, 192, 2, 70),
+         (F16, F16, 128, 5, 1)]
+
+
+@pytest.mark.parametrize("dtype,store,dim,group,nodes", KINDS)
+@pytest.mark.parametrize("lens,page", [([300, 40, 129, 0, 70], 16), ([20000, 3], 64), ([100] * 90, 20)])
+def test_tree_visible_values_that_are_not_finite(kv, dtype, store, dim, group, nodes, lens, page):  # noqa: F811
+    """An infinity is the column's output, two against each other and not-a-numbers are not-a-number, as in `attend`; items of
+    one CTA and cut ones, copies of boxes and of rows, in the sequence and in its nodes."""
+    g, rng = torch.Generator().manual_seed(16), np.random.default_rng(16)
+    heads = 2
+    cache, q, table, n = setup(kv, lens, nodes, heads, group, page, dim, dtype, store, g)
+    tab, inf, nan = table.cpu(), float("inf"), float("nan")
+    put(cache, tab, 0, 7, 0, 5, inf)
+    put(cache, tab, 0, lens[0] - 1, 1, dim - 1, -inf)
+    put(cache, tab, 0, 3, 1, dim - 1, inf)               # not-a-number in that column
+    put(cache, tab, 1, 2, 0, 33, -inf)
+    put(cache, tab, 1, 1, 1, 40, nan)
+    last = len(lens) - 1
+    put(cache, tab, last, lens[last] + nodes - 1, 0, 8, inf)   # a node: its own rows and those of its descendants
+    put(cache, tab, last, lens[last], 1, 9, -inf)
+    put(cache, tab, last, lens[last] + nodes // 2, 1, 9, inf)
+    q *= 0.3                                                # no weight is 0 in 64 bits
+    parents = ints(some_trees(len(lens), nodes, rng))
+    check_special(cache, q, table, n, parents)
+    counts = ints(rng.integers(0, nodes + 1, len(lens)))
+    check_special(cache, q, table, n, parents, counts=counts)
+
+
+@pytest.mark.parametrize("dtype,store,dim,group,nodes", KINDS)
+@pytest.mark.parametrize("lens,page", [([300, 40, 129, 0, 70], 16), ([20000, 3], 64), ([100] * 90, 20)])
+def test_tree_values_near_the_ends_of_their_range(kv, dtype, store, dim, group, nodes, lens, page):  # noqa: F811
+    """Large finite values, whose products with weights that are not normed pass fp32's range: outputs are their means."""
+    if dtype == F16 and store == F16:
+        big = 6e4
+    else:
+        big = 3e38 if dtype == BF16 else 1e4
+    g, rng = torch.Generator().manual_seed(17), np.random.default_rng(17)
+    cache, q, table, n = setup(kv, lens, nodes, 2, group, page, dim, dtype, store, g)
+    if store == I8:
+        cache.v_scale.fill_(big / 127)
+        cache.v[:, :, :, ::2] = torch.randint(90, 128, cache.v[:, :, :, ::2].shape, generator=g).to(DEV, I8)
+    else:
+        cache.v.copy_((torch.rand(cache.v.shape, generator=g) * 2 - 1).to(DEV) * big)
+        cache.v[:, :, :, ::2] = (big * (0.9 + 0.1 * torch.rand(cache.v[:, :, :, ::2].shape, generator=g).to(DEV))).to(store)
+    check_special(cache, q, table, n, ints(some_trees(len(lens), nodes, rng)))
+
+
+def test_tree_not_finite_rows_and_values_together(kv):  # noqa: F811
+    """A query of not-a-numbers beside infinite values: its row is not-a-number in every column; without a place for the sums'
+    logarithms as well."""
+    L = pkg("_lib")
+    g = torch.Generator().manual_seed(18)
+    cache, q, table, n = setup(kv, [9000, 100, 40], 6, 2, 2, 16, 64, BF16, BF16, g)
+    q[0, 2, 1] = float("nan")
+    q[1, 3] = float("nan")
+    tab = table.cpu()
+    for b in range(3):
+        put(cache, tab, b, 5, b % 2, 7, float("inf"))
+    parents = ints([-1, 0, 1, 0, -1, 4])
+    check_special(cache, q, table, n, parents)
+    want, _ = cache.attend_tree(q, table, n, parents)
+    out = torch.full_like(want, float("nan"))
+    work = torch.empty(L.lib().fvs_kv_attend_tree_work(64, 12), dtype=torch.uint8, device=DEV)
+    rc = L.lib().fvs_kv_attend_tree(torch.cuda.current_stream().cuda_stream, cache._ref, L.BF16, q.data_ptr(), *q.stride()[:3], 4,
+                                    table.data_ptr(), 3, table.shape[1], table.stride(0), n.data_ptr(), parents.data_ptr(), 0, None, 6,
+                                    0.125, out.data_ptr(), None, work.data_ptr())
+    torch.cuda.synchronize()
+    assert rc == 0 and torch.equal(out.view(torch.int16) & 0x7fff, want.view(torch.int16) & 0x7fff)
