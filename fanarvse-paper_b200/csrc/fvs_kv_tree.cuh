@@ -182,6 +182,12 @@ __device__ __forceinline__ uint32_t idesc(int N, bool bf16, bool transposed) {
     const uint32_t t = bf16 ? 1u : 0u;
     return (1u << 4) | (t << 7) | (t << 10) | ((transposed ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
 }
+// The scale of a row of int8 keys.  It multiplies the score, where the formula multiplies the codes: with an infinite one their
+// products with q's elements are infinities of both signs, a not-a-number together.
+__device__ __forceinline__ float key_scale(const float* at) {
+    const float x = __ldg(at);
+    return __fadd_rn(__fsub_rn(x, x), x);
+}
 // values as the second operand: keys are the rows of 128 bytes, so N runs along memory; column blocks `lbo` bytes apart,
 // eight keys 1024 bytes apart
 __device__ __forceinline__ uint64_t values_desc(uint32_t addr, uint32_t lbo) {
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                     next_at = (uint32_t)(e / (I8 ? 16 : 8));
                     if (I8) {
                         const int64_t se = (int64_t)page * a.c.scale_page_stride + (int64_t)s * a.c.scale_slot_stride + (int64_t)head * a.c.scale_head_stride;
-                        ks = __ldg(a.c.k_scale + se);
+                        ks = key_scale(a.c.k_scale + se);
                         vs = __ldg(a.c.v_scale + se);
                     }
                 }
@@ -1165,7 +1171,7 @@ __device__ __forceinline__ bool stored(const Args& a, int b, int head, int x, St
     r.ks = r.vs = 1.f;
     if (STORE == FVS_I8) {
         const int64_t se = (int64_t)page * a.c.scale_page_stride + (int64_t)slot * a.c.scale_slot_stride + (int64_t)head * a.c.scale_head_stride;
-        r.ks = __ldg(a.c.k_scale + se);
+        r.ks = key_scale(a.c.k_scale + se);
         r.vs = __ldg(a.c.v_scale + se);
     }
     return true;

@@ -566,3 +566,12 @@ def test_tree_not_finite_rows_and_values_together(kv):  # noqa: F811
                                     0.125, out.data_ptr(), None, work.data_ptr())
     torch.cuda.synchronize()
     assert rc == 0 and torch.equal(out.view(torch.int16) & 0x7fff, want.view(torch.int16) & 0x7fff)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_tree_infinite_key_scales(kv, dtype):  # noqa: F811
+    """Codes of both signs times an infinite scale: a score of not-a-number, whatever the sign of the codes' own product."""
+    g = torch.Generator().manual_seed(20)
+    cache, q, table, n = setup(kv, [90, 300], 5, 2, 2, 16, 64, dtype, I8, g)
+    cache.k_scale[int(table[1, 4]), 1, 3] = float("inf")
+    check_special(cache, q, table, n, ints([-1, 0, 1, 1, -1]))
