@@ -269,9 +269,8 @@ class PagedKV:
         A node sees the visible ones of the first lens [sequences] logical tokens, its ancestors and itself; counts int32
         [sequences]: the nodes that a sequence has (default: all).  Returns (out like q, lse fp32 [sequences, nodes, query
         heads]): zeros and -inf where nothing is visible and for nodes that a sequence does not have.  One node is
-        `attend` with a length of lens + 1.  Hidden slots may hold anything; the nodes' own keys and values are finite (one
-        that is not may reach nodes that do not see it).  Visible values that are not finite do what the formula does; their
-        rows are computed again, which takes longer."""
+        `attend` with a length of lens + 1.  What a node does not see may hold anything.  Visible values that are
+        not finite do what the formula does; rows beside them are computed again, which takes longer."""
         shape = q.shape
         if not (len(shape) == 4 and shape[3] == self.dim and q.get_device() == self._index):
             raise ValueError(f"q is [sequences, nodes, heads, {self.dim}] on the cache's GPU")

@@ -540,9 +540,10 @@ int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, cons
  * counts (nullable) [seqs]: the nodes that a sequence has, all without it.  out and lse as fvs_kv_attend's, contiguous
  * [seqs, nodes, hq, dim] and [seqs, nodes, hq] (lse nullable); out 0 and lse -infinity for a node that sees nothing and for
  * nodes from counts[b] on.  Places before lens[b] that are not there may hold anything, and so may every place behind the
- * nodes; the nodes' own rows are finite (one that is not may reach nodes that do not see it).  Values that are not finite do
- * what the formula does (an infinity is its column's output, two against each other are not-a-number), and finite ones give
- * finite outputs up to the ends of their range; such rows are computed again, which takes longer (131000 tokens: 2 ms).
+ * nodes.  Values that are not finite do what the formula does (an infinity is its column's output, two against each other are
+ * not-a-number; a node's are nothing to nodes that do not see it), and finite ones give finite outputs up to the ends of their
+ * range; such rows are computed again, which takes longer (131000 tokens under 64 nodes: 2 ms, 92 beside a node of
+ * not-a-numbers).
  * A length above the table's row (or below 0) is cut to it; where the nodes reach past the row those places are not
  * there, with FVS_KV_BAD_INDEX.  nodes <= FVS_TREE_NODES (FVS_ERANGE above).  k, v and q span at most 64 GB each
  * (FVS_ERANGE; 16-bit caches whose pages are a multiple of 8 slots any size).

@@ -575,3 +575,29 @@ def test_tree_infinite_key_scales(kv, dtype):  # noqa: F811
     cache, q, table, n = setup(kv, [90, 300], 5, 2, 2, 16, 64, dtype, I8, g)
     cache.k_scale[int(table[1, 4]), 1, 3] = float("inf")
     check_special(cache, q, table, n, ints([-1, 0, 1, 1, -1]))
+
+
+@pytest.mark.parametrize("dtype,store,dim,group,nodes", KINDS[:6])
+@pytest.mark.parametrize("lens,page", [([300, 0, 129], 16), ([15000, 3, 1], 64), ([70] * 80, 20)])
+@pytest.mark.parametrize("x", [float("nan"), float("inf")])
+def test_tree_nodes_that_are_not_finite(kv, dtype, store, dim, group, nodes, lens, page, x):  # noqa: F811
+    """A draft's key or value of not-a-numbers or infinities is seen by itself and its descendants alone."""
+    g, rng = torch.Generator().manual_seed(19), np.random.default_rng(19)
+    cache, q, table, n = setup(kv, lens, nodes, 2, group, page, dim, dtype, store, g)
+    tab, parents = table.cpu(), some_trees(len(lens), nodes, rng)
+    for b in range(min(3, len(lens))):
+        for t, rows, scale in ((lens[b] + 1, cache.k, cache.k_scale), (lens[b] + nodes - 1, cache.v, cache.v_scale), (lens[b] + 2, cache.v, cache.v_scale)):
+            at = int(tab[b, t // page]), b % 2, t % page
+            if scale is None:
+                rows[at] = x
+            else:
+                scale[at] = x
+    q *= 0.3
+    sees = [O.sees(p) for p in parents[:3]]
+    assert any(not m[:, 1].all() and m[:, 1].sum() > 1 for m in sees)
+    check_special(cache, q, table, n, ints(parents))
+    out, lse = cache.attend_tree(q, table, n, ints(parents))
+    for b, m in enumerate(sees[:len(lens)]):
+        fine = torch.isfinite(out[b]).all(-1).all(-1).cpu().numpy()
+        clean = ~(m[:, 1] | m[:, 2] | m[:, nodes - 1])
+        assert fine[clean].all() and clean.any()
