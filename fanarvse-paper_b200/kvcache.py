@@ -351,16 +351,19 @@ class PagedKV:
         return held
 
     def check_status(self):
-        """Raises if a call since the last check, on any stream, met an index outside its table (waits for the GPU)."""
+        """Raises if a call since the last check, on any stream, met an index outside its table or gave up a wait (waits for the
+        GPU)."""
         torch.cuda.synchronize(self.device)
         status = int(self.status.item())
         if status != 0:
             self.status.zero_()
             torch.cuda.synchronize(self.device)  # so that a call on any stream from here on is seen
+            met = []
             if status & _lib.GAVE_UP:
-                raise _lib.FvsError("paged cache: a wait inside attend_tree ran out; its outputs are undefined")
-            raise _lib.FvsError("paged cache: an index was outside its table (page, sequence, token or position); "
-                                "that access was skipped")
+                met.append("a wait inside attend_tree ran out; its outputs are undefined")
+            if status & ~_lib.GAVE_UP:
+                met.append("an index was outside its table (page, sequence, token or position); that access was skipped")
+            raise _lib.FvsError("paged cache: " + "; ".join(met))
 
 
 def release_workspaces():

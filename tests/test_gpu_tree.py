@@ -601,3 +601,15 @@ def test_tree_nodes_that_are_not_finite(kv, dtype, store, dim, group, nodes, len
         fine = torch.isfinite(out[b]).all(-1).all(-1).cpu().numpy()
         clean = ~(m[:, 1] | m[:, 2] | m[:, nodes - 1])
         assert fine[clean].all() and clean.any()
+
+
+def test_tree_status_names_all_that_was_met(kv):  # noqa: F811
+    """A wait that ran out hides no index outside its table."""
+    FvsError = pkg("_lib").FvsError
+    cache = make_cache(kv, 4, 1, 16, 64, F16, torch.Generator().manual_seed(21))
+    for status, words in ((1, ["index"]), (2, ["ran out"]), (3, ["index", "ran out"])):
+        cache.status.fill_(status)
+        with pytest.raises(FvsError) as e:
+            cache.check_status()
+        assert [w for w in ("index", "ran out") if w in str(e.value)] == words
+        cache.check_status()
