@@ -19,9 +19,14 @@
 // for each pair of scores take 660 cycles for 32 columns of two warps of a quarter SM when they run alone (131000 tokens
 // under 64 nodes: 219 us where memory takes 84 and the matrix instructions with two parts of each weight 126).
 //
-// Rounding: scores, maxima, sums and O are fp32.  A weight enters the second product as two parts of the 16-bit type (its
-// rounded value and the rounded rest): 17 bits with bf16, 22 with fp16, where one part would double the error that the output's
-// own rounding makes; a third has no room in TMEM.  int8 codes are multiplied as bf16 with their key's scale in the weight.
+// Rounding: scores, maxima, sums and O are fp32.  A weight enters the second product as two parts of the 16-bit type, its
+// rounded value and the rounded rest: 22 bits over fp16 values and over int8 codes (as fp16, their scale in the weight), 17 over
+// bf16 values.  One part would double the error that the output's own rounding makes.  Outputs that are not the nearest
+// number, 64 sequences of 1 to 7700 keys, one node, heads of 128: bf16 1 in 676 (attend, which has 24 bits, 1 in 4096, products
+// in fp32 1 in 5958), fp16 1 in 333 (attend 512, fp32 705), over int8 codes 1 in 2427 bf16 ones (attend 4096, fp32 3121; 546 with
+// two bf16 parts) and 1 in 349 fp16 ones (attend 809, fp32 705; 84 with two bf16 parts).  64 nodes over 131000 bf16 keys:
+// 1 in 381, fp32 1 in 260.  A third bf16 part would be a third more of the matrix instructions, and half as much more of the TMEM
+// that a tile's scores leave, which heads of 128 do not have.
 // A row's weights are relative to a reference that rises only when they become large (LIMIT): O need not be rescaled at most
 // tiles, and the quotient is the same.
 #pragma once
@@ -275,6 +280,12 @@ __device__ __forceinline__ float exp2_of(float x) {
     return r;
 }
 
+__device__ __forceinline__ float log2_of(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // two fp32 operations in one instruction
 struct Two {
     uint64_t x;
@@ -337,10 +348,13 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     constexpr bool I8 = STORE == FVS_I8;
     constexpr int KEYS = S::KEYS, BUFFERS = S::BUFFERS, PART = S::PART, PARTS = KEYS / PART, W = S::W, RT = ROWS * MT, SLOTS = S::SLOTS, LEAD = S::LEAD;
     constexpr int INFO_BYTES = S::INFO_BYTES, PRODUCERS = S::PRODUCERS;
-    constexpr int VTYPE = I8 ? FVS_BF16 : TYPE;  // of weights and values
-    // the most that 32 weights may add up to before their reference rises; over fp16 values they lie in the upper part of
-    // fp16's range, LIMIT * LIFT at most
-    constexpr float LIMIT = VTYPE == FVS_F16 ? 127.f : 4096.f, LIFT = VTYPE == FVS_F16 ? 512.f : 1.f;
+    constexpr int VTYPE = I8 ? FVS_F16 : TYPE;  // of weights and values
+    // The most that 32 weights may add up to before their reference rises; over fp16 values they lie in the upper part of
+    // fp16's range, LIMIT * LIFT at most.  Over int8 codes it is the weights times the values' scales that enter the product:
+    // the reference follows these, 2^UP below the largest, and the weights alone only have to stay in fp32's range (scales
+    // outside 2^-FAR to 2^FAR count as its ends).
+    constexpr float UP = 9.f, FAR = 100.f, MOST = 0x1p115f;
+    constexpr float LIMIT = I8 ? 127.f * 512.f : VTYPE == FVS_F16 ? 127.f : 4096.f, LIFT = !I8 && VTYPE == FVS_F16 ? 512.f : 1.f;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -714,7 +728,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                             fetch(rk, kbase);
                         }
                     } else {
-                        widen(rv, std::integral_constant<int, FVS_BF16>());
+                        widen(rv, std::integral_constant<int, FVS_F16>());
                         if (t + 1 < t1) fetch(rv, vbase);
                     }
                     advance();
@@ -967,7 +981,10 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                         if (__builtin_expect(raise, 0)) {
                             float top = __int_as_float(0xff800000);
 #pragma unroll
-                            for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(s[j]));
+                            for (int j = 0; j < 32; j++) {
+                                const float x = __uint_as_float(s[j]);
+                                top = fmaxf(top, I8 ? x + fminf(fmaxf(log2_of(fabsf(ks[KEYS + 32 * k + j])), -FAR), FAR) - UP : x);
+                            }
                             if (!I8) top *= lift;
                             const float to = need ? fmaxf(m, top) : m, by = m == to ? 1.f : exp2_of(m - to);
                             m = to;
@@ -1011,17 +1028,35 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                         const float off = m == __int_as_float(0xff800000) ? 0.f : m;
                         const Two minus = two(-off, -off);
                         Two sums[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+                        Two scaled[2] = {two(0.f, 0.f), two(0.f, 0.f)};  // int8: sums with the values' scales
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const Two raw = two(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-                            const float2 x = one(I8 ? add2(raw, minus) : fma2(raw, factor, minus));
-                            s[j] = __float_as_uint(exp2_of(x.x)), s[j + 1] = __float_as_uint(exp2_of(x.y));
-                            sums[(j / 2) & 1] = add2(sums[(j / 2) & 1], two(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+                        for (int j = 0; j < 32; j += 4) {
+                            float4 f;
+                            if (I8) f = *reinterpret_cast<const float4*>(ks + KEYS + 32 * k + j);
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                const int i = j + 2 * y;
+                                const Two raw = two(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                                const float2 x = one(I8 ? add2(raw, minus) : fma2(raw, factor, minus));
+                                Two p = two(exp2_of(x.x), exp2_of(x.y));
+                                sums[y] = add2(sums[y], p);
+                                if (I8) {
+                                    p = mul2(p, y ? two(f.z, f.w) : two(f.x, f.y));
+                                    scaled[y] = add2(scaled[y], p);
+                                }
+                                const float2 w2 = one(p);
+                                s[i] = __float_as_uint(w2.x), s[i + 1] = __float_as_uint(w2.y);
+                            }
                         }
                         const float2 pair = one(add2(sums[0], sums[1]));
                         const float sum = pair.x + pair.y;
                         // (not-a-numbers and rows that have seen nothing yet are taken again once)
-                        need = !(sum <= LIMIT) || m == __int_as_float(0xff800000);
+                        if (I8) {
+                            const float2 both = one(add2(scaled[0], scaled[1]));
+                            need = !(both.x + both.y <= LIMIT && sum <= MOST) || m == __int_as_float(0xff800000);
+                        } else {
+                            need = !(sum <= LIMIT) || m == __int_as_float(0xff800000);
+                        }
                         if (__any_sync(0xffffffffu, need) && !raise) {
                             raise = true;
                             continue;
@@ -1033,12 +1068,9 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
                             uint32_t hi[8], lo[8];
 #pragma unroll
                             for (int j = 0; j < 16; j += 4) {
-                                float4 f;
-                                if (I8) f = *reinterpret_cast<const float4*>(ks + KEYS + 32 * k + h + j);
 #pragma unroll
                                 for (int y = 0; y < 2; y++) {
                                     Two p = two(__uint_as_float(s[h + j + 2 * y]), __uint_as_float(s[h + j + 2 * y + 1]));
-                                    if (I8) p = mul2(p, y ? two(f.z, f.w) : two(f.x, f.y));
                                     if (LIFT != 1.f) p = mul2(p, two(LIFT, LIFT));
                                     const float2 w2 = one(p);
                                     hi[j / 2 + y] = Elem<VTYPE>::down(w2.x, w2.y);

@@ -613,3 +613,130 @@ def test_tree_status_names_all_that_was_met(kv):  # noqa: F811
             cache.check_status()
         assert [w for w in ("index", "ran out") if w in str(e.value)] == words
         cache.check_status()
+
+
+@pytest.mark.parametrize("dtype,dim,group,nodes", [(BF16, 128, 8, 32), (F16, 64, 2, 10), (F16, 96, 4, 40), (BF16, 192, 1, 3)])
+@pytest.mark.parametrize("kind", ["wide", "rising", "falling", "zeros", "signs"])
+def test_tree_value_scales_far_apart(kv, dtype, dim, group, nodes, kind):  # noqa: F811
+    """int8 values whose scales differ by 2^60 from key to key, rise or fall along the sequence, are 0 beside the largest weights,
+    or negative.  Weights times scales enter the product as fp16 numbers of 22 bits, of 2^-25 beside 2^9 for the largest met so
+    far: off by 2^-34 of it a key.  A scale of 0 counts as 2^-100 there: where such a key weighs most, 2^-25 beside 2^(9 + 100) for
+    its weight, which is at most the sum, times a code of 127 is 2^-127 a key."""
+    g, rng = torch.Generator().manual_seed(22), np.random.default_rng(22)
+    lens, page, heads = [300, 40, 1000], 16, 2
+    cache, q, table, n = setup(kv, lens, nodes, heads, group, page, dim, dtype, I8, g)
+    q *= 0.5
+    tab = table.cpu().long()
+    order = torch.zeros(cache.pages * page)
+    for b, m in enumerate(lens):
+        t = torch.arange(m + nodes)
+        order[tab[b, t // page] * page + t % page] = t.float()
+    order = order.view(cache.pages, 1, page).to(DEV)
+    far = torch.rand(cache.v_scale.shape, generator=g).to(DEV)
+    if kind == "wide":
+        cache.v_scale *= 2.0 ** (60 * far - 30).round()
+    elif kind in ("rising", "falling"):
+        cache.v_scale *= 2.0 ** ((order if kind == "rising" else 1000 - order) / 10 - 50).round()
+    elif kind == "zeros":
+        top = far < 0.3                                       # these keys weigh most, and have no value
+        cache.k_scale[top] *= 30
+        cache.v_scale[top] = 0
+    else:
+        cache.v_scale[far < 0.5] *= -1
+    parents = ints(some_trees(len(lens), nodes, rng))
+    out, lse = cache.attend_tree(q, table, n, parents)
+    torch.cuda.synchronize()
+    k, v = values(cache)
+    scale = dim ** -0.5
+    eo, el, pv, mag = O.attend_tree(c(q), k, v, c(table), c(n), c(parents), None, scale)
+    L = max(lens) + nodes
+    es = (dim + 4) * 2.0 ** -23 * mag[..., None]
+    bound = U[dtype] * np.abs(eo) + (2.0 ** -21 + 2 * es + 2.0 ** -20 + (L + 64) * 2.0 ** -22) * pv + L * (2.0 ** -34 * pv.max(-1, keepdims=True) + 2.0 ** -127) + (2.0 ** -25 if dtype == F16 else 0)
+    out = c(out).astype(np.float64)
+    over = np.abs(eo) >= 65504 * (1 - 2.0 ** -12) if dtype == F16 else np.zeros(eo.shape, bool)   # outputs past fp16's range
+    assert np.isfinite(out[~over]).all() and (np.abs(out[over]) >= 65504 * (1 - 2.0 ** -10)).all()
+    with np.errstate(invalid="ignore"):
+        worst = (np.abs(out - eo) / bound)[~over].max(initial=0)
+    assert worst <= 1, f"out is {worst:.2f} of its bound"
+    tol = 2 * es[..., 0] + (L + 64) * 2.0 ** -22 + 2.0 ** -20 * (1 + np.abs(el))
+    assert (np.abs(c(lse) - el) <= tol).all()
+    cache.check_status()
+
+
+@pytest.mark.parametrize("dtype,store,part", [(BF16, BF16, 2.0 ** -17), (F16, F16, 2.0 ** -21), (BF16, I8, 2.0 ** -21), (F16, I8, 2.0 ** -21)])
+@pytest.mark.parametrize("dim,group", [(64, 2), (128, 40), (192, 1)])
+def test_tree_weights_keep_their_second_part(kv, dtype, store, part, dim, group):  # noqa: F811
+    """Two keys whose weighted values all but cancel: what is left shows a weight's own rounding, which with one 16-bit part
+    misses the bound by far.  Scores are single exact products, so that no sum adds to the bound; an exponential is within
+    2^-21, a sum of two and the quotient within 2^-23 together."""
+    g = torch.Generator().manual_seed(23)
+    B, nodes = 24, 5
+    cache, q, table, n = setup(kv, [2] * B, nodes, 1, group, 16, dim, dtype, store, g)
+    at = table[:, 0].long()
+    first = torch.rand(B, generator=g) * 1.4 + 0.1             # scores' difference
+    q.zero_()
+    q[..., 0] = 1.0
+    cache.k[at] = 0
+    if store == I8:
+        cache.k[at, :, 0, 0] = 64
+        cache.k_scale[at] = (first / 64).to(DEV)[:, None, None]
+        cache.v_scale[at] = 1 / 64
+    else:
+        cache.k[at, :, 0, 0] = first.to(DEV, store)[:, None]
+    k, _ = values(cache)
+    d = torch.tensor(k[c(at), 0, 0, 0])                       # 64 bits
+    ratio = torch.exp(d)                                       # of the two weights
+    if store == I8:                                            # w0 a - w1 b, of codes near a / b = w1 / w0
+        b = torch.arange(dim) % 60 + 60
+        a = (b[None] / ratio[:, None]).round()
+        cache.v[at, 0, 0], cache.v[at, 0, 1] = a.to(DEV, I8), -b.expand(B, dim).to(DEV, I8)
+    else:
+        b = 1 + torch.arange(dim) / 256
+        cache.v[at, 0, 0], cache.v[at, 0, 1] = (b[None] / ratio[:, None]).to(DEV, store), -b.expand(B, dim).to(DEV, store)
+    # each node sees the two keys and itself: its own key weighs nothing beside them
+    own = at
+    for i in range(nodes):
+        cache.k[own, 0, 2 + i] = 0
+        if store == I8:
+            cache.k[own, 0, 2 + i, 0], cache.k_scale[own, 0, 2 + i] = -127, 1.0
+        else:
+            cache.k[own, 0, 2 + i, 0] = -100.0
+    parents = ints(np.full(nodes, -1))
+    out, lse = cache.attend_tree(q, table, n, parents, scale=1.0)
+    k, v = values(cache)
+    eo, el, pv, _ = O.attend_tree(c(q), k, v, c(table), c(n), np.broadcast_to(c(parents), (B, nodes)), None, 1.0)
+    bound = U[dtype] * np.abs(eo) + (part + 2.0 ** -21 + 2.0 ** -23 + 2.0 ** -22) * pv + 2.0 ** -34 * np.abs(v[c(at)]).max() + (2.0 ** -25 if dtype == F16 else 0)
+    worst = (np.abs(c(out) - eo) / bound).max()
+    assert worst <= 1, f"out is {worst:.2f} of its bound"
+    # the same with weights rounded to one part
+    w = np.stack([np.ones(B), np.exp(-c(d))], 1)
+    one = torch.tensor(w * (512 if store != BF16 else 1)).to(F16 if store != BF16 else BF16).double().numpy()
+    vv = v[c(at), 0, :2]
+    cut = (one[..., None] * vv).sum(1) / (w.sum(1) * (512 if store != BF16 else 1))[:, None]
+    assert (np.abs(cut - eo[:, 0, 0]) / bound[:, 0, 0]).max() > 20
+
+
+@pytest.mark.parametrize("dtype,store,group,dim,nodes", [(BF16, BF16, 2, 64, 3), (F16, I8, 1, 128, 40), (F16, F16, 8, 64, 33), (BF16, BF16, 4, 192, 5)])
+def test_tree_no_share_is_lost(kv, dtype, store, group, dim, nodes):  # noqa: F811
+    """One long context whose every run of keys has a column of its own: an output without one CTA's share (a 296th of the keys or
+    more) would be far off its bound in that run's column, and so would its lse's tighter one."""
+    g, rng = torch.Generator().manual_seed(24), np.random.default_rng(24)
+    L = 60000
+    cache, q, table, n = setup(kv, [L], nodes, 1, group, 64, dim, dtype, store, g)
+    q *= 0.1
+    run = torch.zeros(cache.pages, 64, dtype=torch.long)
+    t = torch.arange(L + nodes)
+    run[table.cpu()[0, t // 64].long(), t % 64] = t * dim // (L + nodes)
+    one = torch.nn.functional.one_hot(run, dim)[:, None].to(DEV)
+    if store == I8:
+        cache.v.copy_(one)
+        cache.v_scale.fill_(1.0)
+    else:
+        cache.v.copy_(one)
+    parents = ints(some_trees(1, nodes, rng))
+    check_tree(cache, q, table, n, parents)
+    # the same bounds for an output without 200 keys of a run (a share has 202 or more)
+    k, v = values(cache)
+    eo, el, pv, mag = O.attend_tree(c(q), k, v, c(table), c(n), c(parents), None, dim ** -0.5)
+    bound = U[dtype] * np.abs(eo) + (2.0 ** -17 + 2.0 ** -20 + (L + nodes + 64) * 2.0 ** -22) * pv * 1.01
+    assert (eo[..., :dim - 1] * 200 / ((L + nodes) / dim) / 2 > 2 * bound[..., :dim - 1]).all()
