@@ -1521,7 +1521,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, RT == 256 && STORE == FVS_I8 ? 8
                 for (int j = 0; j < COLS; j++) x[j] = p[j * RT];  // of a CTA without a share: anything, and not added
 #pragma unroll
                 for (int j = 0; j < COLS; j++)
-                    if (top != NONE && by != 0.f) o[j] = fmaf(x[j], by, o[j]);
+                    if (top != NONE) o[j] = fmaf(x[j], by, o[j]);
             }
             const float by = l == 0.f ? 0.f : 1.f / l;
             uint32_t packed[COLS / 2];

@@ -740,3 +740,25 @@ def test_tree_no_share_is_lost(kv, dtype, store, group, dim, nodes):  # noqa: F8
     eo, el, pv, mag = O.attend_tree(c(q), k, v, c(table), c(n), c(parents), None, dim ** -0.5)
     bound = U[dtype] * np.abs(eo) + (2.0 ** -17 + 2.0 ** -20 + (L + nodes + 64) * 2.0 ** -22) * pv * 1.01
     assert (eo[..., :dim - 1] * 200 / ((L + nodes) / dim) / 2 > 2 * bound[..., :dim - 1]).all()
+
+
+@pytest.mark.parametrize("dtype,store,dim", [(BF16, BF16, 128), (F16, F16, 64), (BF16, I8, 64)])
+@pytest.mark.parametrize("n", [200, 30000])
+def test_tree_infinite_value_of_a_small_weight(kv, dtype, store, dim, n):  # noqa: F811
+    """A weight that fp32 does not hold is above zero all the same: in its own tile, and as a share of its own."""
+    g = torch.Generator().manual_seed(25)
+    cache, q, table, lens = setup(kv, [n], 6, 1, 4, 16, dim, dtype, store, g)
+    tab = table.cpu()
+    q *= 0.1
+    q[..., 0] = 20.0
+    row = table[0, :3 if n < 1000 else 64].long()           # the first keys (more than a share): 400 nats below the others
+    if store == I8:
+        cache.k_scale.fill_(0.01)
+        cache.k[..., 0] = 0
+        cache.k[row, :, :, 0], cache.k_scale[row] = -127, 20 / 127
+    else:
+        cache.k[..., 0] = 0
+        cache.k[row, :, :, 0] = -20.0
+    put(cache, tab, 0, 5, 0, 7, float("inf"))
+    put(cache, tab, 0, 40, 0, 9, float("-inf"))
+    check_special(cache, q, table, lens, ints([-1, 0, 0, 1, 2, -1]), scale=1.0)
