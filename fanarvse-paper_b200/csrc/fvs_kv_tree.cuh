@@ -351,9 +351,9 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
     constexpr int VTYPE = I8 ? FVS_F16 : TYPE;  // of weights and values
     // The most that 32 weights may add up to before their reference rises; over fp16 values they lie in the upper part of
     // fp16's range, LIMIT * LIFT at most.  Over int8 codes it is the weights times the values' scales that enter the product:
-    // the reference follows these, 2^UP below the largest, and the weights alone only have to stay in fp32's range (scales
-    // outside 2^-FAR to 2^FAR count as its ends).
-    constexpr float UP = 9.f, FAR = 100.f, MOST = 0x1p115f;
+    // the reference follows these, 2^UP below the largest, and the weights alone only have to stay in fp32's range, their sum over
+    // 2^31 keys too (scales outside 2^-FAR to 2^FAR count as its ends; a weight is 2^(UP + FAR) at most where the reference rises).
+    constexpr float UP = 9.f, FAR = 80.f, MOST = 0x1p95f;
     constexpr float LIMIT = I8 ? 127.f * 512.f : VTYPE == FVS_F16 ? 127.f : 4096.f, LIFT = !I8 && VTYPE == FVS_F16 ? 512.f : 1.f;
 
     extern __shared__ uint8_t smem_raw[];

@@ -620,8 +620,8 @@ def test_tree_status_names_all_that_was_met(kv):  # noqa: F811
 def test_tree_value_scales_far_apart(kv, dtype, dim, group, nodes, kind):  # noqa: F811
     """int8 values whose scales differ by 2^60 from key to key, rise or fall along the sequence, are 0 beside the largest weights,
     or negative.  Weights times scales enter the product as fp16 numbers of 22 bits, of 2^-25 beside 2^9 for the largest met so
-    far: off by 2^-34 of it a key.  A scale of 0 counts as 2^-100 there: where such a key weighs most, 2^-25 beside 2^(9 + 100) for
-    its weight, which is at most the sum, times a code of 127 is 2^-127 a key."""
+    far: off by 2^-34 of it a key.  A scale of 0 counts as 2^-80 there: where such a key weighs most, 2^-25 beside 2^(9 + 80) for
+    its weight, which is at most the sum, times a code of 127 is 2^-107 a key."""
     g, rng = torch.Generator().manual_seed(22), np.random.default_rng(22)
     lens, page, heads = [300, 40, 1000], 16, 2
     cache, q, table, n = setup(kv, lens, nodes, heads, group, page, dim, dtype, I8, g)
@@ -651,7 +651,7 @@ def test_tree_value_scales_far_apart(kv, dtype, dim, group, nodes, kind):  # noq
     eo, el, pv, mag = O.attend_tree(c(q), k, v, c(table), c(n), c(parents), None, scale)
     L = max(lens) + nodes
     es = (dim + 4) * 2.0 ** -23 * mag[..., None]
-    bound = U[dtype] * np.abs(eo) + (2.0 ** -21 + 2 * es + 2.0 ** -20 + (L + 64) * 2.0 ** -22) * pv + L * (2.0 ** -34 * pv.max(-1, keepdims=True) + 2.0 ** -127) + (2.0 ** -25 if dtype == F16 else 0)
+    bound = U[dtype] * np.abs(eo) + (2.0 ** -21 + 2 * es + 2.0 ** -20 + (L + 64) * 2.0 ** -22) * pv + L * (2.0 ** -34 * pv.max(-1, keepdims=True) + 2.0 ** -107) + (2.0 ** -25 if dtype == F16 else 0)
     out = c(out).astype(np.float64)
     over = np.abs(eo) >= 65504 * (1 - 2.0 ** -12) if dtype == F16 else np.zeros(eo.shape, bool)   # outputs past fp16's range
     assert np.isfinite(out[~over]).all() and (np.abs(out[over]) >= 65504 * (1 - 2.0 ** -10)).all()
@@ -762,3 +762,18 @@ def test_tree_infinite_value_of_a_small_weight(kv, dtype, store, dim, n):  # noq
     put(cache, tab, 0, 5, 0, 7, float("inf"))
     put(cache, tab, 0, 40, 0, 9, float("-inf"))
     check_special(cache, q, table, lens, ints([-1, 0, 0, 1, 2, -1]), scale=1.0)
+
+
+def test_tree_long_run_of_values_of_zero(kv):  # noqa: F811
+    """Every key but a few has a value scale of 0 and all of the weight: the sum of their weights, 2^89 each, stays finite."""
+    g = torch.Generator().manual_seed(26)
+    n = 400000
+    cache, q, table, lens = setup(kv, [n], 2, 1, 2, 64, 64, BF16, I8, g)
+    cache.v_scale[:] = 0
+    cache.k[:] = 0
+    cache.v_scale[table[0, -1].long(), :, :(n + 2) % 64] = 1.0
+    out, lse = cache.attend_tree(q, table, lens, ints([-1, 0]))
+    k, v = values(cache)
+    eo, el, pv, _ = O.attend_tree(c(q), k, v, c(table), c(lens), np.array([[-1, 0]]), None, 0.125)
+    assert (np.abs(c(lse) - el) <= 2.0 ** -20 * np.abs(el) + (n + 64) * 2.0 ** -22).all() and np.isfinite(c(lse)).all()
+    assert (np.abs(c(out) - eo) <= 2.0 ** -8 * np.abs(eo) + (n + 64) * 2.0 ** -22 * pv).all()
