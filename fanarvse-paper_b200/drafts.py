@@ -2,9 +2,12 @@
 model takes.
 
 A tree of a sequence is `parents`: int32 [nodes], node i stands behind node parents[i], or behind the sequence itself
-where that is -1; parents come before their children.  One step over a `PagedKV` cache: append the nodes at the places
-behind the sequence (rotated at the positions that their depth gives), `PagedKV.attend_tree` in every layer, `verify`, and
-`PagedKV.compact` in every layer.  The reference has no counterpart: it ends with the found rows' ids.
+where that is -1; parents come before their children.  One step over a `PagedKV` cache, with one token of each sequence
+pending (drawn, not in the cache yet): append it and the nodes behind it at the places behind the sequence (rotated at the
+positions that their depth gives) and `PagedKV.attend_tree` in every layer, with the pending token as node 0 of a tree [-1] +
+[p + 1 for p in parents]; `verify`, whose target has a row behind the pending token and one behind each node; and in every layer
+`PagedKV.compact` of 0 and the path's nodes + 1.  The drawn token is pending then.  The reference has no counterpart: it ends
+with the found rows' ids.
 
 Calls run on the current torch stream, neither synchronise nor read device memory on the host, and can be captured into a
 CUDA graph.
