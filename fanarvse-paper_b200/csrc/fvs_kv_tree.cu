@@ -19,7 +19,7 @@ extern template int launch_types<256>(fvs_stream_t, Args, int);
 using namespace fvs::kv;
 
 // two partial results of each CTA, of as many rows as an item has, behind DESC words of each CTA: two CTAs of 128 rows an SM
-// with heads up to 128, else one
+// with heads up to 128, else one.  The same for every number of rows
 extern "C" int fvs_kv_attend_tree_work(int dim, int rows) {
     if (dim < 1 || rows < 0) return FVS_EINVAL;
     if (dim > 256) return FVS_ERANGE;

@@ -2,8 +2,8 @@
 //
 // Node i of sequence b lies at logical place lens[b] + i and sees every token before lens[b], its ancestors and itself:
 // out = sum_t softmax_t(scale <q, k_t>) v_t.  The nodes' query heads of one key head are the rows of one product: rows =
-// nodes * (hq / heads), so that keys and values are read once for all of them.  With 4 rows * dim flops per 4 * dim bytes of a
-// 16-bit key and value, memory bounds a call up to about 250 rows and the matrix instructions above that.
+// nodes * (hq / heads), so that keys and values are read once for all of them.  With 6 rows * dim flops (both parts of a weight
+// count) per 4 * dim bytes of a 16-bit key and value, memory bounds a call up to about 170 rows and the matrix instructions above.
 //
 // One or two CTAs an SM (Shape), each with a share of equal cost of all items (sequence, key head, up to 256 rows), cut anywhere
 // between tiles of KEYS keys; what is cut goes through the workspace and join_kernel.  Inside a CTA, a stream of tiles:
@@ -14,10 +14,12 @@
 //   matrix instructions (a thread for each softmax warpgroup): S = Q K^T into TMEM, and, when the rows' weights lie there in
 //     place of S, O += P V; where TMEM has room a tile's S is issued before the O of the tile before.
 //   softmax warpgroups, a thread per row: weights and their sum; at a segment's end the output or the share of one.
-// What bounds it: up to 128 rows the copies' latency and a segment's beginning and end (64 ragged requests of 64 rows: 82 us
-// where the bytes take 48, a rate of 3.9 TB/s); with 256 rows the softmax warps, whose 11 instructions and 2 exponentials
-// for each pair of scores take 660 cycles for 32 columns of two warps of a quarter SM when they run alone (131000 tokens
-// under 64 nodes: 219 us where memory takes 84 and the matrix instructions with two parts of each weight 126).
+// What bounds it: up to 128 rows no unit (64 ragged requests of 64 rows: 83 us where the bytes take 48, a rate of 3.8 TB/s, tensor
+// pipe 44 %, issue slots 31 %): a CTA's tiles wait for one another (copy, scores, weights, outputs; one O, so that a segment's
+// products wait for the one before to be read out), and 8 us are the join.  With 256 rows the softmax warps, whose 11
+// instructions and 2 exponentials for each pair of scores take 660 cycles for 32 columns of two warps of a quarter SM when they
+// run alone (131000 tokens under 64 nodes: 218 us at best where memory takes 84 and the matrix instructions with two parts of each
+// weight 126).
 //
 // Rounding: scores, maxima, sums and O are fp32.  A weight enters the second product as two parts of the 16-bit type, its
 // rounded value and the rounded rest: 22 bits over fp16 values and over int8 codes (as fp16, their scale in the weight), 17 over

@@ -6,12 +6,12 @@
 // r_{k+1} = max(r_k - m_k q, 0) and m_{k+1} = sum r_{k+1}, unless that is 0.  Where none is taken the next token is drawn from
 // r_k: the first whose running sum passes u_last sum(r_k).  Taken this way the tokens are distributed as the target's own.
 //
-// All of it is in fp64: p and q are exact in it and so is a first difference, so that a decision depends on the order of a
-// sum only within 1e-16 of its border.
+// All of it is in fp64: p and q are exact in it and so is a first difference of numbers less than 2^29 apart, so that a
+// decision depends on the order of a sum only within 1e-16 of its border.
 //
 // Whether a node is taken without a refusal before it needs two numbers, gathered for all nodes at once; a whole row (and
-// the draft's) is read only for a node's refused child and for the last draw: 2 V elements of a sequence where the floor is
-// V (1 + draft), each pass after the first from L2.  A cluster of CTAs shares a row, since one SM reads it at 1/148 of the
+// the draft's) is read only for a node's refused child and for the last draw, a pass over V (1 + draft) elements each: the
+// floor is one pass, more of a row come from L2.  A cluster of CTAs shares a row, since one SM reads it at 1/148 of the
 // memory's rate; the sums of its CTAs are exchanged through distributed shared memory and added in order of rank, so that
 // every CTA comes to the same numbers and walks the same path by itself.
 // What bounds it: a sequence's passes behind one another, each with a cluster's barrier at its end.  64 x 16 nodes over
@@ -76,7 +76,7 @@ struct Shared {
 };
 
 // r_k of element v of the present row: as every m_j and q is at least 0, max(.. max(p - m_0 q, 0) .. - m_{k-1} q, 0) is max(p -
-// M q, 0) with M their sum.  M is 1 for k = 1, and a difference of two fp32 numbers is exact in fp64.
+// M q, 0) with M their sum.  M is 1 for k = 1, and a difference of two fp32 numbers less than 2^29 apart is exact in fp64.
 __device__ __forceinline__ double rest_of(float p, float q, double M) {
     const double r = fma(-M, (double)q, (double)p);
     // the sign over both words: a comparison of fp64 numbers and two selections took 49 us where this takes 45

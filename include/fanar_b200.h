@@ -547,7 +547,8 @@ int fvs_kv_attend(fvs_stream_t stream, const fvs_kv_cache* cache, int type, cons
  * A length above the table's row (or below 0) is cut to it; where the nodes reach past the row those places are not
  * there, with FVS_KV_BAD_INDEX.  nodes <= FVS_TREE_NODES (FVS_ERANGE above).  k, v and q span at most 64 GB each
  * (FVS_ERANGE; 16-bit caches whose pages are a multiple of 8 slots any size).
- * work: fvs_kv_attend_tree_work(dim, nodes * (hq / heads)) bytes of device memory, 16-byte aligned, of any contents.  Calls that
+ * work: fvs_kv_attend_tree_work(dim, nodes * (hq / heads)) bytes of device memory (now the same for every number of rows),
+ * 16-byte aligned, of any contents.  Calls that
  * may run at the same time need their own; those on one stream, from whatever threads, may share one (a call's launches are
  * never between another's).
  */

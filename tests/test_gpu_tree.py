@@ -777,3 +777,36 @@ def test_tree_long_run_of_values_of_zero(kv):  # noqa: F811
     eo, el, pv, _ = O.attend_tree(c(q), k, v, c(table), c(lens), np.array([[-1, 0]]), None, 0.125)
     assert (np.abs(c(lse) - el) <= 2.0 ** -20 * np.abs(el) + (n + 64) * 2.0 ** -22).all() and np.isfinite(c(lse)).all()
     assert (np.abs(c(out) - eo) <= 2.0 ** -8 * np.abs(eo) + (n + 64) * 2.0 ** -22 * pv).all()
+
+
+def test_tree_not_finite_in_graphs_and_on_streams(kv):  # noqa: F811
+    """Rows that are computed again: captured, replayed after the values changed, and beside another stream's calls."""
+    g, rng = torch.Generator().manual_seed(27), np.random.default_rng(27)
+    cache, q, table, n = setup(kv, [5000, 90, 300], 12, 2, 4, 16, 128, BF16, BF16, g)
+    q *= 0.3
+    tab, parents = table.cpu(), ints(some_trees(3, 12, rng))
+    put(cache, tab, 0, 77, 0, 3, float("inf"))
+    put(cache, tab, 2, 301, 1, 100, float("nan"))
+    other, q2, table2, n2 = setup(kv, [4000], 64, 2, 4, 16, 128, BF16, BF16, g)
+    put(other, table2.cpu(), 0, 4001, 1, 5, float("-inf"))
+    parents2 = ints(some_trees(1, 64, rng))
+    want, want2 = cache.attend_tree(q, table, n, parents), other.attend_tree(q2, table2, n2, parents2)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got = cache.attend_tree(q, table, n, parents)
+    same = lambda a, b: all(torch.equal(x.view(torch.int16 if x.element_size() == 2 else torch.int32), y.view(torch.int16 if y.element_size() == 2 else torch.int32)) for x, y in zip(a, b))  # noqa: E731
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            graph.replay()
+        beside = other.attend_tree(q2, table2, n2, parents2)
+        torch.cuda.synchronize()
+        assert same(got, want) and same(beside, want2)
+    check_special(cache, q, table, n, parents, got=got)
+    put(cache, tab, 0, 77, 0, 3, 1.0)
+    put(cache, tab, 1, 3, 1, 60, float("-inf"))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph.replay()
+    torch.cuda.synchronize()
+    check_special(cache, q, table, n, parents, got=got)
