@@ -84,7 +84,7 @@ struct Shape {
     // warpgroups took turns at the tiles took 115 us where this took 107, at 64 ragged requests of 64 rows)
     static constexpr int CTAS = MT == 1 && D <= 128 ? 2 : 1;
     static constexpr int W = MT;  // softmax warpgroups
-    // keys of a tile: 128 where the codes' widening is the slower part (403 us where 64 took 445, at 24 long int8 contexts under
+    // keys of a tile: 128 where the codes' widening is the slower part (388 us where 64 took 436, at 24 long int8 contexts under
     // 32 nodes), else 64, whose scores are computed a tile ahead (229 where 128 took 254, at 131000 tokens under 64 nodes)
     static constexpr int KEYS = MT == 2 && STORE == FVS_I8 ? 128 : 64;
     // keys whose weights enter O together, while the softmax warps are at the next ones: half a tile (131000 tokens under 64
@@ -1183,7 +1183,7 @@ __global__ void __launch_bounds__(Shape<D, STORE, MT, QR>::THREADS, Shape<D, STO
 // is not finite where the sum of weights is) are computed again from the formula, behind everything else, by the block that
 // holds them: a column is what its values that are not finite make of it (weights are above zero), or, where a row sees none,
 // the mean of its values by weights of at most one.  Finite inputs pay for a look at O and for the blocks of this code: 24 long
-// int8 contexts under 32 nodes 386 us (381 without), 32 x 10 passages 64.2 (63.7), 131000 tokens under 64 nodes nothing.  Others
+// int8 contexts under 32 nodes 386 us (381 without), 32 x 10 passages 63.3 (61.7), 131000 tokens under 64 nodes nothing.  Others
 // pay for what is computed again: of those 131000 tokens 2 ms for an infinite value in one key head, 92 for a not-a-number
 // in a node, whose siblings' scores are taken again; one short passage 60 and 120 us.
 constexpr int JOIN_COLS = 32, JOIN_THREADS = 256, JOIN_LEAST = 96;  // JOIN_LEAST: CTAs whose maxima leave room for a Redo
