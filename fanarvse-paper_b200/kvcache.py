@@ -303,10 +303,10 @@ class PagedKV:
         if n == 0 or nodes == 0:
             return out, lse
         stream = self._stream()
+        work = self._tree_workspace(stream, nodes * (hq // self.heads))  # held until the launches are made, whatever others do
         check(self._attend_tree(stream, self._ref, ty, at, s0, s1, s2, hq, *ta, la, parents.data_ptr(),
                                 nodes if parents.dim() == 2 else 0, ca, nodes, self.scale if scale is None else scale, oa,
-                                lse.data_ptr(), self._tree_workspace(stream, nodes * (hq // self.heads)).data_ptr()),
-              "kv_attend_tree")
+                                lse.data_ptr(), work.data_ptr()), "kv_attend_tree")
         self.launches += 2
         return out, lse
 

@@ -8,6 +8,7 @@ Bounds, from the arithmetic alone (u: unit roundoff of the output type):
 * sums over L keys in fp32, cut or rounded: (L + 64) 2^-22 of sum p |v|; one rounding of the output.
 """
 import threading
+import weakref
 
 import numpy as np
 import pytest
@@ -810,3 +811,27 @@ def test_tree_not_finite_in_graphs_and_on_streams(kv):  # noqa: F811
         graph.replay()
     torch.cuda.synchronize()
     check_special(cache, q, table, n, parents, got=got)
+
+
+def test_tree_workspace_is_held_for_the_launches(kv, monkeypatch):  # noqa: F811
+    """Another thread may give the stream's workspace back, or put a larger one in its place, while a call is made: its memory is
+    nobody else's before the launches are on the stream."""
+    g = torch.Generator().manual_seed(28)
+    cache, q, table, n = setup(kv, [70], 3, 1, 2, 16, 64, BF16, BF16, g)
+    held = []
+    find, launch = cache._tree_workspace, cache._attend_tree
+
+    def found(*args):
+        work = find(*args)
+        held.append(weakref.ref(work))
+        kv.release_workspaces()
+        return work
+
+    def launched(*args):
+        assert held[-1]() is not None and args[-1] == held[-1]().data_ptr()
+        return launch(*args)
+
+    monkeypatch.setattr(cache, "_tree_workspace", found)
+    monkeypatch.setattr(cache, "_attend_tree", launched)
+    check_tree(cache, q, table, n, ints([-1, 0, 0]))
+    assert len(held) == 1 and held[0]() is None
