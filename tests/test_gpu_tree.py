@@ -835,3 +835,23 @@ def test_tree_workspace_is_held_for_the_launches(kv, monkeypatch):  # noqa: F811
     monkeypatch.setattr(cache, "_attend_tree", launched)
     check_tree(cache, q, table, n, ints([-1, 0, 0]))
     assert len(held) == 1 and held[0]() is None
+
+
+@pytest.mark.parametrize("dtype,store,part,parts_of_attend", [(BF16, BF16, 2.0 ** -17, 2.0 ** -24), (BF16, I8, 2.0 ** -21, 2.0 ** -21), (F16, I8, 2.0 ** -21, 2.0 ** -21)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_tree_of_one_node_is_attend_in_every_type(kv, dtype, store, part, parts_of_attend, dim):  # noqa: F811
+    """The two calls' outputs are apart by no more than both bounds together, and by one number of the type at most in nearly all."""
+    g = torch.Generator().manual_seed(29)
+    lens = [0, 5, 700, 64, 3000] * 3
+    cache, q, table, n = setup(kv, lens, 1, 2, 4, 16, dim, dtype, store, g)
+    out, lse = cache.attend_tree(q, table, n, ints([-1]))
+    one, olse = cache.attend(q[:, 0].contiguous(), table, n + 1)
+    k, v = values(cache)
+    eo, el, pv, mag = O.attend_tree(c(q), k, v, c(table), c(n), np.full((len(lens), 1), -1), None, dim ** -0.5)
+    es = (dim + 4) * 2.0 ** -23 * mag[:, 0, :, None]
+    L = max(lens) + 1
+    each = U[dtype] * np.abs(eo[:, 0]) + (2 * es + 2.0 ** -20 + (L + 64) * 2.0 ** -22) * pv[:, 0] + (2.0 ** -25 if dtype == F16 else 0)
+    a, b = c(out)[:, 0].astype(np.float64), c(one).astype(np.float64)
+    assert (np.abs(a - b) <= 2 * each + (part + parts_of_attend) * pv[:, 0]).all()
+    assert (np.abs(a - b) <= 4 * U[dtype] * np.abs(eo[:, 0])).mean() > 0.99
+    assert (np.abs(c(lse)[:, 0] - c(olse)) <= 2 * (2 * es[..., 0] + (L + 64) * 2.0 ** -22 + 2.0 ** -20 * (1 + np.abs(el[:, 0])))).all()
